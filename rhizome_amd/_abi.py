@@ -1,4 +1,4 @@
-"""ctypes mirror of include/rhizome_gdr.h and the loader of librhizome_gdr.so.
+"""ctypes mirror of include/rhizome_gdr.h and rhizome_train.h and the loader of librhizome_gdr.so.
 
 The library is loaded from this package directory only (built in-tree by
 rhizome_amd.build); if it is missing, loading raises -- there is no
@@ -18,6 +18,7 @@ ROOT = os.path.dirname(HERE)
 # sanitizer build under _build/asan, for example); there is no other backend.
 LIB_PATH = os.environ.get("RHIZOME_GDR_LIB") or os.path.join(HERE, "librhizome_gdr.so")
 HEADER = os.path.join(ROOT, "include", "rhizome_gdr.h")
+TRAIN_HEADER = os.path.join(ROOT, "include", "rhizome_train.h")
 
 # rhz_status
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_HIP = 0, 1, 2, 3, 4
@@ -71,6 +72,19 @@ class MultistepArgs(Structure):
     ]
 
 
+class PrefillBackwardArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32), ("seq_len", c_int32), ("heads", c_int32), ("d_k", c_int32),
+        ("d_v", c_int32), ("dtype", c_int32), ("gate_kind", c_int32),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("gate", c_void_p), ("beta", c_void_p),
+        ("grad_o", c_void_p), ("cu_seqlens", c_void_p), ("initial_state", c_void_p),
+        ("grad_final_state", c_void_p),
+        ("grad_q", c_void_p), ("grad_k", c_void_p), ("grad_v", c_void_p), ("grad_gate", c_void_p),
+        ("grad_beta", c_void_p), ("grad_initial_state", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class Conv1dArgs(Structure):
     _fields_ = [
         ("batch", c_int32), ("seq_len", c_int32), ("channels", c_int32), ("dtype", c_int32),
@@ -118,9 +132,9 @@ class GdrError(RuntimeError):
 _lib = None
 
 
-def declared_functions() -> list[str]:
-    """Names of the functions declared in include/rhizome_gdr.h."""
-    text = open(HEADER).read()
+def declared_functions(header: str = HEADER) -> list[str]:
+    """Names of the functions declared in include/rhizome_gdr.h (or another header)."""
+    text = open(header).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     return sorted(set(re.findall(r"\b(rhz_\w+)\s*\(", text)))
 
@@ -159,6 +173,10 @@ def lib():
         L.rhz_gdr_decode_step.restype = c_int32
         L.rhz_gdr_multistep.argtypes = [POINTER(MultistepArgs), c_void_p]
         L.rhz_gdr_multistep.restype = c_int32
+        L.rhz_gdr_prefill_backward_workspace_size.argtypes = [POINTER(PrefillBackwardArgs), POINTER(c_size_t)]
+        L.rhz_gdr_prefill_backward_workspace_size.restype = c_int32
+        L.rhz_gdr_prefill_backward.argtypes = [POINTER(PrefillBackwardArgs), c_void_p]
+        L.rhz_gdr_prefill_backward.restype = c_int32
         L.rhz_causal_conv1d.argtypes = [POINTER(Conv1dArgs), c_void_p]
         L.rhz_causal_conv1d.restype = c_int32
         L.rhz_gdr_prepare.argtypes = [POINTER(PrepareArgs), c_void_p]

@@ -117,6 +117,11 @@ rhz_status hip_status(hipError_t e, const char* what) {
 
 }  // namespace
 
+rhz_status rhz::record_error(rhz_status s, const char* detail) {
+    g_last_error = detail;
+    return s;
+}
+
 extern "C" {
 
 int32_t rhz_gdr_abi_version(void) { return RHZ_GDR_ABI_VERSION; }

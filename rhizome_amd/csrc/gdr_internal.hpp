@@ -8,8 +8,12 @@
 #include <stdint.h>
 
 #include "rhizome_gdr.h"
+#include "rhizome_train.h"
 
 namespace rhz {
+
+// Keeps `detail` as the calling thread's last error (rhz_last_error); returns s.
+rhz_status record_error(rhz_status s, const char* detail);
 
 // Whether the runtime launches a grid of `blocks` workgroups of `threads` along
 // x as asked: it truncates one of 2^32 work-items or more without an error.
@@ -63,6 +67,10 @@ hipError_t chunked_range_errors(unsigned int* count, bool reset);
 // The same for the count of workgroups that recomputed their rows with the
 // fp32 recurrence because an input left the fp16 path's domain.
 hipError_t chunked_exact_reruns(unsigned int* count, bool reset);
+
+// Backward pass of the prefill (gdr_backward.hip); d_k <= 128.
+size_t backward_workspace_bytes(const rhz_gdr_prefill_backward_args& a);
+hipError_t launch_backward(const rhz_gdr_prefill_backward_args& a, hipStream_t stream);
 
 // Local-block prologue and epilogue (gdr_aux.hip).
 hipError_t launch_conv1d(const rhz_conv1d_args& a, hipStream_t stream);
