@@ -78,6 +78,95 @@ rhz_status rhz_gdr_prefill_backward_workspace_size(const rhz_gdr_prefill_backwar
 
 rhz_status rhz_gdr_prefill_backward(const rhz_gdr_prefill_backward_args* args, void* stream);
 
+/* Backward pass of rhz_gdr_conv_prepare, the Local block's prologue: from the
+ * gradients of its outputs q, k, v, beta and g (as rhz_gdr_prefill_backward
+ * gives them for RHZ_GATE_LOG_ALPHA) and of the final conv state, those of x,
+ * the weights, the bias, the logits, a_log and the initial conv state.  The
+ * forward call's inputs are given again and the convolution formed again, in
+ * fp32.  The same shapes as the forward call (else RHZ_ERR_UNSUPPORTED).  Rows
+ * of a pack outside every sequence are left as they were and add nothing.  No
+ * output overlaps an input, the workspace or another output. */
+typedef struct rhz_gdr_conv_prepare_backward_args {
+    int32_t batch;    /* dense: B;  packed: number of sequences N (>= 1) */
+    int32_t seq_len;  /* dense: T;  packed: total tokens (>= 0) */
+    int32_t heads;    /* H >= 1 */
+    int32_t d_k;      /* >= 1 */
+    int32_t d_v;      /* >= 1 */
+    int32_t dtype;    /* rhz_dtype of x, of grad_q .. grad_g and of grad_x */
+    float q_scale;    /* as in the forward call; must be finite */
+    const void* x;              /* [tokens, C], C = H (2 d_k + d_v) */
+    const float* weight;        /* [C, 4] */
+    const float* bias;          /* [C], or NULL for zero */
+    const int32_t* cu_seqlens;  /* [N+1] or NULL (dense) */
+    const float* initial_state; /* [batch, C, 3], or NULL for zeros */
+    const float* beta_logit;    /* [tokens, H] */
+    const float* alpha_logit;   /* [tokens, H] */
+    const float* a_log;         /* [H] */
+    const void* grad_q;         /* [tokens, H, d_k] */
+    const void* grad_k;         /* [tokens, H, d_k] */
+    const void* grad_v;         /* [tokens, H, d_v] */
+    const void* grad_beta;      /* [tokens, H] */
+    const void* grad_g;         /* [tokens, H] */
+    const float* grad_final_state; /* [batch, C, 3], or NULL for zeros */
+    void* grad_x;               /* [tokens, C] out */
+    float* grad_weight;         /* [C, 4] out */
+    float* grad_bias;           /* [C] out, or NULL */
+    float* grad_beta_logit;     /* [tokens, H] out */
+    float* grad_alpha_logit;    /* [tokens, H] out */
+    float* grad_a_log;          /* [H] out */
+    float* grad_initial_state;  /* [batch, C, 3] out, or NULL */
+    void* workspace;            /* device scratch, 256-byte aligned */
+    size_t workspace_bytes;
+} rhz_gdr_conv_prepare_backward_args;
+
+rhz_status rhz_gdr_conv_prepare_backward_workspace_size(const rhz_gdr_conv_prepare_backward_args* args,
+                                                        size_t* bytes);
+
+rhz_status rhz_gdr_conv_prepare_backward(const rhz_gdr_conv_prepare_backward_args* args, void* stream);
+
+/* Layer norm of every row of `dim` values: y = (x - mean) / sqrt(variance +
+ * eps) * weight + bias, the variance from the centred values, in fp32.  y may
+ * alias x. */
+typedef struct rhz_layernorm_args {
+    int32_t rows;     /* >= 0 */
+    int32_t dim;      /* 1..8192 */
+    int32_t dtype;    /* rhz_dtype of x and y */
+    float eps;        /* >= 0 */
+    const void* x;        /* [rows, dim] */
+    const float* weight;  /* [dim] */
+    const float* bias;    /* [dim], or NULL for zero */
+    void* y;              /* [rows, dim] */
+} rhz_layernorm_args;
+
+rhz_status rhz_layernorm(const rhz_layernorm_args* args, void* stream);
+
+/* Backward pass of a row norm, rhz_layernorm or rhz_rmsnorm_heads: from grad_y
+ * and the forward call's x, grad_x and the sums over the rows for the weights
+ * (rhz_rmsnorm_heads's scale) and for layer norm's bias.  Statistics and sums
+ * in fp32.  No output overlaps an input, the workspace or another output. */
+typedef struct rhz_norm_backward_args {
+    int32_t rows;     /* >= 0 */
+    int32_t dim;      /* 1..8192 */
+    int32_t dtype;    /* rhz_dtype of grad_y, x and grad_x */
+    float eps;        /* as in the forward call */
+    const void* grad_y;   /* [rows, dim] */
+    const void* x;        /* [rows, dim] */
+    const float* weight;  /* [dim]: layer norm's weight, or RMSNorm's scale */
+    void* grad_x;         /* [rows, dim] out */
+    float* grad_weight;   /* [dim] out */
+    float* grad_bias;     /* [dim] out, or NULL; NULL for RMSNorm */
+    void* workspace;      /* device scratch, 256-byte aligned */
+    size_t workspace_bytes;
+} rhz_norm_backward_args;
+
+/* Bytes of workspace of either of the two calls below: at most 4 KiB per
+ * column. */
+rhz_status rhz_norm_backward_workspace_size(const rhz_norm_backward_args* args, size_t* bytes);
+
+rhz_status rhz_layernorm_backward(const rhz_norm_backward_args* args, void* stream);
+
+rhz_status rhz_rmsnorm_heads_backward(const rhz_norm_backward_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,8 +8,10 @@ and raises if the library is missing.
 from .gdr import (causal_conv1d, conv_prepare, decode_step, exact_reruns, fp16_range_errors,  # noqa: F401
                   local_prefill, multistep, philox_fill, prefill, prepare, query_support,
                   rmsnorm_heads, sync_timeouts)
-from .train import prefill_backward  # noqa: F401
+from .train import (conv_prepare_backward, layernorm, layernorm_backward, prefill_backward,  # noqa: F401
+                    rmsnorm_heads_backward)
 
 __all__ = ["prefill", "prefill_backward", "local_prefill", "decode_step", "multistep", "causal_conv1d", "prepare",
-           "conv_prepare", "rmsnorm_heads", "philox_fill", "query_support", "sync_timeouts", "fp16_range_errors",
+           "conv_prepare", "conv_prepare_backward", "rmsnorm_heads", "rmsnorm_heads_backward", "layernorm",
+           "layernorm_backward", "philox_fill", "query_support", "sync_timeouts", "fp16_range_errors",
            "exact_reruns"]

@@ -85,6 +85,35 @@ class PrefillBackwardArgs(Structure):
     ]
 
 
+class ConvPrepareBackwardArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32), ("seq_len", c_int32), ("heads", c_int32), ("d_k", c_int32),
+        ("d_v", c_int32), ("dtype", c_int32), ("q_scale", c_float),
+        ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("cu_seqlens", c_void_p),
+        ("initial_state", c_void_p), ("beta_logit", c_void_p), ("alpha_logit", c_void_p), ("a_log", c_void_p),
+        ("grad_q", c_void_p), ("grad_k", c_void_p), ("grad_v", c_void_p), ("grad_beta", c_void_p),
+        ("grad_g", c_void_p), ("grad_final_state", c_void_p),
+        ("grad_x", c_void_p), ("grad_weight", c_void_p), ("grad_bias", c_void_p),
+        ("grad_beta_logit", c_void_p), ("grad_alpha_logit", c_void_p), ("grad_a_log", c_void_p),
+        ("grad_initial_state", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class LayernormArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32), ("dim", c_int32), ("dtype", c_int32), ("eps", c_float),
+        ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("y", c_void_p),
+    ]
+
+
+class NormBackwardArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32), ("dim", c_int32), ("dtype", c_int32), ("eps", c_float),
+        ("grad_y", c_void_p), ("x", c_void_p), ("weight", c_void_p), ("grad_x", c_void_p),
+        ("grad_weight", c_void_p), ("grad_bias", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class Conv1dArgs(Structure):
     _fields_ = [
         ("batch", c_int32), ("seq_len", c_int32), ("channels", c_int32), ("dtype", c_int32),
@@ -177,6 +206,15 @@ def lib():
         L.rhz_gdr_prefill_backward_workspace_size.restype = c_int32
         L.rhz_gdr_prefill_backward.argtypes = [POINTER(PrefillBackwardArgs), c_void_p]
         L.rhz_gdr_prefill_backward.restype = c_int32
+        for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
+                           ("rhz_norm_backward", NormBackwardArgs)):
+            size = getattr(L, name + "_workspace_size")
+            size.argtypes, size.restype = [POINTER(args), POINTER(c_size_t)], c_int32
+        for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
+                           ("rhz_layernorm", LayernormArgs), ("rhz_layernorm_backward", NormBackwardArgs),
+                           ("rhz_rmsnorm_heads_backward", NormBackwardArgs)):
+            run = getattr(L, name)
+            run.argtypes, run.restype = [POINTER(args), c_void_p], c_int32
         L.rhz_causal_conv1d.argtypes = [POINTER(Conv1dArgs), c_void_p]
         L.rhz_causal_conv1d.restype = c_int32
         L.rhz_gdr_prepare.argtypes = [POINTER(PrepareArgs), c_void_p]

@@ -81,6 +81,15 @@ hipError_t launch_rmsnorm(const rhz_rmsnorm_args& a, hipStream_t stream);
 bool conv_prepare_supported(int dtype, int d_k, int d_v);
 hipError_t launch_conv_prepare(const rhz_gdr_conv_prepare_args& a, hipStream_t stream);
 
+// The prologue's and the norms' backward passes (gdr_conv_backward.hip,
+// gdr_norm_backward.hip).
+size_t conv_prepare_backward_workspace_bytes(const rhz_gdr_conv_prepare_backward_args& a);
+hipError_t launch_conv_prepare_backward(const rhz_gdr_conv_prepare_backward_args& a, hipStream_t stream);
+hipError_t launch_layernorm(const rhz_layernorm_args& a, hipStream_t stream);
+size_t norm_backward_workspace_bytes(const rhz_norm_backward_args& a);
+// layer: layer norm's, else RMSNorm's
+hipError_t launch_norm_backward(const rhz_norm_backward_args& a, bool layer, hipStream_t stream);
+
 // Device Philox-4x32-10 fill.
 hipError_t launch_philox_fill(int kind, uint64_t seed, uint64_t stream_id, int64_t count,
                               int row_len, double mean, double std_dev, int out_dtype, void* out,

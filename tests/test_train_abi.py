@@ -99,6 +99,85 @@ def test_backward_of_nothing():
     assert _abi.lib().rhz_gdr_prefill_backward(None, None) == _abi.ERR_INVALID_ARG
 
 
+CONV = dict(batch=2, seq_len=100, heads=4, d_k=64, d_v=64, dtype=_abi.BF16, q_scale=8.0)
+CONV_PTRS = ("x", "weight", "beta_logit", "alpha_logit", "a_log", "grad_q", "grad_k", "grad_v", "grad_beta", "grad_g",
+             "grad_x", "grad_weight", "grad_beta_logit", "grad_alpha_logit", "grad_a_log")
+
+
+@pytest.mark.parametrize("over,status,msg", [
+    (dict(batch=0), _abi.ERR_INVALID_ARG, "batch"),
+    (dict(seq_len=-1), _abi.ERR_INVALID_ARG, "seq_len"),
+    (dict(heads=0), _abi.ERR_INVALID_ARG, "heads"),
+    (dict(d_k=0), _abi.ERR_INVALID_ARG, "d_k"),
+    (dict(d_k=24), _abi.ERR_UNSUPPORTED, "power of two"),
+    (dict(d_v=12), _abi.ERR_UNSUPPORTED, "multiples of 8"),
+    (dict(d_k=1024), _abi.ERR_UNSUPPORTED, "exceed"),
+    (dict(dtype=_abi.F64), _abi.ERR_INVALID_ARG, "dtype"),
+    (dict(q_scale=float("nan")), _abi.ERR_INVALID_ARG, "q_scale"),
+    (dict(seq_len=1 << 24), _abi.ERR_INVALID_ARG, "2^31"),
+    (dict(x=A + 8), _abi.ERR_INVALID_ARG, "x is not aligned"),
+    (dict(grad_v=A + 7 * STEP + 8), _abi.ERR_INVALID_ARG, "grad_v is not aligned"),
+    (dict(grad_x=A + 5 * STEP), _abi.ERR_INVALID_ARG, "overlaps"),
+    (dict(grad_weight=A + STEP), _abi.ERR_INVALID_ARG, "overlaps"),
+    (dict(), _abi.ERR_WORKSPACE, "workspace is NULL"),
+    (dict(workspace=A + 50 * STEP, workspace_bytes=64), _abi.ERR_WORKSPACE, "needed"),
+    (dict(workspace=A + 50 * STEP + 16, workspace_bytes=1 << 30), _abi.ERR_WORKSPACE, "256-byte"),
+] + [({p: None}, _abi.ERR_INVALID_ARG, f"{p} is NULL") for p in CONV_PTRS])
+def test_conv_prepare_backward_validation(over, status, msg):
+    a = _fill(_abi.ConvPrepareBackwardArgs, CONV, CONV_PTRS, over)
+    assert _abi.lib().rhz_gdr_conv_prepare_backward(byref(a), None) == status, _abi.last_error()
+    assert msg in _abi.last_error()
+    assert _abi.lib().rhz_gdr_conv_prepare_backward(None, None) == _abi.ERR_INVALID_ARG
+
+
+NORM = dict(rows=100, dim=128, dtype=_abi.BF16, eps=1e-5)
+NORM_PTRS = ("grad_y", "x", "weight", "grad_x", "grad_weight")
+
+
+@pytest.mark.parametrize("over,status,msg", [
+    (dict(rows=-1), _abi.ERR_INVALID_ARG, "rows"),
+    (dict(dim=0), _abi.ERR_INVALID_ARG, "dim"),
+    (dict(dim=8193), _abi.ERR_UNSUPPORTED, "dim"),
+    (dict(dtype=2), _abi.ERR_INVALID_ARG, "dtype"),
+    (dict(eps=-1.0), _abi.ERR_INVALID_ARG, "eps"),
+    (dict(eps=float("nan")), _abi.ERR_INVALID_ARG, "eps"),
+    (dict(rows=1 << 25), _abi.ERR_INVALID_ARG, "2^31"),
+    (dict(x=A + STEP + 1), _abi.ERR_INVALID_ARG, "x is not aligned"),
+    (dict(grad_x=A), _abi.ERR_INVALID_ARG, "overlaps"),
+    (dict(), _abi.ERR_WORKSPACE, "workspace is NULL"),
+    (dict(workspace=A + 50 * STEP, workspace_bytes=64), _abi.ERR_WORKSPACE, "needed"),
+] + [({p: None}, _abi.ERR_INVALID_ARG, f"{p} is NULL") for p in NORM_PTRS])
+def test_norm_backward_validation(over, status, msg):
+    a = _fill(_abi.NormBackwardArgs, NORM, NORM_PTRS, over)
+    for run in (_abi.lib().rhz_layernorm_backward, _abi.lib().rhz_rmsnorm_heads_backward):
+        assert run(byref(a), None) == status, _abi.last_error()
+        assert msg in _abi.last_error()
+
+
+def test_layernorm_validation():
+    run = _abi.lib().rhz_layernorm
+    for over, status in ((dict(rows=-1), _abi.ERR_INVALID_ARG), (dict(dim=9000), _abi.ERR_UNSUPPORTED),
+                         (dict(x=None), _abi.ERR_INVALID_ARG), (dict(y=A + 1), _abi.ERR_INVALID_ARG),
+                         (dict(weight=None), _abi.ERR_INVALID_ARG), (dict(bias=A + 2), _abi.ERR_INVALID_ARG),
+                         (dict(rows=0, x=None, y=None, weight=None), _abi.OK)):
+        assert run(byref(_fill(_abi.LayernormArgs, NORM, ("x", "weight", "y"), over)), None) == status
+    a = _fill(_abi.NormBackwardArgs, NORM, NORM_PTRS + ("grad_bias",), {})
+    assert _abi.lib().rhz_rmsnorm_heads_backward(byref(a), None) == _abi.ERR_INVALID_ARG
+    assert "no bias" in _abi.last_error()
+
+
+@pytest.mark.parametrize("name,struct,values,pointers", [
+    ("rhz_gdr_conv_prepare_backward", _abi.ConvPrepareBackwardArgs, CONV, CONV_PTRS),
+    ("rhz_norm_backward", _abi.NormBackwardArgs, NORM, NORM_PTRS)])
+def test_other_workspace_sizes(name, struct, values, pointers):
+    query = name + "_workspace_size"
+    status, n = _size(_fill(struct, values, pointers, {}), query)
+    assert status == _abi.OK and n > 0
+    empty = {"seq_len": 0} if "seq_len" in values else {"rows": 0}
+    assert _size(_fill(struct, values, pointers, empty), query) == (_abi.OK, 0)
+    assert getattr(_abi.lib(), query)(byref(_fill(struct, values, pointers, {})), None) == _abi.ERR_INVALID_ARG
+
+
 VALIDATION = {_abi.ERR_INVALID_ARG, _abi.ERR_UNSUPPORTED, _abi.ERR_WORKSPACE}
 ints = st.one_of(st.integers(-3, 300), st.sampled_from([0, 1, 64, 128, 1024, 4096, 65536]),
                  st.integers(-2**31, 2**31 - 1))
