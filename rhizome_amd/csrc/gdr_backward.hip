@@ -52,6 +52,12 @@ constexpr int C64 = kChunk;           // tokens of a chunk
 constexpr double kMinLog = -1000.0;   // log-decays below it decay to 0 in fp32 all the same
 constexpr float kTinyAlpha = 1e-18f;  // below: dalpha is formed without dividing by alpha
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
 // ------------------------------------------------------------- operands
 // An MFMA operand is held in "units" of 16 bytes per lane.  Lane (g, m), g =
 // lane / 16, m = lane % 16, holds for row m of a 16-row tile the contraction
@@ -61,6 +67,7 @@ constexpr float kTinyAlpha = 1e-18f;  // below: dalpha is formed without dividin
 struct OpF16 {
     using Elt = _Float16;
     using Unit = f16x8;
+    using Quad = f16x4;
     static constexpr int kBlocks = 2;  // 16-index blocks of a unit
     static constexpr bool kScaled = true;
     static __device__ __forceinline__ f32x4 mma(const Unit& a, const Unit& b, const f32x4& c) {
@@ -87,6 +94,7 @@ struct OpF16 {
 struct OpF32 {
     using Elt = float;
     using Unit = f32x4;
+    using Quad = f32x4;
     static constexpr int kBlocks = 1;
     static constexpr bool kScaled = false;
     static __device__ __forceinline__ f32x4 mma(const Unit& a, const Unit& b, f32x4 c) {
@@ -103,48 +111,78 @@ struct OpF32 {
     static __device__ __forceinline__ void unpack(const Unit& u, f32x4* t) { t[0] = u; }
 };
 
-// A matrix of units in LDS, NKU units along the contraction per 16-row tile.
-// A wave reads one unit of a tile at once, 1 KiB; within it the row is XORed
-// so that the staging writes, which run along tiles, units and g, spread over
-// the banks.
-template <class Op, int NKU>
-struct LdsMat {
-    using Unit = typename Op::Unit;
+template <class Op>
+__device__ __forceinline__ typename Op::Unit lds_unit(const char* p, int i, int lane) {
+    return reinterpret_cast<const typename Op::Unit*>(p)[i * 64 + lane];
+}
+
+// A matrix by rows in LDS.  A unit of it is read along its rows, or along its
+// columns (fp16: ds_read_b64_tr_b16, which gives lane l of 16 the l-th column
+// of four rows), so that one copy serves products over either index.  The
+// padding of a row spreads 16 rows' accesses evenly over the banks.
+template <class Op, int COLS>
+struct RowMat {
     using Elt = typename Op::Elt;
-    static constexpr int kTileBytes = NKU * 1024;
+    using Unit = typename Op::Unit;
+    static constexpr int kStride = COLS * int(sizeof(Elt)) + 16;
+    static constexpr int bytes(int rows) { return rows * kStride; }
     char* p;
-    static __device__ __forceinline__ int slot(int mt, int ku, int g, int m) {
-        return g * 16 + (m ^ (((g << 2) ^ (ku & 3) ^ (mt & 3)) & 15));
+    __device__ __forceinline__ char* at(int row, int col) const { return p + row * kStride + col * int(sizeof(Elt)); }
+    // a unit's 16 bytes of consecutive columns: an order of the contraction
+    // that only another operand read this way shares
+    __device__ __forceinline__ Unit run(int row0, int ku, int lane) const {
+        return *reinterpret_cast<const Unit*>(at(row0 + (lane & 15), (ku * 4 + (lane >> 4)) * (16 / int(sizeof(Elt)))));
     }
-    __device__ __forceinline__ Unit unit(int mt, int ku, int lane) const {
-        return *reinterpret_cast<const Unit*>(p + (mt * NKU + ku) * 1024 + slot(mt, ku, lane >> 4, lane & 15) * 16);
-    }
-    __device__ __forceinline__ void put_unit(int mt, int ku, int lane, const Unit& u) const {
-        *reinterpret_cast<Unit*>(p + (mt * NKU + ku) * 1024 + slot(mt, ku, lane >> 4, lane & 15) * 16) = u;
-    }
-    // the four contraction indices k .. k + 3 (k a multiple of 4) of a row
-    static __device__ __forceinline__ int offset4(int row, int k) {
-        const int b = k >> 4, ku = b / Op::kBlocks, half = b % Op::kBlocks;
-        return ((row >> 4) * NKU + ku) * 1024 + slot(row >> 4, ku, (k >> 2) & 3, row & 15) * 16 + half * 8;
-    }
-    __device__ __forceinline__ void put4(int row, int k, float a, float b, float c, float d) const {
+    // the columns 16 b + 4 g .. of a unit's blocks, as accumulators hold them
+    __device__ __forceinline__ Unit blocks(int row, int ku, int g) const {
         if constexpr (Op::kScaled) {
-            uint2 u = {pack_f16x2(a, b), pack_f16x2(c, d)};
-            *reinterpret_cast<uint2*>(p + offset4(row, k)) = u;
+            const f16x4 a = *reinterpret_cast<const f16x4*>(at(row, 32 * ku + 4 * g));
+            const f16x4 b = *reinterpret_cast<const f16x4*>(at(row, 32 * ku + 16 + 4 * g));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-            *reinterpret_cast<f32x4*>(p + offset4(row, k)) = f32x4{a, b, c, d};
+            return *reinterpret_cast<const Unit*>(at(row, 16 * ku + 4 * g));
         }
     }
-    __device__ __forceinline__ void put4(int row, int k, uint2 u) const {
-        *reinterpret_cast<uint2*>(p + offset4(row, k)) = u;
-    }
-    __device__ __forceinline__ f32x4 get4(int row, int k) const {
+    // column 16 ct + m, rows 16 rb + 4 g ..
+    __device__ __forceinline__ typename Op::Quad col4(int ct, int rb, int lane) const {
+        const int g = lane >> 4, m = lane & 15;
         if constexpr (Op::kScaled) {
-            typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-            const f16x4 h = *reinterpret_cast<const f16x4*>(p + offset4(row, k));
-            return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+            const char* a = at(16 * rb + 4 * g + (m >> 2), 16 * ct + 4 * (m & 3));
+            return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a)));
         } else {
-            return *reinterpret_cast<const f32x4*>(p + offset4(row, k));
+            f32x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const float*>(at(16 * rb + 4 * g + j, 16 * ct + m));
+            return x;
+        }
+    }
+    __device__ __forceinline__ Unit cols(int ct, int ku, int lane) const {
+        if constexpr (Op::kScaled)
+            return __builtin_shufflevector(col4(ct, 2 * ku, lane), col4(ct, 2 * ku + 1, lane), 0, 1, 2, 3, 4, 5, 6, 7);
+        else
+            return col4(ct, ku, lane);
+    }
+    __device__ __forceinline__ void put_unit(int row, int ku, int g, const Unit& u) const {  // the inverse of blocks()
+        if constexpr (Op::kScaled) {
+            *reinterpret_cast<f16x4*>(at(row, 32 * ku + 4 * g)) = __builtin_shufflevector(u, u, 0, 1, 2, 3);
+            *reinterpret_cast<f16x4*>(at(row, 32 * ku + 16 + 4 * g)) = __builtin_shufflevector(u, u, 4, 5, 6, 7);
+        } else {
+            *reinterpret_cast<Unit*>(at(row, 16 * ku + 4 * g)) = u;
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void put(int row, int col, const float (&x)[N], float s) const {
+        if constexpr (Op::kScaled) {
+            typedef _Float16 f16xn __attribute__((ext_vector_type(N)));
+            f16xn h;
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = (_Float16)(x[i] * s);
+            *reinterpret_cast<f16xn*>(at(row, col)) = h;
+        } else {
+            static_assert(N == 4 || N == 8, "");
+#pragma unroll
+            for (int i = 0; i < N; i += 4)
+                *reinterpret_cast<f32x4*>(at(row, col + i)) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
         }
     }
 };
@@ -153,67 +191,114 @@ struct LdsMat {
 __device__ __forceinline__ int sq_at(int r, int c) { return r * 64 + ((((c >> 2) ^ r) & 15) << 2) + (c & 3); }
 
 __device__ __forceinline__ int bits_abs(float x) { return int(__float_as_uint(x) & 0x7fffffffu); }
-// Maximum over the wave of non-negative ints (magnitude bits: a NaN's are the largest).
+// Maximum over the wave of non-negative ints (magnitude bits: a NaN's are the
+// largest), by DPP within rows of 16 and then over the four rows.
+template <int CTRL>
+__device__ __forceinline__ int dpp_max(int x) {
+    return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ int wave_max_bits(int x) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off, kWave));
-    return __builtin_amdgcn_readfirstlane(x);
+    x = dpp_max<0x128>(dpp_max<0x124>(dpp_max<0x4E>(dpp_max<0xB1>(x))));
+    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+               max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
-// The power of two that a tile of largest magnitude `bits` is divided by, so
-// that its largest value lands in [2^to, 2^(to+1)).
-__device__ __forceinline__ int tile_exp(int bits, int to) { return max(min((bits >> 23) - 127, 100), -100) - to; }
+// The exponent of magnitude bits, 100 at most either way.
+__device__ __forceinline__ int bits_exp(int bits) { return max(min((bits >> 23) - 127, 100), -100); }
 
-// Four consecutive elements of a row, zero from `n` on.
+// A run of 16 bytes of a row of T (8 bf16 or 4 fp32), as floats.  VEC: rows
+// are whole runs and aligned, and a run outside the matrix (`in` false) is
+// read from `safe` and cleared, so that no branch parts the loads.
 template <typename T>
-__device__ __forceinline__ float4 row4(const T* p, int n, bool vec) {
-    if (vec && n >= 4) return load4(p);
-    float4 r;
-    r.x = n > 0 ? Elem<T>::load(p, 0) : 0.f;
-    r.y = n > 1 ? Elem<T>::load(p, 1) : 0.f;
-    r.z = n > 2 ? Elem<T>::load(p, 2) : 0.f;
-    r.w = n > 3 ? Elem<T>::load(p, 3) : 0.f;
-    return r;
+constexpr int kRun = 16 / int(sizeof(T));
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4 load_run(const T* p, const T* safe, bool in, int n) {
+    if constexpr (VEC) {
+        const u32x4 u = *reinterpret_cast<const u32x4*>(in ? p : safe);
+        return in ? u : u32x4{0, 0, 0, 0};
+    } else {
+        T x[kRun<T>];
+#pragma unroll
+        for (int i = 0; i < kRun<T>; ++i) x[i] = in && i < n ? p[i] : T(0);
+        return __builtin_bit_cast(u32x4, x);
+    }
 }
 template <typename T>
-__device__ __forceinline__ void put_row4(T* p, int n, bool vec, float a, float b, float c, float d) {
-    if (vec && n >= 4) {
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
-        else
-            *reinterpret_cast<uint2*>(p) = uint2{pack_bf16x2(a, b), pack_bf16x2(c, d)};
-        return;
+__device__ __forceinline__ void unpack_run(const u32x4& u, float (&x)[kRun<T>]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
     }
-    if (n > 0) Elem<T>::store(p, 0, a);
-    if (n > 1) Elem<T>::store(p, 1, b);
-    if (n > 2) Elem<T>::store(p, 2, c);
-    if (n > 3) Elem<T>::store(p, 3, d);
+}
+template <typename T>
+__device__ __forceinline__ int run_max_bits(const u32x4& u) {
+    float x[kRun<T>];
+    unpack_run<T>(u, x);
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < kRun<T>; ++i) m = max(m, bits_abs(x[i]));
+    return m;
+}
+// Two floats as bf16, round to nearest even, by the hardware's conversion.
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+// N consecutive values of a row of which n lie in the matrix; VEC: all or none do.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void store_run(T* p, int n, const float (&x)[N]) {
+    if constexpr (VEC) {
+        if (n <= 0) return;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4)
+                *reinterpret_cast<f32x4*>(p + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        } else if constexpr (N == 8) {
+            *reinterpret_cast<u32x4*>(p) =
+                u32x4{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7])};
+        } else {
+            *reinterpret_cast<uint2*>(p) = uint2{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n) Elem<T>::store(p, i, x[i]);
+    }
 }
 
 // ------------------------------------------------------------ workspace
-// One record per (chunk, head): unit matrices for DK = d_k padded to 32, 64
-// or 128 and d_v padded to 16-row tiles (an even number of them).
+// One record per (chunk, head), in units of DK = d_k padded to 32, 64 or 128
+// and d_v padded to 16-row tiles (an even number of them).
 struct RecLayout {
-    size_t wk, kt, kd, qt, wt, ot, dot, s0, ds1, vec, bytes;
+    size_t wk, kd, kf, qf, wt, ot, dot, w, x, s0, ds1, vec, bytes;
 };
 __host__ __device__ inline RecLayout rec_layout(int DK, int dvt, int es) {
     RecLayout l{};
     const size_t tk = (size_t)64 * DK * es, tv = (size_t)64 * dvt * 16 * es, st = (size_t)DK * dvt * 16 * es;
     size_t at = 0;
     l.wk = at; at += tk;    // T diag(gamma) K          (token; d_k)
-    l.kt = at; at += tk;    // K                        (d_k; token)
     l.kd = at; at += tk;    // T^T diag(beta tail) K    (token; d_k)
-    l.qt = at; at += tk;    // Q                        (d_k; token)
-    l.wt = at; at += tv;    // T V, then W              (d_v; token)
-    l.ot = at; at += tv;    // T^T diag(beta) P^T dO, then dX  (d_v; token)
-    l.dot = at; at += tv;   // dO                       (d_v; token)
-    l.s0 = at; at += st;    // S0                       (d_v; d_k)
-    l.ds1 = at; at += st;   // dS1                      (d_v; d_k)
-    l.vec = at;             // Vec, then the tiles' exponents
+    l.kf = at; at += tk;    // K by rows, as scaled
+    l.qf = at; at += tk;    // Q by rows, as scaled
+    l.wt = at; at += tv;    // T V                            (d_v; token), by 16-row tiles
+    l.ot = at; at += tv;    // T^T diag(beta) P^T dO          (d_v; token), by 16-row tiles
+    l.dot = at; at += tv;   // dO                             (d_v; token), by 16-row tiles
+    l.w = at; at += tv;     // W                              (token; d_v), by units of d_v
+    l.x = at; at += tv;     // dX                             (token; d_v), by units of d_v
+    l.s0 = at; at += st;    // S0                             (d_k; d_v), by units of d_v
+    l.ds1 = at; at += st;   // dS1                            (d_k; d_v), by units of d_v
+    l.vec = at;             // small values, then the tiles' exponents
     at += 256 * 4 + 6 * 64 * 4;
     l.bytes = (at + 255) & ~(size_t)255;
     return l;
 }
-// the record's small values: gamma [64], beta tail [64], gamma_c, exponents of K and Q
+// the record's small values: gamma [64], beta tail [64], gamma_c, exponents of
+// K and Q, whether the chunk leaves the fp16 operands' domain
 enum { kVecGamma = 0, kVecWrite = 64, kVecGc = 128, kVecEK = 129, kVecEQ = 130, kVecBad = 131 };
 // exponents by d_v tile, from float 256 on
 enum { kExpV = 256, kExpO = 320, kExpW = 384, kExpX = 448, kExpS = 512, kExpD = 576 };
@@ -227,8 +312,7 @@ struct BwdParams {
     char* ws;
     RecLayout rec;
     int batch, seq_len, heads, d_k, d_v, dvt, gate_is_alpha;
-    bool vec_k, vec_v;  // rows of q, k (of v, dO) are loaded and stored four elements at a time
-    bool vec_s;         // rows of the states, 16 bytes at a time
+    bool vec_s;  // rows of the states, 16 bytes at a time
 };
 
 // The chunk `ci` of the launch: its sequence, first token and number of
@@ -259,20 +343,22 @@ __device__ __forceinline__ bool find_chunk(const BwdParams& p, int ci, ChunkAt& 
     return true;
 }
 
-// Running log-decays and factors of a chunk, by the first wave.
+// Running log-decays (to base 2, in fp64, so that a difference of two is exact
+// to fp32 whatever came before) and factors of a chunk, by the first wave.
 struct Gates {
     double G[64];
     float gamma[64], tail[64], beta[64], gate[64];
 };
+__device__ __forceinline__ float pow2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 __device__ __forceinline__ bool load_gates(const BwdParams& p, const ChunkAt& at, int h, Gates& gs, int lane) {
     const bool in = lane < at.n;
     const long r = (long)(at.t0 + (in ? lane : 0)) * p.heads + h;
-    const float gate = in ? p.gate[r] : (p.gate_is_alpha ? 1.f : 0.f);
-    const float beta = in ? p.beta[r] : 0.f;
-    double g = p.gate_is_alpha ? log((double)gate) : (double)gate;
-    const bool bad = !(g <= 0.0) || !(beta >= 0.f && beta <= 1.f);
-    if (g < kMinLog) g = kMinLog;
-    double G = g;
+    float gate = p.gate[r], beta = p.beta[r];
+    gate = in ? gate : (p.gate_is_alpha ? 1.f : 0.f);
+    beta = in ? beta : 0.f;
+    const float g = p.gate_is_alpha ? logf(gate) : gate;
+    const bool bad = !(g <= 0.f) || !(beta >= 0.f && beta <= 1.f);
+    double G = (double)(g < kMinLog ? kMinLog : g) * 1.4426950408889634;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const double o = __shfl_up(G, off, kWave);
@@ -280,91 +366,57 @@ __device__ __forceinline__ bool load_gates(const BwdParams& p, const ChunkAt& at
     }
     const double Gc = __shfl(G, 63, kWave);
     gs.G[lane] = G;
-    gs.gamma[lane] = expf((float)G);
-    gs.tail[lane] = expf((float)(Gc - G));
+    gs.gamma[lane] = pow2(G);
+    gs.tail[lane] = pow2(Gc - G);
     gs.beta[lane] = beta;
     gs.gate[lane] = gate;
     return bad;
 }
-__device__ __forceinline__ float decay(const Gates& gs, int r, int s) { return expf((float)(gs.G[r] - gs.G[s])); }
-
-// A 64-token block of q or k: thread blocks of 4 tokens x 4 columns.
-template <typename T, int DK>
-struct Block64 {
-    static constexpr int NB = (16 * (DK / 4) + 255) / 256;
-    float4 x[NB][4];
-    __device__ __forceinline__ int load(const T* base, long ld, int n, int d, bool vec) {
-        int m = 0;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, cb = id % (DK / 4), rb = id / (DK / 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = 4 * rb + j;
-                x[i][j] = t < n && rb < 16 ? row4<T>(base + t * ld + 4 * cb, d - 4 * cb, vec) : float4{0, 0, 0, 0};
-                m = max(m, max(max(bits_abs(x[i][j].x), bits_abs(x[i][j].y)),
-                               max(bits_abs(x[i][j].z), bits_abs(x[i][j].w))));
-            }
-        }
-        return m;
-    }
-    // rows (token; column) and / or columns (column; token) as units, times s
-    template <class Op>
-    __device__ __forceinline__ void put_rows(const LdsMat<Op, DK / (16 * Op::kBlocks)>& a, float s) const {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, cb = id % (DK / 4), rb = id / (DK / 4);
-            if (rb >= 16) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4& y = x[i][j];
-                a.put4(4 * rb + j, 4 * cb, y.x * s, y.y * s, y.z * s, y.w * s);
-            }
-        }
-    }
-    template <class Op>
-    __device__ __forceinline__ void put_cols(const LdsMat<Op, 64 / (16 * Op::kBlocks)>& a, float s) const {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + 256 * i, cb = id % (DK / 4), rb = id / (DK / 4);
-            if (rb >= 16) break;
-            const float4 *y = x[i];
-            a.put4(4 * cb + 0, 4 * rb, y[0].x * s, y[1].x * s, y[2].x * s, y[3].x * s);
-            a.put4(4 * cb + 1, 4 * rb, y[0].y * s, y[1].y * s, y[2].y * s, y[3].y * s);
-            a.put4(4 * cb + 2, 4 * rb, y[0].z * s, y[1].z * s, y[2].z * s, y[3].z * s);
-            a.put4(4 * cb + 3, 4 * rb, y[0].w * s, y[1].w * s, y[2].w * s, y[3].w * s);
-        }
-    }
-};
+__device__ __forceinline__ float decay(const Gates& gs, int r, int s) { return pow2(gs.G[r] - gs.G[s]); }
 
 // ----------------------------------------------------------------- prep
-// One (chunk, head) per workgroup of four waves.  LDS: K by rows (then T in
-// fp32), K by columns, Q by rows (then by columns), L diag(beta) in fp32 (then
-// T^T diag(beta) P^T), P (then each wave's tile of V or dO).
+// One (chunk, head) per workgroup of four waves.  LDS: K by rows (then each
+// wave's tile of V or dO), Q by rows (then T), L diag(beta) in fp32 (then
+// T^T diag(beta) P^T).
 template <class Op, int DK>
 struct PrepLds {
-    static constexpr int kRow = 64 * DK * int(sizeof(typename Op::Elt));
-    static constexpr int kSq = 64 * 64 * 4;
+    using T64 = RowMat<Op, 64>;
+    using Tile = RowMat<Op, 16>;
+    static constexpr int kRow = RowMat<Op, DK>::bytes(64), kTiles = 4 * Tile::bytes(64);
+    static constexpr int kDiag = 4 * 16 * 16 * 4;  // T's diagonal blocks in fp32
     static constexpr int kKr = 0;
-    static constexpr int kKt = kKr + (kRow > kSq ? kRow : kSq);  // T lies where K's rows were
-    static constexpr int kQr = kKt + kRow;
-    static constexpr int kA = kQr + kRow;
-    static constexpr int kP = kA + kSq;
-    static constexpr int kGates = kP + 64 * 64 * int(sizeof(typename Op::Elt));
+    static constexpr int kQr = kRow > kTiles ? kRow : kTiles;
+    static constexpr int kT = kQr, kTd = kQr + T64::bytes(64), kQEnd = kTd + kDiag;
+    static constexpr int kA = kQr + kRow > kQEnd ? kQr + kRow : kQEnd;
+    static constexpr int kGates = kA + 64 * 64 * 4;
     static constexpr int kMisc = kGates + int(sizeof(Gates));
     static constexpr int kBytes = kMisc + 64;
 };
 
-template <class Op, typename T, int DK>
+// every element of a unit times the factor of its contraction index
+template <class Op>
+__device__ __forceinline__ typename Op::Unit times_unit(const typename Op::Unit& u, const float* f, int ku, int g) {
+    f32x4 t[Op::kBlocks];
+    Op::unpack(u, t);
+#pragma unroll
+    for (int b = 0; b < Op::kBlocks; ++b) t[b] *= *reinterpret_cast<const f32x4*>(f + 16 * (ku * Op::kBlocks + b) + 4 * g);
+    return Op::pack(t, 1.f);
+}
+
+template <class Op, typename T, int DK, bool VEC>
 __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at, int h, char* rec, char* lds) {
     using Unit = typename Op::Unit;
+    using Elt = typename Op::Elt;
     using L = PrepLds<Op, DK>;
-    constexpr int NT = DK / 16, NKK = NT / Op::kBlocks, NKT = 4 / Op::kBlocks, NBK = Op::kBlocks;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, m = lane & 15;
-    const LdsMat<Op, NKK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
-    const LdsMat<Op, NKT> Kt{lds + L::kKt}, Qt{lds + L::kQr}, Pm{lds + L::kP}, Bo{lds + L::kA};
+    constexpr int NT = DK / 16, NBK = Op::kBlocks, NKK = NT / NBK, NKT = 4 / NBK, R = kRun<T>;
+    constexpr int NR = 64 * DK / R / 256;  // runs of K (and of Q) per thread
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+              m = lane & 15;
+    const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
+    const RowMat<Op, 64> Th{lds + L::kT};
+    float* Td = reinterpret_cast<float*>(lds + L::kTd);
     float* Af = reinterpret_cast<float*>(lds + L::kA);
-    float* Tf = reinterpret_cast<float*>(lds + L::kKr);
+    char* Bo = lds + L::kA;
     Gates& gs = *reinterpret_cast<Gates*>(lds + L::kGates);
     int* misc = reinterpret_cast<int*>(lds + L::kMisc);  // maxima of K, Q by wave; [8] outside the domain
     float* vec = reinterpret_cast<float*>(rec + p.rec.vec);
@@ -373,31 +425,56 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     const long ldk = (long)p.heads * p.d_k, ldv = (long)p.heads * p.d_v;
     const T* kp = static_cast<const T*>(p.k) + at.t0 * ldk + (long)h * p.d_k;
     const T* qp = static_cast<const T*>(p.q) + at.t0 * ldk + (long)h * p.d_k;
-    Block64<T, DK> kb, qb;
-    const int mk = kb.load(kp, ldk, at.n, p.d_k, p.vec_k), mq = qb.load(qp, ldk, at.n, p.d_k, p.vec_k);
+    u32x4 kb[NR], qb[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int id = tid + 256 * i, t = id / (DK / R), c = id % (DK / R) * R;
+        const bool in = t < at.n && c < p.d_k;
+        kb[i] = load_run<T, VEC>(kp + t * ldk + c, kp, in, p.d_k - c);
+        qb[i] = load_run<T, VEC>(qp + t * ldk + c, qp, in, p.d_k - c);
+    }
     bool bad = false;
     if (wave == 0) bad = load_gates(p, at, h, gs, lane);
     int ek = 0, eq = 0;
     if constexpr (Op::kScaled) {
-        const int wk = wave_max_bits(mk), wq = wave_max_bits(mq);
+        int mk = 0, mq = 0;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            mk = max(mk, run_max_bits<T>(kb[i]));
+            mq = max(mq, run_max_bits<T>(qb[i]));
+        }
+        mk = wave_max_bits(mk);
+        mq = wave_max_bits(mq);
         if (lane == 0) {
-            misc[wave] = wk;
-            misc[4 + wave] = wq;
+            misc[wave] = mk;
+            misc[4 + wave] = mq;
         }
         if (tid == 0) misc[8] = 0;
-    }
-    __syncthreads();
-    if constexpr (Op::kScaled) {
+        __syncthreads();
         const int bk = max(max(misc[0], misc[1]), max(misc[2], misc[3]));
         const int bq = max(max(misc[4], misc[5]), max(misc[6], misc[7]));
-        ek = tile_exp(bk, 0);
-        eq = tile_exp(bq, 0);
+        ek = bits_exp(bk);
+        eq = bits_exp(bq);
         bad = bad || bk >= 0x7f800000 || bq >= 0x7f800000;
     }
-    const float sk = exp2i(-ek), sq = exp2i(-eq);
-    kb.template put_rows<Op>(Kr, sk);
-    kb.template put_cols<Op>(Kt, sk);
-    qb.template put_rows<Op>(Qr, sq);
+    {
+        const float sk = exp2i(-ek), sq = exp2i(-eq);
+        Elt* kf = reinterpret_cast<Elt*>(rec + p.rec.kf);
+        Elt* qf = reinterpret_cast<Elt*>(rec + p.rec.qf);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int id = tid + 256 * i, t = id / (DK / R), c = id % (DK / R) * R;
+            float x[R];
+            typedef Elt EltR __attribute__((ext_vector_type(R)));
+            unpack_run<T>(kb[i], x);
+            Kr.put(t, c, x, sk);
+            *reinterpret_cast<EltR*>(kf + t * DK + c) = *reinterpret_cast<const EltR*>(Kr.at(t, c));
+            unpack_run<T>(qb[i], x);
+            Qr.put(t, c, x, sq);
+            *reinterpret_cast<EltR*>(qf + t * DK + c) = *reinterpret_cast<const EltR*>(Qr.at(t, c));
+        }
+    }
+    __syncthreads();
     if (tid < 64) {
         vec[kVecGamma + tid] = gs.gamma[tid];
         vec[kVecWrite + tid] = gs.beta[tid] * gs.tail[tid];
@@ -407,48 +484,52 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
         exps[kVecEK] = ek;
         exps[kVecEQ] = eq;
     }
-    __syncthreads();
 
-    // L diag(beta) (fp32) and P (scaled as K and Q are): tile pairs over the waves
-    const float kk2 = exp2i(2 * ek);
-#pragma unroll 1
-    for (int id = wave; id < 16; id += 4) {
-        const int mt = id >> 2, nt = id & 3;  // rows, columns
-        if (nt <= mt) {
-            f32x4 c = {0, 0, 0, 0};
+    // column tile `wave` of L diag(beta) (fp32), row tile `wave` of P diag(beta)
+    // (scaled as K and Q are, in registers): five tiles of products each wave
+    Unit pu[NKT];
+    {
+        const float kk2 = exp2i(2 * ek);
+        const int s = 16 * wave + m;
+        const float bs = gs.beta[s];
+        Unit uk[NKK], uq[NKK];
 #pragma unroll
-            for (int ku = 0; ku < NKK; ++ku) c = Op::mma(Kr.unit(mt, ku, lane), Kr.unit(nt, ku, lane), c);
-            const int s = 16 * nt + m;
+        for (int ku = 0; ku < NKK; ++ku) {
+            uk[ku] = Kr.run(16 * wave, ku, lane);
+            uq[ku] = Qr.run(16 * wave, ku, lane);
+        }
+        f32x4 pt[4];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            f32x4 ck = {0, 0, 0, 0}, cq = {0, 0, 0, 0};
+#pragma unroll
+            for (int ku = 0; ku < NKK; ++ku) {
+                const Unit a = Kr.run(16 * mt, ku, lane);
+                if (mt >= wave) ck = Op::mma(a, uk[ku], ck);
+                if (mt <= wave) cq = Op::mma(a, uq[ku], cq);
+            }
+            pt[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * mt + 4 * g + i;
-                const float kk = c[i] * kk2;
-                if (Op::kScaled && r == s && !(kk <= 1.03125f)) bad = true;
-                Af[sq_at(r, s)] = s < r ? kk * decay(gs, r, s) * gs.beta[s] : 0.f;
+                if (mt >= wave) {  // row r of L, column s
+                    const float kk = ck[i] * kk2;
+                    if (Op::kScaled && r == s && !(kk <= 1.03125f)) bad = true;
+                    Af[sq_at(r, s)] = s < r ? kk * decay(gs, r, s) * bs : 0.f;
+                }
+                if (mt <= wave && r <= s) pt[mt][i] = cq[i] * decay(gs, s, r) * gs.beta[r];  // row s of P, column r
             }
         }
-        // P by rows s of q, contraction over rows j of k: tile (j = mt, s = nt)
-        f32x4 c = {0, 0, 0, 0};
-        if (mt <= nt) {
 #pragma unroll
-            for (int ku = 0; ku < NKK; ++ku) c = Op::mma(Kr.unit(mt, ku, lane), Qr.unit(nt, ku, lane), c);
-        }
-        const int s = 16 * nt + m;
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = 16 * mt + 4 * g + i;
-            x[i] = j <= s ? c[i] * decay(gs, s, j) : 0.f;
-        }
-        Pm.put4(s, 16 * mt + 4 * g, x[0], x[1], x[2], x[3]);
+        for (int u = 0; u < NKT; ++u) pu[u] = Op::pack(&pt[u * NBK], 1.f);
     }
     if constexpr (Op::kScaled)
         if (bad) misc[8] = 1;
     __syncthreads();
 
-    // T's diagonal blocks by forward substitution, column m of block `wave`
-    // in lane (., m); Q by columns meanwhile
-    f32x4 tc[4];  // block column `wave` of T as accumulator tiles
+    // T's diagonal blocks by forward substitution in fp32, column m of block
+    // `wave` in lane (., m); then T_iw = -T_ii sum_{w <= b < i} A_ib T_bw down
+    // block column w on fp32 MFMA
     {
         float t[16];
 #pragma unroll
@@ -466,154 +547,124 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
         f32x4 d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[i] = g == 0 ? t[i] : g == 1 ? t[4 + i] : g == 2 ? t[8 + i] : t[12 + i];
+        // row-major, so that a left operand is one read
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tc[b] = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < 4; ++i) Td[wave * 256 + (4 * g + i) * 16 + m] = d[i];
+        __syncthreads();
+        f32x4 tc[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            if (b == wave) tc[b] = d;
-        // T overwrites K's rows, whose last readers passed the barrier
+        for (int i = 0; i < 4; ++i) {
+            tc[i] = f32x4{0, 0, 0, 0};
+            if (i == wave) tc[i] = d;
+            if (i > wave) {
+                f32x4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            if (b <= wave)  // the blocks above the diagonal are zero
+                for (int b = 0; b < i; ++b)
+                    if (b >= wave)
+                        y = OpF32::mma(*reinterpret_cast<const f32x4*>(Af + sq_at(16 * i + m, 16 * b + 4 * g)), tc[b], y);
+                z = OpF32::mma(*reinterpret_cast<const f32x4*>(Td + i * 256 + m * 16 + 4 * g), y, z);
+                tc[i] = -z;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) Tf[sq_at(16 * b + 4 * g + i, 16 * wave + m)] = tc[b][i];
-    }
-    qb.template put_cols<Op>(Qt, sq);
-    __syncthreads();
-    // T_iw = -T_ii sum_{w <= b < i} A_ib T_bw down block column w, in fp32
-#pragma unroll
-    for (int i = 1; i < 4; ++i) {
-        if (i > wave) {
-            f32x4 y = {0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < i; ++b)
-                if (b >= wave)
-                    y = OpF32::mma(*reinterpret_cast<const f32x4*>(Af + sq_at(16 * i + m, 16 * b + 4 * g)), tc[b], y);
-            f32x4 z = {0, 0, 0, 0};
-            z = OpF32::mma(*reinterpret_cast<const f32x4*>(Tf + sq_at(16 * i + m, 16 * i + 4 * g)), y, z);
-            tc[i] = -z;
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<Elt*>(Th.at(16 * i + 4 * g + e, 16 * wave + m)) = (Elt)tc[i][e];
         }
     }
-#pragma unroll
-    for (int i = 1; i < 4; ++i)
-        if (i > wave)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) Tf[sq_at(16 * i + 4 * g + e, 16 * wave + m)] = tc[i][e];
     __syncthreads();
 
-    // right operands of token tile `wave`: T's rows times gamma, T's columns
-    // times beta (and tail)
     {
-        Unit ub[NKT];
-        const int r = 16 * wave + m;
+        // T diag(gamma) K and T^T diag(beta tail) K, rows of token tile `wave`
+        Unit ur[NKT], uc[NKT];
 #pragma unroll
         for (int ku = 0; ku < NKT; ++ku) {
-            f32x4 t[NBK];
+            ur[ku] = times_unit<Op>(Th.blocks(16 * wave + m, ku, g), gs.gamma, ku, g);
+            uc[ku] = times_unit<Op>(times_unit<Op>(Th.cols(wave, ku, lane), gs.beta, ku, g), gs.tail, ku, g);
+        }
+        Unit* ow = reinterpret_cast<Unit*>(rec + p.rec.wk);
+        Unit* od = reinterpret_cast<Unit*>(rec + p.rec.kd);
+#pragma unroll
+        for (int u = 0; u < NKK; ++u) {
+            f32x4 c[NBK], d[NBK];
 #pragma unroll
             for (int b = 0; b < NBK; ++b) {
-                const int s = 16 * (ku * NBK + b) + 4 * g;
-                t[b] = *reinterpret_cast<const f32x4*>(Tf + sq_at(r, s));
+                c[b] = d[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[b][e] *= gs.gamma[s + e];
-            }
-            ub[ku] = Op::pack(t, 1.f);
-        }
-        Unit* out = reinterpret_cast<Unit*>(rec + p.rec.wk);
-        auto times_k = [&] {
-#pragma unroll
-            for (int u = 0; u < NKK; ++u) {
-                f32x4 c[NBK];
-#pragma unroll
-                for (int b = 0; b < NBK; ++b) {
-                    c[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int ku = 0; ku < NKT; ++ku) c[b] = Op::mma(Kt.unit(u * NBK + b, ku, lane), ub[ku], c[b]);
-                }
-                out[(wave * NKK + u) * 64 + lane] = Op::pack(c, 1.f);
-            }
-        };
-        times_k();
-        Unit uo[NKT];
-#pragma unroll
-        for (int ku = 0; ku < NKT; ++ku) {
-            f32x4 t[NBK], o[NBK];
-#pragma unroll
-            for (int b = 0; b < NBK; ++b) {
-                const int j = 16 * (ku * NBK + b) + 4 * g;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[b][e] = Tf[sq_at(j + e, r)] * gs.beta[j + e];
-                    t[b][e] = o[b][e] * gs.tail[j + e];
+                for (int ku = 0; ku < NKT; ++ku) {
+                    const Unit a = Kr.cols(u * NBK + b, ku, lane);
+                    c[b] = Op::mma(a, ur[ku], c[b]);
+                    d[b] = Op::mma(a, uc[ku], d[b]);
                 }
             }
-            ub[ku] = Op::pack(t, 1.f);
-            uo[ku] = Op::pack(o, 1.f);
+            ow[(wave * NKK + u) * 64 + lane] = Op::pack(c, 1.f);
+            od[(wave * NKK + u) * 64 + lane] = Op::pack(d, 1.f);
         }
-        out = reinterpret_cast<Unit*>(rec + p.rec.kd);
-        times_k();
-        // T^T diag(beta) P^T, rows of tile `wave`
+        // T^T diag(beta) P^T as left operand units (row r; s): columns s of this wave's tile
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
+        for (int nt = 0; nt < 4; ++nt) {
             f32x4 c = {0, 0, 0, 0};
 #pragma unroll
-            for (int ku = 0; ku < NKT; ++ku) c = Op::mma(Pm.unit(mt, ku, lane), uo[ku], c);
-            Bo.put4(r, 16 * mt + 4 * g, c[0], c[1], c[2], c[3]);
-        }
-        Unit* okt = reinterpret_cast<Unit*>(rec + p.rec.kt);
-        Unit* oqt = reinterpret_cast<Unit*>(rec + p.rec.qt);
-        for (int mt = wave; mt < NT; mt += 4)
-#pragma unroll
-            for (int ku = 0; ku < NKT; ++ku) {
-                okt[(mt * NKT + ku) * 64 + lane] = Kt.unit(mt, ku, lane);
-                oqt[(mt * NKT + ku) * 64 + lane] = Qt.unit(mt, ku, lane);
+            for (int ku = 0; ku < NKT; ++ku) c = Op::mma(pu[ku], Th.cols(nt, ku, lane), c);
+            // lane (g, m): row r = 16 nt + m, columns s = 16 wave + 4 g ..
+            if constexpr (Op::kScaled) {
+                const f16x4 q = {(_Float16)c[0], (_Float16)c[1], (_Float16)c[2], (_Float16)c[3]};
+                *reinterpret_cast<f16x4*>(Bo + ((nt * NKT + wave / 2) * 64 + lane) * 16 + (wave & 1) * 8) = q;
+            } else {
+                *reinterpret_cast<f32x4*>(Bo + ((nt * NKT + wave) * 64 + lane) * 16) = c;
             }
+        }
     }
     Unit ta[4][NKT];  // T by rows, left operand
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int ku = 0; ku < NKT; ++ku) {
-            f32x4 t[NBK];
-#pragma unroll
-            for (int b = 0; b < NBK; ++b)
-                t[b] = *reinterpret_cast<const f32x4*>(Tf + sq_at(16 * mt + m, 16 * (ku * NBK + b) + 4 * g));
-            ta[mt][ku] = Op::pack(t, 1.f);
-        }
+        for (int ku = 0; ku < NKT; ++ku) ta[mt][ku] = Th.blocks(16 * mt + m, ku, g);
     __syncthreads();
 
     // T V and T^T diag(beta) P^T dO by 16-column tiles of d_v, one wave each
-    const LdsMat<Op, NKT> st{lds + L::kP + wave * (NKT * 1024)};
+    const RowMat<Op, 16> st{lds + L::kKr + wave * RowMat<Op, 16>::bytes(64)};
     const T* vp = static_cast<const T*>(p.v) + at.t0 * ldv + (long)h * p.d_v;
     const T* op = static_cast<const T*>(p.dout) + at.t0 * ldv + (long)h * p.d_v;
-    const int rb = lane >> 2, cb = lane & 3;
-    bool bad_v = false;
+    constexpr int NV = 64 * 16 / R / 64, RPR = 16 / R;  // runs of a tile per lane, and per row
+    auto load_tile = [&](u32x4 (&y)[2][NV], int tile) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int id = lane + 64 * i, t = id / RPR, c = 16 * tile + id % RPR * R;
+                const T* src = which ? op : vp;
+                y[which][i] = load_run<T, VEC>(src + t * ldv + c, src, t < at.n && c < p.d_v, p.d_v - c);
+            }
+    };
+    u32x4 y[2][NV];
+    if (wave < p.dvt) load_tile(y, wave);
     for (int tile = wave; tile < p.dvt; tile += 4) {
+        u32x4 now[2][NV];
+#pragma unroll
+        for (int i = 0; i < 2 * NV; ++i) now[i / NV][i % NV] = y[i / NV][i % NV];
+        if (tile + 4 < p.dvt) load_tile(y, tile + 4);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-            const T* src = which ? op : vp;
-            float4 y[4];
-            int mx = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = 4 * rb + j, c = 16 * tile + 4 * cb;
-                y[j] = t < at.n ? row4<T>(src + t * ldv + c, p.d_v - c, p.vec_v) : float4{0, 0, 0, 0};
-                mx = max(mx, max(max(bits_abs(y[j].x), bits_abs(y[j].y)), max(bits_abs(y[j].z), bits_abs(y[j].w))));
-            }
             float s = 1.f;
             if constexpr (Op::kScaled) {
-                const int bits = wave_max_bits(mx), e = tile_exp(bits, -2);
-                bad_v = bad_v || bits >= 0x7f800000;
+                int mx = 0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) mx = max(mx, run_max_bits<T>(now[which][i]));
+                const int bits = wave_max_bits(mx), e = bits_exp(bits) + 2;  // below 1/2
+                bad = bad || bits >= 0x7f800000;
                 s = exp2i(-e);
                 if (lane == 0) exps[(which ? kExpO : kExpV) + tile] = e;
             }
-            st.put4(4 * cb + 0, 4 * rb, y[0].x * s, y[1].x * s, y[2].x * s, y[3].x * s);
-            st.put4(4 * cb + 1, 4 * rb, y[0].y * s, y[1].y * s, y[2].y * s, y[3].y * s);
-            st.put4(4 * cb + 2, 4 * rb, y[0].z * s, y[1].z * s, y[2].z * s, y[3].z * s);
-            st.put4(4 * cb + 3, 4 * rb, y[0].w * s, y[1].w * s, y[2].w * s, y[3].w * s);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int id = lane + 64 * i;
+                float x[R];
+                unpack_run<T>(now[which][i], x);
+                st.put(id / RPR, id % RPR * R, x, s);
+            }
             __builtin_amdgcn_wave_barrier();
             Unit ub[NKT];
 #pragma unroll
-            for (int ku = 0; ku < NKT; ++ku) ub[ku] = st.unit(0, ku, lane);
+            for (int ku = 0; ku < NKT; ++ku) ub[ku] = st.cols(0, ku, lane);
             __builtin_amdgcn_wave_barrier();
             Unit* o = reinterpret_cast<Unit*>(rec + (which ? p.rec.ot : p.rec.wt)) + (long)tile * NKT * 64;
 #pragma unroll
@@ -625,7 +676,7 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
                     c[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int ku = 0; ku < NKT; ++ku)
-                        c[b] = Op::mma(which ? Bo.unit(mt, ku, lane) : ta[mt][ku], ub[ku], c[b]);
+                        c[b] = Op::mma(which ? lds_unit<Op>(Bo, mt * NKT + ku, lane) : ta[mt][ku], ub[ku], c[b]);
                 }
                 o[u * 64 + lane] = Op::pack(c, 1.f);
             }
@@ -637,41 +688,77 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
         }
     }
     if constexpr (Op::kScaled) {
-        if (bad_v) misc[8] = 1;
+        if (bad) misc[8] = 1;
         __syncthreads();
         if (tid == 0) exps[kVecBad] = misc[8];
     }
 }
 
-template <class Op, typename T, int DK>
-__global__ __launch_bounds__(256) void bwd_prep_kernel(BwdParams p) {
+template <class Op, typename T, int DK, bool VEC>
+__global__ __launch_bounds__(256, Op::kScaled ? 3 : 1) void bwd_prep_kernel(BwdParams p) {
     __shared__ __align__(16) char lds[PrepLds<Op, DK>::kBytes];
     const int ci = blockIdx.x / p.heads, h = blockIdx.x - ci * p.heads;
     ChunkAt at;
     if (!find_chunk(p, ci, at)) return;
-    prep_chunk<Op, T, DK>(p, at, h, p.ws + (size_t)blockIdx.x * p.rec.bytes, lds);
+    prep_chunk<Op, T, DK, VEC>(p, at, h, p.ws + (size_t)blockIdx.x * p.rec.bytes, lds);
 }
 
 // ----------------------------------------------------------------- scan
-// One wave carries 16 rows of S (or of dS) along a sequence's chunks in
-// accumulators: tile b holds d_k indices 16 b + 4 g .. + 3 of row m.  The
-// operands come straight from the record's units, each 1 KiB read by a wave at
-// once, and the state's own operands from its accumulators, so a wave needs no
-// LDS and waits for no other.  A unit of the next chunk is read as soon as the
-// present chunk's has been used.
+// Four waves to a workgroup, each carrying 16 rows of S (or of dS) along the
+// chunks of a (sequence, head) in accumulators: tile b holds d_k indices 16 b +
+// 4 g .. + 3 of row m.  The state's own operands come from its accumulators;
+// the others pass through LDS once for the four waves, read from HBM two
+// chunks ahead.  What the gradients need of a wave's rows is turned through a
+// corner of LDS of its own, so that d_v runs along the units it writes.
+template <class Op, int DK>
+struct ScanLds {
+    static constexpr int kE = int(sizeof(typename Op::Elt));
+    static constexpr int kUnits = 64 * DK * kE;                  // T diag(gamma) K or T^T diag(beta tail) K
+    static constexpr int kRows = RowMat<Op, DK>::bytes(64);      // K, Q
+    static constexpr int kBuf = kUnits + 2 * kRows;
+    static constexpr int kBufs = Op::kScaled ? 2 : 1;
+    static constexpr int kTurnCols = DK > 64 ? DK : 64;
+    static constexpr int kTurn = RowMat<Op, kTurnCols>::bytes(16);
+    static constexpr int kTurnAt = kBufs * kBuf;
+    static constexpr int kBytes = kTurnAt + 4 * kTurn;
+};
+
 template <class Op, int DK>
 struct State {
     static constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK;
     f32x4 s[NT];
-    int e = 0;  // the state is s * 2^e
+    int e;  // the state is s * 2^e, with |s| below 2^15.1: its fp16 operands are s itself
 
+    __device__ __forceinline__ int top() const {  // the exponent of the state's largest value
+        float mx = 0.f;
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+            mx = fmaxf(fmaxf(fmaxf(mx, fabsf(s[b][0])), fabsf(s[b][1])), fmaxf(fabsf(s[b][2]), fabsf(s[b][3])));
+        return bits_exp(bits_abs(wave_max(mx))) + e;
+    }
     __device__ __forceinline__ void load(const BwdParams& p, const float* base, int row, int g) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             const int c = 16 * b + 4 * g;
-            float4 x = {0, 0, 0, 0};
-            if (base && row < p.d_v) x = row4<float>(base + (long)row * p.d_k + c, p.d_k - c, p.vec_s);
-            s[b] = f32x4{x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][i] = 0.f;
+            if (base && row < p.d_v && c < p.d_k) {
+                const float* r = base + (long)row * p.d_k + c;
+                if (p.vec_s) {
+                    s[b] = *reinterpret_cast<const f32x4*>(r);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < p.d_k) s[b][i] = r[i];
+                }
+            }
+        }
+        e = 0;
+        if constexpr (Op::kScaled) {
+            e = top() - 7;
+            const float f = exp2i(-e);
+#pragma unroll
+            for (int b = 0; b < NT; ++b) s[b] *= f;
         }
     }
     __device__ __forceinline__ void store(const BwdParams& p, float* base, int row, int g) const {
@@ -680,257 +767,213 @@ struct State {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             const int c = 16 * b + 4 * g;
-            put_row4<float>(base + (long)row * p.d_k + c, p.d_k - c, p.vec_s, s[b][0] * f, s[b][1] * f, s[b][2] * f,
-                            s[b][3] * f);
+            if (c >= p.d_k) continue;
+            float* r = base + (long)row * p.d_k + c;
+            if (p.vec_s) {
+                *reinterpret_cast<f32x4*>(r) = s[b] * f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < p.d_k) r[i] = s[b][i] * f;
+            }
         }
     }
-    // operand units of the state divided by 2^f; returns f, and through `top`
-    // the exponent of its largest value
-    __device__ __forceinline__ int operands(typename Op::Unit (&u)[NU], int& top) const {
-        int f = 0;
-        top = 0;
-        float sc = 1.f;
-        if constexpr (Op::kScaled) {
-            float mx = 0.f;
+};
+
+// A wave's own reads of a chunk: T V, or T^T diag(beta) P^T dO and dO; the
+// tokens' factors; gamma_c and exponents.
+template <class Op, bool BACK>
+struct TileInputs {
+    static constexpr int NKT = 4 / Op::kBlocks;
+    typename Op::Unit t[NKT], o[BACK ? NKT : 1];
+    f32x4 f[4];
+    float gc;
+    int ek, eq, et;
+    __device__ __forceinline__ void load(const BwdParams& p, const char* rec, int tile, int lane) {
+        const typename Op::Unit* a =
+            reinterpret_cast<const typename Op::Unit*>(rec + (BACK ? p.rec.ot : p.rec.wt)) + tile * NKT * 64 + lane;
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
-                mx = fmaxf(fmaxf(fmaxf(mx, fabsf(s[b][0])), fabsf(s[b][1])), fmaxf(fabsf(s[b][2]), fabsf(s[b][3])));
-            top = tile_exp(bits_abs(wave_max(mx)), 0) + e;
-            f = top - 11;
-            sc = exp2i(e - f);
+        for (int u = 0; u < NKT; ++u) t[u] = a[u * 64];
+        if constexpr (BACK) {
+            const typename Op::Unit* b =
+                reinterpret_cast<const typename Op::Unit*>(rec + p.rec.dot) + tile * NKT * 64 + lane;
+#pragma unroll
+            for (int u = 0; u < NKT; ++u) o[u] = b[u * 64];
         }
+        const float* v = reinterpret_cast<const float*>(rec + p.rec.vec);
 #pragma unroll
-        for (int i = 0; i < NU; ++i) u[i] = Op::pack(&s[i * NBK], sc);
-        return f;
+        for (int b = 0; b < 4; ++b)
+            f[b] = *reinterpret_cast<const f32x4*>(v + (BACK ? kVecGamma : kVecWrite) + 16 * b + 4 * (lane >> 4));
+        gc = v[kVecGc];
+        ek = eq = et = 0;
+        if constexpr (Op::kScaled) {
+            const int* x = reinterpret_cast<const int*>(v);
+            ek = x[kVecEK];
+            eq = x[kVecEQ];
+            et = x[(BACK ? kExpO : kExpV) + tile];
+        }
     }
 };
 
 template <class Op>
-__device__ __forceinline__ int tokens_exp(const f32x4 (&w)[4], int to) {
+__device__ __forceinline__ int tokens_exp(const f32x4 (&w)[4]) {
     if constexpr (!Op::kScaled) return 0;
     float mx = 0.f;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
         mx = fmaxf(fmaxf(fmaxf(mx, fabsf(w[b][0])), fabsf(w[b][1])), fmaxf(fabsf(w[b][2]), fabsf(w[b][3])));
-    return tile_exp(bits_abs(wave_max(mx)), to);
+    return bits_exp(bits_abs(wave_max(mx)));
 }
 
-template <class Op, int NMT, int NKU>
-__device__ __forceinline__ void load_units(typename Op::Unit (&u)[NMT][NKU], const char* base, int lane) {
-    const typename Op::Unit* b = reinterpret_cast<const typename Op::Unit*>(base) + lane;
+// Rows of a wave's tile as units with d_v along the contraction: column tile
+// `b` of the turned matrix to `base` + b KiB, this tile's half of them (fp16:
+// a unit holds two tiles).
+template <class Op, int N, class Mat>
+__device__ __forceinline__ void store_turned(const Mat& turn, char* base, int tile, int lane) {
+    char* o = base + (Op::kScaled ? (tile >> 1) * N * 1024 + (tile & 1) * 8 : tile * N * 1024) + lane * 16;
 #pragma unroll
-    for (int i = 0; i < NMT; ++i)
-#pragma unroll
-        for (int k = 0; k < NKU; ++k) u[i][k] = b[(i * NKU + k) * 64];
+    for (int b = 0; b < N; ++b) *reinterpret_cast<typename Op::Quad*>(o + b * 1024) = turn.col4(b, 0, lane);
 }
 
-// a vector of 64 by tokens, as the accumulators' rows hold them
-__device__ __forceinline__ void load_tokens(f32x4 (&x)[4], const float* v, int g) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const f32x4*>(v + 16 * b + 4 * g);
-}
-
-// what a scan reads of a chunk once for the whole wave: gamma_c and the
-// exponents of K, Q and of the wave's tile
-struct ChunkScalars {
-    float gc;
-    int ek, eq, et;
-};
-template <class Op>
-__device__ __forceinline__ ChunkScalars chunk_scalars(const BwdParams& p, const char* rec, int at) {
-    const float* vec = reinterpret_cast<const float*>(rec + p.rec.vec);
-    const int* exps = reinterpret_cast<const int*>(vec);
-    if constexpr (Op::kScaled) return {vec[kVecGc], exps[kVecEK], exps[kVecEQ], exps[at]};
-    return {vec[kVecGc], 0, 0, 0};
-}
-
-// W and the next state: W = T V - (T diag(gamma) K) S0^T, S1 = gamma_c S0 + (beta tail W)^T K.
-template <class Op, int DK>
-__device__ __forceinline__ void scan_forward(const BwdParams& p, State<Op, DK>& S, char* rec, size_t stride, int nc,
-                                             int tile, int lane) {
+// One chunk of a wave's rows.  Forward: W = T V - (T diag(gamma) K) S0^T and
+// S1 = gamma_c S0 + (beta tail W)^T K.  Back: dX = T^T diag(beta) (P^T dO +
+// diag(tail) K dS1^T) and dS0 = gamma_c dS1 + (gamma dO)^T Q - (gamma dX)^T K.
+template <class Op, int DK, bool BACK>
+__device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S, const TileInputs<Op, BACK>& in, char* rec,
+                                           const char* buf, char* turn, int tile, int lane) {
     using Unit = typename Op::Unit;
+    using L = ScanLds<Op, DK>;
     constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK;
-    const int g = lane >> 4;
-    if (nc == 0) return;
-    Unit wk[4][NU], kt[NT][NKT], wt[1][NKT];
-    f32x4 wr[4];
-    load_units<Op>(wk, rec + p.rec.wk, lane);
-    load_units<Op>(wt, rec + p.rec.wt + (size_t)tile * NKT * 1024, lane);
-    load_tokens(wr, reinterpret_cast<const float*>(rec + p.rec.vec) + kVecWrite, g);
-    if constexpr (Op::kScaled) load_units<Op>(kt, rec + p.rec.kt, lane);
-    ChunkScalars sc = chunk_scalars<Op>(p, rec, kExpV + tile);
-    for (int c = 0; c < nc; ++c) {
-        char* next = rec + (c + 1 < nc ? stride : 0);  // the last chunk reads its own again
-        const float gc = sc.gc;
-        const int ek = sc.ek, ev = sc.et;
-        sc = chunk_scalars<Op>(p, next, kExpV + tile);
-        if constexpr (!Op::kScaled) load_units<Op>(kt, rec + p.rec.kt, lane);
-        Unit su[NU];
-        int top;
-        const int f = S.operands(su, top);
-        Unit* os = reinterpret_cast<Unit*>(rec + p.rec.s0) + (size_t)tile * NU * 64 + lane;
+    const int g = lane >> 4, m = lane & 15;
+    const RowMat<Op, DK> K{const_cast<char*>(buf) + L::kUnits}, Q{const_cast<char*>(buf) + L::kUnits + L::kRows};
+    const RowMat<Op, L::kTurnCols> tn{turn};
+    f32x4 x[4], w[4];
 #pragma unroll
-        for (int i = 0; i < NU; ++i) os[i * 64] = su[i];
-        f32x4 x[4], w[4];
+    for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < NU; ++i) {
+        const Unit su = Op::pack(&S.s[i * NBK], 1.f);
+        tn.put_unit(m, i, g, su);
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) x[b] = Op::mma(wk[b][i], su[i], x[b]);
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) Op::unpack(wt[0][u], &w[u * NBK]);
-        const float sv = exp2i(ev), sx = exp2i(f + ek);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[b][i] = w[b][i] * sv - x[b][i] * sx;
-        load_units<Op>(wk, next + p.rec.wk, lane);
-        load_units<Op>(wt, next + p.rec.wt + (size_t)tile * NKT * 1024, lane);
-        const int ew = tokens_exp<Op>(w, 3);
-        const float si = exp2i(-ew);
-        Unit* ow = reinterpret_cast<Unit*>(rec + p.rec.wt) + (size_t)tile * NKT * 64 + lane;
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) ow[u * 64] = Op::pack(&w[u * NBK], si);
-        if (Op::kScaled && lane == 0) {
-            int* oe = reinterpret_cast<int*>(rec + p.rec.vec);
-            oe[kExpW + tile] = ew;
-            oe[kExpS + tile] = f;
-        }
-        // the next state in units of 2^e: those of the larger of what stays
-        // (gamma_c S0) and what is written; the operand's largest value stays
-        // below 2^12
-        int e = 0;
-        if constexpr (Op::kScaled) e = max(ew + 3 + ek, top + tile_exp(bits_abs(gc), 0)) - 11;
-        const float sw = exp2i(ek - e), sg = gc * exp2i(S.e - e);
-        S.e = e;
-        Unit wu[NKT];
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[b][i] *= wr[b][i];
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) wu[u] = Op::pack(&w[u * NBK], sw);
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S.s[b][i] *= sg;
-#pragma unroll
-        for (int u = 0; u < NKT; ++u)
-#pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(kt[b][u], wu[u], S.s[b]);
-        if constexpr (Op::kScaled) load_units<Op>(kt, next + p.rec.kt, lane);
-        load_tokens(wr, reinterpret_cast<const float*>(next + p.rec.vec) + kVecWrite, g);
-        rec = next;
+        for (int b = 0; b < 4; ++b) x[b] = Op::mma(lds_unit<Op>(buf, b * NU + i, lane), su, x[b]);
     }
-}
-
-// dX and the previous state's gradient: dX = T^T diag(beta) (P^T dO + diag(tail)
-// K dS1^T), dS0 = gamma_c dS1 + (gamma dO)^T Q - (gamma dX)^T K.
-template <class Op, int DK>
-__device__ __forceinline__ void scan_backward(const BwdParams& p, State<Op, DK>& S, char* rec, size_t stride, int nc,
-                                              int tile, int lane) {
-    using Unit = typename Op::Unit;
-    constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK;
-    const int g = lane >> 4;
-    if (nc == 0) return;
-    rec += (size_t)(nc - 1) * stride;
-    Unit kd[4][NU], kt[NT][NKT], qt[NT][NKT], ot[1][NKT], dt[1][NKT];
-    f32x4 ga[4];
-    load_units<Op>(kd, rec + p.rec.kd, lane);
-    load_units<Op>(ot, rec + p.rec.ot + (size_t)tile * NKT * 1024, lane);
-    load_units<Op>(dt, rec + p.rec.dot + (size_t)tile * NKT * 1024, lane);
-    load_tokens(ga, reinterpret_cast<const float*>(rec + p.rec.vec) + kVecGamma, g);
+    __builtin_amdgcn_wave_barrier();
+    store_turned<Op, NT>(tn, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
+    __builtin_amdgcn_wave_barrier();
+    const int top = Op::kScaled ? S.top() : 0;
+#pragma unroll
+    for (int u = 0; u < NKT; ++u) Op::unpack(in.t[u], &w[u * NBK]);
+    const float st = exp2i(BACK ? in.et + in.ek + in.eq : in.et), sx = BACK ? exp2i(S.e + in.ek) : -exp2i(S.e + in.ek);
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[b][i] = w[b][i] * st + x[b][i] * sx;
+    // W is kept with its largest value in [8, 16), dX in [1/4, 1/2)
+    const int tw = tokens_exp<Op>(w), ew = Op::kScaled ? tw + (BACK ? 2 : -3) : 0;
+    const float si = exp2i(-ew);
+#pragma unroll
+    for (int u = 0; u < NKT; ++u) tn.put_unit(m, u, g, Op::pack(&w[u * NBK], si));
+    __builtin_amdgcn_wave_barrier();
+    store_turned<Op, 4>(tn, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
+    __builtin_amdgcn_wave_barrier();
+    if (Op::kScaled && lane == 0) {
+        int* oe = reinterpret_cast<int*>(rec + p.rec.vec);
+        oe[(BACK ? kExpX : kExpW) + tile] = ew;
+        oe[(BACK ? kExpD : kExpS) + tile] = S.e;
+    }
+    // the next state in units of 2^e, of the larger of what stays (gamma_c S,
+    // below 2^9 of them) and what is written (each token's value below 2^8, and
+    // 64 tokens' with rows of K or Q below 2: 2^15)
+    int e = 0;
     if constexpr (Op::kScaled) {
-        load_units<Op>(kt, rec + p.rec.kt, lane);
-        load_units<Op>(qt, rec + p.rec.qt, lane);
+        e = max(tw + in.ek, top + bits_exp(bits_abs(in.gc)));
+        if constexpr (BACK) e = max(e, in.et - 2 + in.eq) + 1;  // two sums of 64 tokens
+        e -= 7;
     }
-    ChunkScalars sc = chunk_scalars<Op>(p, rec, kExpO + tile);
-    for (int c = nc - 1; c >= 0; --c) {
-        char* next = rec - (c > 0 ? stride : 0);
-        const float gc = sc.gc;
-        const int ek = sc.ek, eq = sc.eq, eo = sc.et;
-        sc = chunk_scalars<Op>(p, next, kExpO + tile);
-        Unit su[NU];
-        int top;
-        const int f = S.operands(su, top);
-        Unit* os = reinterpret_cast<Unit*>(rec + p.rec.ds1) + (size_t)tile * NU * 64 + lane;
+    const float sw = BACK ? -exp2i(in.ek - e) : exp2i(in.ek - e), sg = in.gc * exp2i(S.e - e);
+    S.e = e;
 #pragma unroll
-        for (int i = 0; i < NU; ++i) os[i * 64] = su[i];
-        f32x4 x[4], w[4];
+    for (int b = 0; b < NT; ++b) S.s[b] *= sg;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+    for (int u = 0; u < NKT; ++u) {
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
+        for (int b = 0; b < NBK; ++b) w[u * NBK + b] *= in.f[u * NBK + b];
+        const Unit wu = Op::pack(&w[u * NBK], sw);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) x[b] = Op::mma(kd[b][i], su[i], x[b]);
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) Op::unpack(ot[0][u], &w[u * NBK]);
-        const float so = exp2i(eo + ek + eq), sx = exp2i(f + ek);
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[b][i] = w[b][i] * so + x[b][i] * sx;
-        load_units<Op>(kd, next + p.rec.kd, lane);
-        load_units<Op>(ot, next + p.rec.ot + (size_t)tile * NKT * 1024, lane);
-        const int ew = tokens_exp<Op>(w, -2);
-        const float si = exp2i(-ew);
-        Unit* ow = reinterpret_cast<Unit*>(rec + p.rec.ot) + (size_t)tile * NKT * 64 + lane;
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) ow[u * 64] = Op::pack(&w[u * NBK], si);
-        if (Op::kScaled && lane == 0) {
-            int* oe = reinterpret_cast<int*>(rec + p.rec.vec);
-            oe[kExpX + tile] = ew;
-            oe[kExpD + tile] = f;
-        }
-        int e = 0;
-        if constexpr (Op::kScaled)
-            e = max(max(ew - 2 + ek, eo - 2 + eq), top + tile_exp(bits_abs(gc), 0)) - 11;
-        const float sw = -exp2i(ek - e), sd = exp2i(eo + eq - e), sg = gc * exp2i(S.e - e);
-        S.e = e;
-        Unit wu[NKT], du[NKT];
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) {
+        for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
+        if constexpr (BACK) {
             f32x4 d[NBK];
-            Op::unpack(dt[0][u], d);
+            Op::unpack(in.o[u], d);
 #pragma unroll
-            for (int b = 0; b < NBK; ++b)
+            for (int b = 0; b < NBK; ++b) d[b] *= in.f[u * NBK + b];
+            const Unit du = Op::pack(d, exp2i(in.et + in.eq - e));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    d[b][i] *= ga[u * NBK + b][i];
-                    w[u * NBK + b][i] *= ga[u * NBK + b][i];
-                }
-            wu[u] = Op::pack(&w[u * NBK], sw);
-            du[u] = Op::pack(d, sd);
+            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
         }
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S.s[b][i] *= sg;
-        if constexpr (!Op::kScaled) load_units<Op>(qt, rec + p.rec.qt, lane);
-#pragma unroll
-        for (int u = 0; u < NKT; ++u)
-#pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(qt[b][u], du[u], S.s[b]);
-        if constexpr (!Op::kScaled) load_units<Op>(kt, rec + p.rec.kt, lane);
-#pragma unroll
-        for (int u = 0; u < NKT; ++u)
-#pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(kt[b][u], wu[u], S.s[b]);
-        if constexpr (Op::kScaled) {
-            load_units<Op>(kt, next + p.rec.kt, lane);
-            load_units<Op>(qt, next + p.rec.qt, lane);
-        }
-        load_units<Op>(dt, next + p.rec.dot + (size_t)tile * NKT * 1024, lane);
-        load_tokens(ga, reinterpret_cast<const float*>(next + p.rec.vec) + kVecGamma, g);
-        rec = next;
     }
 }
 
-// Waves over (direction, d_v tile) of a (sequence, head); four to a workgroup.
+// A chunk's shared operands on their way from HBM to LDS, by all 256 threads.
+template <class Op, int DK, bool BACK>
+struct ScanStage {
+    static constexpr int kE = int(sizeof(typename Op::Elt)), N = 64 * DK * kE / 16 / 256, RPR = DK * kE / 16;
+    u32x4 a[N], k[N], q[BACK ? N : 1];
+    __device__ __forceinline__ void load(const BwdParams& p, const char* rec) {
+        const u32x4* pa = reinterpret_cast<const u32x4*>(rec + (BACK ? p.rec.kd : p.rec.wk));
+        const u32x4* pk = reinterpret_cast<const u32x4*>(rec + p.rec.kf);
+        const u32x4* pq = reinterpret_cast<const u32x4*>(rec + p.rec.qf);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            a[i] = pa[threadIdx.x + 256 * i];
+            k[i] = pk[threadIdx.x + 256 * i];
+            if constexpr (BACK) q[i] = pq[threadIdx.x + 256 * i];
+        }
+    }
+    __device__ __forceinline__ void store(char* buf) const {
+        using L = ScanLds<Op, DK>;
+        const RowMat<Op, DK> K{buf + L::kUnits}, Q{buf + L::kUnits + L::kRows};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = threadIdx.x + 256 * i;
+            reinterpret_cast<u32x4*>(buf)[id] = a[i];
+            *reinterpret_cast<u32x4*>(K.at(id / RPR, 0) + id % RPR * 16) = k[i];
+            if constexpr (BACK) *reinterpret_cast<u32x4*>(Q.at(id / RPR, 0) + id % RPR * 16) = q[i];
+        }
+    }
+};
+
+template <class Op, int DK, bool BACK>
+__device__ __forceinline__ void scan_sequence(const BwdParams& p, State<Op, DK>& S, char* rec, size_t stride, int nc,
+                                              int tile, bool active, int lane, char* lds) {
+    using L = ScanLds<Op, DK>;
+    if (nc == 0) return;
+    char* turn = lds + L::kTurnAt + (threadIdx.x >> 6) * L::kTurn;
+    auto at = [&](int c) { return rec + (size_t)(BACK ? nc - 1 - c : c) * stride; };  // c < nc
+    ScanStage<Op, DK, BACK> st;
+    TileInputs<Op, BACK> in;
+    st.load(p, at(0));
+    if (active) in.load(p, at(0), tile, lane);
+    st.store(lds);
+    st.load(p, at(min(1, nc - 1)));
+    __syncthreads();
+    for (int c = 0; c < nc; ++c) {
+        char* here = at(c);
+        if (active) {
+            const TileInputs<Op, BACK> now = in;
+            in.load(p, at(min(c + 1, nc - 1)), tile, lane);
+            scan_chunk<Op, DK, BACK>(p, S, now, here, lds + (L::kBufs == 2 ? c & 1 : 0) * L::kBuf, turn, tile, lane);
+        }
+        if constexpr (L::kBufs == 1) __syncthreads();
+        st.store(lds + (L::kBufs == 2 ? (c + 1) & 1 : 0) * L::kBuf);
+        st.load(p, at(min(c + 2, nc - 1)));
+        __syncthreads();
+    }
+}
+
 template <class Op, int DK>
 __global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int splits) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ __align__(16) char lds[ScanLds<Op, DK>::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = blockIdx.x;
     const int part = id % splits;
     id /= splits;
@@ -938,7 +981,7 @@ __global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int split
     id >>= 1;
     const int seq = id / p.heads, h = id - seq * p.heads;
     const int tile = part * 4 + wave;
-    if (tile >= p.dvt) return;
+    const bool active = tile < p.dvt;
     int ci, nc;
     if (p.cu) {
         ci = p.chunk_base[seq];
@@ -954,223 +997,244 @@ __global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int split
     State<Op, DK> S;
     if (!back) {
         S.load(p, p.init ? p.init + st : nullptr, row, lane >> 4);
-        scan_forward<Op, DK>(p, S, rec, stride, nc, tile, lane);
+        scan_sequence<Op, DK, false>(p, S, rec, stride, nc, tile, active, lane, lds);
     } else {
         S.load(p, p.dfinal ? p.dfinal + st : nullptr, row, lane >> 4);
-        scan_backward<Op, DK>(p, S, rec, stride, nc, tile, lane);
-        if (p.dinit) S.store(p, p.dinit + st, row, lane >> 4);
+        scan_sequence<Op, DK, true>(p, S, rec, stride, nc, tile, active, lane, lds);
+        if (p.dinit && active) S.store(p, p.dinit + st, row, lane >> 4);
     }
 }
 
 // ----------------------------------------------------------------- grad
 // One (chunk, head) per workgroup of four waves; wave w owns token tile w of
-// every product.  Tiles of d_v (64 rows of S as fp16, 32 as fp32) pass through
-// LDS, where S0, dS1, W and dX are turned so that d_v runs along the
-// contraction; the products over d_v stay in accumulators (dO S0, dX S0, W dS1
-// by d_k, dO W^T and dX W^T both ways round).  Then K and Q take the tiles'
-// place and the 64 x 64 products follow, right operands from the accumulators.
+// every product.  Tiles of d_v, one unit wide, pass through two buffers of LDS;
+// the products over d_v stay in accumulators (dO S0, dX S0, W dS1 by d_k, and
+// dO W^T and dX W^T: the tiles up to the diagonal with W's rows as rows, those
+// from it on with W's rows as columns).  Then K and Q take the tiles' place and
+// the 64 x 64 products follow, right operands from the accumulators.  The
+// tiles' exponents differ; right operands are scaled to the largest.
 template <class Op, int DK>
 struct GradLds {
-    static constexpr int kE = int(sizeof(typename Op::Elt));
-    static constexpr int kTdv = 32 * Op::kBlocks;  // rows of S in a tile: two units along the contraction
-    static constexpr int kSt = DK * kTdv * kE, kTok = 64 * kTdv * kE;
-    static constexpr int kS0 = 0, kDs = kSt, kW = 2 * kSt, kX = kW + kTok, kO = kX + kTok, kTileEnd = kO + kTok;
-    static constexpr int kRow = 64 * DK * kE, kSq = 64 * 64 * 4;
-    static constexpr int kKr = 0, kQr = kRow;
-    static constexpr int kKt = 2 * kRow > kSq ? 2 * kRow : kSq;  // the pair sums lie where K's and Q's rows were
-    static constexpr int kQt = kKt + kRow, kKqEnd = kQt + kRow;
-    static constexpr int kGates = kTileEnd > kKqEnd ? kTileEnd : kKqEnd;
+    static constexpr int kTdv = 16 * Op::kBlocks;
+    static constexpr int kSt = DK / 16 * 1024, kTok = 4 * 1024;
+    static constexpr int kS0 = 0, kDs = kSt, kW = 2 * kSt, kX = kW + kTok, kO = kX + kTok, kBuf = kO + kTok;
+    static constexpr int kRow = RowMat<Op, DK>::bytes(64), kSq = 64 * 64 * 4;
+    static constexpr int kKr = 0, kQr = kRow, kM = 2 * kRow, kKqEnd = kM + kSq;
+    static constexpr int kGates = 2 * kBuf > kKqEnd ? 2 * kBuf : kKqEnd;
     static constexpr int kVecs = kGates + int(sizeof(Gates));  // a [64], kw [64], partial sums [3][256], reductions [16]
     static constexpr int kBytes = kVecs + (128 + 768 + 16) * 4;
 };
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float unit_dot(const f16x8& a, const f16x8& b) {
-    float s = 0.f;
+// the dot products of a unit's blocks
+__device__ __forceinline__ void unit_dots(const f16x8& a, const f16x8& b, float (&s)[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        s = __builtin_amdgcn_fdot2(f16x2{a[2 * i], a[2 * i + 1]}, f16x2{b[2 * i], b[2 * i + 1]}, s, false);
-    return s;
-}
-__device__ __forceinline__ float unit_dot(const f32x4& a, const f32x4& b) {
-    return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
-}
-
-// Four units of rows 4 mq .. 4 mq + 3 of a (row; column) tile written to LDS as (column; row).
-template <class Op, int NKU>
-__device__ __forceinline__ void put_turned(const LdsMat<Op, NKU>& a, const typename Op::Unit (&u)[4], int col, int row,
-                                           float s) {
-    if constexpr (Op::kScaled) {
-        f16x8 x[4];
-        const _Float16 f = (_Float16)s;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = u[j] * f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const f16x4 y = {x[0][e], x[1][e], x[2][e], x[3][e]};
-            a.put4(col + (e >> 2) * 16 + (e & 3), row, __builtin_bit_cast(uint2, y));
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a.put4(col + e, row, u[0][e], u[1][e], u[2][e], u[3][e]);
+    for (int h = 0; h < 2; ++h) {
+        s[h] = __builtin_amdgcn_fdot2(f16x2{a[4 * h], a[4 * h + 1]}, f16x2{b[4 * h], b[4 * h + 1]}, 0.f, false);
+        s[h] = __builtin_amdgcn_fdot2(f16x2{a[4 * h + 2], a[4 * h + 3]}, f16x2{b[4 * h + 2], b[4 * h + 3]}, s[h], false);
     }
 }
+__device__ __forceinline__ void unit_dots(const f32x4& a, const f32x4& b, float (&s)[1]) {
+    s[0] = a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
+}
+// a unit with its two blocks times 2^d0 and 2^d1, d <= 0
+__device__ __forceinline__ f16x8 shift_unit(f16x8 u, int d0, int d1) {
+    const _Float16 f = (_Float16)exp2i(d0), h = (_Float16)exp2i(d1);
+    const f16x8 s = {f, f, f, f, h, h, h, h};
+    return u * s;
+}
+__device__ __forceinline__ f32x4 shift_unit(const f32x4& u, int, int) { return u; }
 
-template <class Op, typename T, int DK>
-__device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at, int h, const char* rec,
-                                           const char* s0, const char* ds1, char* lds) {
+template <class Op, typename T, int DK, bool VEC>
+__device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at, int h, const char* rec, char* lds) {
     using Unit = typename Op::Unit;
+    using Elt = typename Op::Elt;
     using L = GradLds<Op, DK>;
-    constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK, NKD = 2, NDT = L::kTdv / 16;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, m = lane & 15;
-    const LdsMat<Op, NKD> S0{lds + L::kS0}, Ds{lds + L::kDs}, W{lds + L::kW}, X{lds + L::kX}, O{lds + L::kO};
-    const LdsMat<Op, NU> Kr{lds + L::kKr}, Qr{lds + L::kQr};
-    const LdsMat<Op, NKT> Kt{lds + L::kKt}, Qt{lds + L::kQt};
+    constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK, R = kRun<T>;
+    constexpr int NS = (NT * 64 + 255) / 256;      // 16-byte pieces of S0's tile per thread
+    constexpr int NO = 64 * L::kTdv / R / 256;     // runs of dO's tile per thread
+    constexpr int NK = 64 * DK * int(sizeof(Elt)) / 16 / 256, RPR = DK * int(sizeof(Elt)) / 16;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+              m = lane & 15;
+    const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
+    float* M = reinterpret_cast<float*>(lds + L::kM);
     Gates& gs = *reinterpret_cast<Gates*>(lds + L::kGates);
     float* va = reinterpret_cast<float*>(lds + L::kVecs);  // a
     float* vk = va + 64;                                   // tail k.(W dS1)
     float* part = va + 128;                                // [3][256]
     float* red = part + 768;                               // [16]
     const int* exps = reinterpret_cast<const int*>(rec + p.rec.vec);
-
     const long ldk = (long)p.heads * p.d_k, ldv = (long)p.heads * p.d_v;
     const long ok = at.t0 * ldk + (long)h * p.d_k, ov = at.t0 * ldv + (long)h * p.d_v;
+    const T* op = static_cast<const T*>(p.dout) + ov;
+    T* dvp = static_cast<T*>(p.dv) + ov;
+    const int tiles = (p.dvt + NBK - 1) / NBK;
+
+    // the tiles of d_v on their way to LDS
+    constexpr int NOR = NO > 0 ? NO : 1;
+    u32x4 rs[NS], rd[NS], rw, rx, ro[NOR];
+    auto load_tile = [&](int t) {
+        const u32x4* s0 = reinterpret_cast<const u32x4*>(rec + p.rec.s0) + (long)t * NT * 64;
+        const u32x4* d1 = reinterpret_cast<const u32x4*>(rec + p.rec.ds1) + (long)t * NT * 64;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int id = min(tid + 256 * i, NT * 64 - 1);
+            rs[i] = s0[id];
+            rd[i] = d1[id];
+        }
+        rw = reinterpret_cast<const u32x4*>(rec + p.rec.w)[(long)t * 256 + tid];
+        rx = reinterpret_cast<const u32x4*>(rec + p.rec.x)[(long)t * 256 + tid];
+#pragma unroll
+        for (int i = 0; i < NOR; ++i) {
+            const int id = tid + 256 * i, tk = id / (L::kTdv / R), c = t * L::kTdv + id % (L::kTdv / R) * R;
+            ro[i] = load_run<T, VEC>(op + tk * ldv + c, op, tk < at.n && c < p.d_v, p.d_v - c);
+        }
+    };
+    load_tile(0);
     if (wave == 0) load_gates(p, at, h, gs, lane);
 
-    // one exponent for each matrix: its tiles' largest
-    int eo = 0, ew = 0, ex = 0, es = 0, ed = 0, ek = 0, eq = 0;
+    // exponents: lane t holds those of d_v tile t; e.. the largest of a product's
+    int xs = 0, xd = 0, xw = 0, xx = 0, eo = 0, es = 0, ed = 0, exs = 0, ew = 0, exw = 0, ek = 0, eq = 0;
     if constexpr (Op::kScaled) {
-        auto top = [&](int a) {
-            int x = lane < p.dvt ? exps[a + lane] : -1000;
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) x = max(x, __shfl_xor(x, off, kWave));
-            return __builtin_amdgcn_readfirstlane(x);
-        };
-        eo = top(kExpO), ew = top(kExpW), ex = top(kExpX), es = top(kExpS), ed = top(kExpD);
+        const bool in = lane < p.dvt;
+        xs = in ? exps[kExpS + lane] : -1000, xd = in ? exps[kExpD + lane] : -1000;
+        xw = in ? exps[kExpW + lane] : -1000, xx = in ? exps[kExpX + lane] : -1000;
+        auto top = [](int x) { return wave_max_bits(x + 8192) - 8192; };
+        eo = top(in ? exps[kExpO + lane] : -1000);
+        es = top(xs), ed = top(xw + xd), exs = top(xx + xs), ew = top(xw), exw = top(xx + xw);
         ek = exps[kVecEK], eq = exps[kVecEQ];
     }
+    const float so = exp2i(-eo);
 
-    f32x4 zq[NT], zk[NT], zw[NT], e1a[4], e2a[4], e1b[4], e2b[4];
+    f32x4 zq[NT], zk[NT], zw[NT], e1[5], e2[5];  // [4]: the diagonal tile with W's rows as columns
 #pragma unroll
     for (int b = 0; b < NT; ++b) zq[b] = zk[b] = zw[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int b = 0; b < 4; ++b) e1a[b] = e2a[b] = e1b[b] = e2b[b] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < 5; ++b) e1[b] = e2[b] = f32x4{0, 0, 0, 0};
     float ip = 0.f;  // <dS1, S0>
 
-    const T* op = static_cast<const T*>(p.dout) + ov;
-    T* dvp = static_cast<T*>(p.dv) + ov;
-    const float so = exp2i(-eo), sx = exp2i(ex);
-    for (int d0 = 0; d0 < p.dvt; d0 += NDT) {
-        const int nd = min(NDT, p.dvt - d0);
-        // S0 and dS1: quads of units, NDT tiles x NU units x 16 quads
+    for (int t = 0; t < tiles; ++t) {
+        char* buf = lds + (t & 1) * L::kBuf;
+        int s0e = 0, s1e = 0, d0e = 0, d1e = 0, w0e = 0, w1e = 0, x0e = 0, x1e = 0;
+        if constexpr (Op::kScaled) {
+            s0e = __builtin_amdgcn_readlane(xs, 2 * t), s1e = __builtin_amdgcn_readlane(xs, 2 * t + 1);
+            d0e = __builtin_amdgcn_readlane(xd, 2 * t), d1e = __builtin_amdgcn_readlane(xd, 2 * t + 1);
+            w0e = __builtin_amdgcn_readlane(xw, 2 * t), w1e = __builtin_amdgcn_readlane(xw, 2 * t + 1);
+            x0e = __builtin_amdgcn_readlane(xx, 2 * t), x1e = __builtin_amdgcn_readlane(xx, 2 * t + 1);
+        }
 #pragma unroll
-        for (int i = 0; i < (NDT * NU * 16 + 255) / 256; ++i) {
+        for (int i = 0; i < NS; ++i) {
             const int id = tid + 256 * i;
-            if (id >= NDT * NU * 16) break;
-            const int mt = id / (NU * 16), ku = (id >> 4) % NU, gg = (id >> 2) & 3, mq = id & 3;
-            Unit a[4], b[4];
-            float fa = 0.f, fb = 0.f;
-            if (mt < nd) {
-                const long at4 = ((long)(d0 + mt) * NU + ku) * 64 + gg * 16 + 4 * mq;
+            if (NT * 64 % 256 == 0 || id < NT * 64) {
+                reinterpret_cast<u32x4*>(buf + L::kS0)[id] = rs[i];
+                reinterpret_cast<u32x4*>(buf + L::kDs)[id] = rd[i];
+                float d[NBK];
+                unit_dots(__builtin_bit_cast(Unit, rs[i]), __builtin_bit_cast(Unit, rd[i]), d);
+                ip += d[0] * exp2i(s0e) * exp2i(d0e);
+                if constexpr (NBK == 2) ip += d[NBK - 1] * exp2i(s1e) * exp2i(d1e);
+            }
+        }
+        reinterpret_cast<u32x4*>(buf + L::kW)[tid] = rw;
+        reinterpret_cast<u32x4*>(buf + L::kX)[tid] = rx;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    a[j] = reinterpret_cast<const Unit*>(s0)[at4 + j];
-                    b[j] = reinterpret_cast<const Unit*>(ds1)[at4 + j];
+        for (int i = 0; i < NOR; ++i) {
+            const int id = tid + 256 * i, tk = id / (L::kTdv / R), c = id % (L::kTdv / R) * R;
+            if (NO == 0 && tk >= 64) break;  // half as many runs as threads
+            float x[R];
+            unpack_run<T>(ro[i], x);
+            // unit (token tile; d_v): block c / 16, lanes g = c / 4 % 4 and, of eight columns, the next
+            char* o = buf + L::kO + (tk >> 4) * 1024 + ((c >> 2 & 3) * 16 + (tk & 15)) * 16;
+            if constexpr (Op::kScaled) {
+                o += (c >> 4) * 8;
+#pragma unroll
+                for (int j = 0; j < R; j += 4) {
+                    const f16x4 y = {(_Float16)(x[j] * so), (_Float16)(x[j + 1] * so), (_Float16)(x[j + 2] * so),
+                                     (_Float16)(x[j + 3] * so)};
+                    *reinterpret_cast<f16x4*>(o + j / 4 * 256) = y;
                 }
-                int xa = 0, xb = 0;
-                if constexpr (Op::kScaled) xa = exps[kExpS + d0 + mt], xb = exps[kExpD + d0 + mt];
-                float dot = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dot += unit_dot(a[j], b[j]);
-                ip += dot * exp2i(xa) * exp2i(xb);
-                fa = exp2i(xa - es), fb = exp2i(xb - ed);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = b[j] = Unit{};
+                for (int j = 0; j < R; j += 4)
+                    *reinterpret_cast<f32x4*>(o + j / 4 * 256) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
             }
-            const int col = 16 * ku * NBK + 4 * gg, row = 16 * mt + 4 * mq;
-            put_turned<Op, NKD>(S0, a, col, row, fa);
-            put_turned<Op, NKD>(Ds, b, col, row, fb);
-        }
-        // W and dX: NDT tiles x NKT units x 16 quads each
-#pragma unroll
-        for (int i = 0; i < (2 * NDT * NKT * 16 + 255) / 256; ++i) {
-            const int id = tid + 256 * i;
-            if (id >= 2 * NDT * NKT * 16) break;
-            const bool isx = id >= NDT * NKT * 16;
-            const int q = isx ? id - NDT * NKT * 16 : id;
-            const int mt = q / (NKT * 16), ku = (q >> 4) % NKT, gg = (q >> 2) & 3, mq = q & 3;
-            Unit a[4];
-            float f = 0.f;
-            if (mt < nd) {
-                const long at4 = ((long)(d0 + mt) * NKT + ku) * 64 + gg * 16 + 4 * mq;
-                const Unit* src = reinterpret_cast<const Unit*>(rec + (isx ? p.rec.ot : p.rec.wt));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = src[at4 + j];
-                f = 1.f;
-                if constexpr (Op::kScaled) f = exp2i(exps[(isx ? kExpX : kExpW) + d0 + mt] - (isx ? ex : ew));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = Unit{};
-            }
-            put_turned<Op, NKD>(isx ? X : W, a, 16 * ku * NBK + 4 * gg, 16 * mt + 4 * mq, f);
-        }
-        // dO by rows
-#pragma unroll
-        for (int i = 0; i < 64 * (L::kTdv / 4) / 256; ++i) {
-            const int id = tid + 256 * i, cb = id % (L::kTdv / 4), t = id / (L::kTdv / 4);
-            const int c = 16 * d0 + 4 * cb;
-            const float4 y = t < at.n ? row4<T>(op + t * ldv + c, p.d_v - c, p.vec_v) : float4{0, 0, 0, 0};
-            O.put4(t, 4 * cb, y.x * so, y.y * so, y.z * so, y.w * so);
         }
         __syncthreads();
+        if (t + 1 < tiles) load_tile(t + 1);
         // dV = dX
+        {
+            constexpr int NP = 64 * L::kTdv / 8;  // pieces of eight columns
+            static_assert(NP <= 256, "");
+            if (NP == 256 || tid < NP) {
+                const int tk = tid / (L::kTdv / 8), c = tid % (L::kTdv / 8) * 8;
+                const char* o = buf + L::kX + (tk >> 4) * 1024 + ((c >> 2 & 3) * 16 + (tk & 15)) * 16;
+                float x[8];
+                if constexpr (Op::kScaled) {
+                    const float f = exp2i(c < 16 ? x0e : x1e);
 #pragma unroll
-        for (int i = 0; i < 64 * (L::kTdv / 4) / 256; ++i) {
-            const int id = tid + 256 * i, cb = id % (L::kTdv / 4), t = id / (L::kTdv / 4);
-            const int c = 16 * d0 + 4 * cb;
-            const f32x4 y = X.get4(t, 4 * cb);
-            if (t < at.n)
-                put_row4<T>(dvp + t * ldv + c, p.d_v - c, p.vec_v, y[0] * sx, y[1] * sx, y[2] * sx, y[3] * sx);
+                    for (int j = 0; j < 8; ++j)
+                        x[j] = (float)reinterpret_cast<const f16x4*>(o + (c >> 4) * 8 + j / 4 * 256)[0][j & 3] * f;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = reinterpret_cast<const f32x4*>(o + j / 4 * 256)[0][j & 3];
+                }
+                const int col = t * L::kTdv + c;
+                if (tk < at.n) {
+                    if constexpr (VEC && sizeof(T) == 4) {  // rows are whole runs of four
+                        const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
+                        store_run<T, true, 4>(dvp + tk * ldv + col, p.d_v - col, a);
+                        store_run<T, true, 4>(dvp + tk * ldv + col + 4, p.d_v - col - 4, b);
+                    } else {
+                        store_run<T, VEC, 8>(dvp + tk * ldv + col, p.d_v - col, x);
+                    }
+                }
+            }
         }
-#pragma unroll
-        for (int ku = 0; ku < NKD; ++ku) {
-            const Unit bo = O.unit(wave, ku, lane), bx = X.unit(wave, ku, lane), bw = W.unit(wave, ku, lane);
+        const Unit bo = lds_unit<Op>(buf + L::kO, wave, lane), bx = lds_unit<Op>(buf + L::kX, wave, lane),
+                   bw = lds_unit<Op>(buf + L::kW, wave, lane);
+        {
+            const Unit b1 = shift_unit(bo, s0e - es, s1e - es);
+            const Unit b2 = shift_unit(bx, x0e + s0e - exs, x1e + s1e - exs);
+            const Unit b3 = shift_unit(bw, w0e + d0e - ed, w1e + d1e - ed);
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                const Unit a = S0.unit(b, ku, lane);
-                zq[b] = Op::mma(a, bo, zq[b]);
-                zk[b] = Op::mma(a, bx, zk[b]);
-                zw[b] = Op::mma(Ds.unit(b, ku, lane), bw, zw[b]);
+                const Unit a = lds_unit<Op>(buf + L::kS0, b, lane);
+                zq[b] = Op::mma(a, b1, zq[b]);
+                zk[b] = Op::mma(a, b2, zk[b]);
+                zw[b] = Op::mma(lds_unit<Op>(buf + L::kDs, b, lane), b3, zw[b]);
             }
+        }
+        {
+            const Unit b1 = shift_unit(bo, w0e - ew, w1e - ew), b2 = shift_unit(bx, x0e + w0e - exw, x1e + w1e - exw);
+            const Unit c1 = shift_unit(bw, w0e - ew, w1e - ew), c2 = shift_unit(bw, x0e + w0e - exw, x1e + w1e - exw);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 if (b <= wave) {
-                    const Unit a = W.unit(b, ku, lane);
-                    e1a[b] = Op::mma(a, bo, e1a[b]);
-                    e2a[b] = Op::mma(a, bx, e2a[b]);
-                }
-                if (b >= wave) {
-                    e1b[b] = Op::mma(O.unit(b, ku, lane), bw, e1b[b]);
-                    e2b[b] = Op::mma(X.unit(b, ku, lane), bw, e2b[b]);
+                    const Unit a = lds_unit<Op>(buf + L::kW, b, lane);
+                    e1[b] = Op::mma(a, b1, e1[b]);
+                    e2[b] = Op::mma(a, b2, e2[b]);
+                } else {
+                    e1[b] = Op::mma(lds_unit<Op>(buf + L::kO, b, lane), c1, e1[b]);
+                    e2[b] = Op::mma(lds_unit<Op>(buf + L::kX, b, lane), c2, e2[b]);
                 }
             }
+            e1[4] = Op::mma(bo, c1, e1[4]);
+            e2[4] = Op::mma(bx, c2, e2[4]);
+        }
+    }
+    // K and Q by rows, where the tiles were
+    {
+        u32x4 k[NK], q[NK];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            k[i] = reinterpret_cast<const u32x4*>(rec + p.rec.kf)[tid + 256 * i];
+            q[i] = reinterpret_cast<const u32x4*>(rec + p.rec.qf)[tid + 256 * i];
         }
         __syncthreads();
-    }
-
-    // K and Q in both orders
-    {
-        Block64<T, DK> x;
-        const float sk = exp2i(-ek), sq = exp2i(-eq);
-        x.load(static_cast<const T*>(p.k) + ok, ldk, at.n, p.d_k, p.vec_k);
-        x.template put_rows<Op>(Kr, sk);
-        x.template put_cols<Op>(Kt, sk);
-        x.load(static_cast<const T*>(p.q) + ok, ldk, at.n, p.d_k, p.vec_k);
-        x.template put_rows<Op>(Qr, sq);
-        x.template put_cols<Op>(Qt, sq);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int id = tid + 256 * i;
+            *reinterpret_cast<u32x4*>(Kr.at(id / RPR, 0) + id % RPR * 16) = k[i];
+            *reinterpret_cast<u32x4*>(Qr.at(id / RPR, 0) + id % RPR * 16) = q[i];
+        }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) ip += __shfl_xor(ip, off, kWave);
@@ -1179,76 +1243,70 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
 
     const int tok = 16 * wave + m;  // this lane's token as a column of the products
     const float gam = gs.gamma[tok], tail = gs.tail[tok], bet = gs.beta[tok];
-    // q.(dO S0), k.(dX S0), k.(W dS1) of the lane's token; q.k and k.k with the tokens up to it
+    const float s1 = exp2i(eo + ew), s2 = exp2i(exw);
+    // q.(dO S0), k.(dX S0), k.(W dS1) of the lane's token
     float qz = 0.f, kz = 0.f, kwz = 0.f;
-    f32x4 mh[4];  // rows r of tile b, column s = tok: dO_s.W_r q_s.k_r - dX_s.W_r k_s.k_r
-    const float s1 = exp2i(eo + ew), s2 = exp2i(ex + ew);
-    {
-        Unit uk[NU], uq[NU];
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            uk[i] = Kr.unit(wave, i, lane);
-            uq[i] = Qr.unit(wave, i, lane);
-            f32x4 k[NBK], q[NBK];
-            Op::unpack(uk[i], k);
-            Op::unpack(uq[i], q);
+    for (int i = 0; i < NU; ++i) {
+        f32x4 k[NBK], q[NBK];
+        Op::unpack(Kr.blocks(tok, i, g), k);
+        Op::unpack(Qr.blocks(tok, i, g), q);
 #pragma unroll
-            for (int b = 0; b < NBK; ++b)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    qz += q[b][j] * zq[i * NBK + b][j];
-                    kz += k[b][j] * zk[i * NBK + b][j];
-                    kwz += k[b][j] * zw[i * NBK + b][j];
-                }
-        }
-        qz += __shfl_xor(qz, 16, kWave);
-        kz += __shfl_xor(kz, 16, kWave);
-        kwz += __shfl_xor(kwz, 16, kWave);
-        qz += __shfl_xor(qz, 32, kWave);
-        kz += __shfl_xor(kz, 32, kWave);
-        kwz += __shfl_xor(kwz, 32, kWave);
-        const float sqk = exp2i(eq + ek) * s1, skk = exp2i(2 * ek) * s2;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
-            if (b <= wave) {
-#pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    const Unit a = Kr.unit(b, i, lane);
-                    qk = Op::mma(a, uq[i], qk);
-                    kk = Op::mma(a, uk[i], kk);
-                }
-            }
+        for (int b = 0; b < NBK; ++b)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int r = 16 * b + 4 * g + j;
-                const float x1 = e1a[b][j] * qk[j] * sqk, x2 = e2a[b][j] * kk[j] * skk;
-                mh[b][j] = r < tok ? x1 - x2 : r == tok ? x1 : 0.f;
+                qz += q[b][j] * zq[i * NBK + b][j];
+                kz += k[b][j] * zk[i * NBK + b][j];
+                kwz += k[b][j] * zw[i * NBK + b][j];
             }
-        }
     }
-    const float ah = qz * exp2i(eo + es + eq) - kz * exp2i(ex + es + ek);  // a without gamma
-    const float kwh = kwz * exp2i(ew + ed + ek);                          // k.(W dS1)
+    qz += __shfl_xor(qz, 16, kWave);
+    kz += __shfl_xor(kz, 16, kWave);
+    kwz += __shfl_xor(kwz, 16, kWave);
+    qz += __shfl_xor(qz, 32, kWave);
+    kz += __shfl_xor(kz, 32, kWave);
+    kwz += __shfl_xor(kwz, 32, kWave);
+    const float ah = qz * exp2i(eo + es + eq) - kz * exp2i(exs + ek);  // a without gamma
+    const float kwh = kwz * exp2i(ed + ek);                            // k.(W dS1)
     if (g == 0) {
         va[tok] = gam * ah;
         vk[tok] = tail * kwh;
     }
-    __syncthreads();  // K's and Q's rows are done with
-
-    float* M = reinterpret_cast<float*>(lds + L::kKr);
+    // rows r of tile b, column s = tok: dO_s.W_r q_s.k_r - dX_s.W_r k_s.k_r, and
+    // with its decay to M
+    f32x4 mh[4];
     Unit n1[NKT], n2[NKT];
     {
+        const float sqk = exp2i(eq + ek) * s1, skk = exp2i(2 * ek) * s2;
+        Unit uk[NU], uq[NU];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            uk[i] = Kr.run(16 * wave, i, lane);
+            uq[i] = Qr.run(16 * wave, i, lane);
+        }
         f32x4 x1[4], x2[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            f32x4 y;
+            mh[b] = x1[b] = x2[b] = f32x4{0, 0, 0, 0};
+            f32x4 y = {0, 0, 0, 0};
+            if (b <= wave) {
+                f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 16 * b + 4 * g + j;
-                const float d = r <= tok ? decay(gs, tok, r) : 0.f;
-                x1[b][j] = e1a[b][j] * d * gs.beta[r];
-                x2[b][j] = r < tok ? e2a[b][j] * d * gs.beta[r] : 0.f;
-                y[j] = mh[b][j] * d;
+                for (int i = 0; i < NU; ++i) {
+                    const Unit a = Kr.run(16 * b, i, lane);
+                    qk = Op::mma(a, uq[i], qk);
+                    kk = Op::mma(a, uk[i], kk);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 16 * b + 4 * g + j;
+                    const float d = r <= tok ? decay(gs, tok, r) : 0.f, br = d * gs.beta[r];
+                    const float f1 = e1[b][j] * qk[j] * sqk, f2 = e2[b][j] * kk[j] * skk;
+                    mh[b][j] = r < tok ? f1 - f2 : r == tok ? f1 : 0.f;
+                    y[j] = mh[b][j] * d;
+                    x1[b][j] = e1[b][j] * br;
+                    x2[b][j] = r < tok ? e2[b][j] * br : 0.f;
+                }
             }
             *reinterpret_cast<f32x4*>(M + sq_at(tok, 16 * b + 4 * g)) = y;
         }
@@ -1269,49 +1327,55 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
             f32x4 c = {0, 0, 0, 0};
             ak[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int u = 0; u < NKT; ++u) {
-                const Unit a = Kt.unit(b, u, lane);
-                c = Op::mma(a, n1[u], c);
-                ak[b] = Op::mma(a, n2[u], ak[b]);
-            }
+            for (int u = 0; u < NKT; ++u)
+                if (u * NBK <= wave) {
+                    const Unit a = Kr.cols(b, u, lane);
+                    c = Op::mma(a, n1[u], c);
+                    ak[b] = Op::mma(a, n2[u], ak[b]);
+                }
             const int col = 16 * b + 4 * g;
-            if (tok < at.n)
-                put_row4<T>(dq + col, p.d_k - col, p.vec_k, zq[b][0] * f1 + c[0] * f2, zq[b][1] * f1 + c[1] * f2,
-                            zq[b][2] * f1 + c[2] * f2, zq[b][3] * f1 + c[3] * f2);
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = zq[b][j] * f1 + c[j] * f2;
+            if (tok < at.n) store_run<T, VEC, 4>(dq + col, p.d_k - col, y);
         }
     }
     {
         f32x4 x1[4], x2[4];  // rows s of tile b, column r = tok
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) {
+            x1[b] = x2[b] = f32x4{0, 0, 0, 0};
+            if (b >= wave) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int s = 16 * b + 4 * g + j;
-                const float d = s >= tok ? decay(gs, s, tok) * bet : 0.f;
-                x1[b][j] = e1b[b][j] * d;
-                x2[b][j] = s > tok ? e2b[b][j] * d : 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    const int s = 16 * b + 4 * g + j;
+                    const float d = s >= tok ? decay(gs, s, tok) * bet : 0.f;
+                    x1[b][j] = (b == wave ? e1[4][j] : e1[b][j]) * d;
+                    x2[b][j] = s > tok ? (b == wave ? e2[4][j] : e2[b][j]) * d : 0.f;
+                }
             }
+        }
 #pragma unroll
         for (int u = 0; u < NKT; ++u) {
             n1[u] = Op::pack(&x1[u * NBK], 1.f);
             n2[u] = Op::pack(&x2[u * NBK], 1.f);
         }
-        const float fk = -gam * exp2i(ex + es), fw = bet * tail * exp2i(ew + ed), fq = s1 * exp2i(eq),
-                    fn = -s2 * exp2i(ek);
+        const float fk = -gam * exp2i(exs), fw = bet * tail * exp2i(ed), fq = s1 * exp2i(eq), fn = -s2 * exp2i(ek);
         T* dk = static_cast<T*>(p.dk) + orow;
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             f32x4 c = {0, 0, 0, 0};
 #pragma unroll
-            for (int u = 0; u < NKT; ++u) {
-                c = Op::mma(Qt.unit(b, u, lane), n1[u], c);
-                ak[b] = Op::mma(Kt.unit(b, u, lane), n2[u], ak[b]);
-            }
+            for (int u = 0; u < NKT; ++u)
+                if (u * NBK + NBK > wave) {
+                    c = Op::mma(Qr.cols(b, u, lane), n1[u], c);
+                    ak[b] = Op::mma(Kr.cols(b, u, lane), n2[u], ak[b]);
+                }
             float y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] = zk[b][j] * fk + zw[b][j] * fw + c[j] * fq + ak[b][j] * fn;
             const int col = 16 * b + 4 * g;
-            if (tok < at.n) put_row4<T>(dk + col, p.d_k - col, p.vec_k, y[0], y[1], y[2], y[3]);
+            if (tok < at.n) store_run<T, VEC, 4>(dk + col, p.d_k - col, y);
         }
     }
     __syncthreads();
@@ -1386,7 +1450,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     // dalpha_t where alpha_t is zero or tiny: the same sum with alpha_t's factor left out
     for (int t = 0; t < at.n; ++t) {
         if (!(gs.gate[t] < kTinyAlpha)) continue;  // uniform
-        const double gt = t ? gs.G[t - 1] - gs.G[t] : -gs.G[0];  // -ln alpha_t
+        const double gt = t ? gs.G[t - 1] - gs.G[t] : -gs.G[0];  // -log2 alpha_t
         float x = 0.f;
         if (tok >= t) {
 #pragma unroll
@@ -1394,13 +1458,13 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 16 * b + 4 * g + j;
-                    if (r < t) x += mh[b][j] * gs.beta[r] * expf((float)(gs.G[tok] - gs.G[r] + gt));
+                    if (r < t) x += mh[b][j] * gs.beta[r] * pow2(gs.G[tok] - gs.G[r] + gt);
                 }
-            if (g == 0) x += ah * expf((float)(gs.G[tok] + gt));
+            if (g == 0) x += ah * pow2(gs.G[tok] + gt);
         } else if (g == 0) {
-            x += bet * kwh * expf((float)(gs.G[63] - gs.G[tok] + gt));
+            x += bet * kwh * pow2(gs.G[63] - gs.G[tok] + gt);
         }
-        if (tid == 0) x += ipt * expf((float)(gs.G[63] + gt));
+        if (tid == 0) x += ipt * pow2(gs.G[63] + gt);
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, kWave);
         if (lane == 0) red[4 + wave] = x;
@@ -1410,14 +1474,13 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     }
 }
 
-template <class Op, typename T, int DK>
-__global__ __launch_bounds__(256) void bwd_grad_kernel(BwdParams p) {
+template <class Op, typename T, int DK, bool VEC>
+__global__ __launch_bounds__(256, Op::kScaled ? 2 : 1) void bwd_grad_kernel(BwdParams p) {
     __shared__ __align__(16) char lds[GradLds<Op, DK>::kBytes];
     const int ci = blockIdx.x / p.heads, h = blockIdx.x - ci * p.heads;
     ChunkAt at;
     if (!find_chunk(p, ci, at)) return;
-    const char* rec = p.ws + (size_t)blockIdx.x * p.rec.bytes;
-    grad_chunk<Op, T, DK>(p, at, h, rec, rec + p.rec.s0, rec + p.rec.ds1, lds);
+    grad_chunk<Op, T, DK, VEC>(p, at, h, p.ws + (size_t)blockIdx.x * p.rec.bytes, lds);
 }
 
 // ---------------------------------------------------------------- exact
@@ -1432,6 +1495,7 @@ __device__ __forceinline__ void load_state(State<Op, DK>& S, const char* base, i
     const f32x4* b = reinterpret_cast<const f32x4*>(base) + (size_t)tile * (DK / 16) * 64 + lane;
 #pragma unroll
     for (int i = 0; i < DK / 16; ++i) S.s[i] = b[i * 64];
+    S.e = 0;
 }
 template <class Op, int DK>
 __device__ __forceinline__ void store_state(const State<Op, DK>& S, char* base, int tile, int lane) {
@@ -1443,16 +1507,18 @@ __host__ __device__ inline size_t exact_scratch(int DK, int dvt) {
     return rec_layout(DK, dvt, 4).bytes + (size_t)DK * dvt * 16 * 4;
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool VEC>
 __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* scratch) {
-    constexpr int kLds = PrepLds<OpF32, DK>::kBytes > GradLds<OpF32, DK>::kBytes ? PrepLds<OpF32, DK>::kBytes
-                                                                                : GradLds<OpF32, DK>::kBytes;
-    __shared__ __align__(16) char lds[kLds];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+    using L = ScanLds<OpF32, DK>;
+    constexpr int kPrep = PrepLds<OpF32, DK>::kBytes, kGrad = GradLds<OpF32, DK>::kBytes;
+    __shared__ __align__(16) char lds[std::max(std::max(kPrep, kGrad), L::kBytes)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15,
+              g = lane >> 4;
     BwdParams e = p;
     e.rec = rec_layout(DK, p.dvt, 4);
     char* rec = scratch + blockIdx.x * exact_scratch(DK, p.dvt);
     char* carry = rec + e.rec.bytes;
+    char* turn = lds + L::kTurnAt + wave * L::kTurn;
     const size_t stride = (size_t)p.heads * p.rec.bytes;
     for (int unit = blockIdx.x; unit < p.batch * p.heads; unit += gridDim.x) {
         const int seq = unit / p.heads, h = unit - seq * p.heads;
@@ -1478,9 +1544,22 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
             at.n = min(C64, t1 - at.t0);
             return at;
         };
-        for (int c = 0; c < nc; ++c) {
-            prep_chunk<OpF32, T, DK>(e, chunk(c), h, rec, lds);
+        // forward over chunk c from state S, or back over it from its gradient
+        auto step = [&](auto back, State<OpF32, DK>& S, int tile) {
+            TileInputs<OpF32, back.value> in;
+            in.load(e, rec, tile, lane);
+            scan_chunk<OpF32, DK, back.value>(e, S, in, rec, lds, turn, tile, lane);
+        };
+        auto stage = [&](auto back) {
             __syncthreads();
+            ScanStage<OpF32, DK, back.value> sg;
+            sg.load(e, rec);
+            sg.store(lds);
+            __syncthreads();
+        };
+        for (int c = 0; c < nc; ++c) {
+            prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
+            stage(std::false_type{});
             for (int tile = wave; tile < p.dvt; tile += 4) {
                 char* kept = first + c * stride + p.rec.s0;
                 State<OpF32, DK> S;
@@ -1491,7 +1570,7 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
                     load_state(S, kept, tile, lane);
                 }
                 if (c + 1 < nc) {
-                    scan_forward<OpF32, DK>(e, S, rec, 0, 1, tile, lane);
+                    step(std::false_type{}, S, tile);
                     store_state(S, kept + stride, tile, lane);
                 }
             }
@@ -1504,18 +1583,22 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
         }
         for (int c = nc - 1; c >= 0; --c) {
             const char* kept = first + c * stride + p.rec.s0;
-            prep_chunk<OpF32, T, DK>(e, chunk(c), h, rec, lds);
-            __syncthreads();
+            prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
+            stage(std::false_type{});
             for (int tile = wave; tile < p.dvt; tile += 4) {
                 State<OpF32, DK> S;
                 load_state(S, kept, tile, lane);
-                scan_forward<OpF32, DK>(e, S, rec, 0, 1, tile, lane);
+                step(std::false_type{}, S, tile);
+            }
+            stage(std::true_type{});
+            for (int tile = wave; tile < p.dvt; tile += 4) {
+                State<OpF32, DK> S;
                 load_state(S, carry, tile, lane);
-                scan_backward<OpF32, DK>(e, S, rec, 0, 1, tile, lane);
+                step(std::true_type{}, S, tile);
                 store_state(S, carry, tile, lane);
             }
             __syncthreads();
-            grad_chunk<OpF32, T, DK>(e, chunk(c), h, rec, rec + e.rec.s0, rec + e.rec.ds1, lds);
+            grad_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
             __syncthreads();
         }
         if (p.dinit)
@@ -1572,7 +1655,7 @@ size_t base_bytes(const rhz_gdr_prefill_backward_args& a) {
     return a.cu_seqlens ? (((size_t)a.batch + 1) * 4 + 255) & ~(size_t)255 : 0;
 }
 
-template <class Op, typename T, int DK>
+template <class Op, typename T, int DK, bool VEC>
 hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hipStream_t st) {
     hipError_t e;
     const int64_t grid = chunks * p.heads;
@@ -1581,7 +1664,7 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     if ((e = check_grid(grid, 256)) != hipSuccess) return e;
     if ((e = check_grid(scans, 256)) != hipSuccess) return e;
     if (grid > 0) {
-        hipLaunchKernelGGL((bwd_prep_kernel<Op, T, DK>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((bwd_prep_kernel<Op, T, DK, VEC>), dim3((unsigned)grid), dim3(256), 0, st, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0 || p.dinit) {
@@ -1589,10 +1672,10 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0) {
-        hipLaunchKernelGGL((bwd_grad_kernel<Op, T, DK>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((bwd_grad_kernel<Op, T, DK, VEC>), dim3((unsigned)grid), dim3(256), 0, st, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         if constexpr (Op::kScaled) {
-            hipLaunchKernelGGL((bwd_exact_kernel<T, DK>), dim3(blocks), dim3(256), 0, st, p, scratch);
+            hipLaunchKernelGGL((bwd_exact_kernel<T, DK, VEC>), dim3(blocks), dim3(256), 0, st, p, scratch);
             e = hipGetLastError();
         }
     }
@@ -1600,11 +1683,17 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
 }
 
 template <class Op, typename T>
-hipError_t pick_dk(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hipStream_t st) {
+hipError_t pick_dk(const BwdParams& p, bool vec, int64_t chunks, char* scratch, int blocks, hipStream_t st) {
     switch (padded_dk(p.d_k)) {
-        case 32: return go<Op, T, 32>(p, chunks, scratch, blocks, st);
-        case 64: return go<Op, T, 64>(p, chunks, scratch, blocks, st);
-        default: return go<Op, T, 128>(p, chunks, scratch, blocks, st);
+        case 32:
+            return vec ? go<Op, T, 32, true>(p, chunks, scratch, blocks, st)
+                       : go<Op, T, 32, false>(p, chunks, scratch, blocks, st);
+        case 64:
+            return vec ? go<Op, T, 64, true>(p, chunks, scratch, blocks, st)
+                       : go<Op, T, 64, false>(p, chunks, scratch, blocks, st);
+        default:
+            return vec ? go<Op, T, 128, true>(p, chunks, scratch, blocks, st)
+                       : go<Op, T, 128, false>(p, chunks, scratch, blocks, st);
     }
 }
 
@@ -1647,10 +1736,10 @@ hipError_t launch_backward(const rhz_gdr_prefill_backward_args& a, hipStream_t s
     p.dvt = tiles_dv(a.d_v);
     p.gate_is_alpha = a.gate_kind == RHZ_GATE_ALPHA;
     p.rec = rec_layout(DK, p.dvt, es);
-    const size_t four = 4 * (size_t)es;
-    p.vec_k = a.d_k % 4 == 0 && aligned(a.q, four) && aligned(a.k, four) && aligned(a.grad_q, four) &&
-              aligned(a.grad_k, four);
-    p.vec_v = a.d_v % 4 == 0 && aligned(a.v, four) && aligned(a.grad_o, four) && aligned(a.grad_v, four);
+    // rows of q, k, v, dO and of their gradients as whole runs of 16 bytes
+    const int run = 16 / es;
+    const bool vec = a.d_k % run == 0 && a.d_v % run == 0 && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&
+                     aligned(a.grad_o, 16) && aligned(a.grad_q, 16) && aligned(a.grad_k, 16) && aligned(a.grad_v, 16);
     p.vec_s = a.d_k % 4 == 0 && aligned(a.initial_state, 16) && aligned(a.grad_final_state, 16) &&
               aligned(a.grad_initial_state, 16);
     char* ws = static_cast<char*>(a.workspace);
@@ -1665,8 +1754,8 @@ hipError_t launch_backward(const rhz_gdr_prefill_backward_args& a, hipStream_t s
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (a.dtype == RHZ_F32) return pick_dk<OpF32, float>(p, chunks, scratch, exact_blocks(a), st);
-    return pick_dk<OpF16, uint16_t>(p, chunks, scratch, exact_blocks(a), st);
+    if (a.dtype == RHZ_F32) return pick_dk<OpF32, float>(p, vec, chunks, scratch, exact_blocks(a), st);
+    return pick_dk<OpF16, uint16_t>(p, vec, chunks, scratch, exact_blocks(a), st);
 }
 
 }  // namespace rhz
