@@ -70,9 +70,9 @@ typedef struct rhz_gdr_prefill_backward_args {
 
 /* Bytes of device workspace rhz_gdr_prefill_backward needs for these arguments
  * (cu_seqlens tells a pack; no other pointer is read): per chunk of 64 tokens
- * and head some 1280 bytes per padded d_k and d_v at d_k = d_v (160 KiB at 128
- * for bf16, 320 for fp32).  Two calls that may run at the same time need a
- * workspace each. */
+ * and head the states on its either side and what the scans hand on, at d_k =
+ * d_v = 128 some 115 KiB for bf16 and 227 for fp32.  Two calls that may run at
+ * the same time need a workspace each. */
 rhz_status rhz_gdr_prefill_backward_workspace_size(const rhz_gdr_prefill_backward_args* args,
                                                    size_t* bytes);
 

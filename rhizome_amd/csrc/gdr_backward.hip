@@ -205,16 +205,19 @@ __device__ __forceinline__ int wave_max_bits(int x) {
 // The exponent of magnitude bits, 100 at most either way.
 __device__ __forceinline__ int bits_exp(int bits) { return max(min((bits >> 23) - 127, 100), -100); }
 
-// A run of 16 bytes of a row of T (8 bf16 or 4 fp32), as floats.  VEC: rows
-// are whole runs and aligned, and a run outside the matrix (`in` false) is
-// read from `safe` and cleared, so that no branch parts the loads.
+// A run of 16 bytes of a row of T (8 bf16 or 4 fp32).  VEC: rows are whole runs
+// and aligned, and a run outside the matrix (`in` false) is read from zeros
+// kept for it: nothing touches the loaded registers before their use, so that
+// loads issued ahead stay in flight.
 template <typename T>
 constexpr int kRun = 16 / int(sizeof(T));
+__device__ const u32x4 kZeroRun = {0, 0, 0, 0};
+typedef const __attribute__((address_space(1))) u32x4 global_u32x4;
 template <typename T, bool VEC>
-__device__ __forceinline__ u32x4 load_run(const T* p, const T* safe, bool in, int n) {
+__device__ __forceinline__ u32x4 load_run(const T* p, bool in, int n) {
     if constexpr (VEC) {
-        const u32x4 u = *reinterpret_cast<const u32x4*>(in ? p : safe);
-        return in ? u : u32x4{0, 0, 0, 0};
+        const u32x4* u = in ? reinterpret_cast<const u32x4*>(p) : &kZeroRun;
+        return *(global_u32x4*)(u);
     } else {
         T x[kRun<T>];
 #pragma unroll
@@ -272,36 +275,31 @@ __device__ __forceinline__ void store_run(T* p, int n, const float (&x)[N]) {
 }
 
 // ------------------------------------------------------------ workspace
-// One record per (chunk, head), in units of DK = d_k padded to 32, 64 or 128
-// and d_v padded to 16-row tiles (an even number of them).
+// One record per (chunk, head), for DK = d_k padded to 32, 64 or 128 and d_v
+// padded to 16-row tiles (an even number of them).
 struct RecLayout {
-    size_t wk, kd, kf, qf, wt, ot, dot, w, x, s0, ds1, vec, bytes;
+    size_t t, p, w, x, s0, ds1, vec, bytes;
 };
 __host__ __device__ inline RecLayout rec_layout(int DK, int dvt, int es) {
     RecLayout l{};
-    const size_t tk = (size_t)64 * DK * es, tv = (size_t)64 * dvt * 16 * es, st = (size_t)DK * dvt * 16 * es;
+    const size_t tt = (size_t)64 * 64 * es, tv = (size_t)64 * dvt * 16 * es, st = (size_t)DK * dvt * 16 * es;
     size_t at = 0;
-    l.wk = at; at += tk;    // T diag(gamma) K          (token; d_k)
-    l.kd = at; at += tk;    // T^T diag(beta tail) K    (token; d_k)
-    l.kf = at; at += tk;    // K by rows, as scaled
-    l.qf = at; at += tk;    // Q by rows, as scaled
-    l.wt = at; at += tv;    // T V                            (d_v; token), by 16-row tiles
-    l.ot = at; at += tv;    // T^T diag(beta) P^T dO          (d_v; token), by 16-row tiles
-    l.dot = at; at += tv;   // dO                             (d_v; token), by 16-row tiles
+    l.t = at; at += tt;     // T by rows
+    l.p = at; at += tt;     // P by rows, scaled as K and Q are
     l.w = at; at += tv;     // W                              (token; d_v), by units of d_v
     l.x = at; at += tv;     // dX                             (token; d_v), by units of d_v
     l.s0 = at; at += st;    // S0                             (d_k; d_v), by units of d_v
     l.ds1 = at; at += st;   // dS1                            (d_k; d_v), by units of d_v
     l.vec = at;             // small values, then the tiles' exponents
-    at += 256 * 4 + 6 * 64 * 4;
+    at += 256 * 4 + 5 * 64 * 4;
     l.bytes = (at + 255) & ~(size_t)255;
     return l;
 }
-// the record's small values: gamma [64], beta tail [64], gamma_c, exponents of
-// K and Q, whether the chunk leaves the fp16 operands' domain
-enum { kVecGamma = 0, kVecWrite = 64, kVecGc = 128, kVecEK = 129, kVecEQ = 130, kVecBad = 131 };
+// the record's small values: gamma, beta tail and beta by token, gamma_c,
+// exponents of K and Q, whether the chunk leaves the fp16 operands' domain
+enum { kVecGamma = 0, kVecWrite = 64, kVecBeta = 128, kVecGc = 192, kVecEK = 193, kVecEQ = 194, kVecBad = 195, kVecs = 196 };
 // exponents by d_v tile, from float 256 on
-enum { kExpV = 256, kExpO = 320, kExpW = 384, kExpX = 448, kExpS = 512, kExpD = 576 };
+enum { kExpO = 256, kExpW = 320, kExpX = 384, kExpS = 448, kExpD = 512 };
 
 struct BwdParams {
     const void *q, *k, *v, *dout;
@@ -375,33 +373,20 @@ __device__ __forceinline__ bool load_gates(const BwdParams& p, const ChunkAt& at
 __device__ __forceinline__ float decay(const Gates& gs, int r, int s) { return pow2(gs.G[r] - gs.G[s]); }
 
 // ----------------------------------------------------------------- prep
-// One (chunk, head) per workgroup of four waves.  LDS: K by rows (then each
-// wave's tile of V or dO), Q by rows (then T), L diag(beta) in fp32 (then
-// T^T diag(beta) P^T).
+// One (chunk, head) per workgroup of four waves.  LDS: K by rows (then T), Q by
+// rows (then P and T's diagonal blocks in fp32), L diag(beta) in fp32.
 template <class Op, int DK>
 struct PrepLds {
     using T64 = RowMat<Op, 64>;
-    using Tile = RowMat<Op, 16>;
-    static constexpr int kRow = RowMat<Op, DK>::bytes(64), kTiles = 4 * Tile::bytes(64);
-    static constexpr int kDiag = 4 * 16 * 16 * 4;  // T's diagonal blocks in fp32
-    static constexpr int kKr = 0;
-    static constexpr int kQr = kRow > kTiles ? kRow : kTiles;
-    static constexpr int kT = kQr, kTd = kQr + T64::bytes(64), kQEnd = kTd + kDiag;
-    static constexpr int kA = kQr + kRow > kQEnd ? kQr + kRow : kQEnd;
+    static constexpr int kRow = RowMat<Op, DK>::bytes(64), kT64 = T64::bytes(64), kDiag = 4 * 16 * 16 * 4;
+    static constexpr int kKr = 0, kT = 0;
+    static constexpr int kQr = kRow > kT64 ? kRow : kT64;
+    static constexpr int kP = kQr, kTd = kQr + kT64;
+    static constexpr int kA = kQr + (kRow > kT64 + kDiag ? kRow : kT64 + kDiag);
     static constexpr int kGates = kA + 64 * 64 * 4;
     static constexpr int kMisc = kGates + int(sizeof(Gates));
     static constexpr int kBytes = kMisc + 64;
 };
-
-// every element of a unit times the factor of its contraction index
-template <class Op>
-__device__ __forceinline__ typename Op::Unit times_unit(const typename Op::Unit& u, const float* f, int ku, int g) {
-    f32x4 t[Op::kBlocks];
-    Op::unpack(u, t);
-#pragma unroll
-    for (int b = 0; b < Op::kBlocks; ++b) t[b] *= *reinterpret_cast<const f32x4*>(f + 16 * (ku * Op::kBlocks + b) + 4 * g);
-    return Op::pack(t, 1.f);
-}
 
 template <class Op, typename T, int DK, bool VEC>
 __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at, int h, char* rec, char* lds) {
@@ -413,16 +398,15 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
               m = lane & 15;
     const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
-    const RowMat<Op, 64> Th{lds + L::kT};
+    const RowMat<Op, 64> Th{lds + L::kT}, Ph{lds + L::kP};
     float* Td = reinterpret_cast<float*>(lds + L::kTd);
     float* Af = reinterpret_cast<float*>(lds + L::kA);
-    char* Bo = lds + L::kA;
     Gates& gs = *reinterpret_cast<Gates*>(lds + L::kGates);
     int* misc = reinterpret_cast<int*>(lds + L::kMisc);  // maxima of K, Q by wave; [8] outside the domain
     float* vec = reinterpret_cast<float*>(rec + p.rec.vec);
     int* exps = reinterpret_cast<int*>(vec);
 
-    const long ldk = (long)p.heads * p.d_k, ldv = (long)p.heads * p.d_v;
+    const long ldk = (long)p.heads * p.d_k;
     const T* kp = static_cast<const T*>(p.k) + at.t0 * ldk + (long)h * p.d_k;
     const T* qp = static_cast<const T*>(p.q) + at.t0 * ldk + (long)h * p.d_k;
     u32x4 kb[NR], qb[NR];
@@ -430,8 +414,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     for (int i = 0; i < NR; ++i) {
         const int id = tid + 256 * i, t = id / (DK / R), c = id % (DK / R) * R;
         const bool in = t < at.n && c < p.d_k;
-        kb[i] = load_run<T, VEC>(kp + t * ldk + c, kp, in, p.d_k - c);
-        qb[i] = load_run<T, VEC>(qp + t * ldk + c, qp, in, p.d_k - c);
+        kb[i] = load_run<T, VEC>(kp + t * ldk + c, in, p.d_k - c);
+        qb[i] = load_run<T, VEC>(qp + t * ldk + c, in, p.d_k - c);
     }
     bool bad = false;
     if (wave == 0) bad = load_gates(p, at, h, gs, lane);
@@ -459,25 +443,21 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     }
     {
         const float sk = exp2i(-ek), sq = exp2i(-eq);
-        Elt* kf = reinterpret_cast<Elt*>(rec + p.rec.kf);
-        Elt* qf = reinterpret_cast<Elt*>(rec + p.rec.qf);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             const int id = tid + 256 * i, t = id / (DK / R), c = id % (DK / R) * R;
             float x[R];
-            typedef Elt EltR __attribute__((ext_vector_type(R)));
             unpack_run<T>(kb[i], x);
             Kr.put(t, c, x, sk);
-            *reinterpret_cast<EltR*>(kf + t * DK + c) = *reinterpret_cast<const EltR*>(Kr.at(t, c));
             unpack_run<T>(qb[i], x);
             Qr.put(t, c, x, sq);
-            *reinterpret_cast<EltR*>(qf + t * DK + c) = *reinterpret_cast<const EltR*>(Qr.at(t, c));
         }
     }
     __syncthreads();
     if (tid < 64) {
         vec[kVecGamma + tid] = gs.gamma[tid];
         vec[kVecWrite + tid] = gs.beta[tid] * gs.tail[tid];
+        vec[kVecBeta + tid] = gs.beta[tid];
     }
     if (tid == 0) {
         vec[kVecGc] = gs.gamma[63];
@@ -485,8 +465,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
         exps[kVecEQ] = eq;
     }
 
-    // column tile `wave` of L diag(beta) (fp32), row tile `wave` of P diag(beta)
-    // (scaled as K and Q are, in registers): five tiles of products each wave
+    // column tile `wave` of L diag(beta) (fp32), row tile `wave` of P (scaled as
+    // K and Q are, in registers): five tiles of products each wave
     Unit pu[NKT];
     {
         const float kk2 = exp2i(2 * ek);
@@ -517,7 +497,7 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
                     if (Op::kScaled && r == s && !(kk <= 1.03125f)) bad = true;
                     Af[sq_at(r, s)] = s < r ? kk * decay(gs, r, s) * bs : 0.f;
                 }
-                if (mt <= wave && r <= s) pt[mt][i] = cq[i] * decay(gs, s, r) * gs.beta[r];  // row s of P, column r
+                if (mt <= wave && r <= s) pt[mt][i] = cq[i] * decay(gs, s, r);  // row s of P, column r
             }
         }
 #pragma unroll
@@ -526,6 +506,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     if constexpr (Op::kScaled)
         if (bad) misc[8] = 1;
     __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NKT; ++u) Ph.put_unit(16 * wave + m, u, g, pu[u]);
 
     // T's diagonal blocks by forward substitution in fp32, column m of block
     // `wave` in lane (., m); then T_iw = -T_ii sum_{w <= b < i} A_ib T_bw down
@@ -572,126 +554,16 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     }
     __syncthreads();
 
-    {
-        // T diag(gamma) K and T^T diag(beta tail) K, rows of token tile `wave`
-        Unit ur[NKT], uc[NKT];
+    constexpr int NP = 64 * int(sizeof(Elt)) / 16;  // 16-byte pieces of a row of T and P
+    u32x4* ot = reinterpret_cast<u32x4*>(rec + p.rec.t);
+    u32x4* op = reinterpret_cast<u32x4*>(rec + p.rec.p);
 #pragma unroll
-        for (int ku = 0; ku < NKT; ++ku) {
-            ur[ku] = times_unit<Op>(Th.blocks(16 * wave + m, ku, g), gs.gamma, ku, g);
-            uc[ku] = times_unit<Op>(times_unit<Op>(Th.cols(wave, ku, lane), gs.beta, ku, g), gs.tail, ku, g);
-        }
-        Unit* ow = reinterpret_cast<Unit*>(rec + p.rec.wk);
-        Unit* od = reinterpret_cast<Unit*>(rec + p.rec.kd);
-#pragma unroll
-        for (int u = 0; u < NKK; ++u) {
-            f32x4 c[NBK], d[NBK];
-#pragma unroll
-            for (int b = 0; b < NBK; ++b) {
-                c[b] = d[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int ku = 0; ku < NKT; ++ku) {
-                    const Unit a = Kr.cols(u * NBK + b, ku, lane);
-                    c[b] = Op::mma(a, ur[ku], c[b]);
-                    d[b] = Op::mma(a, uc[ku], d[b]);
-                }
-            }
-            ow[(wave * NKK + u) * 64 + lane] = Op::pack(c, 1.f);
-            od[(wave * NKK + u) * 64 + lane] = Op::pack(d, 1.f);
-        }
-        // T^T diag(beta) P^T as left operand units (row r; s): columns s of this wave's tile
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            f32x4 c = {0, 0, 0, 0};
-#pragma unroll
-            for (int ku = 0; ku < NKT; ++ku) c = Op::mma(pu[ku], Th.cols(nt, ku, lane), c);
-            // lane (g, m): row r = 16 nt + m, columns s = 16 wave + 4 g ..
-            if constexpr (Op::kScaled) {
-                const f16x4 q = {(_Float16)c[0], (_Float16)c[1], (_Float16)c[2], (_Float16)c[3]};
-                *reinterpret_cast<f16x4*>(Bo + ((nt * NKT + wave / 2) * 64 + lane) * 16 + (wave & 1) * 8) = q;
-            } else {
-                *reinterpret_cast<f32x4*>(Bo + ((nt * NKT + wave) * 64 + lane) * 16) = c;
-            }
-        }
+    for (int i = 0; i < 64 * NP / 256; ++i) {
+        const int id = tid + 256 * i;
+        ot[id] = *reinterpret_cast<const u32x4*>(Th.at(id / NP, 0) + id % NP * 16);
+        op[id] = *reinterpret_cast<const u32x4*>(Ph.at(id / NP, 0) + id % NP * 16);
     }
-    Unit ta[4][NKT];  // T by rows, left operand
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int ku = 0; ku < NKT; ++ku) ta[mt][ku] = Th.blocks(16 * mt + m, ku, g);
-    __syncthreads();
-
-    // T V and T^T diag(beta) P^T dO by 16-column tiles of d_v, one wave each
-    const RowMat<Op, 16> st{lds + L::kKr + wave * RowMat<Op, 16>::bytes(64)};
-    const T* vp = static_cast<const T*>(p.v) + at.t0 * ldv + (long)h * p.d_v;
-    const T* op = static_cast<const T*>(p.dout) + at.t0 * ldv + (long)h * p.d_v;
-    constexpr int NV = 64 * 16 / R / 64, RPR = 16 / R;  // runs of a tile per lane, and per row
-    auto load_tile = [&](u32x4 (&y)[2][NV], int tile) {
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int id = lane + 64 * i, t = id / RPR, c = 16 * tile + id % RPR * R;
-                const T* src = which ? op : vp;
-                y[which][i] = load_run<T, VEC>(src + t * ldv + c, src, t < at.n && c < p.d_v, p.d_v - c);
-            }
-    };
-    u32x4 y[2][NV];
-    if (wave < p.dvt) load_tile(y, wave);
-    for (int tile = wave; tile < p.dvt; tile += 4) {
-        u32x4 now[2][NV];
-#pragma unroll
-        for (int i = 0; i < 2 * NV; ++i) now[i / NV][i % NV] = y[i / NV][i % NV];
-        if (tile + 4 < p.dvt) load_tile(y, tile + 4);
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            float s = 1.f;
-            if constexpr (Op::kScaled) {
-                int mx = 0;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) mx = max(mx, run_max_bits<T>(now[which][i]));
-                const int bits = wave_max_bits(mx), e = bits_exp(bits) + 2;  // below 1/2
-                bad = bad || bits >= 0x7f800000;
-                s = exp2i(-e);
-                if (lane == 0) exps[(which ? kExpO : kExpV) + tile] = e;
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int id = lane + 64 * i;
-                float x[R];
-                unpack_run<T>(now[which][i], x);
-                st.put(id / RPR, id % RPR * R, x, s);
-            }
-            __builtin_amdgcn_wave_barrier();
-            Unit ub[NKT];
-#pragma unroll
-            for (int ku = 0; ku < NKT; ++ku) ub[ku] = st.cols(0, ku, lane);
-            __builtin_amdgcn_wave_barrier();
-            Unit* o = reinterpret_cast<Unit*>(rec + (which ? p.rec.ot : p.rec.wt)) + (long)tile * NKT * 64;
-#pragma unroll
-            for (int u = 0; u < NKT; ++u) {
-                f32x4 c[NBK];
-#pragma unroll
-                for (int b = 0; b < NBK; ++b) {
-                    const int mt = u * NBK + b;
-                    c[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int ku = 0; ku < NKT; ++ku)
-                        c[b] = Op::mma(which ? lds_unit<Op>(Bo, mt * NKT + ku, lane) : ta[mt][ku], ub[ku], c[b]);
-                }
-                o[u * 64 + lane] = Op::pack(c, 1.f);
-            }
-            if (which) {
-                Unit* od = reinterpret_cast<Unit*>(rec + p.rec.dot) + (long)tile * NKT * 64;
-#pragma unroll
-                for (int ku = 0; ku < NKT; ++ku) od[ku * 64 + lane] = ub[ku];
-            }
-        }
-    }
-    if constexpr (Op::kScaled) {
-        if (bad) misc[8] = 1;
-        __syncthreads();
-        if (tid == 0) exps[kVecBad] = misc[8];
-    }
+    if (Op::kScaled && tid == 0) exps[kVecBad] = misc[8];
 }
 
 template <class Op, typename T, int DK, bool VEC>
@@ -707,18 +579,19 @@ __global__ __launch_bounds__(256, Op::kScaled ? 3 : 1) void bwd_prep_kernel(BwdP
 // Four waves to a workgroup, each carrying 16 rows of S (or of dS) along the
 // chunks of a (sequence, head) in accumulators: tile b holds d_k indices 16 b +
 // 4 g .. + 3 of row m.  The state's own operands come from its accumulators;
-// the others pass through LDS once for the four waves, read from HBM two
-// chunks ahead.  What the gradients need of a wave's rows is turned through a
-// corner of LDS of its own, so that d_v runs along the units it writes.
+// K, Q, T and P pass through LDS once for the four waves, read from HBM two
+// chunks ahead, and serve as rows and as columns.  What a wave alone reads (its
+// columns of V or dO) and writes (S0, W, dS1, dX in the order the gradients'
+// products take) is turned through a corner of LDS of its own.
 template <class Op, int DK>
 struct ScanLds {
-    static constexpr int kE = int(sizeof(typename Op::Elt));
-    static constexpr int kUnits = 64 * DK * kE;                  // T diag(gamma) K or T^T diag(beta tail) K
-    static constexpr int kRows = RowMat<Op, DK>::bytes(64);      // K, Q
-    static constexpr int kBuf = kUnits + 2 * kRows;
+    static constexpr int kRow = RowMat<Op, DK>::bytes(64), kT64 = RowMat<Op, 64>::bytes(64);
+    static constexpr int kK = 0, kT = kRow, kVec = kT + kT64, kQ = kVec + 1024, kP = kQ + kRow;
+    static constexpr int kBuf = kP + kT64;
     static constexpr int kBufs = Op::kScaled ? 2 : 1;
     static constexpr int kTurnCols = DK > 64 ? DK : 64;
-    static constexpr int kTurn = RowMat<Op, kTurnCols>::bytes(16);
+    static constexpr int kTurnRows = RowMat<Op, kTurnCols>::bytes(16), kTile = 64 * (16 * int(sizeof(typename Op::Elt)) + 16);
+    static constexpr int kTurn = kTurnRows > kTile ? kTurnRows : kTile;
     static constexpr int kTurnAt = kBufs * kBuf;
     static constexpr int kBytes = kTurnAt + 4 * kTurn;
 };
@@ -780,49 +653,64 @@ struct State {
     }
 };
 
-// A wave's own reads of a chunk: T V, or T^T diag(beta) P^T dO and dO; the
-// tokens' factors; gamma_c and exponents.
-template <class Op, bool BACK>
-struct TileInputs {
-    static constexpr int NKT = 4 / Op::kBlocks;
-    typename Op::Unit t[NKT], o[BACK ? NKT : 1];
-    f32x4 f[4];
-    float gc;
-    int ek, eq, et;
-    __device__ __forceinline__ void load(const BwdParams& p, const char* rec, int tile, int lane) {
-        const typename Op::Unit* a =
-            reinterpret_cast<const typename Op::Unit*>(rec + (BACK ? p.rec.ot : p.rec.wt)) + tile * NKT * 64 + lane;
+// The chunk's tokens of a sequence.
+template <typename T>
+struct SeqAt {
+    const T *k, *q, *vo;  // the sequence's first token of this head: K, Q, and V or dO
+    int tokens;
+};
+
+// A wave's 16 columns of V (or dO) of a chunk, as the rows come from HBM.
+template <typename T, bool VEC>
+struct TileRuns {
+    static constexpr int R = kRun<T>, N = 64 * 16 / R / 64, RPR = 16 / R;
+    u32x4 r[N];
+    __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, int tile, int lane) {
+        const long ld = (long)p.heads * p.d_v;
 #pragma unroll
-        for (int u = 0; u < NKT; ++u) t[u] = a[u * 64];
-        if constexpr (BACK) {
-            const typename Op::Unit* b =
-                reinterpret_cast<const typename Op::Unit*>(rec + p.rec.dot) + tile * NKT * 64 + lane;
-#pragma unroll
-            for (int u = 0; u < NKT; ++u) o[u] = b[u * 64];
+        for (int i = 0; i < N; ++i) {
+            const int id = lane + 64 * i, t = c * C64 + id / RPR, col = 16 * tile + id % RPR * R;
+            r[i] = load_run<T, VEC>(at.vo + t * ld + col, t < at.tokens && col < p.d_v, p.d_v - col);
         }
-        const float* v = reinterpret_cast<const float*>(rec + p.rec.vec);
+    }
+    __device__ __forceinline__ int max_bits() const {
+        int m = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            f[b] = *reinterpret_cast<const f32x4*>(v + (BACK ? kVecGamma : kVecWrite) + 16 * b + 4 * (lane >> 4));
-        gc = v[kVecGc];
-        ek = eq = et = 0;
-        if constexpr (Op::kScaled) {
-            const int* x = reinterpret_cast<const int*>(v);
-            ek = x[kVecEK];
-            eq = x[kVecEQ];
-            et = x[(BACK ? kExpO : kExpV) + tile];
+        for (int i = 0; i < N; ++i) m = max(m, run_max_bits<T>(r[i]));
+        return wave_max_bits(m);
+    }
+    // the tokens 16 b + 4 g .. of column m, through the wave's corner of LDS
+    __device__ __forceinline__ void turn(char* corner, f32x4 (&x)[4], int lane) const {
+        using Raw = typename std::conditional<sizeof(T) == 2, OpF16, OpF32>::type;  // 16 bits are moved as such
+        const RowMat<Raw, 16> tn{corner};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = lane + 64 * i;
+            *reinterpret_cast<u32x4*>(tn.at(id / RPR, id % RPR * R)) = r[i];
         }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if constexpr (sizeof(T) == 2) {
+                const s16x4 h = __builtin_bit_cast(s16x4, tn.col4(0, b, lane));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[b][i] = __uint_as_float(uint32_t(uint16_t(h[i])) << 16);
+            } else {
+                x[b] = tn.col4(0, b, lane);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 };
 
-template <class Op>
-__device__ __forceinline__ int tokens_exp(const f32x4 (&w)[4]) {
-    if constexpr (!Op::kScaled) return 0;
-    float mx = 0.f;
+// Magnitude bits of the largest of a wave's values; a NaN's are the largest.
+__device__ __forceinline__ int tokens_bits(const f32x4 (&w)[4]) {
+    int mx = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
-        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(w[b][0])), fabsf(w[b][1])), fmaxf(fabsf(w[b][2]), fabsf(w[b][3])));
-    return bits_exp(bits_abs(wave_max(mx)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = max(mx, bits_abs(w[b][i]));
+    return wave_max_bits(mx);
 }
 
 // Rows of a wave's tile as units with d_v along the contraction: column tile
@@ -835,19 +723,29 @@ __device__ __forceinline__ void store_turned(const Mat& turn, char* base, int ti
     for (int b = 0; b < N; ++b) *reinterpret_cast<typename Op::Quad*>(o + b * 1024) = turn.col4(b, 0, lane);
 }
 
-// One chunk of a wave's rows.  Forward: W = T V - (T diag(gamma) K) S0^T and
-// S1 = gamma_c S0 + (beta tail W)^T K.  Back: dX = T^T diag(beta) (P^T dO +
-// diag(tail) K dS1^T) and dS0 = gamma_c dS1 + (gamma dO)^T Q - (gamma dX)^T K.
-template <class Op, int DK, bool BACK>
-__device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S, const TileInputs<Op, BACK>& in, char* rec,
-                                           const char* buf, char* turn, int tile, int lane) {
+// One chunk of a wave's rows.  Forward: W = T (V - diag(gamma) K S0^T) and S1 =
+// gamma_c S0 + (beta tail W)^T K.  Back: dX = T^T (diag(beta) P^T dO +
+// diag(beta tail) K dS1^T) and dS0 = gamma_c dS1 + (gamma dO)^T Q - (gamma dX)^T K.
+template <class Op, typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S, const TileRuns<T, VEC>& in, char* rec,
+                                           char* buf, char* turn, int tile, int lane) {
     using Unit = typename Op::Unit;
     using L = ScanLds<Op, DK>;
     constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK;
     const int g = lane >> 4, m = lane & 15;
-    const RowMat<Op, DK> K{const_cast<char*>(buf) + L::kUnits}, Q{const_cast<char*>(buf) + L::kUnits + L::kRows};
+    const RowMat<Op, DK> K{buf + L::kK}, Q{buf + L::kQ};
+    const RowMat<Op, 64> Tm{buf + L::kT}, P{buf + L::kP};
     const RowMat<Op, L::kTurnCols> tn{turn};
-    f32x4 x[4], w[4];
+    const float* vec = reinterpret_cast<const float*>(buf + L::kVec);
+    auto by_token = [&](int v, int b) { return *reinterpret_cast<const f32x4*>(vec + v + 16 * b + 4 * g); };
+    const float gc = vec[kVecGc];
+    int ek = 0, eq = 0;
+    if constexpr (Op::kScaled) {
+        ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
+        eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
+    }
+    f32x4 x[4], w[4], vo[4];
+    in.turn(turn, vo, lane);
 #pragma unroll
     for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -855,21 +753,62 @@ __device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S,
         const Unit su = Op::pack(&S.s[i * NBK], 1.f);
         tn.put_unit(m, i, g, su);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = Op::mma(lds_unit<Op>(buf, b * NU + i, lane), su, x[b]);
+        for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su, x[b]);
     }
     __builtin_amdgcn_wave_barrier();
     store_turned<Op, NT>(tn, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
     __builtin_amdgcn_wave_barrier();
     const int top = Op::kScaled ? S.top() : 0;
+    const float sx = exp2i(S.e + ek);
+    int eo = 0;
+    if constexpr (!BACK) {
 #pragma unroll
-    for (int u = 0; u < NKT; ++u) Op::unpack(in.t[u], &w[u * NBK]);
-    const float st = exp2i(BACK ? in.et + in.ek + in.eq : in.et), sx = BACK ? exp2i(S.e + in.ek) : -exp2i(S.e + in.ek);
+        for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * (x[b] * sx);
+    } else {
+        if constexpr (Op::kScaled) eo = bits_exp(in.max_bits()) + 2;  // dO below 1/2
+        const float so = exp2i(-eo), sz = exp2i(eo + ek + eq);
+        f32x4 z[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) z[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[b][i] = w[b][i] * st + x[b][i] * sx;
+        for (int u = 0; u < NKT; ++u) {
+            const Unit du = Op::pack(&vo[u * NBK], so);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (u * NBK + NBK > b) z[b] = Op::mma(P.cols(b, u, lane), du, z[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) w[b] = by_token(kVecBeta, b) * (z[b] * sz) + by_token(kVecWrite, b) * (x[b] * sx);
+    }
+    // T or T^T times it, the operand below 2^5
+    int er = 0, rbits = 0;
+    if constexpr (Op::kScaled) {
+        rbits = tokens_bits(w);
+        er = bits_exp(rbits) - 4;
+    }
+    {
+        const float sr = exp2i(-er);
+        f32x4 y[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) y[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < NKT; ++u) {
+            const Unit ru = Op::pack(&w[u * NBK], sr);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (!BACK && u * NBK <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), ru, y[b]);
+                if (BACK && u * NBK + NBK > b) y[b] = Op::mma(Tm.cols(b, u, lane), ru, y[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) w[b] = y[b];
+    }
     // W is kept with its largest value in [8, 16), dX in [1/4, 1/2)
-    const int tw = tokens_exp<Op>(w), ew = Op::kScaled ? tw + (BACK ? 2 : -3) : 0;
+    int tw = 0, ew = 0;
+    if constexpr (Op::kScaled) {
+        tw = bits_exp(tokens_bits(w));
+        ew = tw + (BACK ? 2 : -3);
+    }
     const float si = exp2i(-ew);
 #pragma unroll
     for (int u = 0; u < NKT; ++u) tn.put_unit(m, u, g, Op::pack(&w[u * NBK], si));
@@ -878,35 +817,37 @@ __device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S,
     __builtin_amdgcn_wave_barrier();
     if (Op::kScaled && lane == 0) {
         int* oe = reinterpret_cast<int*>(rec + p.rec.vec);
-        oe[(BACK ? kExpX : kExpW) + tile] = ew;
+        oe[(BACK ? kExpX : kExpW) + tile] = ew + er;
         oe[(BACK ? kExpD : kExpS) + tile] = S.e;
+        if constexpr (BACK) oe[kExpO + tile] = eo;
+        if (rbits >= 0x7f800000) oe[kVecBad] = 1;
     }
     // the next state in units of 2^e, of the larger of what stays (gamma_c S,
     // below 2^9 of them) and what is written (each token's value below 2^8, and
-    // 64 tokens' with rows of K or Q below 2: 2^15)
+    // 64 tokens' with rows of K or Q below 2: 2^15; back, two such sums of 2^14)
     int e = 0;
     if constexpr (Op::kScaled) {
-        e = max(tw + in.ek, top + bits_exp(bits_abs(in.gc)));
-        if constexpr (BACK) e = max(e, in.et - 2 + in.eq) + 1;  // two sums of 64 tokens
+        e = max(tw + er + ek, top + bits_exp(bits_abs(gc)));
+        if constexpr (BACK) e = max(e, eo - 2 + eq) + 1;
         e -= 7;
     }
-    const float sw = BACK ? -exp2i(in.ek - e) : exp2i(in.ek - e), sg = in.gc * exp2i(S.e - e);
+    const float sw = BACK ? -exp2i(er + ek - e) : exp2i(er + ek - e), sd = exp2i(eq - e), sg = gc * exp2i(S.e - e);
     S.e = e;
 #pragma unroll
     for (int b = 0; b < NT; ++b) S.s[b] *= sg;
 #pragma unroll
     for (int u = 0; u < NKT; ++u) {
 #pragma unroll
-        for (int b = 0; b < NBK; ++b) w[u * NBK + b] *= in.f[u * NBK + b];
+        for (int b = 0; b < NBK; ++b) {
+            const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u * NBK + b);
+            w[u * NBK + b] *= f;
+            if constexpr (BACK) vo[u * NBK + b] *= f;
+        }
         const Unit wu = Op::pack(&w[u * NBK], sw);
 #pragma unroll
         for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
         if constexpr (BACK) {
-            f32x4 d[NBK];
-            Op::unpack(in.o[u], d);
-#pragma unroll
-            for (int b = 0; b < NBK; ++b) d[b] *= in.f[u * NBK + b];
-            const Unit du = Op::pack(d, exp2i(in.et + in.eq - e));
+            const Unit du = Op::pack(&vo[u * NBK], sd);
 #pragma unroll
             for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
         }
@@ -914,71 +855,113 @@ __device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S,
 }
 
 // A chunk's shared operands on their way from HBM to LDS, by all 256 threads.
-template <class Op, int DK, bool BACK>
+template <class Op, typename T, int DK, bool VEC, bool BACK>
 struct ScanStage {
-    static constexpr int kE = int(sizeof(typename Op::Elt)), N = 64 * DK * kE / 16 / 256, RPR = DK * kE / 16;
-    u32x4 a[N], k[N], q[BACK ? N : 1];
-    __device__ __forceinline__ void load(const BwdParams& p, const char* rec) {
-        const u32x4* pa = reinterpret_cast<const u32x4*>(rec + (BACK ? p.rec.kd : p.rec.wk));
-        const u32x4* pk = reinterpret_cast<const u32x4*>(rec + p.rec.kf);
-        const u32x4* pq = reinterpret_cast<const u32x4*>(rec + p.rec.qf);
+    static constexpr int R = kRun<T>, N = 64 * DK / R / 256;
+    static constexpr int NP = 64 * int(sizeof(typename Op::Elt)) / 16, NT = 64 * NP / 256;
+    u32x4 k[N], q[BACK ? N : 1], t[NT], pp[BACK ? NT : 1];
+    float vec;
+    int ek, eq;
+    __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, const char* rec) {
+        const int tid = threadIdx.x;
+        const long ld = (long)p.heads * p.d_k;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            a[i] = pa[threadIdx.x + 256 * i];
-            k[i] = pk[threadIdx.x + 256 * i];
-            if constexpr (BACK) q[i] = pq[threadIdx.x + 256 * i];
+            const int id = tid + 256 * i, tk = c * C64 + id / (DK / R), col = id % (DK / R) * R;
+            const bool in = tk < at.tokens && col < p.d_k;
+            k[i] = load_run<T, VEC>(at.k + tk * ld + col, in, p.d_k - col);
+            if constexpr (BACK) q[i] = load_run<T, VEC>(at.q + tk * ld + col, in, p.d_k - col);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            t[i] = reinterpret_cast<const u32x4*>(rec + p.rec.t)[tid + 256 * i];
+            if constexpr (BACK) pp[i] = reinterpret_cast<const u32x4*>(rec + p.rec.p)[tid + 256 * i];
+        }
+        const float* v = reinterpret_cast<const float*>(rec + p.rec.vec);
+        vec = v[min(tid, kVecs - 1)];
+        ek = eq = 0;
+        if constexpr (Op::kScaled) {
+            ek = reinterpret_cast<const int*>(v)[kVecEK];
+            eq = reinterpret_cast<const int*>(v)[kVecEQ];
         }
     }
     __device__ __forceinline__ void store(char* buf) const {
         using L = ScanLds<Op, DK>;
-        const RowMat<Op, DK> K{buf + L::kUnits}, Q{buf + L::kUnits + L::kRows};
+        const int tid = threadIdx.x;
+        const RowMat<Op, DK> K{buf + L::kK}, Q{buf + L::kQ};
+        const RowMat<Op, 64> Tm{buf + L::kT}, P{buf + L::kP};
+        const float sk = exp2i(-ek), sq = exp2i(-eq);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + 256 * i;
-            reinterpret_cast<u32x4*>(buf)[id] = a[i];
-            *reinterpret_cast<u32x4*>(K.at(id / RPR, 0) + id % RPR * 16) = k[i];
-            if constexpr (BACK) *reinterpret_cast<u32x4*>(Q.at(id / RPR, 0) + id % RPR * 16) = q[i];
+            const int id = tid + 256 * i;
+            float x[R];
+            unpack_run<T>(k[i], x);
+            K.put(id / (DK / R), id % (DK / R) * R, x, sk);
+            if constexpr (BACK) {
+                unpack_run<T>(q[i], x);
+                Q.put(id / (DK / R), id % (DK / R) * R, x, sq);
+            }
         }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int id = tid + 256 * i;
+            *reinterpret_cast<u32x4*>(Tm.at(id / NP, 0) + id % NP * 16) = t[i];
+            if constexpr (BACK) *reinterpret_cast<u32x4*>(P.at(id / NP, 0) + id % NP * 16) = pp[i];
+        }
+        if (tid < kVecs) reinterpret_cast<float*>(buf + L::kVec)[tid] = vec;
     }
 };
 
-template <class Op, int DK, bool BACK>
-__device__ __forceinline__ void scan_sequence(const BwdParams& p, State<Op, DK>& S, char* rec, size_t stride, int nc,
-                                              int tile, bool active, int lane, char* lds) {
+template <class Op, typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan_sequence(const BwdParams& p, State<Op, DK>& S, const SeqAt<T>& at, char* rec,
+                                              size_t stride, int nc, int tile, bool active, int lane, char* lds) {
     using L = ScanLds<Op, DK>;
     if (nc == 0) return;
     char* turn = lds + L::kTurnAt + (threadIdx.x >> 6) * L::kTurn;
-    auto at = [&](int c) { return rec + (size_t)(BACK ? nc - 1 - c : c) * stride; };  // c < nc
-    ScanStage<Op, DK, BACK> st;
-    TileInputs<Op, BACK> in;
-    st.load(p, at(0));
-    if (active) in.load(p, at(0), tile, lane);
+    auto chunk = [&](int c) { return BACK ? nc - 1 - min(c, nc - 1) : min(c, nc - 1); };
+    ScanStage<Op, T, DK, VEC, BACK> st;
+    TileRuns<T, VEC> in;
+    st.load(p, at, chunk(0), rec + chunk(0) * stride);
+    if (active) in.load(p, at, chunk(0), tile, lane);
     st.store(lds);
-    st.load(p, at(min(1, nc - 1)));
+    st.load(p, at, chunk(1), rec + chunk(1) * stride);
     __syncthreads();
     for (int c = 0; c < nc; ++c) {
-        char* here = at(c);
         if (active) {
-            const TileInputs<Op, BACK> now = in;
-            in.load(p, at(min(c + 1, nc - 1)), tile, lane);
-            scan_chunk<Op, DK, BACK>(p, S, now, here, lds + (L::kBufs == 2 ? c & 1 : 0) * L::kBuf, turn, tile, lane);
+            const TileRuns<T, VEC> now = in;
+            in.load(p, at, chunk(c + 1), tile, lane);
+            scan_chunk<Op, T, DK, VEC, BACK>(p, S, now, rec + chunk(c) * stride,
+                                             lds + (L::kBufs == 2 ? c & 1 : 0) * L::kBuf, turn, tile, lane);
         }
         if constexpr (L::kBufs == 1) __syncthreads();
         st.store(lds + (L::kBufs == 2 ? (c + 1) & 1 : 0) * L::kBuf);
-        st.load(p, at(min(c + 2, nc - 1)));
+        st.load(p, at, chunk(c + 2), rec + chunk(c + 2) * stride);
         __syncthreads();
     }
 }
 
-template <class Op, int DK>
+template <typename T>
+__device__ __forceinline__ SeqAt<T> seq_at(const BwdParams& p, int seq, int h, bool back) {
+    int t0, t1;
+    seq_bounds(p.cu, seq, p.seq_len, t0, t1);
+    const long rk = ((long)t0 * p.heads + h) * p.d_k, rv = ((long)t0 * p.heads + h) * p.d_v;
+    return {static_cast<const T*>(p.k) + rk, static_cast<const T*>(p.q) + rk,
+            static_cast<const T*>(back ? p.dout : p.v) + rv, t1 - t0};
+}
+
+template <class Op, typename T, int DK, bool VEC>
 __global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int splits) {
     __shared__ __align__(16) char lds[ScanLds<Op, DK>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id = blockIdx.x;
-    const int part = id % splits;
-    id /= splits;
+    // the workgroups that share a (sequence, head, direction) follow each other
+    // on one XCD (blocks go round the eight), whose L2 then serves their K, Q, T
+    // and P
+    const int per = 8 * splits, grp = blockIdx.x / per, in = blockIdx.x - grp * per;
+    const int part = in >> 3;
+    int id = grp * 8 + (in & 7);
     const bool back = id & 1;
     id >>= 1;
+    if (id >= p.batch * p.heads) return;
     const int seq = id / p.heads, h = id - seq * p.heads;
     const int tile = part * 4 + wave;
     const bool active = tile < p.dvt;
@@ -994,13 +977,14 @@ __global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int split
     const size_t stride = (size_t)p.heads * p.rec.bytes;
     const long st = ((long)seq * p.heads + h) * p.d_v * p.d_k;
     const int row = 16 * tile + (lane & 15);
+    const SeqAt<T> at = seq_at<T>(p, seq, h, back);
     State<Op, DK> S;
     if (!back) {
         S.load(p, p.init ? p.init + st : nullptr, row, lane >> 4);
-        scan_sequence<Op, DK, false>(p, S, rec, stride, nc, tile, active, lane, lds);
+        scan_sequence<Op, T, DK, VEC, false>(p, S, at, rec, stride, nc, tile, active, lane, lds);
     } else {
         S.load(p, p.dfinal ? p.dfinal + st : nullptr, row, lane >> 4);
-        scan_sequence<Op, DK, true>(p, S, rec, stride, nc, tile, active, lane, lds);
+        scan_sequence<Op, T, DK, VEC, true>(p, S, at, rec, stride, nc, tile, active, lane, lds);
         if (p.dinit && active) S.store(p, p.dinit + st, row, lane >> 4);
     }
 }
@@ -1047,12 +1031,11 @@ __device__ __forceinline__ f32x4 shift_unit(const f32x4& u, int, int) { return u
 template <class Op, typename T, int DK, bool VEC>
 __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at, int h, const char* rec, char* lds) {
     using Unit = typename Op::Unit;
-    using Elt = typename Op::Elt;
     using L = GradLds<Op, DK>;
     constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK, R = kRun<T>;
     constexpr int NS = (NT * 64 + 255) / 256;      // 16-byte pieces of S0's tile per thread
     constexpr int NO = 64 * L::kTdv / R / 256;     // runs of dO's tile per thread
-    constexpr int NK = 64 * DK * int(sizeof(Elt)) / 16 / 256, RPR = DK * int(sizeof(Elt)) / 16;
+    constexpr int NK = 64 * DK / R / 256;          // runs of K (and of Q) per thread
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
               m = lane & 15;
     const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
@@ -1086,7 +1069,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
 #pragma unroll
         for (int i = 0; i < NOR; ++i) {
             const int id = tid + 256 * i, tk = id / (L::kTdv / R), c = t * L::kTdv + id % (L::kTdv / R) * R;
-            ro[i] = load_run<T, VEC>(op + tk * ldv + c, op, tk < at.n && c < p.d_v, p.d_v - c);
+            ro[i] = load_run<T, VEC>(op + tk * ldv + c, tk < at.n && c < p.d_v, p.d_v - c);
         }
     };
     load_tile(0);
@@ -1222,18 +1205,26 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     }
     // K and Q by rows, where the tiles were
     {
-        u32x4 k[NK], q[NK];
+        const T* kp = static_cast<const T*>(p.k) + ok;
+        const T* qp = static_cast<const T*>(p.q) + ok;
+        u32x4 rk[NK], rq[NK];
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            k[i] = reinterpret_cast<const u32x4*>(rec + p.rec.kf)[tid + 256 * i];
-            q[i] = reinterpret_cast<const u32x4*>(rec + p.rec.qf)[tid + 256 * i];
+            const int id = tid + 256 * i, tk = id / (DK / R), c = id % (DK / R) * R;
+            const bool in = tk < at.n && c < p.d_k;
+            rk[i] = load_run<T, VEC>(kp + tk * ldk + c, in, p.d_k - c);
+            rq[i] = load_run<T, VEC>(qp + tk * ldk + c, in, p.d_k - c);
         }
+        const float sk = exp2i(-ek), sq = exp2i(-eq);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            const int id = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(Kr.at(id / RPR, 0) + id % RPR * 16) = k[i];
-            *reinterpret_cast<u32x4*>(Qr.at(id / RPR, 0) + id % RPR * 16) = q[i];
+            const int id = tid + 256 * i, tk = id / (DK / R), c = id % (DK / R) * R;
+            float x[R];
+            unpack_run<T>(rk[i], x);
+            Kr.put(tk, c, x, sk);
+            unpack_run<T>(rq[i], x);
+            Qr.put(tk, c, x, sq);
         }
     }
 #pragma unroll
@@ -1545,21 +1536,21 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
             return at;
         };
         // forward over chunk c from state S, or back over it from its gradient
-        auto step = [&](auto back, State<OpF32, DK>& S, int tile) {
-            TileInputs<OpF32, back.value> in;
-            in.load(e, rec, tile, lane);
-            scan_chunk<OpF32, DK, back.value>(e, S, in, rec, lds, turn, tile, lane);
+        auto step = [&](auto back, State<OpF32, DK>& S, int c, int tile) {
+            TileRuns<T, VEC> in;
+            in.load(e, seq_at<T>(p, seq, h, back.value), c, tile, lane);
+            scan_chunk<OpF32, T, DK, VEC, back.value>(e, S, in, rec, lds, turn, tile, lane);
         };
-        auto stage = [&](auto back) {
+        auto stage = [&](auto back, int c) {
             __syncthreads();
-            ScanStage<OpF32, DK, back.value> sg;
-            sg.load(e, rec);
+            ScanStage<OpF32, T, DK, VEC, back.value> sg;
+            sg.load(e, seq_at<T>(p, seq, h, back.value), c, rec);
             sg.store(lds);
             __syncthreads();
         };
         for (int c = 0; c < nc; ++c) {
             prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
-            stage(std::false_type{});
+            stage(std::false_type{}, c);
             for (int tile = wave; tile < p.dvt; tile += 4) {
                 char* kept = first + c * stride + p.rec.s0;
                 State<OpF32, DK> S;
@@ -1570,7 +1561,7 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
                     load_state(S, kept, tile, lane);
                 }
                 if (c + 1 < nc) {
-                    step(std::false_type{}, S, tile);
+                    step(std::false_type{}, S, c, tile);
                     store_state(S, kept + stride, tile, lane);
                 }
             }
@@ -1584,17 +1575,17 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
         for (int c = nc - 1; c >= 0; --c) {
             const char* kept = first + c * stride + p.rec.s0;
             prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
-            stage(std::false_type{});
+            stage(std::false_type{}, c);
             for (int tile = wave; tile < p.dvt; tile += 4) {
                 State<OpF32, DK> S;
                 load_state(S, kept, tile, lane);
-                step(std::false_type{}, S, tile);
+                step(std::false_type{}, S, c, tile);
             }
-            stage(std::true_type{});
+            stage(std::true_type{}, c);
             for (int tile = wave; tile < p.dvt; tile += 4) {
                 State<OpF32, DK> S;
                 load_state(S, carry, tile, lane);
-                step(std::true_type{}, S, tile);
+                step(std::true_type{}, S, c, tile);
                 store_state(S, carry, tile, lane);
             }
             __syncthreads();
@@ -1660,7 +1651,7 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     hipError_t e;
     const int64_t grid = chunks * p.heads;
     const int splits = (p.dvt + 3) / 4;
-    const int64_t scans = (int64_t)p.batch * p.heads * 2 * splits;
+    const int64_t scans = ((int64_t)p.batch * p.heads * 2 + 7) / 8 * 8 * splits;
     if ((e = check_grid(grid, 256)) != hipSuccess) return e;
     if ((e = check_grid(scans, 256)) != hipSuccess) return e;
     if (grid > 0) {
@@ -1668,7 +1659,7 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0 || p.dinit) {
-        hipLaunchKernelGGL((bwd_scan_kernel<Op, DK>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
+        hipLaunchKernelGGL((bwd_scan_kernel<Op, T, DK, VEC>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0) {
