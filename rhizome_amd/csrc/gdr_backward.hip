@@ -576,25 +576,30 @@ __global__ __launch_bounds__(256, Op::kScaled ? 3 : 1) void bwd_prep_kernel(BwdP
 }
 
 // ----------------------------------------------------------------- scan
-// Four waves to a workgroup, each carrying 16 rows of S (or of dS) along the
-// chunks of a (sequence, head) in accumulators: tile b holds d_k indices 16 b +
-// 4 g .. + 3 of row m.  The state's own operands come from its accumulators;
-// K, Q, T and P pass through LDS once for the four waves, read from HBM two
-// chunks ahead, and serve as rows and as columns.  What a wave alone reads (its
-// columns of V or dO) and writes (S0, W, dS1, dX in the order the gradients'
-// products take) is turned through a corner of LDS of its own.
+// A wave carries 16 rows of S (or of dS) along the chunks of a (sequence, head)
+// in accumulators: tile b holds d_k indices 16 b + 4 g .. + 3 of row m.  The
+// state's own operands come from its accumulators; K, Q, T and P pass through
+// LDS once for a workgroup's four such waves and serve as rows and as columns.
+// Forward: W = T (V - diag(gamma) K S0^T), S1 = gamma_c S0 + (beta tail W)^T K.
+// Back: dX = T^T (diag(beta) P^T dO + diag(beta tail) K dS1^T), dS0 = gamma_c
+// dS1 + (gamma dO)^T Q - (gamma dX)^T K.  What the gradients need (S0, W, dS1,
+// dX) is turned through LDS into the order that their products take.
 template <class Op, int DK>
-struct ScanLds {
+struct ScanBuf {  // a chunk's shared operands
     static constexpr int kRow = RowMat<Op, DK>::bytes(64), kT64 = RowMat<Op, 64>::bytes(64);
     static constexpr int kK = 0, kT = kRow, kVec = kT + kT64, kQ = kVec + 1024, kP = kQ + kRow;
-    static constexpr int kBuf = kP + kT64;
-    static constexpr int kBufs = Op::kScaled ? 2 : 1;
-    static constexpr int kTurnCols = DK > 64 ? DK : 64;
-    static constexpr int kTurnRows = RowMat<Op, kTurnCols>::bytes(16), kTile = 64 * (16 * int(sizeof(typename Op::Elt)) + 16);
-    static constexpr int kTurn = kTurnRows > kTile ? kTurnRows : kTile;
-    static constexpr int kTurnAt = kBufs * kBuf;
-    static constexpr int kBytes = kTurnAt + 4 * kTurn;
+    static constexpr int kBytes = kP + kT64;
 };
+
+// The exponent of the largest value of a wave's tiles (NaNs do not count).
+template <int N>
+__device__ __forceinline__ int tiles_exp(const f32x4 (&w)[N]) {
+    float mx = 0.f;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(w[b][0])), fabsf(w[b][1])), fmaxf(fabsf(w[b][2]), fabsf(w[b][3])));
+    return bits_exp(wave_max_bits(bits_abs(mx)));
+}
 
 template <class Op, int DK>
 struct State {
@@ -602,13 +607,7 @@ struct State {
     f32x4 s[NT];
     int e;  // the state is s * 2^e, with |s| below 2^15.1: its fp16 operands are s itself
 
-    __device__ __forceinline__ int top() const {  // the exponent of the state's largest value
-        float mx = 0.f;
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-            mx = fmaxf(fmaxf(fmaxf(mx, fabsf(s[b][0])), fabsf(s[b][1])), fmaxf(fabsf(s[b][2]), fabsf(s[b][3])));
-        return bits_exp(bits_abs(wave_max(mx))) + e;
-    }
+    __device__ __forceinline__ int top() const { return tiles_exp<NT>(s) + e; }  // the largest value's exponent
     __device__ __forceinline__ void load(const BwdParams& p, const float* base, int row, int g) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
@@ -679,16 +678,18 @@ struct TileRuns {
         for (int i = 0; i < N; ++i) m = max(m, run_max_bits<T>(r[i]));
         return wave_max_bits(m);
     }
-    // the tokens 16 b + 4 g .. of column m, through the wave's corner of LDS
-    __device__ __forceinline__ void turn(char* corner, f32x4 (&x)[4], int lane) const {
-        using Raw = typename std::conditional<sizeof(T) == 2, OpF16, OpF32>::type;  // 16 bits are moved as such
-        const RowMat<Raw, 16> tn{corner};
+    // through LDS, 16-bit values as they are: rows in, then the tokens 16 b + 4 g .. of column m out
+    using Raw = RowMat<typename std::conditional<sizeof(T) == 2, OpF16, OpF32>::type, 16>;
+    __device__ __forceinline__ void put(char* corner, int lane) const {
+        const Raw tn{corner};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = lane + 64 * i;
             *reinterpret_cast<u32x4*>(tn.at(id / RPR, id % RPR * R)) = r[i];
         }
-        __builtin_amdgcn_wave_barrier();
+    }
+    static __device__ __forceinline__ void get(char* corner, f32x4 (&x)[4], int lane) {
+        const Raw tn{corner};
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             if constexpr (sizeof(T) == 2) {
@@ -699,19 +700,8 @@ struct TileRuns {
                 x[b] = tn.col4(0, b, lane);
             }
         }
-        __builtin_amdgcn_wave_barrier();
     }
 };
-
-// Magnitude bits of the largest of a wave's values; a NaN's are the largest.
-__device__ __forceinline__ int tokens_bits(const f32x4 (&w)[4]) {
-    int mx = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = max(mx, bits_abs(w[b][i]));
-    return wave_max_bits(mx);
-}
 
 // Rows of a wave's tile as units with d_v along the contraction: column tile
 // `b` of the turned matrix to `base` + b KiB, this tile's half of them (fp16:
@@ -723,138 +713,7 @@ __device__ __forceinline__ void store_turned(const Mat& turn, char* base, int ti
     for (int b = 0; b < N; ++b) *reinterpret_cast<typename Op::Quad*>(o + b * 1024) = turn.col4(b, 0, lane);
 }
 
-// One chunk of a wave's rows.  Forward: W = T (V - diag(gamma) K S0^T) and S1 =
-// gamma_c S0 + (beta tail W)^T K.  Back: dX = T^T (diag(beta) P^T dO +
-// diag(beta tail) K dS1^T) and dS0 = gamma_c dS1 + (gamma dO)^T Q - (gamma dX)^T K.
-template <class Op, typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan_chunk(const BwdParams& p, State<Op, DK>& S, const TileRuns<T, VEC>& in, char* rec,
-                                           char* buf, char* turn, int tile, int lane) {
-    using Unit = typename Op::Unit;
-    using L = ScanLds<Op, DK>;
-    constexpr int NT = DK / 16, NBK = Op::kBlocks, NU = NT / NBK, NKT = 4 / NBK;
-    const int g = lane >> 4, m = lane & 15;
-    const RowMat<Op, DK> K{buf + L::kK}, Q{buf + L::kQ};
-    const RowMat<Op, 64> Tm{buf + L::kT}, P{buf + L::kP};
-    const RowMat<Op, L::kTurnCols> tn{turn};
-    const float* vec = reinterpret_cast<const float*>(buf + L::kVec);
-    auto by_token = [&](int v, int b) { return *reinterpret_cast<const f32x4*>(vec + v + 16 * b + 4 * g); };
-    const float gc = vec[kVecGc];
-    int ek = 0, eq = 0;
-    if constexpr (Op::kScaled) {
-        ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
-        eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
-    }
-    f32x4 x[4], w[4], vo[4];
-    in.turn(turn, vo, lane);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-        const Unit su = Op::pack(&S.s[i * NBK], 1.f);
-        tn.put_unit(m, i, g, su);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su, x[b]);
-    }
-    __builtin_amdgcn_wave_barrier();
-    store_turned<Op, NT>(tn, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
-    __builtin_amdgcn_wave_barrier();
-    const int top = Op::kScaled ? S.top() : 0;
-    const float sx = exp2i(S.e + ek);
-    int eo = 0;
-    if constexpr (!BACK) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * (x[b] * sx);
-    } else {
-        if constexpr (Op::kScaled) eo = bits_exp(in.max_bits()) + 2;  // dO below 1/2
-        const float so = exp2i(-eo), sz = exp2i(eo + ek + eq);
-        f32x4 z[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) z[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) {
-            const Unit du = Op::pack(&vo[u * NBK], so);
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (u * NBK + NBK > b) z[b] = Op::mma(P.cols(b, u, lane), du, z[b]);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = by_token(kVecBeta, b) * (z[b] * sz) + by_token(kVecWrite, b) * (x[b] * sx);
-    }
-    // T or T^T times it, the operand below 2^5
-    int er = 0, rbits = 0;
-    if constexpr (Op::kScaled) {
-        rbits = tokens_bits(w);
-        er = bits_exp(rbits) - 4;
-    }
-    {
-        const float sr = exp2i(-er);
-        f32x4 y[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) y[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) {
-            const Unit ru = Op::pack(&w[u * NBK], sr);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                if (!BACK && u * NBK <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), ru, y[b]);
-                if (BACK && u * NBK + NBK > b) y[b] = Op::mma(Tm.cols(b, u, lane), ru, y[b]);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = y[b];
-    }
-    // W is kept with its largest value in [8, 16), dX in [1/4, 1/2)
-    int tw = 0, ew = 0;
-    if constexpr (Op::kScaled) {
-        tw = bits_exp(tokens_bits(w));
-        ew = tw + (BACK ? 2 : -3);
-    }
-    const float si = exp2i(-ew);
-#pragma unroll
-    for (int u = 0; u < NKT; ++u) tn.put_unit(m, u, g, Op::pack(&w[u * NBK], si));
-    __builtin_amdgcn_wave_barrier();
-    store_turned<Op, 4>(tn, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
-    __builtin_amdgcn_wave_barrier();
-    if (Op::kScaled && lane == 0) {
-        int* oe = reinterpret_cast<int*>(rec + p.rec.vec);
-        oe[(BACK ? kExpX : kExpW) + tile] = ew + er;
-        oe[(BACK ? kExpD : kExpS) + tile] = S.e;
-        if constexpr (BACK) oe[kExpO + tile] = eo;
-        if (rbits >= 0x7f800000) oe[kVecBad] = 1;
-    }
-    // the next state in units of 2^e, of the larger of what stays (gamma_c S,
-    // below 2^9 of them) and what is written (each token's value below 2^8, and
-    // 64 tokens' with rows of K or Q below 2: 2^15; back, two such sums of 2^14)
-    int e = 0;
-    if constexpr (Op::kScaled) {
-        e = max(tw + er + ek, top + bits_exp(bits_abs(gc)));
-        if constexpr (BACK) e = max(e, eo - 2 + eq) + 1;
-        e -= 7;
-    }
-    const float sw = BACK ? -exp2i(er + ek - e) : exp2i(er + ek - e), sd = exp2i(eq - e), sg = gc * exp2i(S.e - e);
-    S.e = e;
-#pragma unroll
-    for (int b = 0; b < NT; ++b) S.s[b] *= sg;
-#pragma unroll
-    for (int u = 0; u < NKT; ++u) {
-#pragma unroll
-        for (int b = 0; b < NBK; ++b) {
-            const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u * NBK + b);
-            w[u * NBK + b] *= f;
-            if constexpr (BACK) vo[u * NBK + b] *= f;
-        }
-        const Unit wu = Op::pack(&w[u * NBK], sw);
-#pragma unroll
-        for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
-        if constexpr (BACK) {
-            const Unit du = Op::pack(&vo[u * NBK], sd);
-#pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
-        }
-    }
-}
-
-// A chunk's shared operands on their way from HBM to LDS, by all 256 threads.
+// A chunk's shared operands on their way from HBM to LDS, by 256 threads (`tid`).
 template <class Op, typename T, int DK, bool VEC, bool BACK>
 struct ScanStage {
     static constexpr int R = kRun<T>, N = 64 * DK / R / 256;
@@ -862,8 +721,7 @@ struct ScanStage {
     u32x4 k[N], q[BACK ? N : 1], t[NT], pp[BACK ? NT : 1];
     float vec;
     int ek, eq;
-    __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, const char* rec) {
-        const int tid = threadIdx.x;
+    __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, const char* rec, int tid) {
         const long ld = (long)p.heads * p.d_k;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -885,9 +743,8 @@ struct ScanStage {
             eq = reinterpret_cast<const int*>(v)[kVecEQ];
         }
     }
-    __device__ __forceinline__ void store(char* buf) const {
-        using L = ScanLds<Op, DK>;
-        const int tid = threadIdx.x;
+    __device__ __forceinline__ void store(char* buf, int tid) const {
+        using L = ScanBuf<Op, DK>;
         const RowMat<Op, DK> K{buf + L::kK}, Q{buf + L::kQ};
         const RowMat<Op, 64> Tm{buf + L::kT}, P{buf + L::kP};
         const float sk = exp2i(-ek), sq = exp2i(-eq);
@@ -912,34 +769,6 @@ struct ScanStage {
     }
 };
 
-template <class Op, typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan_sequence(const BwdParams& p, State<Op, DK>& S, const SeqAt<T>& at, char* rec,
-                                              size_t stride, int nc, int tile, bool active, int lane, char* lds) {
-    using L = ScanLds<Op, DK>;
-    if (nc == 0) return;
-    char* turn = lds + L::kTurnAt + (threadIdx.x >> 6) * L::kTurn;
-    auto chunk = [&](int c) { return BACK ? nc - 1 - min(c, nc - 1) : min(c, nc - 1); };
-    ScanStage<Op, T, DK, VEC, BACK> st;
-    TileRuns<T, VEC> in;
-    st.load(p, at, chunk(0), rec + chunk(0) * stride);
-    if (active) in.load(p, at, chunk(0), tile, lane);
-    st.store(lds);
-    st.load(p, at, chunk(1), rec + chunk(1) * stride);
-    __syncthreads();
-    for (int c = 0; c < nc; ++c) {
-        if (active) {
-            const TileRuns<T, VEC> now = in;
-            in.load(p, at, chunk(c + 1), tile, lane);
-            scan_chunk<Op, T, DK, VEC, BACK>(p, S, now, rec + chunk(c) * stride,
-                                             lds + (L::kBufs == 2 ? c & 1 : 0) * L::kBuf, turn, tile, lane);
-        }
-        if constexpr (L::kBufs == 1) __syncthreads();
-        st.store(lds + (L::kBufs == 2 ? (c + 1) & 1 : 0) * L::kBuf);
-        st.load(p, at, chunk(c + 2), rec + chunk(c + 2) * stride);
-        __syncthreads();
-    }
-}
-
 template <typename T>
 __device__ __forceinline__ SeqAt<T> seq_at(const BwdParams& p, int seq, int h, bool back) {
     int t0, t1;
@@ -949,44 +778,373 @@ __device__ __forceinline__ SeqAt<T> seq_at(const BwdParams& p, int seq, int h, b
             static_cast<const T*>(back ? p.dout : p.v) + rv, t1 - t0};
 }
 
-template <class Op, typename T, int DK, bool VEC>
-__global__ __launch_bounds__(256, 1) void bwd_scan_kernel(BwdParams p, int splits) {
-    __shared__ __align__(16) char lds[ScanLds<Op, DK>::kBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // the workgroups that share a (sequence, head, direction) follow each other
-    // on one XCD (blocks go round the eight), whose L2 then serves their K, Q, T
-    // and P
+// The rows that a workgroup of a scan launch carries: the workgroups that share
+// a (sequence, head, direction) follow each other on one XCD (blocks go round
+// the eight), whose L2 then serves their K, Q, T and P.
+struct ScanAt {
+    bool back;
+    int seq, h, part, nc;
+    char* rec;        // the first chunk's record
+    size_t stride;    // from chunk to chunk
+    long state;       // index of the head's state
+};
+__device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& a) {
     const int per = 8 * splits, grp = blockIdx.x / per, in = blockIdx.x - grp * per;
-    const int part = in >> 3;
     int id = grp * 8 + (in & 7);
-    const bool back = id & 1;
+    a.part = in >> 3;
+    a.back = id & 1;
     id >>= 1;
-    if (id >= p.batch * p.heads) return;
-    const int seq = id / p.heads, h = id - seq * p.heads;
-    const int tile = part * 4 + wave;
-    const bool active = tile < p.dvt;
-    int ci, nc;
+    if (id >= p.batch * p.heads) return false;
+    a.seq = id / p.heads;
+    a.h = id - a.seq * p.heads;
+    int ci;
     if (p.cu) {
-        ci = p.chunk_base[seq];
-        nc = p.chunk_base[seq + 1] - ci;
+        ci = p.chunk_base[a.seq];
+        a.nc = p.chunk_base[a.seq + 1] - ci;
     } else {
-        nc = (p.seq_len + C64 - 1) / C64;
-        ci = seq * nc;
+        a.nc = (p.seq_len + C64 - 1) / C64;
+        ci = a.seq * a.nc;
     }
-    char* rec = p.ws + ((size_t)ci * p.heads + h) * p.rec.bytes;
-    const size_t stride = (size_t)p.heads * p.rec.bytes;
-    const long st = ((long)seq * p.heads + h) * p.d_v * p.d_k;
-    const int row = 16 * tile + (lane & 15);
-    const SeqAt<T> at = seq_at<T>(p, seq, h, back);
+    a.rec = p.ws + ((size_t)ci * p.heads + a.h) * p.rec.bytes;
+    a.stride = (size_t)p.heads * p.rec.bytes;
+    a.state = (long)id * p.d_v * p.d_k;
+    return true;
+}
+
+// bf16 tensors, fp16 operands.  A wave's chunk is one chain of LDS reads,
+// products and exponents that a SIMD's single wave cannot fill, so four more
+// waves do what is off it: they read K, Q, T, P and each carrying wave's
+// columns of V or dO two chunks ahead, convert them to LDS one chunk ahead, and
+// turn and store the previous chunk's S0 and W (dS1 and dX).  Two barriers a
+// chunk: A, the buffers of the chunk are full and its predecessor's results lie
+// in LDS; B, these have been read.
+template <int DK>
+struct Scan16Lds {
+    using Buf = ScanBuf<OpF16, DK>;
+    static constexpr int kTile = 64 * 48;                                         // a wave's columns of V or dO
+    static constexpr int kTurnS = RowMat<OpF16, DK>::bytes(16), kTurnW = RowMat<OpF16, 64>::bytes(16);
+    static constexpr int kTiles = 2 * Buf::kBytes, kTurn = kTiles + 8 * kTile, kExps = kTurn + 4 * (kTurnS + kTurnW);
+    static constexpr int kBytes = kExps + 8 * 4;
+};
+
+template <typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a, int tile, int wave, int lane, char* lds) {
+    using Op = OpF16;
+    using Unit = f16x8;
+    using L = Scan16Lds<DK>;
+    using Buf = typename L::Buf;
+    constexpr int NT = DK / 16, NU = NT / 2;
+    const int g = lane >> 4, m = lane & 15, row = 16 * tile + m;
+    const float* from = BACK ? p.dfinal : p.init;
     State<Op, DK> S;
-    if (!back) {
-        S.load(p, p.init ? p.init + st : nullptr, row, lane >> 4);
-        scan_sequence<Op, T, DK, VEC, false>(p, S, at, rec, stride, nc, tile, active, lane, lds);
-    } else {
-        S.load(p, p.dfinal ? p.dfinal + st : nullptr, row, lane >> 4);
-        scan_sequence<Op, T, DK, VEC, true>(p, S, at, rec, stride, nc, tile, active, lane, lds);
-        if (p.dinit && active) S.store(p, p.dinit + st, row, lane >> 4);
+    S.load(p, from ? from + a.state : nullptr, row, g);
+    const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
+    const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
+    for (int c = 0; c < a.nc; ++c) {
+        __syncthreads();  // A
+        char* buf = lds + (c & 1) * Buf::kBytes;
+        const RowMat<Op, DK> K{buf + Buf::kK}, Q{buf + Buf::kQ};
+        const RowMat<Op, 64> Tm{buf + Buf::kT}, P{buf + Buf::kP};
+        const float* vec = reinterpret_cast<const float*>(buf + Buf::kVec);
+        auto by_token = [&](int v, int b) { return *reinterpret_cast<const f32x4*>(vec + v + 16 * b + 4 * g); };
+        const float gc = vec[kVecGc];
+        const int ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
+        const int eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
+        const int eo = BACK ? __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(lds + L::kExps)[(c & 1) * 4 + wave]) : 0;
+        f32x4 x[4], w[4], vo[4];
+        TileRuns<T, VEC>::get(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, vo, lane);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
+        Unit su[NU];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) su[i] = Op::pack(&S.s[i * 2], 1.f);
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su[i], x[b]);
+        const int top = S.top(), se = S.e;
+        const float sx = exp2i(se + ek);
+        if constexpr (!BACK) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * (x[b] * sx);
+        } else {
+            const float so = exp2i(-eo), sz = exp2i(eo + ek + eq);
+            f32x4 z[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) z[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Unit du = Op::pack(&vo[u * 2], so);
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (u * 2 + 2 > b) z[b] = Op::mma(P.cols(b, u, lane), du, z[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[b] = by_token(kVecBeta, b) * (z[b] * sz) + by_token(kVecWrite, b) * (x[b] * sx);
+        }
+        // T or T^T times it, the operand below 2^5
+        const int er = tiles_exp<4>(w) - 4;
+        {
+            const float sr = exp2i(-er);
+            f32x4 y[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) y[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Unit ru = Op::pack(&w[u * 2], sr);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (!BACK && u * 2 <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), ru, y[b]);
+                    if (BACK && u * 2 + 2 > b) y[b] = Op::mma(Tm.cols(b, u, lane), ru, y[b]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[b] = y[b];
+        }
+        // W is kept with its largest value in [8, 16), dX in [1/4, 1/2)
+        const int tx = tiles_exp<4>(w), ew = tx + (BACK ? 2 : -3);
+        if (lane == 0) {
+            int* oe = reinterpret_cast<int*>(a.rec + (BACK ? a.nc - 1 - c : c) * a.stride + p.rec.vec);
+            oe[(BACK ? kExpX : kExpW) + tile] = ew + er;
+            oe[(BACK ? kExpD : kExpS) + tile] = se;
+            if constexpr (BACK) oe[kExpO + tile] = eo;
+        }
+        __syncthreads();  // B
+        const float si = exp2i(-ew);
+#pragma unroll
+        for (int i = 0; i < NU; ++i) ts.put_unit(m, i, g, su[i]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) tw.put_unit(m, u, g, Op::pack(&w[u * 2], si));
+        // the next state in units of 2^e, of the larger of what stays (gamma_c S,
+        // below 2^9 of them) and what is written (each token's value below 2^8, and
+        // 64 tokens' with rows of K or Q below 2: 2^15; back, two such sums of 2^14)
+        int e = max(tx + er + ek, top + bits_exp(bits_abs(gc)));
+        if constexpr (BACK) e = max(e, eo - 2 + eq) + 1;
+        e -= 7;
+        const float sw = BACK ? -exp2i(er + ek - e) : exp2i(er + ek - e), sd = exp2i(eq - e), sg = gc * exp2i(se - e);
+        S.e = e;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) S.s[b] *= sg;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u * 2 + b);
+                w[u * 2 + b] *= f;
+                if constexpr (BACK) vo[u * 2 + b] *= f;
+            }
+            const Unit wu = Op::pack(&w[u * 2], sw);
+#pragma unroll
+            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
+            if constexpr (BACK) {
+                const Unit du = Op::pack(&vo[u * 2], sd);
+#pragma unroll
+                for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
+            }
+        }
     }
+    __syncthreads();  // the last chunk's results lie in LDS
+    // a value that is not finite, or a product out of fp16's range, anywhere on
+    // the way is in the state still (0 times it is NaN): the head is done again
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad = bad || !(fabsf(S.s[b][i]) < INFINITY);
+    if (bad && a.nc > 0) reinterpret_cast<int*>(a.rec + p.rec.vec)[kVecBad] = 1;
+    if (BACK && p.dinit) S.store(p, p.dinit + a.state, row, g);
+}
+
+template <typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a, int tile, int wave, int lane, char* lds) {
+    using Op = OpF16;
+    using L = Scan16Lds<DK>;
+    constexpr int NT = DK / 16;
+    const int tid = wave * 64 + lane;
+    const bool active = tile < p.dvt;
+    const SeqAt<T> at = seq_at<T>(p, a.seq, a.h, BACK);
+    const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
+    const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
+    auto chunk = [&](int c) { return BACK ? a.nc - 1 - min(c, a.nc - 1) : min(c, a.nc - 1); };
+    ScanStage<Op, T, DK, VEC, BACK> st;
+    TileRuns<T, VEC> in;
+    auto load = [&](int c) {
+        st.load(p, at, chunk(c), a.rec + chunk(c) * a.stride, tid);
+        if (active) in.load(p, at, chunk(c), tile, lane);
+    };
+    auto store = [&](int c) {
+        st.store(lds + (c & 1) * L::Buf::kBytes, tid);
+        if (active) {
+            in.put(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, lane);
+            if constexpr (BACK) {  // dO below 1/2
+                const int e = bits_exp(in.max_bits()) + 2;
+                if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[(c & 1) * 4 + wave] = e;
+            }
+        }
+    };
+    auto results = [&](int c) {
+        char* rec = a.rec + chunk(c) * a.stride;
+        if (!active) return;
+        store_turned<Op, NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
+        store_turned<Op, 4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
+    };
+    if (a.nc > 0) {
+        load(0);
+        store(0);
+        load(1);
+    }
+    for (int c = 0; c < a.nc; ++c) {
+        __syncthreads();  // A
+        if (c > 0) results(c - 1);
+        if (c + 1 < a.nc) {
+            store(c + 1);
+            load(c + 2);
+        }
+        __syncthreads();  // B
+    }
+    __syncthreads();
+    if (a.nc > 0) results(a.nc - 1);
+}
+
+template <typename T, int DK, bool VEC>
+__global__ __launch_bounds__(512) void bwd_scan16_kernel(BwdParams p, int splits) {
+    __shared__ __align__(16) char lds[Scan16Lds<DK>::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    ScanAt a;
+    if (!scan_at(p, splits, a)) return;
+    const int tile = a.part * 4 + (wave & 3);
+    if (wave >= 4) {
+        if (a.back) scan16_serve<T, DK, VEC, true>(p, a, tile, wave - 4, lane, lds);
+        else scan16_serve<T, DK, VEC, false>(p, a, tile, wave - 4, lane, lds);
+    } else if (tile < p.dvt) {
+        if (a.back) scan16_carry<T, DK, VEC, true>(p, a, tile, wave, lane, lds);
+        else scan16_carry<T, DK, VEC, false>(p, a, tile, wave, lane, lds);
+    } else {  // no rows: the barriers alone
+        for (int c = 0; c < 2 * a.nc + 1; ++c) __syncthreads();
+    }
+}
+
+// fp32 operands: bound by the fp32 matrix rate, four waves that each do the
+// whole of it, the next chunk's shared operands in registers meanwhile.
+template <int DK>
+struct Scan32Lds {
+    using Buf = ScanBuf<OpF32, DK>;
+    static constexpr int kTurnCols = DK > 64 ? DK : 64;
+    static constexpr int kTurnRows = RowMat<OpF32, kTurnCols>::bytes(16), kTile = 64 * 80;
+    static constexpr int kTurn = kTurnRows > kTile ? kTurnRows : kTile;
+    static constexpr int kTurnAt = Buf::kBytes, kBytes = kTurnAt + 4 * kTurn;
+};
+
+template <typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan32_chunk(const BwdParams& p, State<OpF32, DK>& S, const TileRuns<T, VEC>& in, char* rec,
+                                             char* buf, char* turn, int tile, int lane) {
+    using Op = OpF32;
+    using Unit = f32x4;
+    using Buf = ScanBuf<Op, DK>;
+    constexpr int NT = DK / 16;
+    const int g = lane >> 4, m = lane & 15;
+    const RowMat<Op, DK> K{buf + Buf::kK}, Q{buf + Buf::kQ};
+    const RowMat<Op, 64> Tm{buf + Buf::kT}, P{buf + Buf::kP};
+    const RowMat<Op, Scan32Lds<DK>::kTurnCols> tn{turn};
+    const float* vec = reinterpret_cast<const float*>(buf + Buf::kVec);
+    auto by_token = [&](int v, int b) { return *reinterpret_cast<const f32x4*>(vec + v + 16 * b + 4 * g); };
+    const float gc = vec[kVecGc];
+    f32x4 x[4], w[4], y[4], vo[4];
+    in.put(turn, lane);
+    __builtin_amdgcn_wave_barrier();
+    TileRuns<T, VEC>::get(turn, vo, lane);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int b = 0; b < 4; ++b) x[b] = y[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        tn.put_unit(m, i, g, S.s[i]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), S.s[i], x[b]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    store_turned<Op, NT>(tn, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
+    __builtin_amdgcn_wave_barrier();
+    if constexpr (!BACK) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * x[b];
+    } else {
+        f32x4 z[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            z[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = b; u < 4; ++u) z[b] = Op::mma(P.cols(b, u, lane), vo[u], z[b]);
+            w[b] = by_token(kVecBeta, b) * z[b] + by_token(kVecWrite, b) * x[b];
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (!BACK && u <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), w[u], y[b]);
+            if (BACK && u >= b) y[b] = Op::mma(Tm.cols(b, u, lane), w[u], y[b]);
+        }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) tn.put_unit(m, u, g, y[u]);
+    __builtin_amdgcn_wave_barrier();
+    store_turned<Op, 4>(tn, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int b = 0; b < NT; ++b) S.s[b] *= gc;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u);
+        const Unit wu = BACK ? -y[u] * f : y[u] * f;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
+        if constexpr (BACK) {
+            const Unit du = vo[u] * f;
+#pragma unroll
+            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
+        }
+    }
+}
+
+template <typename T, int DK, bool VEC, bool BACK>
+__device__ __forceinline__ void scan32(const BwdParams& p, const ScanAt& a, int tile, int lane, char* lds) {
+    using L = Scan32Lds<DK>;
+    const bool active = tile < p.dvt;
+    const int row = 16 * tile + (lane & 15);
+    const float* from = BACK ? p.dfinal : p.init;
+    const SeqAt<T> at = seq_at<T>(p, a.seq, a.h, BACK);
+    State<OpF32, DK> S;
+    S.load(p, from ? from + a.state : nullptr, row, lane >> 4);
+    char* turn = lds + L::kTurnAt + (threadIdx.x >> 6) * L::kTurn;
+    auto chunk = [&](int c) { return BACK ? a.nc - 1 - min(c, a.nc - 1) : min(c, a.nc - 1); };
+    ScanStage<OpF32, T, DK, VEC, BACK> st;
+    TileRuns<T, VEC> in;
+    if (a.nc > 0) {
+        st.load(p, at, chunk(0), a.rec + chunk(0) * a.stride, threadIdx.x);
+        if (active) in.load(p, at, chunk(0), tile, lane);
+    }
+    for (int c = 0; c < a.nc; ++c) {
+        st.store(lds, threadIdx.x);
+        st.load(p, at, chunk(c + 1), a.rec + chunk(c + 1) * a.stride, threadIdx.x);
+        __syncthreads();
+        if (active) {
+            const TileRuns<T, VEC> now = in;
+            in.load(p, at, chunk(c + 1), tile, lane);
+            scan32_chunk<T, DK, VEC, BACK>(p, S, now, a.rec + chunk(c) * a.stride, lds, turn, tile, lane);
+        }
+        __syncthreads();
+    }
+    if (BACK && p.dinit && active) S.store(p, p.dinit + a.state, row, lane >> 4);
+}
+
+template <typename T, int DK, bool VEC>
+__global__ __launch_bounds__(256, 1) void bwd_scan32_kernel(BwdParams p, int splits) {
+    __shared__ __align__(16) char lds[Scan32Lds<DK>::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    ScanAt a;
+    if (!scan_at(p, splits, a)) return;
+    if (a.back) scan32<T, DK, VEC, true>(p, a, a.part * 4 + wave, lane, lds);
+    else scan32<T, DK, VEC, false>(p, a, a.part * 4 + wave, lane, lds);
 }
 
 // ----------------------------------------------------------------- grad
@@ -1500,7 +1658,7 @@ __host__ __device__ inline size_t exact_scratch(int DK, int dvt) {
 
 template <typename T, int DK, bool VEC>
 __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* scratch) {
-    using L = ScanLds<OpF32, DK>;
+    using L = Scan32Lds<DK>;
     constexpr int kPrep = PrepLds<OpF32, DK>::kBytes, kGrad = GradLds<OpF32, DK>::kBytes;
     __shared__ __align__(16) char lds[std::max(std::max(kPrep, kGrad), L::kBytes)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15,
@@ -1539,13 +1697,13 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
         auto step = [&](auto back, State<OpF32, DK>& S, int c, int tile) {
             TileRuns<T, VEC> in;
             in.load(e, seq_at<T>(p, seq, h, back.value), c, tile, lane);
-            scan_chunk<OpF32, T, DK, VEC, back.value>(e, S, in, rec, lds, turn, tile, lane);
+            scan32_chunk<T, DK, VEC, back.value>(e, S, in, rec, lds, turn, tile, lane);
         };
         auto stage = [&](auto back, int c) {
             __syncthreads();
             ScanStage<OpF32, T, DK, VEC, back.value> sg;
-            sg.load(e, seq_at<T>(p, seq, h, back.value), c, rec);
-            sg.store(lds);
+            sg.load(e, seq_at<T>(p, seq, h, back.value), c, rec, threadIdx.x);
+            sg.store(lds, threadIdx.x);
             __syncthreads();
         };
         for (int c = 0; c < nc; ++c) {
@@ -1653,13 +1811,16 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     const int splits = (p.dvt + 3) / 4;
     const int64_t scans = ((int64_t)p.batch * p.heads * 2 + 7) / 8 * 8 * splits;
     if ((e = check_grid(grid, 256)) != hipSuccess) return e;
-    if ((e = check_grid(scans, 256)) != hipSuccess) return e;
+    if ((e = check_grid(scans, 512)) != hipSuccess) return e;
     if (grid > 0) {
         hipLaunchKernelGGL((bwd_prep_kernel<Op, T, DK, VEC>), dim3((unsigned)grid), dim3(256), 0, st, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0 || p.dinit) {
-        hipLaunchKernelGGL((bwd_scan_kernel<Op, T, DK, VEC>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
+        if constexpr (Op::kScaled)
+            hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(512), 0, st, p, splits);
+        else
+            hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0) {
