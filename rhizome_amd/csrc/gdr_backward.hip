@@ -608,10 +608,10 @@ struct State {
     int e;  // the state is s * 2^e, with |s| below 2^15.1: its fp16 operands are s itself
 
     __device__ __forceinline__ int top() const { return tiles_exp<NT>(s) + e; }  // the largest value's exponent
-    __device__ __forceinline__ void load(const BwdParams& p, const float* base, int row, int g) {
+    __device__ __forceinline__ void load(const BwdParams& p, const float* base, int row, int c0) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            const int c = 16 * b + 4 * g;
+            const int c = c0 + 16 * b;
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[b][i] = 0.f;
             if (base && row < p.d_v && c < p.d_k) {
@@ -633,12 +633,12 @@ struct State {
             for (int b = 0; b < NT; ++b) s[b] *= f;
         }
     }
-    __device__ __forceinline__ void store(const BwdParams& p, float* base, int row, int g) const {
+    __device__ __forceinline__ void store(const BwdParams& p, float* base, int row, int c0) const {
         if (row >= p.d_v) return;
         const float f = exp2i(e);
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            const int c = 16 * b + 4 * g;
+            const int c = c0 + 16 * b;
             if (c >= p.d_k) continue;
             float* r = base + (long)row * p.d_k + c;
             if (p.vec_s) {
@@ -659,17 +659,18 @@ struct SeqAt {
     int tokens;
 };
 
-// A wave's 16 columns of V (or dO) of a chunk, as the rows come from HBM.
-template <typename T, bool VEC>
+// 16 columns of V (or dO) of a chunk, as the rows come from HBM to `THREADS`
+// threads; `lane` counts them.
+template <typename T, bool VEC, int THREADS = 64>
 struct TileRuns {
-    static constexpr int R = kRun<T>, N = 64 * 16 / R / 64, RPR = 16 / R;
+    static constexpr int R = kRun<T>, RUNS = 64 * 16 / R, N = (RUNS + THREADS - 1) / THREADS, RPR = 16 / R;
     u32x4 r[N];
     __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, int tile, int lane) {
         const long ld = (long)p.heads * p.d_v;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = lane + 64 * i, t = c * C64 + id / RPR, col = 16 * tile + id % RPR * R;
-            r[i] = load_run<T, VEC>(at.vo + t * ld + col, t < at.tokens && col < p.d_v, p.d_v - col);
+            r[i] = load_run<T, VEC>(at.vo + t * ld + col, id < RUNS && t < at.tokens && col < p.d_v, p.d_v - col);
         }
     }
     __device__ __forceinline__ int max_bits() const {
@@ -685,7 +686,7 @@ struct TileRuns {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = lane + 64 * i;
-            *reinterpret_cast<u32x4*>(tn.at(id / RPR, id % RPR * R)) = r[i];
+            if (id < RUNS) *reinterpret_cast<u32x4*>(tn.at(id / RPR, id % RPR * R)) = r[i];
         }
     }
     static __device__ __forceinline__ void get(char* corner, f32x4 (&x)[4], int lane) {
@@ -704,20 +705,20 @@ struct TileRuns {
 };
 
 // Rows of a wave's tile as units with d_v along the contraction: column tile
-// `b` of the turned matrix to `base` + b KiB, this tile's half of them (fp16:
-// a unit holds two tiles).
-template <class Op, int N, class Mat>
+// `b` of the turned matrix to `base` + b KiB, this tile's half of them (a unit
+// holds two tiles).
+template <int N, class Mat>
 __device__ __forceinline__ void store_turned(const Mat& turn, char* base, int tile, int lane) {
-    char* o = base + (Op::kScaled ? (tile >> 1) * N * 1024 + (tile & 1) * 8 : tile * N * 1024) + lane * 16;
+    char* o = base + (tile >> 1) * N * 1024 + (tile & 1) * 8 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < N; ++b) *reinterpret_cast<typename Op::Quad*>(o + b * 1024) = turn.col4(b, 0, lane);
+    for (int b = 0; b < N; ++b) *reinterpret_cast<f16x4*>(o + b * 1024) = turn.col4(b, 0, lane);
 }
 
-// A chunk's shared operands on their way from HBM to LDS, by 256 threads (`tid`).
-template <class Op, typename T, int DK, bool VEC, bool BACK>
+// A chunk's shared operands on their way from HBM to LDS, by `THREADS` threads.
+template <class Op, typename T, int DK, bool VEC, bool BACK, int THREADS = 256>
 struct ScanStage {
-    static constexpr int R = kRun<T>, N = 64 * DK / R / 256;
-    static constexpr int NP = 64 * int(sizeof(typename Op::Elt)) / 16, NT = 64 * NP / 256;
+    static constexpr int R = kRun<T>, N = 64 * DK / R / THREADS;
+    static constexpr int NP = 64 * int(sizeof(typename Op::Elt)) / 16, NT = 64 * NP / THREADS;
     u32x4 k[N], q[BACK ? N : 1], t[NT], pp[BACK ? NT : 1];
     float vec;
     int ek, eq;
@@ -725,15 +726,15 @@ struct ScanStage {
         const long ld = (long)p.heads * p.d_k;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = tid + 256 * i, tk = c * C64 + id / (DK / R), col = id % (DK / R) * R;
+            const int id = tid + THREADS * i, tk = c * C64 + id / (DK / R), col = id % (DK / R) * R;
             const bool in = tk < at.tokens && col < p.d_k;
             k[i] = load_run<T, VEC>(at.k + tk * ld + col, in, p.d_k - col);
             if constexpr (BACK) q[i] = load_run<T, VEC>(at.q + tk * ld + col, in, p.d_k - col);
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            t[i] = reinterpret_cast<const u32x4*>(rec + p.rec.t)[tid + 256 * i];
-            if constexpr (BACK) pp[i] = reinterpret_cast<const u32x4*>(rec + p.rec.p)[tid + 256 * i];
+            t[i] = reinterpret_cast<const u32x4*>(rec + p.rec.t)[tid + THREADS * i];
+            if constexpr (BACK) pp[i] = reinterpret_cast<const u32x4*>(rec + p.rec.p)[tid + THREADS * i];
         }
         const float* v = reinterpret_cast<const float*>(rec + p.rec.vec);
         vec = v[min(tid, kVecs - 1)];
@@ -750,7 +751,7 @@ struct ScanStage {
         const float sk = exp2i(-ek), sq = exp2i(-eq);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = tid + 256 * i;
+            const int id = tid + THREADS * i;
             float x[R];
             unpack_run<T>(k[i], x);
             K.put(id / (DK / R), id % (DK / R) * R, x, sk);
@@ -761,7 +762,7 @@ struct ScanStage {
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const int id = tid + 256 * i;
+            const int id = tid + THREADS * i;
             *reinterpret_cast<u32x4*>(Tm.at(id / NP, 0) + id % NP * 16) = t[i];
             if constexpr (BACK) *reinterpret_cast<u32x4*>(P.at(id / NP, 0) + id % NP * 16) = pp[i];
         }
@@ -837,7 +838,7 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
     const int g = lane >> 4, m = lane & 15, row = 16 * tile + m;
     const float* from = BACK ? p.dfinal : p.init;
     State<Op, DK> S;
-    S.load(p, from ? from + a.state : nullptr, row, g);
+    S.load(p, from ? from + a.state : nullptr, row, 4 * g);
     const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
     const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
     for (int c = 0; c < a.nc; ++c) {
@@ -952,7 +953,7 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
 #pragma unroll
         for (int i = 0; i < 4; ++i) bad = bad || !(fabsf(S.s[b][i]) < INFINITY);
     if (bad && a.nc > 0) reinterpret_cast<int*>(a.rec + p.rec.vec)[kVecBad] = 1;
-    if (BACK && p.dinit) S.store(p, p.dinit + a.state, row, g);
+    if (BACK && p.dinit) S.store(p, p.dinit + a.state, row, 4 * g);
 }
 
 template <typename T, int DK, bool VEC, bool BACK>
@@ -985,8 +986,8 @@ __device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a
     auto results = [&](int c) {
         char* rec = a.rec + chunk(c) * a.stride;
         if (!active) return;
-        store_turned<Op, NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
-        store_turned<Op, 4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
+        store_turned<NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
+        store_turned<4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
     };
     if (a.nc > 0) {
         load(0);
@@ -1026,125 +1027,133 @@ __global__ __launch_bounds__(512) void bwd_scan16_kernel(BwdParams p, int splits
 
 // fp32 operands: bound by the fp32 matrix rate, four waves that each do the
 // whole of it, the next chunk's shared operands in registers meanwhile.
-template <int DK>
+// fp32.  An fp32 product takes its SIMD 16 times as long as an fp16 one, and few
+// heads leave most SIMDs idle, so a tile has four waves: each owns a quarter of
+// the state's columns (its update, 1/4 of the products) and a block of 16 tokens
+// (x, w and y), and they exchange state, w and y through LDS.  2 x 1003 tokens, 8
+// heads, d = 64: 53 us, where one wave a tile took 106.
+template <int DK, int TILES>
 struct Scan32Lds {
     using Buf = ScanBuf<OpF32, DK>;
-    static constexpr int kTurnCols = DK > 64 ? DK : 64;
-    static constexpr int kTurnRows = RowMat<OpF32, kTurnCols>::bytes(16), kTile = 64 * 80;
-    static constexpr int kTurn = kTurnRows > kTile ? kTurnRows : kTile;
-    static constexpr int kTurnAt = Buf::kBytes, kBytes = kTurnAt + 4 * kTurn;
+    static constexpr int kTile = RowMat<OpF32, 16>::bytes(64), kW = RowMat<OpF32, 64>::bytes(16);
+    static constexpr int kS = RowMat<OpF32, DK>::bytes(16);
+    // by tile: its columns of V or dO, which y overlays, then w and the state
+    static constexpr int kWAt = std::max(kTile, kW), kSAt = kWAt + kW, kEach = kSAt + kS;
+    static constexpr int kTiles = Buf::kBytes, kBytes = kTiles + TILES * kEach;
 };
+// d_k columns of the state that one of a tile's four waves carries
+template <int DK>
+constexpr int kOwn = DK > 64 ? DK / 4 : 16;
 
-template <typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan32_chunk(const BwdParams& p, State<OpF32, DK>& S, const TileRuns<T, VEC>& in, char* rec,
-                                             char* buf, char* turn, int tile, int lane) {
+// One chunk of a tile, by its four waves (`w`); every wave of the workgroup
+// calls it.  The operands, the tile's columns of V or dO and its state lie in
+// LDS, behind a barrier.
+template <typename T, int DK, int TILES, bool BACK>
+__device__ __forceinline__ void scan32_chunk(const BwdParams& p, State<OpF32, kOwn<DK>>& S, char* rec, char* buf,
+                                             char* mine, int tile, int w, int lane) {
     using Op = OpF32;
-    using Unit = f32x4;
-    using Buf = ScanBuf<Op, DK>;
-    constexpr int NT = DK / 16;
+    using L = Scan32Lds<DK, TILES>;
+    using Buf = typename L::Buf;
+    constexpr int NT = DK / 16, NO = kOwn<DK> / 16;
     const int g = lane >> 4, m = lane & 15;
-    const RowMat<Op, DK> K{buf + Buf::kK}, Q{buf + Buf::kQ};
-    const RowMat<Op, 64> Tm{buf + Buf::kT}, P{buf + Buf::kP};
-    const RowMat<Op, Scan32Lds<DK>::kTurnCols> tn{turn};
+    const bool own = w * NO < NT;
+    const RowMat<Op, DK> K{buf + Buf::kK}, Q{buf + Buf::kQ}, turn_s{mine + L::kSAt};
+    const RowMat<Op, 64> Tm{buf + Buf::kT}, P{buf + Buf::kP}, turn_w{mine + L::kWAt}, turn_y{mine};
     const float* vec = reinterpret_cast<const float*>(buf + Buf::kVec);
     auto by_token = [&](int v, int b) { return *reinterpret_cast<const f32x4*>(vec + v + 16 * b + 4 * g); };
-    const float gc = vec[kVecGc];
-    f32x4 x[4], w[4], y[4], vo[4];
-    in.put(turn, lane);
-    __builtin_amdgcn_wave_barrier();
-    TileRuns<T, VEC>::get(turn, vo, lane);
-    __builtin_amdgcn_wave_barrier();
+    // column tiles of a turned matrix to the record, `n` of them from `first`
+    auto keep = [&](const auto& turn, char* base, int tiles, int first, int n) {
+        char* o = base + ((size_t)tile * tiles + first) * 1024 + lane * 16;
+        for (int b = 0; b < n; ++b) *reinterpret_cast<f32x4*>(o + b * 1024) = turn.col4(first + b, 0, lane);
+    };
+    f32x4 vo[4], x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+    TileRuns<T, true>::get(mine, vo, lane);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = y[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        tn.put_unit(m, i, g, S.s[i]);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), S.s[i], x[b]);
-    }
-    __builtin_amdgcn_wave_barrier();
-    store_turned<Op, NT>(tn, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
-    __builtin_amdgcn_wave_barrier();
+    for (int i = 0; i < NT; ++i) x = Op::mma(K.blocks(16 * w + m, i, g), turn_s.blocks(m, i, g), x);
+    if (own) keep(turn_s, rec + (BACK ? p.rec.ds1 : p.rec.s0), NT, w * NO, NO);
     if constexpr (!BACK) {
+        f32x4 v = vo[0];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * x[b];
+        for (int u = 1; u < 4; ++u) v = w == u ? vo[u] : v;
+        x = v - by_token(kVecGamma, w) * x;
     } else {
-        f32x4 z[4];
+        f32x4 z = {0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            z[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int u = b; u < 4; ++u) z[b] = Op::mma(P.cols(b, u, lane), vo[u], z[b]);
-            w[b] = by_token(kVecBeta, b) * z[b] + by_token(kVecWrite, b) * x[b];
-        }
+        for (int u = 0; u < 4; ++u)
+            if (u >= w) z = Op::mma(P.cols(w, u, lane), vo[u], z);
+        x = by_token(kVecBeta, w) * z + by_token(kVecWrite, w) * x;
     }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (!BACK && u <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), w[u], y[b]);
-            if (BACK && u >= b) y[b] = Op::mma(Tm.cols(b, u, lane), w[u], y[b]);
-        }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) tn.put_unit(m, u, g, y[u]);
-    __builtin_amdgcn_wave_barrier();
-    store_turned<Op, 4>(tn, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int b = 0; b < NT; ++b) S.s[b] *= gc;
+    turn_w.put_unit(m, w, g, x);
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u);
-        const Unit wu = BACK ? -y[u] * f : y[u] * f;
+        if (!BACK && u <= w) y = Op::mma(Tm.blocks(16 * w + m, u, g), turn_w.blocks(m, u, g), y);
+        if (BACK && u >= w) y = Op::mma(Tm.cols(w, u, lane), turn_w.blocks(m, u, g), y);
+    }
+    turn_y.put_unit(m, w, g, y);
+    __syncthreads();
+    keep(turn_y, rec + (BACK ? p.rec.x : p.rec.w), 4, w, 1);
+    if (!own) return;
+    const float gc = vec[kVecGc];
 #pragma unroll
-        for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
+    for (int b = 0; b < NO; ++b) S.s[b] *= gc;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u), yu = turn_y.blocks(m, u, g);
+        const f32x4 wu = BACK ? -yu * f : yu * f, du = vo[u] * f;
+#pragma unroll
+        for (int b = 0; b < NO; ++b) S.s[b] = Op::mma(K.cols(w * NO + b, u, lane), wu, S.s[b]);
         if constexpr (BACK) {
-            const Unit du = vo[u] * f;
 #pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
+            for (int b = 0; b < NO; ++b) S.s[b] = Op::mma(Q.cols(w * NO + b, u, lane), du, S.s[b]);
         }
     }
+#pragma unroll
+    for (int b = 0; b < NO; ++b) turn_s.put_unit(m, w * NO + b, g, S.s[b]);
 }
 
-template <typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan32(const BwdParams& p, const ScanAt& a, int tile, int lane, char* lds) {
-    using L = Scan32Lds<DK>;
-    const bool active = tile < p.dvt;
-    const int row = 16 * tile + (lane & 15);
+template <typename T, int DK, bool VEC, int TILES, bool BACK>
+__device__ __forceinline__ void scan32(const BwdParams& p, const ScanAt& a, char* lds) {
+    using L = Scan32Lds<DK, TILES>;
+    constexpr int NO = kOwn<DK> / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, g = lane >> 4;
+    const int tile = a.part * TILES + (wave >> 2), row = 16 * tile + (lane & 15), c0 = kOwn<DK> * w + 4 * g;
+    const bool own = w * NO < DK / 16;
     const float* from = BACK ? p.dfinal : p.init;
     const SeqAt<T> at = seq_at<T>(p, a.seq, a.h, BACK);
-    State<OpF32, DK> S;
-    S.load(p, from ? from + a.state : nullptr, row, lane >> 4);
-    char* turn = lds + L::kTurnAt + (threadIdx.x >> 6) * L::kTurn;
+    char* mine = lds + L::kTiles + (wave >> 2) * L::kEach;
+    State<OpF32, kOwn<DK>> S;
+    S.load(p, from ? from + a.state : nullptr, row, c0);
+    const RowMat<OpF32, DK> turn_s{mine + L::kSAt};
+    if (own)
+#pragma unroll
+        for (int b = 0; b < NO; ++b) turn_s.put_unit(lane & 15, w * NO + b, g, S.s[b]);
     auto chunk = [&](int c) { return BACK ? a.nc - 1 - min(c, a.nc - 1) : min(c, a.nc - 1); };
-    ScanStage<OpF32, T, DK, VEC, BACK> st;
-    TileRuns<T, VEC> in;
+    ScanStage<OpF32, T, DK, VEC, BACK, 256 * TILES> st;
+    TileRuns<T, VEC, 256> in;
     if (a.nc > 0) {
         st.load(p, at, chunk(0), a.rec + chunk(0) * a.stride, threadIdx.x);
-        if (active) in.load(p, at, chunk(0), tile, lane);
+        in.load(p, at, chunk(0), tile, threadIdx.x & 255);
     }
     for (int c = 0; c < a.nc; ++c) {
         st.store(lds, threadIdx.x);
-        st.load(p, at, chunk(c + 1), a.rec + chunk(c + 1) * a.stride, threadIdx.x);
+        in.put(mine, threadIdx.x & 255);
         __syncthreads();
-        if (active) {
-            const TileRuns<T, VEC> now = in;
-            in.load(p, at, chunk(c + 1), tile, lane);
-            scan32_chunk<T, DK, VEC, BACK>(p, S, now, a.rec + chunk(c) * a.stride, lds, turn, tile, lane);
-        }
+        st.load(p, at, chunk(c + 1), a.rec + chunk(c + 1) * a.stride, threadIdx.x);
+        in.load(p, at, chunk(c + 1), tile, threadIdx.x & 255);
+        scan32_chunk<T, DK, TILES, BACK>(p, S, a.rec + chunk(c) * a.stride, lds, mine, tile, w, lane);
         __syncthreads();
     }
-    if (BACK && p.dinit && active) S.store(p, p.dinit + a.state, row, lane >> 4);
+    if (BACK && p.dinit && own) S.store(p, p.dinit + a.state, row, c0);
 }
 
-template <typename T, int DK, bool VEC>
-__global__ __launch_bounds__(256, 1) void bwd_scan32_kernel(BwdParams p, int splits) {
-    __shared__ __align__(16) char lds[Scan32Lds<DK>::kBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <typename T, int DK, bool VEC, int TILES>
+__global__ __launch_bounds__(256 * TILES) void bwd_scan32_kernel(BwdParams p, int splits) {
+    __shared__ __align__(16) char lds[Scan32Lds<DK, TILES>::kBytes];
     ScanAt a;
     if (!scan_at(p, splits, a)) return;
-    if (a.back) scan32<T, DK, VEC, true>(p, a, a.part * 4 + wave, lane, lds);
-    else scan32<T, DK, VEC, false>(p, a, a.part * 4 + wave, lane, lds);
+    if (a.back) scan32<T, DK, VEC, TILES, true>(p, a, lds);
+    else scan32<T, DK, VEC, TILES, false>(p, a, lds);
 }
 
 // ----------------------------------------------------------------- grad
@@ -1639,18 +1648,9 @@ __global__ __launch_bounds__(256, Op::kScaled ? 2 : 1) void bwd_grad_kernel(BwdP
 // states before the chunks are kept in fp32 where the records' S0 and dS1 were
 // (the same bytes), and everything else of the present chunk in the
 // workgroup's own scratch: a record of fp32 units and the state's gradient.
-template <class Op, int DK>
-__device__ __forceinline__ void load_state(State<Op, DK>& S, const char* base, int tile, int lane) {
-    const f32x4* b = reinterpret_cast<const f32x4*>(base) + (size_t)tile * (DK / 16) * 64 + lane;
-#pragma unroll
-    for (int i = 0; i < DK / 16; ++i) S.s[i] = b[i * 64];
-    S.e = 0;
-}
-template <class Op, int DK>
-__device__ __forceinline__ void store_state(const State<Op, DK>& S, char* base, int tile, int lane) {
-    f32x4* b = reinterpret_cast<f32x4*>(base) + (size_t)tile * (DK / 16) * 64 + lane;
-#pragma unroll
-    for (int i = 0; i < DK / 16; ++i) b[i * 64] = S.s[i];
+template <int DK>
+__device__ __forceinline__ f32x4* kept_state(char* base, int tile, int w, int lane) {
+    return reinterpret_cast<f32x4*>(base) + ((size_t)tile * (DK / 16) + w * (kOwn<DK> / 16)) * 64 + lane;
 }
 __host__ __device__ inline size_t exact_scratch(int DK, int dvt) {
     return rec_layout(DK, dvt, 4).bytes + (size_t)DK * dvt * 16 * 4;
@@ -1658,16 +1658,19 @@ __host__ __device__ inline size_t exact_scratch(int DK, int dvt) {
 
 template <typename T, int DK, bool VEC>
 __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* scratch) {
-    using L = Scan32Lds<DK>;
+    using L = Scan32Lds<DK, 1>;
+    constexpr int NO = kOwn<DK> / 16;
     constexpr int kPrep = PrepLds<OpF32, DK>::kBytes, kGrad = GradLds<OpF32, DK>::kBytes;
     __shared__ __align__(16) char lds[std::max(std::max(kPrep, kGrad), L::kBytes)];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15,
-              g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+    const int c0 = kOwn<DK> * w + 4 * g;
+    const bool own = w * NO < DK / 16;
     BwdParams e = p;
     e.rec = rec_layout(DK, p.dvt, 4);
     char* rec = scratch + blockIdx.x * exact_scratch(DK, p.dvt);
     char* carry = rec + e.rec.bytes;
-    char* turn = lds + L::kTurnAt + wave * L::kTurn;
+    char* mine = lds + L::kTiles;
+    const RowMat<OpF32, DK> turn_s{mine + L::kSAt};
     const size_t stride = (size_t)p.heads * p.rec.bytes;
     for (int unit = blockIdx.x; unit < p.batch * p.heads; unit += gridDim.x) {
         const int seq = unit / p.heads, h = unit - seq * p.heads;
@@ -1693,68 +1696,71 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
             at.n = min(C64, t1 - at.t0);
             return at;
         };
-        // forward over chunk c from state S, or back over it from its gradient
-        auto step = [&](auto back, State<OpF32, DK>& S, int c, int tile) {
-            TileRuns<T, VEC> in;
-            in.load(e, seq_at<T>(p, seq, h, back.value), c, tile, lane);
-            scan32_chunk<T, DK, VEC, back.value>(e, S, in, rec, lds, turn, tile, lane);
+        using St = State<OpF32, kOwn<DK>>;
+        auto get = [&](St& S, char* base, int tile) {
+            const f32x4* b = kept_state<DK>(base, tile, w, lane);
+            S.e = 0;
+            if (own)
+#pragma unroll
+                for (int i = 0; i < NO; ++i) S.s[i] = b[i * 64];
         };
-        auto stage = [&](auto back, int c) {
+        auto put = [&](const St& S, char* base, int tile) {
+            f32x4* b = kept_state<DK>(base, tile, w, lane);
+            if (own)
+#pragma unroll
+                for (int i = 0; i < NO; ++i) b[i * 64] = S.s[i];
+        };
+        // chunk c of every tile: forward from the states of `kept` to those of
+        // `next`, or back over it on the states' gradients, in place
+        auto step = [&](auto back, int c, char* kept, char* next) {
+            const SeqAt<T> from = seq_at<T>(p, seq, h, back.value);
             __syncthreads();
             ScanStage<OpF32, T, DK, VEC, back.value> sg;
-            sg.load(e, seq_at<T>(p, seq, h, back.value), c, rec, threadIdx.x);
+            sg.load(e, from, c, rec, threadIdx.x);
             sg.store(lds, threadIdx.x);
+            for (int tile = 0; tile < p.dvt; ++tile) {
+                St S;
+                get(S, kept, tile);
+                __syncthreads();
+                TileRuns<T, VEC, 256> in;
+                in.load(e, from, c, tile, threadIdx.x);
+                in.put(mine, threadIdx.x);
+                if (own)
+#pragma unroll
+                    for (int b = 0; b < NO; ++b) turn_s.put_unit(m, w * NO + b, g, S.s[b]);
+                __syncthreads();
+                scan32_chunk<T, DK, 1, back.value>(e, S, rec, lds, mine, tile, w, lane);
+                if (next) put(S, next, tile);
+            }
             __syncthreads();
         };
-        for (int c = 0; c < nc; ++c) {
-            prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
-            stage(std::false_type{}, c);
-            for (int tile = wave; tile < p.dvt; tile += 4) {
-                char* kept = first + c * stride + p.rec.s0;
-                State<OpF32, DK> S;
-                if (c == 0) {
-                    S.load(p, p.init ? p.init + st : nullptr, 16 * tile + row, g);
-                    store_state(S, kept, tile, lane);
-                } else {
-                    load_state(S, kept, tile, lane);
-                }
-                if (c + 1 < nc) {
-                    step(std::false_type{}, S, c, tile);
-                    store_state(S, kept + stride, tile, lane);
-                }
+        // a state's tiles from where the caller has it
+        auto begin = [&](const float* from, char* base) {
+            for (int tile = 0; tile < p.dvt; ++tile) {
+                St S;
+                S.load(p, from ? from + st : nullptr, 16 * tile + m, c0);
+                put(S, base, tile);
             }
-            __syncthreads();
+        };
+        begin(p.init, first + p.rec.s0);
+        for (int c = 0; c + 1 < nc; ++c) {
+            char* kept = first + c * stride + p.rec.s0;
+            prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
+            step(std::false_type{}, c, kept, kept + stride);
         }
-        for (int tile = wave; tile < p.dvt; tile += 4) {
-            State<OpF32, DK> S;
-            S.load(p, p.dfinal ? p.dfinal + st : nullptr, 16 * tile + row, g);
-            store_state(S, carry, tile, lane);
-        }
+        begin(p.dfinal, carry);
         for (int c = nc - 1; c >= 0; --c) {
-            const char* kept = first + c * stride + p.rec.s0;
             prep_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
-            stage(std::false_type{}, c);
-            for (int tile = wave; tile < p.dvt; tile += 4) {
-                State<OpF32, DK> S;
-                load_state(S, kept, tile, lane);
-                step(std::false_type{}, S, c, tile);
-            }
-            stage(std::true_type{}, c);
-            for (int tile = wave; tile < p.dvt; tile += 4) {
-                State<OpF32, DK> S;
-                load_state(S, carry, tile, lane);
-                step(std::true_type{}, S, c, tile);
-                store_state(S, carry, tile, lane);
-            }
-            __syncthreads();
+            step(std::false_type{}, c, first + c * stride + p.rec.s0, nullptr);
+            step(std::true_type{}, c, carry, carry);
             grad_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
             __syncthreads();
         }
         if (p.dinit)
-            for (int tile = wave; tile < p.dvt; tile += 4) {
-                State<OpF32, DK> S;
-                load_state(S, carry, tile, lane);
-                S.store(p, p.dinit + st, 16 * tile + row, g);
+            for (int tile = 0; tile < p.dvt; ++tile) {
+                St S;
+                get(S, carry, tile);
+                if (own) S.store(p, p.dinit + st, 16 * tile + m, c0);
             }
     }
 }
@@ -1804,12 +1810,20 @@ size_t base_bytes(const rhz_gdr_prefill_backward_args& a) {
     return a.cu_seqlens ? (((size_t)a.batch + 1) * 4 + 255) & ~(size_t)255 : 0;
 }
 
+// 16-row tiles of fp32 scans up to which each has a workgroup of its own; two
+// share one, its K, Q, T and P and each SIMD, where the card has more tiles than
+// CUs.  d = 128, 1024 tokens, whole call: 256 tiles 140 us with one and 162 with
+// two a workgroup, 512 tiles 268 and 221; d = 64: 117 and 134, 227 and 198.
+constexpr int64_t kOneTile = 256;
+
 template <class Op, typename T, int DK, bool VEC>
 hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hipStream_t st) {
     hipError_t e;
     const int64_t grid = chunks * p.heads;
-    const int splits = (p.dvt + 3) / 4;
-    const int64_t scans = ((int64_t)p.batch * p.heads * 2 + 7) / 8 * 8 * splits;
+    const int64_t walks = (int64_t)p.batch * p.heads * 2;
+    const int tiles = Op::kScaled ? 4 : walks * p.dvt > kOneTile ? 2 : 1;
+    const int splits = (p.dvt + tiles - 1) / tiles;  // dvt is even
+    const int64_t scans = (walks + 7) / 8 * 8 * splits;
     if ((e = check_grid(grid, 256)) != hipSuccess) return e;
     if ((e = check_grid(scans, 512)) != hipSuccess) return e;
     if (grid > 0) {
@@ -1819,8 +1833,10 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     if (grid > 0 || p.dinit) {
         if constexpr (Op::kScaled)
             hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(512), 0, st, p, splits);
+        else if (tiles == 1)
+            hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC, 1>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
         else
-            hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
+            hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC, 2>), dim3((unsigned)scans), dim3(512), 0, st, p, splits);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (grid > 0) {

@@ -112,6 +112,14 @@ def test_shapes(device, dtype, lengths, H, dk, dv):
         check(call(d, lengths, device, dense=True), want, dtype, "dense")
 
 
+@pytest.mark.parametrize("dk", [20, 64, 100, 128])
+def test_more_state_tiles_than_cus(device, dk):
+    """Two sequences of 16 heads and 80 value channels: 384 tiles of 16 state
+    rows over both scans, which share workgroups."""
+    d = inputs(torch.float32, [70, 3], 16, dk, 80, seed=dk)
+    check(call(d, [70, 3], device), reference(d, [70, 3]), torch.float32)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("gate", ["g", "alpha"])
 @pytest.mark.parametrize("g_mean", [-6.0, 3.0])
