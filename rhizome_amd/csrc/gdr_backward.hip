@@ -704,20 +704,20 @@ struct TileRuns {
     }
 };
 
-// Rows of a wave's tile as units with d_v along the contraction: column tile
-// `b` of the turned matrix to `base` + b KiB, this tile's half of them (a unit
+// Rows of a wave's tile as units with d_v along the contraction, one half of the
+// turned matrix: its column tile `b` to `base` + b KiB, this tile's half of them (a unit
 // holds two tiles).
 template <int N, class Mat>
-__device__ __forceinline__ void store_turned(const Mat& turn, char* base, int tile, int lane) {
-    char* o = base + (tile >> 1) * N * 1024 + (tile & 1) * 8 + lane * 16;
+__device__ __forceinline__ void store_turned(const Mat& turn, char* base, int tile, int half, int lane) {
+    char* o = base + ((tile >> 1) * N + half * (N / 2)) * 1024 + (tile & 1) * 8 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < N; ++b) *reinterpret_cast<f16x4*>(o + b * 1024) = turn.col4(b, 0, lane);
+    for (int b = 0; b < N / 2; ++b) *reinterpret_cast<f16x4*>(o + b * 1024) = turn.col4(half * (N / 2) + b, 0, lane);
 }
 
 // A chunk's shared operands on their way from HBM to LDS, by `THREADS` threads.
 template <class Op, typename T, int DK, bool VEC, bool BACK, int THREADS = 256>
 struct ScanStage {
-    static constexpr int R = kRun<T>, N = 64 * DK / R / THREADS;
+    static constexpr int R = kRun<T>, RUNS = 64 * DK / R, N = (RUNS + THREADS - 1) / THREADS;
     static constexpr int NP = 64 * int(sizeof(typename Op::Elt)) / 16, NT = 64 * NP / THREADS;
     u32x4 k[N], q[BACK ? N : 1], t[NT], pp[BACK ? NT : 1];
     float vec;
@@ -727,7 +727,7 @@ struct ScanStage {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = tid + THREADS * i, tk = c * C64 + id / (DK / R), col = id % (DK / R) * R;
-            const bool in = tk < at.tokens && col < p.d_k;
+            const bool in = id < RUNS && tk < at.tokens && col < p.d_k;
             k[i] = load_run<T, VEC>(at.k + tk * ld + col, in, p.d_k - col);
             if constexpr (BACK) q[i] = load_run<T, VEC>(at.q + tk * ld + col, in, p.d_k - col);
         }
@@ -752,6 +752,7 @@ struct ScanStage {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = tid + THREADS * i;
+            if (id >= RUNS) break;
             float x[R];
             unpack_run<T>(k[i], x);
             K.put(id / (DK / R), id % (DK / R) * R, x, sk);
@@ -813,19 +814,20 @@ __device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& 
 }
 
 // bf16 tensors, fp16 operands.  A wave's chunk is one chain of LDS reads,
-// products and exponents that a SIMD's single wave cannot fill, so four more
-// waves do what is off it: they read K, Q, T, P and each carrying wave's
-// columns of V or dO two chunks ahead, convert them to LDS one chunk ahead, and
-// turn and store the previous chunk's S0 and W (dS1 and dX).  Two barriers a
-// chunk: A, the buffers of the chunk are full and its predecessor's results lie
-// in LDS; B, these have been read.
+// products and exponents that a SIMD's single wave cannot fill, so eight more
+// waves do what is off it: they read K, Q, T, P and the carrying waves' columns
+// of V or dO two chunks ahead, convert them to LDS one chunk ahead, and turn and
+// store the previous chunk's S0 and W (dS1 and dX).  Two barriers a chunk: A,
+// the buffers of the chunk are full and its predecessor's results lie in LDS; B,
+// these have been read.  Four waves instead of eight were behind the chain (16384
+// tokens, 16 heads, d_v = 256: 860 us, and 802 with eight).
 template <int DK>
 struct Scan16Lds {
     using Buf = ScanBuf<OpF16, DK>;
     static constexpr int kTile = 64 * 48;                                         // a wave's columns of V or dO
     static constexpr int kTurnS = RowMat<OpF16, DK>::bytes(16), kTurnW = RowMat<OpF16, 64>::bytes(16);
     static constexpr int kTiles = 2 * Buf::kBytes, kTurn = kTiles + 8 * kTile, kExps = kTurn + 4 * (kTurnS + kTurnW);
-    static constexpr int kBytes = kExps + 8 * 4;
+    static constexpr int kBytes = kExps + 16 * 4;
 };
 
 template <typename T, int DK, bool VEC, bool BACK>
@@ -851,7 +853,8 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         const float gc = vec[kVecGc];
         const int ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
         const int eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
-        const int eo = BACK ? __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(lds + L::kExps)[(c & 1) * 4 + wave]) : 0;
+        const int2 eos = reinterpret_cast<const int2*>(lds + L::kExps)[(c & 1) * 4 + wave];
+        const int eo = BACK ? __builtin_amdgcn_readfirstlane(max(eos.x, eos.y)) : 0;
         f32x4 x[4], w[4], vo[4];
         TileRuns<T, VEC>::get(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, vo, lane);
 #pragma unroll
@@ -957,37 +960,37 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
 }
 
 template <typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a, int tile, int wave, int lane, char* lds) {
+__device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a, int tile, int tid, char* lds) {
+    const int wave = (tid >> 6) & 3, half = __builtin_amdgcn_readfirstlane(tid >> 8), lane = tid & 63;
     using Op = OpF16;
     using L = Scan16Lds<DK>;
     constexpr int NT = DK / 16;
-    const int tid = wave * 64 + lane;
     const bool active = tile < p.dvt;
     const SeqAt<T> at = seq_at<T>(p, a.seq, a.h, BACK);
     const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
     const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
     auto chunk = [&](int c) { return BACK ? a.nc - 1 - min(c, a.nc - 1) : min(c, a.nc - 1); };
-    ScanStage<Op, T, DK, VEC, BACK> st;
-    TileRuns<T, VEC> in;
+    ScanStage<Op, T, DK, VEC, BACK, 512> st;
+    TileRuns<T, VEC, 128> in;
     auto load = [&](int c) {
         st.load(p, at, chunk(c), a.rec + chunk(c) * a.stride, tid);
-        if (active) in.load(p, at, chunk(c), tile, lane);
+        if (active) in.load(p, at, chunk(c), tile, half * 64 + lane);
     };
     auto store = [&](int c) {
         st.store(lds + (c & 1) * L::Buf::kBytes, tid);
         if (active) {
-            in.put(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, lane);
+            in.put(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, half * 64 + lane);
             if constexpr (BACK) {  // dO below 1/2
                 const int e = bits_exp(in.max_bits()) + 2;
-                if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[(c & 1) * 4 + wave] = e;
+                if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[((c & 1) * 4 + wave) * 2 + half] = e;
             }
         }
     };
     auto results = [&](int c) {
         char* rec = a.rec + chunk(c) * a.stride;
         if (!active) return;
-        store_turned<NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, lane);
-        store_turned<4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, lane);
+        store_turned<NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, half, lane);
+        store_turned<4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, half, lane);
     };
     if (a.nc > 0) {
         load(0);
@@ -997,26 +1000,26 @@ __device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a
     for (int c = 0; c < a.nc; ++c) {
         __syncthreads();  // A
         if (c > 0) results(c - 1);
+        __syncthreads();  // B
         if (c + 1 < a.nc) {
             store(c + 1);
             load(c + 2);
         }
-        __syncthreads();  // B
     }
     __syncthreads();
     if (a.nc > 0) results(a.nc - 1);
 }
 
 template <typename T, int DK, bool VEC>
-__global__ __launch_bounds__(512) void bwd_scan16_kernel(BwdParams p, int splits) {
+__global__ __launch_bounds__(768) void bwd_scan16_kernel(BwdParams p, int splits) {
     __shared__ __align__(16) char lds[Scan16Lds<DK>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ScanAt a;
     if (!scan_at(p, splits, a)) return;
     const int tile = a.part * 4 + (wave & 3);
     if (wave >= 4) {
-        if (a.back) scan16_serve<T, DK, VEC, true>(p, a, tile, wave - 4, lane, lds);
-        else scan16_serve<T, DK, VEC, false>(p, a, tile, wave - 4, lane, lds);
+        if (a.back) scan16_serve<T, DK, VEC, true>(p, a, tile, threadIdx.x - 256, lds);
+        else scan16_serve<T, DK, VEC, false>(p, a, tile, threadIdx.x - 256, lds);
     } else if (tile < p.dvt) {
         if (a.back) scan16_carry<T, DK, VEC, true>(p, a, tile, wave, lane, lds);
         else scan16_carry<T, DK, VEC, false>(p, a, tile, wave, lane, lds);
@@ -1025,8 +1028,6 @@ __global__ __launch_bounds__(512) void bwd_scan16_kernel(BwdParams p, int splits
     }
 }
 
-// fp32 operands: bound by the fp32 matrix rate, four waves that each do the
-// whole of it, the next chunk's shared operands in registers meanwhile.
 // fp32.  An fp32 product takes its SIMD 16 times as long as an fp16 one, and few
 // heads leave most SIMDs idle, so a tile has four waves: each owns a quarter of
 // the state's columns (its update, 1/4 of the products) and a block of 16 tokens
@@ -1832,7 +1833,7 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     }
     if (grid > 0 || p.dinit) {
         if constexpr (Op::kScaled)
-            hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(512), 0, st, p, splits);
+            hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(768), 0, st, p, splits);
         else if (tiles == 1)
             hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC, 1>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
         else
