@@ -119,15 +119,28 @@ __device__ __forceinline__ typename Op::Unit lds_unit(const char* p, int i, int 
 // A matrix by rows in LDS.  A unit of it is read along its rows, or along its
 // columns (fp16: ds_read_b64_tr_b16, which gives lane l of 16 the l-th column
 // of four rows), so that one copy serves products over either index.  The
-// padding of a row spreads 16 rows' accesses evenly over the banks.
+// 16-byte groups of a row are XORed by the row: of the lanes that LDS serves at
+// once, 16 with 16 bytes or 32 with 8, none share a bank, whether they run down
+// 16 rows or along eight rows' 32 bytes (padded rows served only one of the
+// two: the bwd scan lost 1500 LDS cycles a chunk to the other).
 template <class Op, int COLS>
 struct RowMat {
     using Elt = typename Op::Elt;
     using Unit = typename Op::Unit;
-    static constexpr int kStride = COLS * int(sizeof(Elt)) + 16;
+    static constexpr int kStride = COLS * int(sizeof(Elt));
     static constexpr int bytes(int rows) { return rows * kStride; }
     char* p;
-    __device__ __forceinline__ char* at(int row, int col) const { return p + row * kStride + col * int(sizeof(Elt)); }
+    static __device__ __forceinline__ int swizzle(int row) {  // in bytes
+        constexpr int kSpan = kStride >= 256 ? 0 : kStride == 128 ? 1 : kStride == 64 ? 2 : 3;  // log2 rows per 64 banks
+        static_assert(kStride >= 32, "");
+        if constexpr (Op::kScaled)
+            return (((row >> kSpan) & (COLS / 16 - 1)) << 5) | ((row & 8) << 1);
+        else
+            return ((row >> kSpan) & (COLS / 4 < 16 ? COLS / 4 - 1 : 15)) << 4;
+    }
+    __device__ __forceinline__ char* at(int row, int col) const {
+        return p + row * kStride + ((col * int(sizeof(Elt))) ^ swizzle(row));
+    }
     // a unit's 16 bytes of consecutive columns: an order of the contraction
     // that only another operand read this way shares
     __device__ __forceinline__ Unit run(int row0, int ku, int lane) const {
@@ -173,19 +186,30 @@ struct RowMat {
     template <int N>
     __device__ __forceinline__ void put(int row, int col, const float (&x)[N], float s) const {
         if constexpr (Op::kScaled) {
-            typedef _Float16 f16xn __attribute__((ext_vector_type(N)));
-            f16xn h;
+            // bf16 values times a power of two: their 8 bits fit fp16's 11, so the
+            // conversion towards zero, two in one instruction, rounds subnormals alone
+            typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+            words h;
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = (_Float16)(x[i] * s);
-            *reinterpret_cast<f16xn*>(at(row, col)) = h;
+            for (int i = 0; i < N; i += 2)
+                h[i / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[i] * s, x[i + 1] * s));
+            *reinterpret_cast<words*>(at(row, col)) = h;
         } else {
-            static_assert(N == 4 || N == 8, "");
 #pragma unroll
             for (int i = 0; i < N; i += 4)
                 *reinterpret_cast<f32x4*>(at(row, col + i)) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
         }
     }
 };
+
+// The thread's index, computed anew: what depends on it does not move out of a
+// loop around the call, where the exact kernel's loops over chunks would keep
+// all of it in registers (1.8 KiB of spills a lane, and 7 us a launch for them).
+__device__ __forceinline__ int thread_index() {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    return tid;
+}
 
 // 64 x 64 fp32 in LDS, 16-byte groups of a row XORed by the row.
 __device__ __forceinline__ int sq_at(int r, int c) { return r * 64 + ((((c >> 2) ^ r) & 15) << 2) + (c & 3); }
@@ -204,6 +228,13 @@ __device__ __forceinline__ int wave_max_bits(int x) {
 }
 // The exponent of magnitude bits, 100 at most either way.
 __device__ __forceinline__ int bits_exp(int bits) { return max(min((bits >> 23) - 127, 100), -100); }
+// The exponent that K or Q of a chunk is divided by before its rounding to fp16:
+// none for values of ordinary size (largest in [2^-8, 16): fp16's steps of 2^-24
+// below 2^-14 are then 2^-16 of it at most), else the largest value's.
+__device__ __forceinline__ int rows_exp(int bits) {
+    const int e = bits_exp(bits);
+    return e >= -8 && e < 4 ? 0 : e;
+}
 
 // A run of 16 bytes of a row of T (8 bf16 or 4 fp32).  VEC: rows are whole runs
 // and aligned, and a run outside the matrix (`in` false) is read from zeros
@@ -225,6 +256,10 @@ __device__ __forceinline__ u32x4 load_run(const T* p, bool in, int n) {
         return __builtin_bit_cast(u32x4, x);
     }
 }
+// Whole rows of a chunk: 16 bytes at `offset` bytes behind a pointer that the wave shares.
+__device__ __forceinline__ u32x4 load_at(const void* p, unsigned offset) {
+    return *(global_u32x4*)(reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + offset));
+}
 template <typename T>
 __device__ __forceinline__ void unpack_run(const u32x4& u, float (&x)[kRun<T>]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -240,12 +275,15 @@ __device__ __forceinline__ void unpack_run(const u32x4& u, float (&x)[kRun<T>]) 
 }
 template <typename T>
 __device__ __forceinline__ int run_max_bits(const u32x4& u) {
-    float x[kRun<T>];
-    unpack_run<T>(u, x);
-    int m = 0;
+    if constexpr (sizeof(T) == 2) {  // as pairs of 15-bit integers
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 m = {0, 0};
 #pragma unroll
-    for (int i = 0; i < kRun<T>; ++i) m = max(m, bits_abs(x[i]));
-    return m;
+        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
+        return max(int(m.x), int(m.y)) << 16;
+    } else {
+        return int(max(max(u.x & 0x7fffffffu, u.y & 0x7fffffffu), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu)));
+    }
 }
 // Two floats as bf16, round to nearest even, by the hardware's conversion.
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
@@ -310,6 +348,7 @@ struct BwdParams {
     char* ws;
     RecLayout rec;
     int batch, seq_len, heads, d_k, d_v, dvt, gate_is_alpha;
+    bool short_rows;  // a chunk's rows lie within 2 GiB
     bool vec_s;  // rows of the states, 16 bytes at a time
 };
 
@@ -395,7 +434,7 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     using L = PrepLds<Op, DK>;
     constexpr int NT = DK / 16, NBK = Op::kBlocks, NKK = NT / NBK, NKT = 4 / NBK, R = kRun<T>;
     constexpr int NR = 64 * DK / R / 256;  // runs of K (and of Q) per thread
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+    const int tid = thread_index(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
               m = lane & 15;
     const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
     const RowMat<Op, 64> Th{lds + L::kT}, Ph{lds + L::kP};
@@ -437,8 +476,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
         __syncthreads();
         const int bk = max(max(misc[0], misc[1]), max(misc[2], misc[3]));
         const int bq = max(max(misc[4], misc[5]), max(misc[6], misc[7]));
-        ek = bits_exp(bk);
-        eq = bits_exp(bq);
+        ek = rows_exp(bk);
+        eq = rows_exp(bq);
         bad = bad || bk >= 0x7f800000 || bq >= 0x7f800000;
     }
     {
@@ -560,8 +599,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
 #pragma unroll
     for (int i = 0; i < 64 * NP / 256; ++i) {
         const int id = tid + 256 * i;
-        ot[id] = *reinterpret_cast<const u32x4*>(Th.at(id / NP, 0) + id % NP * 16);
-        op[id] = *reinterpret_cast<const u32x4*>(Ph.at(id / NP, 0) + id % NP * 16);
+        ot[id] = *reinterpret_cast<const u32x4*>(Th.at(id / NP, id % NP * (64 / NP)));
+        op[id] = *reinterpret_cast<const u32x4*>(Ph.at(id / NP, id % NP * (64 / NP)));
     }
     if (Op::kScaled && tid == 0) exps[kVecBad] = misc[8];
 }
@@ -667,9 +706,16 @@ struct TileRuns {
     u32x4 r[N];
     __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, int tile, int lane) {
         const long ld = (long)p.heads * p.d_v;
+        if (VEC && sizeof(T) == 2 && RUNS % THREADS == 0 && p.short_rows && at.tokens - c * C64 >= C64 && 16 * tile + 16 <= p.d_v) {
+            const T* base = at.vo + c * C64 * ld + 16 * tile;
+            const unsigned off = ((unsigned)(lane / RPR) * (unsigned)ld + lane % RPR * R) * sizeof(T);
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = load_at(base + i * (THREADS / RPR) * ld, off);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = lane + 64 * i, t = c * C64 + id / RPR, col = 16 * tile + id % RPR * R;
+            const int id = lane + THREADS * i, t = c * C64 + id / RPR, col = 16 * tile + id % RPR * R;
             r[i] = load_run<T, VEC>(at.vo + t * ld + col, id < RUNS && t < at.tokens && col < p.d_v, p.d_v - col);
         }
     }
@@ -685,7 +731,7 @@ struct TileRuns {
         const Raw tn{corner};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = lane + 64 * i;
+            const int id = lane + THREADS * i;
             if (id < RUNS) *reinterpret_cast<u32x4*>(tn.at(id / RPR, id % RPR * R)) = r[i];
         }
     }
@@ -704,14 +750,15 @@ struct TileRuns {
     }
 };
 
-// Rows of a wave's tile as units with d_v along the contraction, one half of the
-// turned matrix: its column tile `b` to `base` + b KiB, this tile's half of them (a unit
-// holds two tiles).
+// Rows of two tiles as units with d_v along the contraction: `N` column
+// tiles of the turned matrices from `first` on, 1 KiB each.
 template <int N, class Mat>
-__device__ __forceinline__ void store_turned(const Mat& turn, char* base, int tile, int half, int lane) {
-    char* o = base + ((tile >> 1) * N + half * (N / 2)) * 1024 + (tile & 1) * 8 + lane * 16;
+__device__ __forceinline__ void store_turned(const Mat& even, const Mat& odd, char* base, int first, int lane) {
+    char* o = base + first * 1024 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < N / 2; ++b) *reinterpret_cast<f16x4*>(o + b * 1024) = turn.col4(half * (N / 2) + b, 0, lane);
+    for (int b = 0; b < N; ++b)
+        *reinterpret_cast<f16x8*>(o + b * 1024) = __builtin_shufflevector(
+            even.col4(first + b, 0, lane), odd.col4(first + b, 0, lane), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // A chunk's shared operands on their way from HBM to LDS, by `THREADS` threads.
@@ -724,12 +771,23 @@ struct ScanStage {
     int ek, eq;
     __device__ __forceinline__ void load(const BwdParams& p, const SeqAt<T>& at, int c, const char* rec, int tid) {
         const long ld = (long)p.heads * p.d_k;
+        constexpr int RPR = DK / R;
+        if (VEC && sizeof(T) == 2 && RUNS % THREADS == 0 && p.short_rows && at.tokens - c * C64 >= C64 && p.d_k == DK) {
+            const unsigned off = ((unsigned)(tid / RPR) * (unsigned)ld + tid % RPR * R) * sizeof(T);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = tid + THREADS * i, tk = c * C64 + id / (DK / R), col = id % (DK / R) * R;
-            const bool in = id < RUNS && tk < at.tokens && col < p.d_k;
-            k[i] = load_run<T, VEC>(at.k + tk * ld + col, in, p.d_k - col);
-            if constexpr (BACK) q[i] = load_run<T, VEC>(at.q + tk * ld + col, in, p.d_k - col);
+            for (int i = 0; i < N; ++i) {
+                const long from = (c * C64 + i * (THREADS / RPR)) * ld;
+                k[i] = load_at(at.k + from, off);
+                if constexpr (BACK) q[i] = load_at(at.q + from, off);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int id = tid + THREADS * i, tk = c * C64 + id / RPR, col = id % RPR * R;
+                const bool in = id < RUNS && tk < at.tokens && col < p.d_k;
+                k[i] = load_run<T, VEC>(at.k + tk * ld + col, in, p.d_k - col);
+                if constexpr (BACK) q[i] = load_run<T, VEC>(at.q + tk * ld + col, in, p.d_k - col);
+            }
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -744,30 +802,43 @@ struct ScanStage {
             eq = reinterpret_cast<const int*>(v)[kVecEQ];
         }
     }
-    __device__ __forceinline__ void store(char* buf, int tid) const {
-        using L = ScanBuf<Op, DK>;
-        const RowMat<Op, DK> K{buf + L::kK}, Q{buf + L::kQ};
-        const RowMat<Op, 64> Tm{buf + L::kT}, P{buf + L::kP};
-        const float sk = exp2i(-ek), sq = exp2i(-eq);
+    template <bool SCALE>
+    static __device__ __forceinline__ void put_rows_as(char* to, const u32x4* from, int e, int tid) {
+        const RowMat<Op, DK> rows{to};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = tid + THREADS * i;
             if (id >= RUNS) break;
             float x[R];
-            unpack_run<T>(k[i], x);
-            K.put(id / (DK / R), id % (DK / R) * R, x, sk);
-            if constexpr (BACK) {
-                unpack_run<T>(q[i], x);
-                Q.put(id / (DK / R), id % (DK / R) * R, x, sq);
-            }
+            unpack_run<T>(from[i], x);
+            rows.put(id / (DK / R), id % (DK / R) * R, x, SCALE ? exp2i(-e) : 1.f);
         }
+    }
+    static __device__ __forceinline__ void put_rows(char* to, const u32x4* from, int e, int tid) {
+        if (Op::kScaled && __builtin_amdgcn_readfirstlane(e) != 0) put_rows_as<true>(to, from, e, tid);
+        else put_rows_as<false>(to, from, e, tid);
+    }
+    static __device__ __forceinline__ void put_square(char* to, const u32x4* from, int tid) {
+        const RowMat<Op, 64> sq{to};
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int id = tid + THREADS * i;
-            *reinterpret_cast<u32x4*>(Tm.at(id / NP, 0) + id % NP * 16) = t[i];
-            if constexpr (BACK) *reinterpret_cast<u32x4*>(P.at(id / NP, 0) + id % NP * 16) = pp[i];
+            *reinterpret_cast<u32x4*>(sq.at(id / NP, id % NP * (64 / NP))) = from[i];
         }
+    }
+    // K, T and the small values, then Q and P (back)
+    __device__ __forceinline__ void store(char* buf, int tid) const {
+        using L = ScanBuf<Op, DK>;
+        put_rows(buf + L::kK, k, ek, tid);
+        put_square(buf + L::kT, t, tid);
         if (tid < kVecs) reinterpret_cast<float*>(buf + L::kVec)[tid] = vec;
+    }
+    __device__ __forceinline__ void store_back(char* buf, int tid) const {
+        using L = ScanBuf<Op, DK>;
+        if constexpr (BACK) {
+            put_rows(buf + L::kQ, q, eq, tid);
+            put_square(buf + L::kP, pp, tid);
+        }
     }
 };
 
@@ -813,22 +884,39 @@ __device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& 
     return true;
 }
 
-// bf16 tensors, fp16 operands.  A wave's chunk is one chain of LDS reads,
-// products and exponents that a SIMD's single wave cannot fill, so eight more
-// waves do what is off it: they read K, Q, T, P and the carrying waves' columns
-// of V or dO two chunks ahead, convert them to LDS one chunk ahead, and turn and
-// store the previous chunk's S0 and W (dS1 and dX).  Two barriers a chunk: A,
-// the buffers of the chunk are full and its predecessor's results lie in LDS; B,
-// these have been read.  Four waves instead of eight were behind the chain (16384
-// tokens, 16 heads, d_v = 256: 860 us, and 802 with eight).
+// bf16 tensors, fp16 operands.  A wave's chunk is one chain of LDS reads and
+// products, and a wave issues an instruction every four to five cycles at best,
+// so four more waves do what is off the chain: they read K, Q, T, P and the
+// carrying waves' columns of V or dO two chunks ahead, convert them to LDS one
+// chunk ahead, and turn and store the previous chunk's S0 and W (dS1 and dX).
+// Two barriers a chunk: A, the buffers of the chunk are full and its
+// predecessor's results lie in LDS; B, these have been read.  What the serving
+// waves do is split around B as the chain is.
+//
+// The chain has no exponent of its own results to wait for: a chunk's values
+// are scaled by the larger of the state's and of V's (dO's) largest value,
+// which leaves them 2^10 below fp16's range and 2^19 above its subnormals.
+// Growth beyond that shows as an infinity or NaN in the state, and the head is
+// done again in fp32.
+//
+// 16384 tokens, 16 heads, d_k = 128, d_v = 256: 770 us, 5900 cycles a chunk, of
+// which the chain waits 350; eight serving waves leave it 168 registers: 816.
+// 4 x 4096 tokens, d = 128 (a workgroup on every CU): 235 us for 0.92 GB, 75 % of
+// a copy's rate.
 template <int DK>
 struct Scan16Lds {
     using Buf = ScanBuf<OpF16, DK>;
-    static constexpr int kTile = 64 * 48;                                         // a wave's columns of V or dO
+    static constexpr int kTile = RowMat<OpF16, 16>::bytes(64);                    // a wave's columns of V or dO
     static constexpr int kTurnS = RowMat<OpF16, DK>::bytes(16), kTurnW = RowMat<OpF16, 64>::bytes(16);
     static constexpr int kTiles = 2 * Buf::kBytes, kTurn = kTiles + 8 * kTile, kExps = kTurn + 4 * (kTurnS + kTurnW);
-    static constexpr int kBytes = kExps + 16 * 4;
+    static constexpr int kBytes = kExps + 8 * 4;
 };
+
+// two products rounded to a pair of fp16
+__device__ __forceinline__ OpF16::Unit pack_products(const f32x4* x, const f32x4* f) {
+    const f32x4 t[2] = {x[0] * f[0], x[1] * f[1]};
+    return OpF16::pack(t, 1.f);
+}
 
 template <typename T, int DK, bool VEC, bool BACK>
 __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a, int tile, int wave, int lane, char* lds) {
@@ -839,11 +927,25 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
     constexpr int NT = DK / 16, NU = NT / 2;
     const int g = lane >> 4, m = lane & 15, row = 16 * tile + m;
     const float* from = BACK ? p.dfinal : p.init;
+    __builtin_amdgcn_s_setprio(2);  // the chain goes before the wave that serves it on the same SIMD
     State<Op, DK> S;
     S.load(p, from ? from + a.state : nullptr, row, 4 * g);
     const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
     const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
+    int* exps = reinterpret_cast<int*>(a.rec + (BACK ? a.nc - 1 : 0) * a.stride + p.rec.vec);
     for (int c = 0; c < a.nc; ++c) {
+        // the state's largest value between 2^-4 and 2^10
+        int top = tiles_exp<NT>(S.s);
+        if (top < -4 || top > 9) {
+            const float f = exp2i(5 - top);
+#pragma unroll
+            for (int b = 0; b < NT; ++b) S.s[b] *= f;
+            S.e += top - 5;
+            top = 5;
+        }
+        Unit su[NU];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) su[i] = Op::pack(&S.s[i * 2], 1.f);
         __syncthreads();  // A
         char* buf = lds + (c & 1) * Buf::kBytes;
         const RowMat<Op, DK> K{buf + Buf::kK}, Q{buf + Buf::kQ};
@@ -853,26 +955,27 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         const float gc = vec[kVecGc];
         const int ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
         const int eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
-        const int2 eos = reinterpret_cast<const int2*>(lds + L::kExps)[(c & 1) * 4 + wave];
-        const int eo = BACK ? __builtin_amdgcn_readfirstlane(max(eos.x, eos.y)) : 0;
+        // of V, or dO: its largest value below 2^ev
+        const int ev = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(lds + L::kExps)[(c & 1) * 4 + wave]);
         f32x4 x[4], w[4], vo[4];
         TileRuns<T, VEC>::get(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, vo, lane);
 #pragma unroll
         for (int b = 0; b < 4; ++b) x[b] = f32x4{0, 0, 0, 0};
-        Unit su[NU];
-#pragma unroll
-        for (int i = 0; i < NU; ++i) su[i] = Op::pack(&S.s[i * 2], 1.f);
 #pragma unroll
         for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su[i], x[b]);
-        const int top = S.top(), se = S.e;
-        const float sx = exp2i(se + ek);
+        // the next state is S times 2^-e, W and dX are kept times 2^-(e - ek):
+        // the larger of the state and of V (of dO times rows of Q or P) at 2^5 or 2^6
+        const int se = S.e, e = max(top + se, ev + (BACK ? eq + 2 : 0)) - 5;
+        Unit ru[2];
         if constexpr (!BACK) {
+            const float sv = exp2i(ek - e), sx = -exp2i(se + ek + ek - e);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) w[b] = vo[b] - by_token(kVecGamma, b) * (x[b] * sx);
+            for (int b = 0; b < 4; ++b) w[b] = vo[b] * sv + (by_token(kVecGamma, b) * sx) * x[b];
         } else {
-            const float so = exp2i(-eo), sz = exp2i(eo + ek + eq);
+            const int eo = ev + 1;  // dO as an operand: below 1/2
+            const float so = exp2i(-eo), sz = exp2i(eo + eq + ek + ek - e), sx = exp2i(se + ek + ek - e);
             f32x4 z[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) z[b] = f32x4{0, 0, 0, 0};
@@ -884,64 +987,51 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
                     if (u * 2 + 2 > b) z[b] = Op::mma(P.cols(b, u, lane), du, z[b]);
             }
 #pragma unroll
-            for (int b = 0; b < 4; ++b) w[b] = by_token(kVecBeta, b) * (z[b] * sz) + by_token(kVecWrite, b) * (x[b] * sx);
+            for (int b = 0; b < 4; ++b) w[b] = (by_token(kVecBeta, b) * sz) * z[b] + (by_token(kVecWrite, b) * sx) * x[b];
         }
-        // T or T^T times it, the operand below 2^5
-        const int er = tiles_exp<4>(w) - 4;
-        {
-            const float sr = exp2i(-er);
-            f32x4 y[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) y[b] = f32x4{0, 0, 0, 0};
+        for (int u = 0; u < 2; ++u) ru[u] = Op::pack(&w[u * 2], 1.f);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Unit ru = Op::pack(&w[u * 2], sr);
+        for (int b = 0; b < 4; ++b) w[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    if (!BACK && u * 2 <= b) y[b] = Op::mma(Tm.blocks(16 * b + m, u, g), ru, y[b]);
-                    if (BACK && u * 2 + 2 > b) y[b] = Op::mma(Tm.cols(b, u, lane), ru, y[b]);
-                }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (!BACK && u * 2 <= b) w[b] = Op::mma(Tm.blocks(16 * b + m, u, g), ru[u], w[b]);
+                if (BACK && u * 2 + 2 > b) w[b] = Op::mma(Tm.cols(b, u, lane), ru[u], w[b]);
             }
+        Unit kc[NT];  // read ahead of the barrier, to be there behind it
 #pragma unroll
-            for (int b = 0; b < 4; ++b) w[b] = y[b];
-        }
-        // W is kept with its largest value in [8, 16), dX in [1/4, 1/2)
-        const int tx = tiles_exp<4>(w), ew = tx + (BACK ? 2 : -3);
+        for (int b = 0; b < NT; ++b) kc[b] = K.cols(b, 0, lane);
+        const float sg = gc * exp2i(se - e);
+#pragma unroll
+        for (int b = 0; b < NT; ++b) S.s[b] *= sg;
+        S.e = e;
         if (lane == 0) {
-            int* oe = reinterpret_cast<int*>(a.rec + (BACK ? a.nc - 1 - c : c) * a.stride + p.rec.vec);
-            oe[(BACK ? kExpX : kExpW) + tile] = ew + er;
-            oe[(BACK ? kExpD : kExpS) + tile] = se;
-            if constexpr (BACK) oe[kExpO + tile] = eo;
+            exps[(BACK ? kExpX : kExpW) + tile] = e - ek;
+            exps[(BACK ? kExpD : kExpS) + tile] = se;
+            if constexpr (BACK) exps[kExpO + tile] = ev + 1;
         }
+        exps += (BACK ? -(long)a.stride : (long)a.stride) / 4;
         __syncthreads();  // B
-        const float si = exp2i(-ew);
 #pragma unroll
         for (int i = 0; i < NU; ++i) ts.put_unit(m, i, g, su[i]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) tw.put_unit(m, u, g, Op::pack(&w[u * 2], si));
-        // the next state in units of 2^e, of the larger of what stays (gamma_c S,
-        // below 2^9 of them) and what is written (each token's value below 2^8, and
-        // 64 tokens' with rows of K or Q below 2: 2^15; back, two such sums of 2^14)
-        int e = max(tx + er + ek, top + bits_exp(bits_abs(gc)));
-        if constexpr (BACK) e = max(e, eo - 2 + eq) + 1;
-        e -= 7;
-        const float sw = BACK ? -exp2i(er + ek - e) : exp2i(er + ek - e), sd = exp2i(eq - e), sg = gc * exp2i(se - e);
-        S.e = e;
-#pragma unroll
-        for (int b = 0; b < NT; ++b) S.s[b] *= sg;
+        for (int u = 0; u < 2; ++u) tw.put_unit(m, u, g, Op::pack(&w[u * 2], 1.f));
+        const float sd = exp2i(eq - e);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            f32x4 f[2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const f32x4 f = by_token(BACK ? kVecGamma : kVecWrite, u * 2 + b);
-                w[u * 2 + b] *= f;
-                if constexpr (BACK) vo[u * 2 + b] *= f;
-            }
-            const Unit wu = Op::pack(&w[u * 2], sw);
+            for (int b = 0; b < 2; ++b) f[b] = by_token(BACK ? kVecGamma : kVecWrite, u * 2 + b);
+            Unit wu = pack_products(&w[u * 2], f);
+            if constexpr (BACK) wu = -wu;
 #pragma unroll
-            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(K.cols(b, u, lane), wu, S.s[b]);
+            for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(u ? K.cols(b, u, lane) : kc[b], wu, S.s[b]);
             if constexpr (BACK) {
-                const Unit du = Op::pack(&vo[u * 2], sd);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) f[b] *= sd;
+                const Unit du = pack_products(&vo[u * 2], f);
 #pragma unroll
                 for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(Q.cols(b, u, lane), du, S.s[b]);
             }
@@ -959,50 +1049,60 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
     if (BACK && p.dinit) S.store(p, p.dinit + a.state, row, 4 * g);
 }
 
-template <typename T, int DK, bool VEC, bool BACK>
-__device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a, int tile, int tid, char* lds) {
-    const int wave = (tid >> 6) & 3, half = __builtin_amdgcn_readfirstlane(tid >> 8), lane = tid & 63;
-    using Op = OpF16;
+// ACTIVE: the tiles it serves carry rows.  The loop's body has no branches around
+// loads or stores, so that a wait for loads leaves the later stores in flight;
+// beyond the last chunk it stages that one again.
+template <typename T, int DK, bool VEC, bool BACK, bool ACTIVE>
+__device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a, int tid, char* lds) {
     using L = Scan16Lds<DK>;
     constexpr int NT = DK / 16;
-    const bool active = tile < p.dvt;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    // half the columns of two tiles' results, and V or dO of one of them
+    const int pair = wave & 1, half = wave >> 1, mine = 2 * pair + half, tile = a.part * 4 + mine, first = a.part * 2 + pair;
     const SeqAt<T> at = seq_at<T>(p, a.seq, a.h, BACK);
-    const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
-    const RowMat<Op, 64> tw{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW) + L::kTurnS};
+    auto turn = [&](int t) { return lds + L::kTurn + (2 * pair + t) * (L::kTurnS + L::kTurnW); };
+    const RowMat<OpF16, DK> ts0{turn(0)}, ts1{turn(1)};
+    const RowMat<OpF16, 64> tw0{turn(0) + L::kTurnS}, tw1{turn(1) + L::kTurnS};
     auto chunk = [&](int c) { return BACK ? a.nc - 1 - min(c, a.nc - 1) : min(c, a.nc - 1); };
-    ScanStage<Op, T, DK, VEC, BACK, 512> st;
-    TileRuns<T, VEC, 128> in;
+    ScanStage<OpF16, T, DK, VEC, BACK> st;
+    TileRuns<T, VEC> in;
     auto load = [&](int c) {
         st.load(p, at, chunk(c), a.rec + chunk(c) * a.stride, tid);
-        if (active) in.load(p, at, chunk(c), tile, half * 64 + lane);
+        if constexpr (ACTIVE) in.load(p, at, chunk(c), tile, lane);
     };
-    auto store = [&](int c) {
-        st.store(lds + (c & 1) * L::Buf::kBytes, tid);
-        if (active) {
-            in.put(lds + L::kTiles + ((c & 1) * 4 + wave) * L::kTile, half * 64 + lane);
-            if constexpr (BACK) {  // dO below 1/2
-                const int e = bits_exp(in.max_bits()) + 2;
-                if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[((c & 1) * 4 + wave) * 2 + half] = e;
-            }
+    auto store = [&](int c) { st.store(lds + (c & 1) * L::Buf::kBytes, tid); };
+    auto store_rest = [&](int c) {
+        st.store_back(lds + (c & 1) * L::Buf::kBytes, tid);
+        if constexpr (ACTIVE) {
+            const int slot = (c & 1) * 4 + mine;
+            in.put(lds + L::kTiles + slot * L::kTile, lane);
+            const int e = bits_exp(in.max_bits()) + 1;  // below 2^e
+            if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[slot] = e;
         }
     };
     auto results = [&](int c) {
-        char* rec = a.rec + chunk(c) * a.stride;
-        if (!active) return;
-        store_turned<NT>(ts, rec + (BACK ? p.rec.ds1 : p.rec.s0), tile, half, lane);
-        store_turned<4>(tw, rec + (BACK ? p.rec.x : p.rec.w), tile, half, lane);
+        if constexpr (ACTIVE) {
+            char* rec = a.rec + chunk(c) * a.stride;
+            store_turned<NT / 2>(ts0, ts1, rec + (BACK ? p.rec.ds1 : p.rec.s0) + first * NT * 1024, half * (NT / 2), lane);
+            store_turned<2>(tw0, tw1, rec + (BACK ? p.rec.x : p.rec.w) + first * 4 * 1024, half * 2, lane);
+        }
     };
     if (a.nc > 0) {
         load(0);
         store(0);
+        store_rest(0);
         load(1);
-    }
-    for (int c = 0; c < a.nc; ++c) {
         __syncthreads();  // A
-        if (c > 0) results(c - 1);
+        store(1);
         __syncthreads();  // B
-        if (c + 1 < a.nc) {
+        store_rest(1);
+        load(2);
+        for (int c = 1; c < a.nc; ++c) {
+            __syncthreads();  // A
+            results(c - 1);
             store(c + 1);
+            __syncthreads();  // B
+            store_rest(c + 1);
             load(c + 2);
         }
     }
@@ -1011,15 +1111,19 @@ __device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a
 }
 
 template <typename T, int DK, bool VEC>
-__global__ __launch_bounds__(768) void bwd_scan16_kernel(BwdParams p, int splits) {
+__global__ __launch_bounds__(512) void bwd_scan16_kernel(BwdParams p, int splits) {
     __shared__ __align__(16) char lds[Scan16Lds<DK>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ScanAt a;
     if (!scan_at(p, splits, a)) return;
-    const int tile = a.part * 4 + (wave & 3);
+    const int tile = a.part * 4 + wave;
+    auto serve = [&](auto back, auto active) {
+        scan16_serve<T, DK, VEC, back.value, active.value>(p, a, threadIdx.x - 256, lds);
+    };
     if (wave >= 4) {
-        if (a.back) scan16_serve<T, DK, VEC, true>(p, a, tile, threadIdx.x - 256, lds);
-        else scan16_serve<T, DK, VEC, false>(p, a, tile, threadIdx.x - 256, lds);
+        const bool active = a.part * 4 + 2 * (wave & 1) < p.dvt;  // dvt is even
+        if (a.back) active ? serve(std::true_type{}, std::true_type{}) : serve(std::true_type{}, std::false_type{});
+        else active ? serve(std::false_type{}, std::true_type{}) : serve(std::false_type{}, std::false_type{});
     } else if (tile < p.dvt) {
         if (a.back) scan16_carry<T, DK, VEC, true>(p, a, tile, wave, lane, lds);
         else scan16_carry<T, DK, VEC, false>(p, a, tile, wave, lane, lds);
@@ -1138,6 +1242,7 @@ __device__ __forceinline__ void scan32(const BwdParams& p, const ScanAt& a, char
     }
     for (int c = 0; c < a.nc; ++c) {
         st.store(lds, threadIdx.x);
+        st.store_back(lds, threadIdx.x);
         in.put(mine, threadIdx.x & 255);
         __syncthreads();
         st.load(p, at, chunk(c + 1), a.rec + chunk(c + 1) * a.stride, threadIdx.x);
@@ -1204,7 +1309,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     constexpr int NS = (NT * 64 + 255) / 256;      // 16-byte pieces of S0's tile per thread
     constexpr int NO = 64 * L::kTdv / R / 256;     // runs of dO's tile per thread
     constexpr int NK = 64 * DK / R / 256;          // runs of K (and of Q) per thread
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
+    const int tid = thread_index(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4,
               m = lane & 15;
     const RowMat<Op, DK> Kr{lds + L::kKr}, Qr{lds + L::kQr};
     float* M = reinterpret_cast<float*>(lds + L::kM);
@@ -1663,9 +1768,14 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
     constexpr int NO = kOwn<DK> / 16;
     constexpr int kPrep = PrepLds<OpF32, DK>::kBytes, kGrad = GradLds<OpF32, DK>::kBytes;
     __shared__ __align__(16) char lds[std::max(std::max(kPrep, kGrad), L::kBytes)];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-    const int c0 = kOwn<DK> * w + 4 * g;
-    const bool own = w * NO < DK / 16;
+    struct Thread {
+        int tid, w, lane, m, g, c0;
+        bool own;
+    };
+    auto thread = [] {
+        const int tid = thread_index(), w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4;
+        return Thread{tid, w, lane, lane & 15, g, kOwn<DK> * w + 4 * g, w * NO < DK / 16};
+    };
     BwdParams e = p;
     e.rec = rec_layout(DK, p.dvt, 4);
     char* rec = scratch + blockIdx.x * exact_scratch(DK, p.dvt);
@@ -1698,49 +1808,52 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
             return at;
         };
         using St = State<OpF32, kOwn<DK>>;
-        auto get = [&](St& S, char* base, int tile) {
-            const f32x4* b = kept_state<DK>(base, tile, w, lane);
+        auto get = [&](const Thread& id, St& S, char* base, int tile) {
+            const f32x4* b = kept_state<DK>(base, tile, id.w, id.lane);
             S.e = 0;
-            if (own)
+            if (id.own)
 #pragma unroll
                 for (int i = 0; i < NO; ++i) S.s[i] = b[i * 64];
         };
-        auto put = [&](const St& S, char* base, int tile) {
-            f32x4* b = kept_state<DK>(base, tile, w, lane);
-            if (own)
+        auto put = [&](const Thread& id, const St& S, char* base, int tile) {
+            f32x4* b = kept_state<DK>(base, tile, id.w, id.lane);
+            if (id.own)
 #pragma unroll
                 for (int i = 0; i < NO; ++i) b[i * 64] = S.s[i];
         };
         // chunk c of every tile: forward from the states of `kept` to those of
         // `next`, or back over it on the states' gradients, in place
         auto step = [&](auto back, int c, char* kept, char* next) {
+            const Thread id = thread();
             const SeqAt<T> from = seq_at<T>(p, seq, h, back.value);
             __syncthreads();
             ScanStage<OpF32, T, DK, VEC, back.value> sg;
-            sg.load(e, from, c, rec, threadIdx.x);
-            sg.store(lds, threadIdx.x);
+            sg.load(e, from, c, rec, id.tid);
+            sg.store(lds, id.tid);
+            sg.store_back(lds, id.tid);
             for (int tile = 0; tile < p.dvt; ++tile) {
                 St S;
-                get(S, kept, tile);
+                get(id, S, kept, tile);
                 __syncthreads();
                 TileRuns<T, VEC, 256> in;
-                in.load(e, from, c, tile, threadIdx.x);
-                in.put(mine, threadIdx.x);
-                if (own)
+                in.load(e, from, c, tile, id.tid);
+                in.put(mine, id.tid);
+                if (id.own)
 #pragma unroll
-                    for (int b = 0; b < NO; ++b) turn_s.put_unit(m, w * NO + b, g, S.s[b]);
+                    for (int b = 0; b < NO; ++b) turn_s.put_unit(id.m, id.w * NO + b, id.g, S.s[b]);
                 __syncthreads();
-                scan32_chunk<T, DK, 1, back.value>(e, S, rec, lds, mine, tile, w, lane);
-                if (next) put(S, next, tile);
+                scan32_chunk<T, DK, 1, back.value>(e, S, rec, lds, mine, tile, id.w, id.lane);
+                if (next) put(id, S, next, tile);
             }
             __syncthreads();
         };
         // a state's tiles from where the caller has it
         auto begin = [&](const float* from, char* base) {
+            const Thread id = thread();
             for (int tile = 0; tile < p.dvt; ++tile) {
                 St S;
-                S.load(p, from ? from + st : nullptr, 16 * tile + m, c0);
-                put(S, base, tile);
+                S.load(p, from ? from + st : nullptr, 16 * tile + id.m, id.c0);
+                put(id, S, base, tile);
             }
         };
         begin(p.init, first + p.rec.s0);
@@ -1757,12 +1870,14 @@ __global__ __launch_bounds__(256, 1) void bwd_exact_kernel(BwdParams p, char* sc
             grad_chunk<OpF32, T, DK, VEC>(e, chunk(c), h, rec, lds);
             __syncthreads();
         }
-        if (p.dinit)
+        if (p.dinit) {
+            const Thread id = thread();
             for (int tile = 0; tile < p.dvt; ++tile) {
                 St S;
-                get(S, carry, tile);
-                if (own) S.store(p, p.dinit + st, 16 * tile + m, c0);
+                get(id, S, carry, tile);
+                if (id.own) S.store(p, p.dinit + st, 16 * tile + id.m, id.c0);
             }
+        }
     }
 }
 
@@ -1833,7 +1948,7 @@ hipError_t go(const BwdParams& p, int64_t chunks, char* scratch, int blocks, hip
     }
     if (grid > 0 || p.dinit) {
         if constexpr (Op::kScaled)
-            hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(768), 0, st, p, splits);
+            hipLaunchKernelGGL((bwd_scan16_kernel<T, DK, VEC>), dim3((unsigned)scans), dim3(512), 0, st, p, splits);
         else if (tiles == 1)
             hipLaunchKernelGGL((bwd_scan32_kernel<T, DK, VEC, 1>), dim3((unsigned)scans), dim3(256), 0, st, p, splits);
         else
@@ -1905,6 +2020,7 @@ hipError_t launch_backward(const rhz_gdr_prefill_backward_args& a, hipStream_t s
     p.dvt = tiles_dv(a.d_v);
     p.gate_is_alpha = a.gate_kind == RHZ_GATE_ALPHA;
     p.rec = rec_layout(DK, p.dvt, es);
+    p.short_rows = (int64_t)a.heads * std::max(a.d_k, a.d_v) * C64 * es < INT32_MAX;
     // rows of q, k, v, dO and of their gradients as whole runs of 16 bytes
     const int run = 16 / es;
     const bool vec = a.d_k % run == 0 && a.d_v % run == 0 && aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) &&

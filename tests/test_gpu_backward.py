@@ -198,6 +198,20 @@ def test_magnitudes_along_a_bf16_sequence(device):
             assert float((x - y).norm()) <= TOL[torch.bfloat16] * float(y.norm()), (part, NAMES[i])
 
 
+@pytest.mark.parametrize("decay", [0.0, -0.05])
+@pytest.mark.parametrize("d_k,d_v", [(128, 64), (32, 64)])
+def test_tokens_that_agree_in_bf16(device, d_k, d_v, decay):
+    """Queries, keys, values and output gradients all along one direction: a
+    chunk's sums over its tokens and channels have every term of one sign."""
+    d = inputs(torch.bfloat16, [200, 64], 2, d_k, d_v, seed=8, state=False)
+    for name, x in (("q", 1.9), ("v", 1.0), ("do", 1.9)):
+        d[name] = (d[name].double() * 0.01 + x).to(torch.bfloat16)
+    d["k"].fill_(d_k ** -0.5)
+    d["beta"].fill_(0.02)
+    d["g"].fill_(decay)
+    check(call(d, [200, 64], device), reference(d, [200, 64]), torch.bfloat16)
+
+
 @pytest.mark.parametrize("what", ["long keys", "beta above 1", "alpha above 1"])
 def test_bf16_outside_the_domain(device, what):
     """One head of two leaves the fp16 path's domain and is computed in fp32;
