@@ -1368,7 +1368,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     for (int b = 0; b < 5; ++b) e1[b] = e2[b] = f32x4{0, 0, 0, 0};
     float ip = 0.f;  // <dS1, S0>
 
-    for (int t = 0; t < tiles; ++t) {
+    auto tile = [&](int t, auto ahead) {
         char* buf = lds + (t & 1) * L::kBuf;
         int s0e = 0, s1e = 0, d0e = 0, d1e = 0, w0e = 0, w1e = 0, x0e = 0, x1e = 0;
         if constexpr (Op::kScaled) {
@@ -1414,7 +1414,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
             }
         }
         __syncthreads();
-        if (t + 1 < tiles) load_tile(t + 1);
+        ahead();
         // dV = dX
         {
             constexpr int NP = 64 * L::kTdv / 8;  // pieces of eight columns
@@ -1475,12 +1475,13 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
             e1[4] = Op::mma(bo, c1, e1[4]);
             e2[4] = Op::mma(bx, c2, e2[4]);
         }
-    }
+    };
+    for (int t = 0; t + 1 < tiles; ++t) tile(t, [&] { load_tile(t + 1); });
     // K and Q by rows, where the tiles were
-    {
+    u32x4 rk[NK], rq[NK];
+    tile(tiles - 1, [&] {
         const T* kp = static_cast<const T*>(p.k) + ok;
         const T* qp = static_cast<const T*>(p.q) + ok;
-        u32x4 rk[NK], rq[NK];
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             const int id = tid + 256 * i, tk = id / (DK / R), c = id % (DK / R) * R;
@@ -1488,6 +1489,8 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
             rk[i] = load_run<T, VEC>(kp + tk * ldk + c, in, p.d_k - c);
             rq[i] = load_run<T, VEC>(qp + tk * ldk + c, in, p.d_k - c);
         }
+    });
+    {
         const float sk = exp2i(-ek), sq = exp2i(-eq);
         __syncthreads();
 #pragma unroll
