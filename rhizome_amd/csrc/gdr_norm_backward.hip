@@ -13,6 +13,10 @@
 // The rows of a block run along its persistent threads, each of which keeps
 // its columns' share of dw and db in registers; the blocks' shares go to the
 // workspace and a second kernel adds them in a fixed order.
+//
+// bf16, of a copy's 5.2 TB/s: layer norm of 16384 rows of 2048, 0.13 GB in 27 us
+// (5.0 TB/s); its backward pass, 0.21 GB in 43 us (4.9) and 4 us for the sums;
+// RMSNorm's backward pass of 262144 rows of 128, 0.20 GB in 38 us (5.3) and 4 us.
 
 #include <algorithm>
 
@@ -277,14 +281,17 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, in
     }
 }
 
-constexpr int kNormBlocks = 512;  // two per CU
+constexpr int kNormBlocks = 512;  // two per CU (four: 16384 rows of 2048 backward 54 us instead of 47)
 
 struct NormShape {
     bool vec;
     int g, nv, unroll;
 };
 // Lanes per row and vectors per lane: as few lanes as hold the row in one
-// vector each, a wave with up to eight (scalar: sixteen), then the block.
+// vector each, a wave with up to four (scalar: sixteen), then the block.  bf16,
+// layer norm and its backward pass: rows of 64 on 8 lanes 28 and 52 us, on 16
+// lanes 44 and 81 (524288 rows); of 2048 on a wave 28 and 47 us, on a block 34
+// and 112 (16384 rows); of 4096 on a wave 29 and 92 us, on a block 27 and 62.
 NormShape norm_shape(int dtype, int dim, bool vec) {
     const int n = dtype == RHZ_F32 ? 4 : 8;
     if (vec && dim % n == 0) {
@@ -295,7 +302,7 @@ NormShape norm_shape(int dtype, int dim, bool vec) {
         if (v <= 64) return {true, 64, 1, 4};
         if (v <= 128) return {true, 64, 2, 2};
         if (v <= 256) return {true, 64, 4, 1};
-        if (v <= 512) return {true, 64, 8, 1};
+        if (v <= 512) return {true, 256, 2, 1};
         if (v <= 1024) return {true, 256, 4, 1};
         return {true, 256, 8, 1};
     }
@@ -323,7 +330,7 @@ hipError_t go_norm(const NormParams& p, const NormShape& s, int64_t blocks, hipS
     RHZ_NORM(true, 64, 1);
     RHZ_NORM(true, 64, 2);
     RHZ_NORM(true, 64, 4);
-    RHZ_NORM(true, 64, 8);
+    RHZ_NORM(true, 256, 2);
     RHZ_NORM(true, 256, 4);
     RHZ_NORM(true, 256, 8);
     RHZ_NORM(false, 16, 4);
