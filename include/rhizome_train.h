@@ -30,8 +30,9 @@ extern "C" {
  * operands, scaled tile by tile by powers of two, with fp32 accumulation and
  * fp32 states; fp32 tensors in fp32 throughout.  A bf16 head whose inputs
  * leave the prefill's domain (a key row with |k|^2 > 1.03125, a beta or alpha
- * outside [0, 1], a value that is not finite, q, k, v and grad_o included) is
- * computed in fp32 in the same call, several times slower.  fp32 tensors are
+ * outside [0, 1], a value that is not finite, q, k, v and grad_o included, or a
+ * sum that leaves fp16's range) is computed in fp32 in the same call, several
+ * times slower.  fp32 tensors are
  * accurate where beta |k|^2 <= 2 and alpha <= 1.
  *
  * grad_gate is the gradient of the gate as it is given: of g, or of alpha

@@ -17,6 +17,11 @@
 // span of tokens: dy_t adds to the four open dx_{t-3} .. dx_t, the first of
 // which is then complete.  Spans are long, so that the spans' shares of dw and
 // db, which go through the workspace, stay small next to the tensors.
+//
+// 16384 tokens of 6144 channels in bf16: 150 us for 0.65 GB (4.3 TB/s, a copy
+// reaches 5.2; 5 % of it the spans' edges and shares) and 5 us for the sums.  The
+// rest is the row norms' chain, y.dq and |y|^2 over a head's lanes before dy of a
+// token is there.
 
 #include <algorithm>
 
