@@ -18,8 +18,8 @@
 // which is then complete.  Spans are long, so that the spans' shares of dw and
 // db, which go through the workspace, stay small next to the tensors.
 //
-// 16384 tokens of 6144 channels in bf16: 150 us for 0.65 GB (4.3 TB/s, a copy
-// reaches 5.2; 5 % of it the spans' edges and shares) and 5 us for the sums.  The
+// 16384 tokens of 6144 channels in bf16: 140 us for 0.65 GB (4.6 TB/s, a copy
+// reaches 5.2; 5 % of it the spans' edges and shares) and 8 us for the sums.  The
 // rest is the row norms' chain, y.dq and |y|^2 over a head's lanes before dy of a
 // token is there.
 
@@ -302,9 +302,13 @@ __global__ __launch_bounds__(1024) void conv_backward_sums_kernel(ConvBackParams
 struct ConvBackShape {
     int total, n, ncb, span, spans, gate_tokens, gates;
 };
-// About kBlocks blocks of 256 threads (two per CU): fewer would leave HBM
-// waiting, more would write more shares of dw (20 bytes per channel and span).
-constexpr int kBlocks = 512, kMinSpan = 16;
+// About kBlocks blocks of 256 threads (four per CU): fewer leave HBM waiting,
+// more write more shares of dw (20 bytes per channel and span).  16384 tokens of
+// 6144 channels in bf16, whole call: 174 us with 256 blocks, 159 with 512, 148
+// with 1024, 158 with 1536, 166 with 2048.  Spans are 8 tokens at least: six more
+// are read at their edges.  64 tokens, waited for: 43 us, 48 with spans of 16; 1080
+// tokens of 1536 channels in fp32 29.3 and 28.8 us.
+constexpr int kBlocks = 1024, kMinSpan = 8;
 ConvBackShape conv_back_shape(const rhz_gdr_conv_prepare_backward_args& a) {
     ConvBackShape s{};
     s.total = a.cu_seqlens ? a.seq_len : a.batch * a.seq_len;
