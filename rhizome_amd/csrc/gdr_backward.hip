@@ -936,7 +936,6 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
     constexpr int NT = DK / 16, NU = NT / 2;
     const int g = lane >> 4, m = lane & 15, row = 16 * tile + m;
     const float* from = BACK ? p.dfinal : p.init;
-    __builtin_amdgcn_s_setprio(2);  // the chain goes before the wave that serves it on the same SIMD
     State<Op, DK> S;
     S.load(p, from ? from + a.state : nullptr, row, 4 * g);
     const RowMat<Op, DK> ts{lds + L::kTurn + wave * (L::kTurnS + L::kTurnW)};
