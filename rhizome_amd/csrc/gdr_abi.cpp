@@ -58,10 +58,10 @@ rhz_status check_prefill(const rhz_gdr_prefill_args* a, bool check_ptrs, int* al
     if (a->d_k > 256) return fail(RHZ_ERR_UNSUPPORTED, "d_k = %d exceeds the supported 256", a->d_k);
     if (a->d_v > 1024) return fail(RHZ_ERR_UNSUPPORTED, "d_v = %d exceeds the supported 1024", a->d_v);
     const int64_t tokens = a->cu_seqlens ? (int64_t)a->seq_len : (int64_t)a->batch * a->seq_len;
-    if (tokens * a->heads > kMaxIndex)
-        return fail(RHZ_ERR_INVALID_ARG, "tokens * heads = %lld exceeds 2^31 - 1", (long long)(tokens * a->heads));
+    if (rhz::exceeds(tokens, a->heads, kMaxIndex))
+        return fail(RHZ_ERR_INVALID_ARG, "tokens * heads = %lld * %d exceeds 2^31 - 1", (long long)tokens, a->heads);
     const int64_t units = (int64_t)a->batch * a->heads;
-    if (units * ((a->d_v + 7) / 8) > kMaxIndex)
+    if (rhz::exceeds(units, (a->d_v + 7) / 8, kMaxIndex))
         return fail(RHZ_ERR_INVALID_ARG, "batch * heads = %lld is too large", (long long)units);
 
     int algo = a->algo;
@@ -329,7 +329,7 @@ rhz_status rhz_gdr_multistep(const rhz_gdr_multistep_args* a, void* stream) {
         return fail(RHZ_ERR_UNSUPPORTED, "steps = %d exceeds the supported %d", a->steps, RHZ_MULTISTEP_MAX);
     if (a->d_k > 256) return fail(RHZ_ERR_UNSUPPORTED, "d_k = %d exceeds the supported 256", a->d_k);
     if (a->d_v > 1024) return fail(RHZ_ERR_UNSUPPORTED, "d_v = %d exceeds the supported 1024", a->d_v);
-    if ((int64_t)a->batch * a->heads * a->steps > kMaxIndex)
+    if (rhz::exceeds((int64_t)a->batch * a->heads, a->steps, kMaxIndex))
         return fail(RHZ_ERR_INVALID_ARG, "batch * steps * heads exceeds 2^31 - 1");
     if (!a->q) return fail(RHZ_ERR_INVALID_ARG, "q is NULL");
     if (!a->k) return fail(RHZ_ERR_INVALID_ARG, "k is NULL");
@@ -363,7 +363,7 @@ rhz_status rhz_causal_conv1d(const rhz_conv1d_args* a, void* stream) {
     if (a->dtype != RHZ_F32 && a->dtype != RHZ_BF16)
         return fail(RHZ_ERR_INVALID_ARG, "dtype must be RHZ_F32 or RHZ_BF16 (got %d)", a->dtype);
     const int64_t tokens = a->cu_seqlens ? a->seq_len : (int64_t)a->batch * a->seq_len;
-    if (tokens * a->channels > kMaxIndex || (int64_t)a->batch * a->channels * 3 > kMaxIndex)
+    if (rhz::exceeds(tokens, a->channels, kMaxIndex) || rhz::exceeds(a->batch, (int64_t)a->channels * 3, kMaxIndex))
         return fail(RHZ_ERR_INVALID_ARG, "tokens * channels and batch * channels * 3 must stay below 2^31");
     if (tokens > 0 && (!a->x || !a->y)) return fail(RHZ_ERR_INVALID_ARG, "x or y is NULL");
     if (!a->weight) return fail(RHZ_ERR_INVALID_ARG, "weight is NULL");
@@ -384,7 +384,7 @@ rhz_status rhz_gdr_prepare(const rhz_gdr_prepare_args* a, void* stream) {
     if (a->dtype != RHZ_F32 && a->dtype != RHZ_BF16)
         return fail(RHZ_ERR_INVALID_ARG, "dtype must be RHZ_F32 or RHZ_BF16 (got %d)", a->dtype);
     if (a->d_k > 256) return fail(RHZ_ERR_UNSUPPORTED, "d_k = %d exceeds the supported 256", a->d_k);
-    if ((int64_t)a->tokens * a->heads * a->d_k > kMaxIndex)
+    if (rhz::exceeds((int64_t)a->tokens * a->heads, a->d_k, kMaxIndex))
         return fail(RHZ_ERR_INVALID_ARG, "tokens * heads * d_k exceeds 2^31 - 1");
     if (!std::isfinite(a->q_scale)) return fail(RHZ_ERR_INVALID_ARG, "q_scale must be finite");
     if (a->tokens == 0) return ok();
@@ -418,7 +418,7 @@ rhz_status rhz_gdr_conv_prepare(const rhz_gdr_conv_prepare_args* a, void* stream
                     a->d_k, a->d_v, a->dtype == RHZ_F32 ? 4 : 8, a->dtype == RHZ_F32 ? 4 : 8);
     const int64_t C = (int64_t)a->heads * (2 * a->d_k + a->d_v);
     const int64_t tokens = a->cu_seqlens ? a->seq_len : (int64_t)a->batch * a->seq_len;
-    if (tokens * C > kMaxIndex || (int64_t)a->batch * C * 3 > kMaxIndex)
+    if (rhz::exceeds(tokens, C, kMaxIndex) || rhz::exceeds(a->batch, C * 3, kMaxIndex))
         return fail(RHZ_ERR_INVALID_ARG, "tokens * channels and batch * channels * 3 must stay below 2^31");
     if (!a->weight) return fail(RHZ_ERR_INVALID_ARG, "weight is NULL");
     if (tokens > 0) {

@@ -15,6 +15,9 @@ namespace rhz {
 // Keeps `detail` as the calling thread's last error (rhz_last_error); returns s.
 rhz_status record_error(rhz_status s, const char* detail);
 
+// a * b > limit, of sizes whose product may leave 64 bits
+inline bool exceeds(int64_t a, int64_t b, int64_t limit) { return b > 0 && a > limit / b; }
+
 // Whether the runtime launches a grid of `blocks` workgroups of `threads` along
 // x as asked: it truncates one of 2^32 work-items or more without an error.
 inline hipError_t check_grid(int64_t blocks, int threads) {

@@ -85,8 +85,8 @@ rhz_status check_backward(const rhz_gdr_prefill_backward_args* a) {
     if (a->d_k > 128) return fail(RHZ_ERR_UNSUPPORTED, "d_k = %d exceeds the backward pass's 128", a->d_k);
     if (a->d_v > 1024) return fail(RHZ_ERR_UNSUPPORTED, "d_v = %d exceeds the supported 1024", a->d_v);
     const int64_t tokens = a->cu_seqlens ? (int64_t)a->seq_len : (int64_t)a->batch * a->seq_len;
-    if (tokens * a->heads > kMaxIndex)
-        return fail(RHZ_ERR_INVALID_ARG, "tokens * heads = %lld exceeds 2^31 - 1", (long long)(tokens * a->heads));
+    if (rhz::exceeds(tokens, a->heads, kMaxIndex))
+        return fail(RHZ_ERR_INVALID_ARG, "tokens * heads = %lld * %d exceeds 2^31 - 1", (long long)tokens, a->heads);
     if ((int64_t)a->batch * a->heads > kMaxIndex / 128)
         return fail(RHZ_ERR_INVALID_ARG, "batch * heads = %lld is too large", (long long)a->batch * a->heads);
     return ok();
@@ -111,7 +111,7 @@ rhz_status check_conv_backward(const rhz_gdr_conv_prepare_backward_args* a) {
     }
     const int64_t C = (int64_t)a->heads * (2 * a->d_k + a->d_v);
     const int64_t tokens = a->cu_seqlens ? a->seq_len : (int64_t)a->batch * a->seq_len;
-    if (tokens * C > kMaxIndex || (int64_t)a->batch * C * 3 > kMaxIndex || C * 4 > kMaxIndex)
+    if (rhz::exceeds(tokens, C, kMaxIndex) || rhz::exceeds(a->batch, C * 3, kMaxIndex) || C * 4 > kMaxIndex)
         return fail(RHZ_ERR_INVALID_ARG, "tokens * channels and batch * channels * 3 must stay below 2^31");
     return ok();
 }
