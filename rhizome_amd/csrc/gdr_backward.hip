@@ -237,7 +237,7 @@ __device__ __forceinline__ int bits_exp(int bits) { return max(min((bits >> 23) 
 // below 2^-14 are then 2^-16 of it at most), else the largest value's.
 __device__ __forceinline__ int rows_exp(int bits) {
     const int e = bits_exp(bits);
-    return e >= -8 && e < 4 ? 0 : e;
+    return bits == 0 || (e >= -8 && e < 4) ? 0 : e;
 }
 
 // A run of 16 bytes of a row of T (8 bf16 or 4 fp32).  VEC: rows are whole runs
@@ -973,17 +973,19 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su[i], x[b]);
-        // the next state is S times 2^-e, W and dX are kept times 2^-(e - ek):
-        // the larger of the state and of V (of dO times rows of Q or P) at 2^5 or 2^6
-        const int se = S.e, e = max(top + se, ev + (BACK ? eq + 2 : 0)) - 5;
+        // the next state is S times 2^-e, W or dX are kept times 2^-ew, the larger of
+        // what the state and V (dO times rows of Q) give at 2^5 or 2^6: with ek < 0
+        // (small keys) W is of V's size, its share of the state 2^ek of it
+        const int se = S.e, other = ev + (BACK ? eq + 2 : ek);
+        const int e = max(top + se, other) - 5, ew = BACK ? e + ek : max(top + se + ek, ev) - 5;
         Unit ru[2];
         if constexpr (!BACK) {
-            const float sv = exp2i(ek - e), sx = -exp2i(se + ek + ek - e);
+            const float sv = exp2i(-ew), sx = -exp2i(se + ek - ew);
 #pragma unroll
             for (int b = 0; b < 4; ++b) w[b] = vo[b] * sv + (by_token(kVecGamma, b) * sx) * x[b];
         } else {
             const int eo = ev + 1;  // dO as an operand: below 1/2
-            const float so = exp2i(-eo), sz = exp2i(eo + eq + ek + ek - e), sx = exp2i(se + ek + ek - e);
+            const float so = exp2i(-eo), sz = exp2i(eo + eq + ek - ew), sx = exp2i(se + ek - ew);
             f32x4 z[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) z[b] = f32x4{0, 0, 0, 0};
@@ -1016,7 +1018,7 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         for (int b = 0; b < NT; ++b) S.s[b] *= sg;
         S.e = e;
         if (lane == 0) {
-            exps[(BACK ? kExpX : kExpW) + tile] = e - ek;
+            exps[(BACK ? kExpX : kExpW) + tile] = ew;
             exps[(BACK ? kExpD : kExpS) + tile] = se;
             if constexpr (BACK) exps[kExpO + tile] = ev + 1;
         }
@@ -1026,13 +1028,14 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         for (int i = 0; i < NU; ++i) ts.put_unit(m, i, g, su[i]);
 #pragma unroll
         for (int u = 0; u < 2; ++u) tw.put_unit(m, u, g, Op::pack(&w[u * 2], 1.f));
-        const float sd = exp2i(eq - e);
+        const float sd = exp2i(eq - e), sw = exp2i(ew + ek - e);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f32x4 f[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b) f[b] = by_token(BACK ? kVecGamma : kVecWrite, u * 2 + b);
-            Unit wu = pack_products(&w[u * 2], f);
+            const f32x4 fw[2] = {f[0] * sw, f[1] * sw};
+            Unit wu = pack_products(&w[u * 2], fw);
             if constexpr (BACK) wu = -wu;
 #pragma unroll
             for (int b = 0; b < NT; ++b) S.s[b] = Op::mma(u ? K.cols(b, u, lane) : kc[b], wu, S.s[b]);

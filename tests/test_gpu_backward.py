@@ -198,6 +198,19 @@ def test_magnitudes_along_a_bf16_sequence(device):
             assert float((x - y).norm()) <= TOL[torch.bfloat16] * float(y.norm()), (part, NAMES[i])
 
 
+@pytest.mark.parametrize("size", [0.0, 1e-2, 1e-4, 2e-5, 1e-6, 1e-12])
+def test_small_keys_in_bf16(device, size):
+    """Keys of a chunk that are zero or small: what they multiply keeps its
+    size, and so do the gradients that do not pass through them."""
+    d = inputs(torch.bfloat16, [200, 64], 2, 64, 64, seed=9)
+    d["k"][64:128] = (d["k"][64:128].double() * size).to(torch.bfloat16)
+    d["k"][200:, 1] = (d["k"][200:, 1].double() * size).to(torch.bfloat16)
+    got, want = call(d, [200, 64], device), reference(d, [200, 64])
+    check(got, want, torch.bfloat16)
+    for rows in (slice(64, 128), slice(200, 264)):  # each chunk against its own norm
+        check([x[rows] for x in got[:3]], [x[rows] for x in want[:3]], torch.bfloat16, str(rows))
+
+
 @pytest.mark.parametrize("decay", [0.0, -0.05])
 @pytest.mark.parametrize("d_k,d_v", [(128, 64), (32, 64)])
 def test_tokens_that_agree_in_bf16(device, d_k, d_v, decay):
