@@ -1307,6 +1307,16 @@ __device__ __forceinline__ void unit_dots(const f16x8& a, const f16x8& b, float 
 __device__ __forceinline__ void unit_dots(const f32x4& a, const f32x4& b, float (&s)[1]) {
     s[0] = a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
 }
+// The exponent of the largest value of a column of four tiles, whose rows lie in
+// the lanes m, 16 + m, 32 + m and 48 + m.
+__device__ __forceinline__ int column_exp(const f32x4 (&x)[4]) {
+    float mx = 0.f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x[b][0])), fabsf(x[b][1])), fmaxf(fabsf(x[b][2]), fabsf(x[b][3])));
+    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+    return bits_exp(bits_abs(fmaxf(mx, __shfl_xor(mx, 32, kWave))));
+}
 // a unit with its two blocks times 2^d0 and 2^d1, d <= 0
 __device__ __forceinline__ f16x8 shift_unit(f16x8 u, int d0, int d1) {
     const _Float16 f = (_Float16)exp2i(d0), h = (_Float16)exp2i(d1);
@@ -1557,6 +1567,24 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
     // with its decay to M
     f32x4 mh[4];
     Unit n1[NKT], n2[NKT];
+    // A column of N1 or N2 is rounded to fp16 by a power of two of its own, which
+    // the products' results, columns of the same token, take back: its values are
+    // sums over all of d_v, without a bound within fp16's range (ones everywhere,
+    // beta = 1/2, d_v = 256: 84000), and proportional to beta, without one from
+    // its subnormals either.
+    int en1 = 0, en2 = 0;
+    auto pack_n = [&](const f32x4 (&x1)[4], const f32x4 (&x2)[4]) {
+        if constexpr (Op::kScaled) {
+            en1 = column_exp(x1);
+            en2 = column_exp(x2);
+        }
+        const float f1 = exp2i(-en1), f2 = exp2i(-en2);
+#pragma unroll
+        for (int u = 0; u < NKT; ++u) {
+            n1[u] = Op::pack(&x1[u * NBK], f1);
+            n2[u] = Op::pack(&x2[u * NBK], f2);
+        }
+    };
     {
         const float sqk = exp2i(eq + ek) * s1, skk = exp2i(2 * ek) * s2;
         Unit uk[NU], uq[NU];
@@ -1591,17 +1619,13 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
             }
             *reinterpret_cast<f32x4*>(M + sq_at(tok, 16 * b + 4 * g)) = y;
         }
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) {
-            n1[u] = Op::pack(&x1[u * NBK], 1.f);
-            n2[u] = Op::pack(&x2[u * NBK], 1.f);
-        }
+        pack_n(x1, x2);
     }
     // dQ = diag(gamma) dO S0 + N1 K;  K's share of dK: -N2 K - N2^T K
     const long orow = ok + tok * ldk;
     f32x4 ak[NT];
     {
-        const float f1 = gam * exp2i(eo + es), f2 = s1 * exp2i(ek);
+        const float f1 = gam * exp2i(eo + es), f2 = exp2i(eo + ew + ek + en1), fn = -exp2i(exw + ek + en2);
         T* dq = static_cast<T*>(p.dq) + orow;
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
@@ -1619,6 +1643,7 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] = zq[b][j] * f1 + c[j] * f2;
             if (tok < at.n) store_run<T, VEC, 4>(dq + col, p.d_k - col, y);
+            ak[b] *= fn;
         }
     }
     {
@@ -1636,25 +1661,22 @@ __device__ __forceinline__ void grad_chunk(const BwdParams& p, const ChunkAt& at
                 }
             }
         }
-#pragma unroll
-        for (int u = 0; u < NKT; ++u) {
-            n1[u] = Op::pack(&x1[u * NBK], 1.f);
-            n2[u] = Op::pack(&x2[u * NBK], 1.f);
-        }
-        const float fk = -gam * exp2i(exs), fw = bet * tail * exp2i(ed), fq = s1 * exp2i(eq), fn = -s2 * exp2i(ek);
+        pack_n(x1, x2);
+        const float fk = -gam * exp2i(exs), fw = bet * tail * exp2i(ed);
+        const float fq = exp2i(eo + ew + eq + en1), fn = -exp2i(exw + ek + en2);
         T* dk = static_cast<T*>(p.dk) + orow;
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            f32x4 c = {0, 0, 0, 0};
+            f32x4 c = {0, 0, 0, 0}, n = {0, 0, 0, 0};
 #pragma unroll
             for (int u = 0; u < NKT; ++u)
                 if (u * NBK + NBK > wave) {
                     c = Op::mma(Qr.cols(b, u, lane), n1[u], c);
-                    ak[b] = Op::mma(Kr.cols(b, u, lane), n2[u], ak[b]);
+                    n = Op::mma(Kr.cols(b, u, lane), n2[u], n);
                 }
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = zk[b][j] * fk + zw[b][j] * fw + c[j] * fq + ak[b][j] * fn;
+            for (int j = 0; j < 4; ++j) y[j] = zk[b][j] * fk + zw[b][j] * fw + c[j] * fq + (ak[b][j] + n[j] * fn);
             const int col = 16 * b + 4 * g;
             if (tok < at.n) store_run<T, VEC, 4>(dk + col, p.d_k - col, y);
         }

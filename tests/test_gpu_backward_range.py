@@ -1,0 +1,60 @@
+"""The bf16 backward pass of the delta-rule prefill where its fp16 operands
+come near the ends of fp16's range, against the same reference and with the
+same tolerances as test_gpu_backward.py.
+
+The inputs are such that a gradient does not cancel to a small remainder of the
+terms that it is summed from, whose rounding the tolerances count: keys that
+repeat have beta up to 1/2, a decay beside it, and so on.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_backward import call, check, inputs, reference
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def alike(lengths, H, dk, dv, keys, beta, decay):
+    """Queries, values and output gradients near one direction.  `keys`: one key
+    for all tokens, unit vectors in turn, or random ones with a mean."""
+    d = inputs(BF16, lengths, H, dk, dv, seed=31, state=False)
+    noise = 1.0 if keys == "random" else 0.01
+    for name, x in (("q", 1.0), ("v", 1.0), ("do", 1.9)):
+        d[name] = (d[name].double() * noise + (2.0 if keys == "random" else x)).to(BF16)
+    n = d["k"].shape[0]
+    if keys == "one":
+        d["k"].fill_(dk ** -0.5)
+    elif keys == "units":
+        d["k"] = torch.eye(dk)[torch.arange(n) % dk][:, None].expand(n, H, dk).contiguous().to(BF16)
+    else:
+        d["q"], k = d["q"].double(), d["k"].double() * math.sqrt(dk) + 2.0
+        d["q"] = (d["q"] / d["q"].norm(dim=-1, keepdim=True) * math.sqrt(dk)).to(BF16)
+        d["k"] = (k / k.norm(dim=-1, keepdim=True)).to(BF16)
+    d["beta"].fill_(beta)
+    d["g"].fill_(decay)
+    return d
+
+
+@pytest.mark.parametrize("keys,d_v,beta,decay", [
+    ("one", 1024, 0.1, -0.05), ("one", 256, 0.5, -0.5), ("one", 1024, 0.5, -0.5), ("units", 64, 1.0, 0.0),
+    ("units", 256, 0.5, -0.05), ("units", 1024, 1.0, 0.0), ("random", 1024, 1.0, -0.5), ("random", 1024, 0.5, -0.05)])
+def test_sums_over_channels_that_agree(device, keys, d_v, beta, decay):
+    """dX.W over the value channels, all terms of one sign: up to 4e6 in units
+    of its operands' exponents, where fp16 ends at 65504."""
+    d = alike([200, 64], 1, 128, d_v, keys, beta, decay)
+    check(call(d, [200, 64], device), reference(d, [200, 64]), BF16)
+
+
+def test_a_large_state_that_channels_share(device):
+    """dO.W over the value channels: W is the state's share of a value, here
+    1000 times the value itself and the same in every channel."""
+    d = inputs(BF16, [100, 200], 1, 128, 1024, seed=32)
+    d["do"] = (d["do"].double() * 0.01 + 1.9).to(BF16)
+    k = 128 ** -0.5 + 0.01 * d["k"].double() * math.sqrt(128)
+    d["k"] = (k / k.norm(dim=-1, keepdim=True)).to(BF16)
+    d["initial_state"] = 1000.0 + d["initial_state"] * 10.0
+    d["g"].fill_(-0.05)
+    check(call(d, [100, 200], device), reference(d, [100, 200]), BF16)
