@@ -277,13 +277,17 @@ __device__ __forceinline__ void unpack_run(const u32x4& u, float (&x)[kRun<T>]) 
         }
     }
 }
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+// the larger magnitude bits of a pair of 16-bit floats and of those of `m`
+__device__ __forceinline__ u16x2 pair_max_bits(u16x2 m, uint32_t x) {
+    return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x & 0x7fff7fffu));
+}
 template <typename T>
 __device__ __forceinline__ int run_max_bits(const u32x4& u) {
     if constexpr (sizeof(T) == 2) {  // as pairs of 15-bit integers
-        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
         u16x2 m = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u[i] & 0x7fff7fffu));
+        for (int i = 0; i < 4; ++i) m = pair_max_bits(m, u[i]);
         return max(int(m.x), int(m.y)) << 16;
     } else {
         return int(max(max(u.x & 0x7fffffffu, u.y & 0x7fffffffu), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu)));
@@ -760,14 +764,20 @@ struct TileRuns {
 };
 
 // Rows of two tiles as units with d_v along the contraction: `N` column
-// tiles of the turned matrices from `first` on, 1 KiB each.
+// tiles of the turned matrices from `first` on, 1 KiB each.  `top` becomes the
+// largest magnitude bits stored.
 template <int N, class Mat>
-__device__ __forceinline__ void store_turned(const Mat& even, const Mat& odd, char* base, int first, int lane) {
+__device__ __forceinline__ void store_turned(const Mat& even, const Mat& odd, char* base, int first, int lane, u16x2& top) {
     char* o = base + first * 1024 + lane * 16;
 #pragma unroll
-    for (int b = 0; b < N; ++b)
-        *reinterpret_cast<f16x8*>(o + b * 1024) = __builtin_shufflevector(
-            even.col4(first + b, 0, lane), odd.col4(first + b, 0, lane), 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int b = 0; b < N; ++b) {
+        const f16x8 u = __builtin_shufflevector(even.col4(first + b, 0, lane), odd.col4(first + b, 0, lane), 0, 1, 2, 3, 4,
+                                                5, 6, 7);
+        *reinterpret_cast<f16x8*>(o + b * 1024) = u;
+        const u32x4 w = __builtin_bit_cast(u32x4, u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = pair_max_bits(top, w[i]);
+    }
 }
 
 // A chunk's shared operands on their way from HBM to LDS, by `THREADS` threads.
@@ -905,8 +915,11 @@ __device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& 
 // The chain has no exponent of its own results to wait for: a chunk's values
 // are scaled by the larger of the state's and of V's (dO's) largest value,
 // which leaves them 2^10 below fp16's range and 2^19 above its subnormals.
-// Growth beyond that shows as an infinity or NaN in the state, and the head is
-// done again in fp32.
+// Growth beyond that shows as an infinity or NaN in the state or in the W or dX
+// that is handed on (rows of q of some 180 along all of a chunk's keys, say,
+// whose state decays before it takes them up), and the head is done again in
+// fp32.  The serving waves watch W and dX as they store them, off the chain (no
+// difference in time).
 //
 // 16384 tokens, 16 heads, d_k = 128, d_v = 256: 770 us, 5900 cycles a chunk, of
 // which the chain waits 350; eight serving waves leave it 168 registers: 816.
@@ -1049,8 +1062,8 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         }
     }
     __syncthreads();  // the last chunk's results lie in LDS
-    // a value that is not finite, or a product out of fp16's range, anywhere on
-    // the way is in the state still (0 times it is NaN): the head is done again
+    // a state's operand that is not finite, or one of V or dO, is in the state still
+    // (0 times it is NaN): the head is done again
     bool bad = false;
 #pragma unroll
     for (int b = 0; b < NT; ++b)
@@ -1091,11 +1104,14 @@ __device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a
             if (lane == 0) reinterpret_cast<int*>(lds + L::kExps)[slot] = e;
         }
     };
+    u16x2 top_w = {0, 0};
     auto results = [&](int c) {
         if constexpr (ACTIVE) {
             char* rec = a.rec + chunk(c) * a.stride;
-            store_turned<NT / 2>(ts0, ts1, rec + (BACK ? p.rec.ds1 : p.rec.s0) + first * NT * 1024, half * (NT / 2), lane);
-            store_turned<2>(tw0, tw1, rec + (BACK ? p.rec.x : p.rec.w) + first * 4 * 1024, half * 2, lane);
+            u16x2 top_s = {0, 0};  // not needed: the state's operands are in the state
+            store_turned<NT / 2>(ts0, ts1, rec + (BACK ? p.rec.ds1 : p.rec.s0) + first * NT * 1024, half * (NT / 2), lane,
+                                 top_s);
+            store_turned<2>(tw0, tw1, rec + (BACK ? p.rec.x : p.rec.w) + first * 4 * 1024, half * 2, lane, top_w);
         }
     };
     if (a.nc > 0) {
@@ -1119,6 +1135,7 @@ __device__ __forceinline__ void scan16_serve(const BwdParams& p, const ScanAt& a
     }
     __syncthreads();
     if (a.nc > 0) results(a.nc - 1);
+    if (max(top_w.x, top_w.y) >= 0x7c00) reinterpret_cast<int*>(a.rec + p.rec.vec)[kVecBad] = 1;  // not finite in fp16
 }
 
 template <typename T, int DK, bool VEC>

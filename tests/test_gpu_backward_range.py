@@ -58,3 +58,19 @@ def test_a_large_state_that_channels_share(device):
     d["initial_state"] = 1000.0 + d["initial_state"] * 10.0
     d["g"].fill_(-0.05)
     check(call(d, [100, 200], device), reference(d, [100, 200]), BF16)
+
+
+def test_a_value_gradient_beyond_fp16(device):
+    """The first token's dX is 69 000 in units of its exponent, from operands
+    that fp16 holds, and the state takes a fifth of it: nothing but dX itself
+    says that the head has left fp16's range."""
+    d = inputs(BF16, [64], 2, 128, 16, seed=33, state=False)
+    up, across = torch.ones(128, dtype=torch.float64) / math.sqrt(128), torch.ones(128, dtype=torch.float64) / math.sqrt(128)
+    across[1::2] *= -1
+    d["q"][:, 0] = 15.875
+    for t, side in ((0, 1), (1, -1)):
+        d["k"][t, 0] = (math.cos(math.radians(50)) * up + side * math.sin(math.radians(50)) * across).to(BF16)
+    d["do"][:, 0] = 1.9921875
+    d["g"][:, 0], d["beta"][:, 0] = 0.0, 0.0
+    d["g"][0, 0], d["beta"][:2, 0] = math.log(0.2), 1.0
+    check(call(d, [64], device), reference(d, [64]), BF16)
