@@ -33,13 +33,25 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr() or None
 
 
-def _stream(stream) -> int | None:
-    if stream is None:
-        # the current stream's handle without a Stream object around it, for
-        # calls that the host bounds (with _empty's allocations, one decode
-        # position of one sequence: 10.4 -> 7.8 us a call)
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None
-    return stream.cuda_stream or None
+def _stream() -> int | None:
+    # the current stream's handle without a Stream object around it, for
+    # calls that the host bounds (with _empty's allocations, one decode
+    # position of one sequence: 10.4 -> 7.8 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) or None
+
+
+def _on_stream(run, args):
+    """``run`` with its parameters ``args`` on the stream among them: what it
+    allocates is that stream's memory from the start, not memory that the
+    current stream's earlier work may still use, and its results stay whole
+    until the current stream's work is done with them too."""
+    stream, here = args["stream"], torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        out = run(**{**args, "stream": None})
+    for t in out if isinstance(out, tuple) else (out,):
+        if t is not None:
+            t.record_stream(here)
+    return out
 
 
 def _empty(like, shape, dtype=None):
@@ -116,6 +128,8 @@ def prefill(q, k, v, g=None, beta=None, *, alpha=None, cu_seqlens=None, initial_
     g is the per-token log-decay (alpha = exp(g)); pass alpha= instead to give
     alpha itself.  ``initial_state=None`` starts from zeros.
     """
+    if stream is not None:
+        return _on_stream(prefill, locals())
     gate, gate_kind = _gate(g, alpha)
     n = _check_prefill_shapes(q, k, v, gate, beta, cu_seqlens, initial_state)
     o = out if out is not None else _empty(q, v.shape)
@@ -129,7 +143,7 @@ def prefill(q, k, v, g=None, beta=None, *, alpha=None, cu_seqlens=None, initial_
         workspace = _empty(q, (need,), torch.uint8)
     if workspace is not None:
         args.workspace, args.workspace_bytes = _ptr(workspace), workspace.numel()
-    _abi.check(_abi.lib().rhz_gdr_prefill(byref(args), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_prefill(byref(args), _stream()))
     return o, fin
 
 
@@ -143,6 +157,8 @@ def local_prefill(q, k, v, beta_logit, alpha_logit, a_log, *, q_scale=None, cu_s
     Returns (o, final_state or None), as :func:`prefill` does on the
     prepared inputs.
     """
+    if stream is not None:
+        return _on_stream(local_prefill, locals())
     n = _check_prefill_shapes(q, k, v, alpha_logit, beta_logit, cu_seqlens, initial_state)
     H = q.shape[-2]
     if a_log.shape != (H,) or a_log.dtype != torch.float32:
@@ -161,7 +177,7 @@ def local_prefill(q, k, v, beta_logit, alpha_logit, a_log, *, q_scale=None, cu_s
         workspace = _empty(q, (need,), torch.uint8)
     if workspace is not None:
         la.prefill.workspace, la.prefill.workspace_bytes = _ptr(workspace), workspace.numel()
-    _abi.check(_abi.lib().rhz_gdr_local_prefill(byref(la), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_local_prefill(byref(la), _stream()))
     return o, fin
 
 
@@ -215,6 +231,8 @@ def decode_args(q, k, v, gate, beta, gate_kind, state, o) -> _abi.DecodeArgs:
 
 def decode_step(q, k, v, g=None, beta=None, *, alpha=None, state, out=None, stream=None):
     """One decode position for every (b, h); ``state`` [B,H,d_v,d_k] fp32 is updated in place."""
+    if stream is not None:
+        return _on_stream(decode_step, locals())
     gate, gate_kind = _gate(g, alpha)
     B, H, dk = q.shape
     dv = v.shape[-1]
@@ -224,7 +242,7 @@ def decode_step(q, k, v, g=None, beta=None, *, alpha=None, state, out=None, stre
         raise ValueError("state must be fp32 [B,H,d_v,d_k]")
     o = out if out is not None else _empty(q, (B, H, dv))
     args = decode_args(q, k, v, gate, beta, gate_kind, state, o)
-    _abi.check(_abi.lib().rhz_gdr_decode_step(byref(args), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_decode_step(byref(args), _stream()))
     return o
 
 
@@ -247,6 +265,8 @@ def multistep(q, k, v, g=None, beta=None, *, alpha=None, state, out=None, states
     (o [B, n, H, d_v], states [B, n, H, d_v, d_k]) with the state after each
     position.  A segment change at position t is ``alpha[:, t] = 0``.
     """
+    if stream is not None:
+        return _on_stream(multistep, locals())
     gate, gate_kind = _gate(g, alpha)
     B, n, H, dk = q.shape
     dv = v.shape[-1]
@@ -259,7 +279,7 @@ def multistep(q, k, v, g=None, beta=None, *, alpha=None, state, out=None, states
     if states is None:
         states = _empty(q, (B, n, H, dv, dk), torch.float32)
     args = multistep_args(q, k, v, gate, beta, gate_kind, state, states, o)
-    _abi.check(_abi.lib().rhz_gdr_multistep(byref(args), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_multistep(byref(args), _stream()))
     return o, states
 
 
@@ -270,6 +290,8 @@ def causal_conv1d(x, weight, bias=None, *, cu_seqlens=None, initial_state=None,
     x [B, T, C] (dense) or [tokens, C] with ``cu_seqlens``; weight [C, 4]
     fp32; bias [C]; initial_state [N, C, 3].  Returns (y, final_state or None).
     """
+    if stream is not None:
+        return _on_stream(causal_conv1d, locals())
     if cu_seqlens is None:
         B, T, C = x.shape
         batch, seq_len = B, T
@@ -286,7 +308,7 @@ def causal_conv1d(x, weight, bias=None, *, cu_seqlens=None, initial_state=None,
     a.batch, a.seq_len, a.channels, a.dtype = batch, seq_len, C, _DTYPES[x.dtype]
     a.x, a.weight, a.bias, a.y = _ptr(x), _ptr(weight), _ptr(bias), _ptr(y)
     a.cu_seqlens, a.initial_state, a.final_state = _ptr(cu_seqlens), _ptr(initial_state), _ptr(fin)
-    _abi.check(_abi.lib().rhz_causal_conv1d(byref(a), _stream(stream)))
+    _abi.check(_abi.lib().rhz_causal_conv1d(byref(a), _stream()))
     return y, fin
 
 
@@ -297,6 +319,8 @@ def prepare(q, k, beta_logit, alpha_logit, a_log, *, q_scale=None, q_out=None, k
 
     q, k [..., H, d_k]; logits [..., H]; a_log [H].  Returns (q, k, beta, g).
     """
+    if stream is not None:
+        return _on_stream(prepare, locals())
     *lead, H, dk = q.shape
     tokens = 1
     for n in lead:
@@ -311,7 +335,7 @@ def prepare(q, k, beta_logit, alpha_logit, a_log, *, q_scale=None, q_out=None, k
     a.q_in, a.k_in, a.q_out, a.k_out = _ptr(q), _ptr(k), _ptr(qo), _ptr(ko)
     a.beta_logit, a.alpha_logit, a.a_log = _ptr(beta_logit), _ptr(alpha_logit), _ptr(a_log)
     a.beta, a.g = _ptr(beta), _ptr(g)
-    _abi.check(_abi.lib().rhz_gdr_prepare(byref(a), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_prepare(byref(a), _stream()))
     return qo, ko, beta, g
 
 
@@ -328,6 +352,8 @@ def conv_prepare(x, weight, bias, beta_logit, alpha_logit, a_log, *, heads, d_k,
     [heads]; initial_state [N, C, 3].  Returns (q, k, v, beta, g,
     final_state or None) with q, k [..., heads, d_k] and v [..., heads, d_v].
     """
+    if stream is not None:
+        return _on_stream(conv_prepare, locals())
     if cu_seqlens is None:
         B, T, C = x.shape
         batch, seq_len, lead = B, T, (B, T)
@@ -352,18 +378,20 @@ def conv_prepare(x, weight, bias, beta_logit, alpha_logit, a_log, *, heads, d_k,
     a.cu_seqlens, a.initial_state, a.final_state = _ptr(cu_seqlens), _ptr(initial_state), _ptr(fin)
     a.beta_logit, a.alpha_logit, a.a_log = _ptr(beta_logit), _ptr(alpha_logit), _ptr(a_log)
     a.q, a.k, a.v, a.beta, a.g = _ptr(q), _ptr(k), _ptr(v), _ptr(beta), _ptr(g)
-    _abi.check(_abi.lib().rhz_gdr_conv_prepare(byref(a), _stream(stream)))
+    _abi.check(_abi.lib().rhz_gdr_conv_prepare(byref(a), _stream()))
     return q, k, v, beta, g, fin
 
 
 def rmsnorm_heads(x, scale, eps: float = 1e-6, *, out=None, stream=None):
     """RMSNorm over the last dimension with a learned scale (norm.rs:8-13, 48-59)."""
+    if stream is not None:
+        return _on_stream(rmsnorm_heads, locals())
     dim = x.shape[-1]
     y = out if out is not None else torch.empty_like(x)
     a = _abi.RmsnormArgs()
     a.rows, a.dim, a.dtype, a.eps = x.numel() // dim, dim, _DTYPES[x.dtype], eps
     a.x, a.scale, a.y = _ptr(x), _ptr(scale), _ptr(y)
-    _abi.check(_abi.lib().rhz_rmsnorm_heads(byref(a), _stream(stream)))
+    _abi.check(_abi.lib().rhz_rmsnorm_heads(byref(a), _stream()))
     return y
 
 
@@ -376,10 +404,12 @@ _FILL_DTYPES = {torch.float64: _abi.F64, torch.float32: _abi.F32, torch.bfloat16
 def philox_fill(kind: str, seed: int, stream_id: int, shape, dtype=torch.float32, *,
                 mean: float = 0.0, std: float = 1.0, device="cuda", out=None, stream=None):
     """Seeded Philox-4x32-10 synthetic tensor generated on the device (see rhz_philox_fill)."""
+    if stream is not None:
+        return _on_stream(philox_fill, locals())
     t = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
     row_len = t.shape[-1] if t.dim() else 1
     _abi.check(_abi.lib().rhz_philox_fill(_FILL[kind], seed, stream_id, t.numel(), row_len, mean,
-                                          std, _FILL_DTYPES[t.dtype], _ptr(t), _stream(stream)))
+                                          std, _FILL_DTYPES[t.dtype], _ptr(t), _stream()))
     return t
 
 

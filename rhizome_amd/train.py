@@ -14,7 +14,7 @@ from ctypes import byref, c_size_t
 import torch
 
 from . import _abi
-from .gdr import _DTYPES, _check_prefill_shapes, _empty, _gate, _ptr, _stream
+from .gdr import _DTYPES, _check_prefill_shapes, _empty, _gate, _on_stream, _ptr, _stream
 
 
 def _same_device(*tensors):
@@ -23,15 +23,6 @@ def _same_device(*tensors):
     for t in tensors:
         if t is not None and t.is_cuda and t.device.index != here:
             raise ValueError(f"all tensors must be on the current device, cuda:{here}")
-
-
-def _used_on(stream, *tensors):
-    """Tensors that this module allocated, kept from reuse until a stream
-    other than the current one is done with them."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
 
 
 def _workspace(like, args, query, workspace):
@@ -56,6 +47,8 @@ def prefill_backward(q, k, v, g=None, beta=None, do=None, *, alpha=None, dfinal_
     alpha, whichever was passed; all but the fp32 dinitial_state have q's dtype.
     Two calls that may run at the same time must not share a workspace.
     """
+    if stream is not None:
+        return _on_stream(prefill_backward, locals())
     gate, gate_kind = _gate(g, alpha)
     if beta is None or do is None:
         raise ValueError("beta and do are needed")
@@ -78,8 +71,7 @@ def prefill_backward(q, k, v, g=None, beta=None, do=None, *, alpha=None, dfinal_
     a.grad_q, a.grad_k, a.grad_v = _ptr(dq), _ptr(dk), _ptr(dv)
     a.grad_gate, a.grad_beta, a.grad_initial_state = _ptr(dgate), _ptr(dbeta), _ptr(dinit)
     workspace = _workspace(q, a, _abi.lib().rhz_gdr_prefill_backward_workspace_size, workspace)
-    _abi.check(_abi.lib().rhz_gdr_prefill_backward(byref(a), _stream(stream)))
-    _used_on(stream, dq, dk, dv, dgate, dbeta, dinit, workspace)
+    _abi.check(_abi.lib().rhz_gdr_prefill_backward(byref(a), _stream()))
     return dq, dk, dv, dgate, dbeta, dinit
 
 
@@ -95,6 +87,8 @@ def conv_prepare_backward(x, weight, bias, beta_logit, alpha_logit, a_log, dq, d
     there is a bias, dinitial_state where there is an initial state; all but dx
     are fp32.
     """
+    if stream is not None:
+        return _on_stream(conv_prepare_backward, locals())
     C = heads * (2 * d_k + d_v)
     lead = x.shape[:-1]
     if x.shape[-1] != C or x.dim() != (3 if cu_seqlens is None else 2) or x.dtype not in _DTYPES:
@@ -130,8 +124,7 @@ def conv_prepare_backward(x, weight, bias, beta_logit, alpha_logit, a_log, dq, d
     a.grad_x, a.grad_weight, a.grad_bias, a.grad_initial_state = _ptr(dx), _ptr(dw), _ptr(db), _ptr(dinit)
     a.grad_beta_logit, a.grad_alpha_logit, a.grad_a_log = _ptr(dbl), _ptr(dal), _ptr(da)
     workspace = _workspace(x, a, _abi.lib().rhz_gdr_conv_prepare_backward_workspace_size, workspace)
-    _abi.check(_abi.lib().rhz_gdr_conv_prepare_backward(byref(a), _stream(stream)))
-    _used_on(stream, dx, dw, db, dbl, dal, da, dinit, workspace)
+    _abi.check(_abi.lib().rhz_gdr_conv_prepare_backward(byref(a), _stream()))
     return dx, dw, db, dbl, dal, da, dinit
 
 
@@ -149,6 +142,8 @@ def _check_norm(x, weight, *like_x):
 
 def layernorm(x, weight, bias=None, eps: float = 1e-5, *, out=None, stream=None):
     """Layer norm over the last dimension: (x - mean) / sqrt(variance + eps) * weight + bias."""
+    if stream is not None:
+        return _on_stream(layernorm, locals())
     y = out if out is not None else _empty(x, x.shape)
     dim = _check_norm(x, weight, y)
     if bias is not None and (tuple(bias.shape) != (dim,) or bias.dtype != torch.float32):
@@ -157,13 +152,11 @@ def layernorm(x, weight, bias=None, eps: float = 1e-5, *, out=None, stream=None)
     a = _abi.LayernormArgs()
     a.rows, a.dim, a.dtype, a.eps = x.numel() // max(dim, 1), dim, _DTYPES[x.dtype], eps
     a.x, a.weight, a.bias, a.y = _ptr(x), _ptr(weight), _ptr(bias), _ptr(y)
-    _abi.check(_abi.lib().rhz_layernorm(byref(a), _stream(stream)))
-    if out is None:
-        _used_on(stream, y)
+    _abi.check(_abi.lib().rhz_layernorm(byref(a), _stream()))
     return y
 
 
-def _norm_backward(run, dy, x, weight, eps, bias, workspace, stream):
+def _norm_backward(run, dy, x, weight, eps, bias, workspace):
     dim = _check_norm(x, weight, dy)
     _same_device(dy, x, weight, workspace)
     a = _abi.NormBackwardArgs()
@@ -173,8 +166,7 @@ def _norm_backward(run, dy, x, weight, eps, bias, workspace, stream):
     a.grad_y, a.x, a.weight = _ptr(dy), _ptr(x), _ptr(weight)
     a.grad_x, a.grad_weight, a.grad_bias = _ptr(dx), _ptr(dw), _ptr(db)
     workspace = _workspace(x, a, _abi.lib().rhz_norm_backward_workspace_size, workspace)
-    _abi.check(run(byref(a), _stream(stream)))
-    _used_on(stream, dx, dw, db, workspace)
+    _abi.check(run(byref(a), _stream()))
     return dx, dw, db
 
 
@@ -182,11 +174,15 @@ def layernorm_backward(dy, x, weight, eps: float = 1e-5, *, workspace=None, stre
     """Backward pass of :func:`layernorm` from the gradient dy of its output
     and its x.  Returns (dx, dweight, dbias), the last two summed over the
     rows in fp32."""
-    return _norm_backward(_abi.lib().rhz_layernorm_backward, dy, x, weight, eps, True, workspace, stream)
+    if stream is not None:
+        return _on_stream(layernorm_backward, locals())
+    return _norm_backward(_abi.lib().rhz_layernorm_backward, dy, x, weight, eps, True, workspace)
 
 
 def rmsnorm_heads_backward(dy, x, scale, eps: float = 1e-6, *, workspace=None, stream=None):
     """Backward pass of :func:`rmsnorm_heads` from the gradient dy of its
     output and its x.  Returns (dx, dscale), dscale summed over the rows in
     fp32."""
-    return _norm_backward(_abi.lib().rhz_rmsnorm_heads_backward, dy, x, scale, eps, False, workspace, stream)[:2]
+    if stream is not None:
+        return _on_stream(rmsnorm_heads_backward, locals())
+    return _norm_backward(_abi.lib().rhz_rmsnorm_heads_backward, dy, x, scale, eps, False, workspace)[:2]
