@@ -342,8 +342,12 @@ __host__ __device__ inline RecLayout rec_layout(int DK, int dvt, int es) {
     return l;
 }
 // the record's small values: gamma, beta tail and beta by token, gamma_c,
-// exponents of K and Q, whether the chunk leaves the fp16 operands' domain
-enum { kVecGamma = 0, kVecWrite = 64, kVecBeta = 128, kVecGc = 192, kVecEK = 193, kVecEQ = 194, kVecBad = 195, kVecs = 196 };
+// exponents of K and Q, whether the chunk leaves the fp16 operands' domain,
+// exponents of the largest beta and beta tail
+enum {
+    kVecGamma = 0, kVecWrite = 64, kVecBeta = 128, kVecGc = 192, kVecEK = 193, kVecEQ = 194, kVecBad = 195, kVecEB = 196,
+    kVecEW = 197, kVecs = 198
+};
 // exponents by d_v tile, from float 256 on
 enum { kExpO = 256, kExpW = 320, kExpX = 384, kExpS = 448, kExpD = 512 };
 
@@ -507,9 +511,17 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
     }
     __syncthreads();
     if (tid < 64) {
+        const float beta = gs.beta[tid], write = beta * gs.tail[tid];
         vec[kVecGamma + tid] = gs.gamma[tid];
-        vec[kVecWrite + tid] = gs.beta[tid] * gs.tail[tid];
-        vec[kVecBeta + tid] = gs.beta[tid];
+        vec[kVecWrite + tid] = write;
+        vec[kVecBeta + tid] = beta;
+        if constexpr (Op::kScaled) {
+            const int eb = bits_exp(wave_max_bits(bits_abs(beta))), ew = bits_exp(wave_max_bits(bits_abs(write)));
+            if (tid == 0) {
+                exps[kVecEB] = eb;
+                exps[kVecEW] = ew;
+            }
+        }
     }
     if (tid == 0) {
         vec[kVecGc] = gs.gamma[63];
@@ -913,8 +925,10 @@ __device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& 
 // waves do is split around B as the chain is.
 //
 // The chain has no exponent of its own results to wait for: a chunk's values
-// are scaled by the larger of the state's and of V's (dO's) largest value,
-// which leaves them 2^10 below fp16's range and 2^19 above its subnormals.
+// are scaled by the larger of the state's and of V's (dO's) largest value and
+// those of the factors on their way.  A single term is thereby some 2^10 below
+// fp16's range and 2^19 above its subnormals; sums of terms of one sign reach
+// 2^10 in W and 2^14 in dX.
 // Growth beyond that shows as an infinity or NaN in the state or in the W or dX
 // that is handed on (rows of q of some 180 along all of a chunk's keys, say,
 // whose state decays before it takes them up), and the head is done again in
@@ -976,6 +990,8 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         const float gc = vec[kVecGc];
         const int ek = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEK]);
         const int eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
+        const int eb = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEB]);
+        const int et = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEW]);
         // of V, or dO: its largest value below 2^ev
         const int ev = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(lds + L::kExps)[(c & 1) * 4 + wave]);
         f32x4 x[4], w[4], vo[4];
@@ -986,11 +1002,13 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su[i], x[b]);
-        // the next state is S times 2^-e, W or dX are kept times 2^-ew, the larger of
-        // what the state and V (dO times rows of Q) give at 2^5 or 2^6: with ek < 0
-        // (small keys) W is of V's size, its share of the state 2^ek of it
-        const int se = S.e, other = ev + (BACK ? eq + 2 : ek);
-        const int e = max(top + se, other) - 5, ew = BACK ? e + ek : max(top + se + ek, ev) - 5;
+        // W or dX are kept times 2^-ew, the next state is S times 2^-e: the larger of
+        // what the state and V (dO times rows of Q) give, with the factors that K, and
+        // dX's and W's beta, bring, at 2^5 to 2^7.  So small keys or betas leave what
+        // they multiply its bits.
+        const int se = S.e, own = top + se - 5, in = ev + (BACK ? eq + 2 : 0) - 5;
+        const int ew = BACK ? ek + max(own + et, in + eb) : max(own + ek, in);
+        const int e = max(own, BACK ? in : ew + ek + et);
         Unit ru[2];
         if constexpr (!BACK) {
             const float sv = exp2i(-ew), sx = -exp2i(se + ek - ew);

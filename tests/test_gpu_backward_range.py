@@ -74,3 +74,17 @@ def test_a_value_gradient_beyond_fp16(device):
     d["g"][:, 0], d["beta"][:, 0] = 0.0, 0.0
     d["g"][0, 0], d["beta"][:2, 0] = math.log(0.2), 1.0
     check(call(d, [64], device), reference(d, [64]), BF16)
+
+
+@pytest.mark.parametrize("state", [True, False])
+@pytest.mark.parametrize("beta", [1e-5, 1e-7, 1e-9, 1e-20])
+def test_small_betas(device, beta, state):
+    """Gates that are all but shut in every token of a head, or of a chunk of
+    it: every gradient keeps its bits, however small it is."""
+    d = inputs(BF16, [200, 64], 2, 128, 128, seed=34, state=state)
+    d["beta"][:, 0] = beta
+    d["beta"][64:128, 1] = beta
+    got, want = call(d, [200, 64], device), reference(d, [200, 64])
+    for h in (0, 1):  # each head against its own norms
+        check([x[:, h] for x in got], [x[:, h] for x in want], BF16, f"head {h}")
+    check([got[2][64:128, 1]], [want[2][64:128, 1]], BF16, "the chunk's")
