@@ -343,10 +343,10 @@ __host__ __device__ inline RecLayout rec_layout(int DK, int dvt, int es) {
 }
 // the record's small values: gamma, beta tail and beta by token, gamma_c,
 // exponents of K and Q, whether the chunk leaves the fp16 operands' domain,
-// exponents of the largest beta and beta tail
+// exponents of the largest beta, beta tail and gamma (the first token's) and of gamma_c
 enum {
     kVecGamma = 0, kVecWrite = 64, kVecBeta = 128, kVecGc = 192, kVecEK = 193, kVecEQ = 194, kVecBad = 195, kVecEB = 196,
-    kVecEW = 197, kVecs = 198
+    kVecEW = 197, kVecEG = 198, kVecEGc = 199, kVecs = 200
 };
 // exponents by d_v tile, from float 256 on
 enum { kExpO = 256, kExpW = 320, kExpX = 384, kExpS = 448, kExpD = 512 };
@@ -520,6 +520,8 @@ __device__ __forceinline__ void prep_chunk(const BwdParams& p, const ChunkAt& at
             if (tid == 0) {
                 exps[kVecEB] = eb;
                 exps[kVecEW] = ew;
+                exps[kVecEG] = bits_exp(bits_abs(gs.gamma[0]));
+                exps[kVecEGc] = bits_exp(bits_abs(gs.gamma[63]));
             }
         }
     }
@@ -992,6 +994,8 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
         const int eq = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEQ]);
         const int eb = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEB]);
         const int et = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEW]);
+        const int eg = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEG]);
+        const int egc = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(vec)[kVecEGc]);
         // of V, or dO: its largest value below 2^ev
         const int ev = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(lds + L::kExps)[(c & 1) * 4 + wave]);
         f32x4 x[4], w[4], vo[4];
@@ -1003,12 +1007,13 @@ __device__ __forceinline__ void scan16_carry(const BwdParams& p, const ScanAt& a
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = Op::mma(K.blocks(16 * b + m, i, g), su[i], x[b]);
         // W or dX are kept times 2^-ew, the next state is S times 2^-e: the larger of
-        // what the state and V (dO times rows of Q) give, with the factors that K, and
-        // dX's and W's beta, bring, at 2^5 to 2^7.  So small keys or betas leave what
-        // they multiply its bits.
+        // what the state and V (dO times rows of Q) give, with the largest factors that
+        // K, beta and the decays bring, at 2^5 to 2^7.  So small keys or betas leave
+        // what they multiply its bits, and a state that is forgotten leaves those of
+        // what follows it.
         const int se = S.e, own = top + se - 5, in = ev + (BACK ? eq + 2 : 0) - 5;
-        const int ew = BACK ? ek + max(own + et, in + eb) : max(own + ek, in);
-        const int e = max(own, BACK ? in : ew + ek + et);
+        const int ew = BACK ? ek + max(own + et, in + eb) : max(own + ek + eg, in);
+        const int e = max(own + egc, BACK ? max(in + eg, ew + ek + eg) : ew + ek + et);
         Unit ru[2];
         if constexpr (!BACK) {
             const float sv = exp2i(-ew), sx = -exp2i(se + ek - ew);

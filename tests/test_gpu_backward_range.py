@@ -88,3 +88,30 @@ def test_small_betas(device, beta, state):
     for h in (0, 1):  # each head against its own norms
         check([x[:, h] for x in got], [x[:, h] for x in want], BF16, f"head {h}")
     check([got[2][64:128, 1]], [want[2][64:128, 1]], BF16, "the chunk's")
+
+
+@pytest.mark.parametrize("gate", ["g", "alpha"])
+@pytest.mark.parametrize("g", [-12.0, -20.0, -60.0])
+def test_strong_decays_keep_the_state_gradients(device, g, gate):
+    """Decays of 6e-6 to 9e-27 a token.  The state's gradient is dO's and dX's
+    share times the first token's decay, and as accurate for it."""
+    d = inputs(BF16, [200, 64, 1], 2, 64, 64, seed=35, gate=gate)
+    d[gate][:, 0] = g if gate == "g" else math.exp(g)
+    d[gate][[0, 200, 264], 1] = g if gate == "g" else math.exp(g)  # the first token's alone
+    got, want = call(d, [200, 64, 1], device), reference(d, [200, 64, 1])
+    for h in (0, 1):
+        check([x[:, h] for x in got], [x[:, h] for x in want], BF16, f"head {h}")
+
+
+@pytest.mark.parametrize("g", [-25.0, -40.0, -math.inf])
+@pytest.mark.parametrize("at", [64, 128])
+def test_a_large_state_forgotten(device, at, g):
+    """A state 1e9 times what the values make of it, up to a chunk's first
+    token, which forgets it: the tokens behind keep their gradients."""
+    d = inputs(BF16, [200], 2, 64, 64, seed=36)
+    d["initial_state"] *= 1e10
+    d["g"].fill_(-0.02)
+    d["g"][at] = g
+    got, want = call(d, [200], device), reference(d, [200])
+    want[3] = torch.nan_to_num(want[3])  # 0 * inf in the derivative of exp at -inf, whose value is 0
+    check([x[at:] for x in got[:5]], [x[at:] for x in want[:5]], BF16)
