@@ -148,11 +148,13 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
         for (int e = 0; e < N; ++e) aw[i][e] = ab[i][e] = 0.f;
     if constexpr (R::kKeepW) R::weights(w, p.w, li, p.dim);
     typename V::Raw rx[U][NV], ry[U][NV];
-    auto load = [&](int first) {
+    // rows go up to 2^31 - 1 (dim = 1) and the counter two steps beyond: unsigned
+    const unsigned rows = p.rows;
+    auto load = [&](unsigned first) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int row = first + u * RPB;
-            if (row < p.rows) {
+            const unsigned row = first + u * RPB;
+            if (row < rows) {
                 R::load_raw(rx[u], static_cast<const T*>(p.x) + (long)row * p.dim, li, p.dim);
                 R::load_raw(ry[u], static_cast<const T*>(p.dy) + (long)row * p.dim, li, p.dim);
             } else {
@@ -161,10 +163,10 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
             }
         }
     };
-    const int step = gridDim.x * RPB * U;
-    int base = blockIdx.x * RPB * U;  // the same for the whole block
+    const unsigned step = gridDim.x * RPB * U;
+    unsigned base = blockIdx.x * RPB * U;  // the same for the whole block
     load(base + grp);
-    for (; base < p.rows; base += step) {
+    for (; base < rows; base += step) {
         float x[U][NV][N], y[U][NV][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -174,9 +176,9 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
         load(base + step + grp);  // rows beyond the last are zero
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int row = base + grp + u * RPB;
+            const unsigned row = base + grp + u * RPB;
             float r = R::template stats<CENTER>(x[u], li, p.dim, p.eps, red);
-            if (row >= p.rows) r = 0.f;  // no row: nothing is added, with eps = 0 too
+            if (row >= rows) r = 0.f;  // no row: nothing is added, with eps = 0 too
             float st = 0.f, sx = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormParams p) {
             }
             const float mx = group_total<G>(sx, red) / (float)p.dim;
             const float mt = CENTER ? group_total<G>(st, red) / (float)p.dim : 0.f;
-            if (row < p.rows) {
+            if (row < rows) {
                 T* o = static_cast<T*>(p.out) + (long)row * p.dim;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
