@@ -33,6 +33,13 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr() or None
 
 
+def _count(n: int) -> int:
+    """A size for a 32-bit field of an argument struct, which would take a larger one modulo 2^32."""
+    if n > 0x7fffffff:
+        raise ValueError(f"{n} rows or tokens: at most 2^31 - 1")
+    return n
+
+
 def _stream() -> int | None:
     # the current stream's handle without a Stream object around it, for
     # calls that the host bounds (with _empty's allocations, one decode
@@ -76,7 +83,7 @@ def prefill_args(q, k, v, gate, beta, gate_kind, cu_seqlens=None, initial_state=
         batch, seq_len = B, T
     else:
         _, H, dk = q.shape
-        batch, seq_len = cu_seqlens.numel() - 1, q.shape[0]
+        batch, seq_len = cu_seqlens.numel() - 1, _count(q.shape[0])
     dv = v.shape[-1]
     a = _abi.PrefillArgs()
     a.batch, a.seq_len, a.heads, a.d_k, a.d_v = batch, seq_len, H, dk, dv
@@ -298,6 +305,7 @@ def causal_conv1d(x, weight, bias=None, *, cu_seqlens=None, initial_state=None,
     else:
         seq_len, C = x.shape
         batch = cu_seqlens.numel() - 1
+        _count(seq_len)
     if tuple(weight.shape) != (C, 4) or weight.dtype != torch.float32:
         raise ValueError("weight must be fp32 [C, 4]")
     y = out if out is not None else torch.empty_like(x)
@@ -330,7 +338,7 @@ def prepare(q, k, beta_logit, alpha_logit, a_log, *, q_scale=None, q_out=None, k
     beta = _empty(q, beta_logit.shape, torch.float32)
     g = torch.empty_like(beta)
     a = _abi.PrepareArgs()
-    a.tokens, a.heads, a.d_k, a.dtype = tokens, H, dk, _DTYPES[q.dtype]
+    a.tokens, a.heads, a.d_k, a.dtype = _count(tokens), H, dk, _DTYPES[q.dtype]
     a.q_scale = float(dk) ** 0.5 if q_scale is None else float(q_scale)
     a.q_in, a.k_in, a.q_out, a.k_out = _ptr(q), _ptr(k), _ptr(qo), _ptr(ko)
     a.beta_logit, a.alpha_logit, a.a_log = _ptr(beta_logit), _ptr(alpha_logit), _ptr(a_log)
@@ -359,7 +367,7 @@ def conv_prepare(x, weight, bias, beta_logit, alpha_logit, a_log, *, heads, d_k,
         batch, seq_len, lead = B, T, (B, T)
     else:
         seq_len, C = x.shape
-        batch, lead = cu_seqlens.numel() - 1, (seq_len,)
+        batch, lead = cu_seqlens.numel() - 1, (_count(seq_len),)
     if C != heads * (2 * d_k + d_v):
         raise ValueError(f"x has {C} channels, not heads * (2 d_k + d_v) = {heads * (2 * d_k + d_v)}")
     if tuple(weight.shape) != (C, 4) or weight.dtype != torch.float32:
@@ -389,7 +397,7 @@ def rmsnorm_heads(x, scale, eps: float = 1e-6, *, out=None, stream=None):
     dim = x.shape[-1]
     y = out if out is not None else torch.empty_like(x)
     a = _abi.RmsnormArgs()
-    a.rows, a.dim, a.dtype, a.eps = x.numel() // dim, dim, _DTYPES[x.dtype], eps
+    a.rows, a.dim, a.dtype, a.eps = _count(x.numel() // dim), dim, _DTYPES[x.dtype], eps
     a.x, a.scale, a.y = _ptr(x), _ptr(scale), _ptr(y)
     _abi.check(_abi.lib().rhz_rmsnorm_heads(byref(a), _stream()))
     return y

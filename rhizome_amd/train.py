@@ -14,7 +14,7 @@ from ctypes import byref, c_size_t
 import torch
 
 from . import _abi
-from .gdr import _DTYPES, _check_prefill_shapes, _empty, _gate, _on_stream, _ptr, _stream
+from .gdr import _DTYPES, _check_prefill_shapes, _count, _empty, _gate, _on_stream, _ptr, _stream
 
 
 def _same_device(*tensors):
@@ -61,7 +61,7 @@ def prefill_backward(q, k, v, g=None, beta=None, do=None, *, alpha=None, dfinal_
         raise ValueError(f"dfinal_state must be fp32 {want}")
     _same_device(q, k, v, gate, beta, do, dfinal_state, cu_seqlens, initial_state, workspace)
     a = _abi.PrefillBackwardArgs()
-    a.batch, a.seq_len = (q.shape[0], q.shape[1]) if cu_seqlens is None else (n, q.shape[0])
+    a.batch, a.seq_len = (q.shape[0], q.shape[1]) if cu_seqlens is None else (n, _count(q.shape[0]))
     a.heads, a.d_k, a.d_v, a.dtype, a.gate_kind = H, d_k, d_v, _DTYPES[q.dtype], gate_kind
     a.q, a.k, a.v, a.gate, a.beta, a.grad_o = _ptr(q), _ptr(k), _ptr(v), _ptr(gate), _ptr(beta), _ptr(do)
     a.cu_seqlens, a.initial_state, a.grad_final_state = _ptr(cu_seqlens), _ptr(initial_state), _ptr(dfinal_state)
@@ -93,7 +93,7 @@ def conv_prepare_backward(x, weight, bias, beta_logit, alpha_logit, a_log, dq, d
     lead = x.shape[:-1]
     if x.shape[-1] != C or x.dim() != (3 if cu_seqlens is None else 2) or x.dtype not in _DTYPES:
         raise ValueError(f"x must be fp32 or bf16 [B, T, {C}] (dense) or [tokens, {C}] (packed)")
-    batch, seq_len = (x.shape[0], x.shape[1]) if cu_seqlens is None else (cu_seqlens.numel() - 1, x.shape[0])
+    batch, seq_len = (x.shape[0], x.shape[1]) if cu_seqlens is None else (cu_seqlens.numel() - 1, _count(x.shape[0]))
     if cu_seqlens is not None and cu_seqlens.dtype != torch.int32:
         raise ValueError("cu_seqlens must be int32")
     f32 = torch.float32
@@ -150,7 +150,7 @@ def layernorm(x, weight, bias=None, eps: float = 1e-5, *, out=None, stream=None)
         raise ValueError(f"bias must be fp32 ({dim},)")
     _same_device(x, weight, bias, y)
     a = _abi.LayernormArgs()
-    a.rows, a.dim, a.dtype, a.eps = x.numel() // max(dim, 1), dim, _DTYPES[x.dtype], eps
+    a.rows, a.dim, a.dtype, a.eps = _count(x.numel() // max(dim, 1)), dim, _DTYPES[x.dtype], eps
     a.x, a.weight, a.bias, a.y = _ptr(x), _ptr(weight), _ptr(bias), _ptr(y)
     _abi.check(_abi.lib().rhz_layernorm(byref(a), _stream()))
     return y
@@ -160,7 +160,7 @@ def _norm_backward(run, dy, x, weight, eps, bias, workspace):
     dim = _check_norm(x, weight, dy)
     _same_device(dy, x, weight, workspace)
     a = _abi.NormBackwardArgs()
-    a.rows, a.dim, a.dtype, a.eps = x.numel() // max(dim, 1), dim, _DTYPES[x.dtype], eps
+    a.rows, a.dim, a.dtype, a.eps = _count(x.numel() // max(dim, 1)), dim, _DTYPES[x.dtype], eps
     dx, dw = _empty(x, x.shape), _empty(weight, weight.shape)
     db = _empty(weight, weight.shape) if bias else None
     a.grad_y, a.x, a.weight = _ptr(dy), _ptr(x), _ptr(weight)

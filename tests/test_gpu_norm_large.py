@@ -39,3 +39,13 @@ def test_backward_of_the_most_rows(device, layer):
     else:
         terms = ys * xs * r
         assert abs(float(dw) - float(terms.sum())) <= 2.0 ** -24 * 18000 * float(terms.abs().sum())
+
+
+@pytest.mark.parametrize("name", ["rmsnorm_heads", "layernorm", "rmsnorm_heads_backward", "layernorm_backward"])
+def test_more_rows_than_the_sizes_hold(device, name):
+    """2^32 + 5 rows are refused, not taken for five."""
+    x = torch.empty(((1 << 32) + 5, 1), dtype=torch.bfloat16, device=device)
+    w = torch.ones(1, device=device)
+    args = (x, x, w) if "backward" in name else (x, w)
+    with pytest.raises(ValueError, match="2\\^31"):
+        getattr(rhizome_amd, name)(*args)
