@@ -127,7 +127,7 @@ rhz_status rhz_gdr_conv_prepare_backward(const rhz_gdr_conv_prepare_backward_arg
 
 /* Layer norm of every row of `dim` values: y = (x - mean) / sqrt(variance +
  * eps) * weight + bias, the variance from the centred values, in fp32.  y may
- * alias x. */
+ * be x itself; else it overlaps no input. */
 typedef struct rhz_layernorm_args {
     int32_t rows;     /* >= 0 */
     int32_t dim;      /* 1..8192 */

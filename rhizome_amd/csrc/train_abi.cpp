@@ -240,13 +240,17 @@ rhz_status rhz_gdr_conv_prepare_backward(const rhz_gdr_conv_prepare_backward_arg
 
 rhz_status rhz_layernorm(const rhz_layernorm_args* a, void* stream) {
     if (!a) return fail(RHZ_ERR_INVALID_ARG, "args is NULL");
-    const rhz_status s = check_norm(a->rows, a->dim, a->dtype, a->eps);
+    rhz_status s = check_norm(a->rows, a->dim, a->dtype, a->eps);
     if (s != RHZ_OK) return s;
     if (a->rows == 0) return ok();
-    if (!a->x || !a->y || !a->weight) return fail(RHZ_ERR_INVALID_ARG, "x, y or weight is NULL");
-    const size_t es = a->dtype == RHZ_F32 ? 4 : 2;
-    if (misaligned(a->x, es) || misaligned(a->y, es) || misaligned(a->weight, 4) || misaligned(a->bias, 4))
-        return fail(RHZ_ERR_INVALID_ARG, "x, y, weight or bias is not aligned");
+    const size_t es = a->dtype == RHZ_F32 ? 4 : 2, n = (size_t)a->rows * a->dim * es, nd = (size_t)a->dim * 4;
+    const Buffer b[] = {
+        {"y", a->y, n, es, true, true},
+        {"weight", a->weight, nd, 4, true, false},
+        {"bias", a->bias, nd, 4, false, false},
+        {"x", a->x, n, es, true, false},  // last: y may be x itself
+    };
+    if ((s = check_buffers(b, a->x == a->y && a->x ? 3 : 4)) != RHZ_OK) return s;
     return hip_status(rhz::launch_layernorm(*a, static_cast<hipStream_t>(stream)), "layernorm launch");
 }
 

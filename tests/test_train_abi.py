@@ -238,3 +238,15 @@ def test_rust_bindings_agree():
 
 def params_of(text):
     return [" ".join(x.split()) for x in text.split(",") if x.strip()]
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(y=A + 4), "x"), (dict(x=A + 7 * STEP - 4, y=A + 7 * STEP), "x"), (dict(weight=A + 64, y=A), "weight"),
+    (dict(bias=A + 2 * STEP + 4), "bias"), (dict(x=A, y=A, weight=A), "weight")])
+def test_layernorm_overlaps(over, msg):
+    """y may be x itself, but not lie across it, a weight or a bias."""
+    a = _fill(_abi.LayernormArgs, NORM, ("x", "weight", "y"), over)
+    if "weight" in over and "x" not in over:
+        a.x = A + 5 * STEP
+    assert _abi.lib().rhz_layernorm(byref(a), None) == _abi.ERR_INVALID_ARG
+    assert "y overlaps " + msg in _abi.last_error()
