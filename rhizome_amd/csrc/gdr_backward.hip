@@ -34,14 +34,15 @@
 // of every (chunk, head) at once from S0, dS1, W and dX.  What passes between
 // them lies in the workspace: a chunk's S0 and dS1 are four times its K, and
 // keeping them is what lets the last kernel, 3/4 of the products, run on all
-// chunks at once.  4 x 4096 tokens, 16 heads, d = 128, bf16: 485 us, 1.9 GB of
+// chunks at once.  4 x 4096 tokens, 16 heads, d = 128, bf16: 484 us, 1.9 GB of
 // HBM traffic (the inputs and outputs alone: 0.47), 370 us at a copy's rate.
 //
 // bf16 tensors are multiplied as fp16 (11 significant bits) on MFMA with fp32
-// accumulation: each fp16 operand is scaled by a power of two of its own, from
-// the largest magnitude of the tile it is rounded in, so that the magnitude of
-// the inputs (a loss's gradient of 1e-8, say) does not matter.  S, dS and every
-// sum are fp32.  fp32 tensors are multiplied in fp32 throughout.
+// accumulation: each fp16 operand is scaled by a power of two, from the largest
+// magnitude of the tile it is rounded in (of V and dO) or of the chunk's factors
+// that it is made of, so that the magnitude of the inputs (a loss's gradient of
+// 1e-8, say) does not matter.  S, dS and every sum are fp32.  fp32 tensors are
+// multiplied in fp32 throughout.
 
 #include <algorithm>
 #include <type_traits>
@@ -428,7 +429,7 @@ __device__ __forceinline__ float decay(const Gates& gs, int r, int s) { return p
 // rows (then P and T's diagonal blocks in fp32), L diag(beta) in fp32.  T and P
 // (16 KiB) are handed on rather than T K, T V, P^T dO and their like (80 KiB):
 // the scans multiply by them twice instead, which cost less than the traffic
-// (prep 152 -> 66 us, the whole call 594 -> 528 us at the size above).  68 us
+// (prep 152 -> 66 us, the whole call 594 -> 528 us at the size above).  73 us
 // for 0.22 GB: bound by the latency of the forward substitution and the products
 // down T's block columns, three workgroups a CU.
 template <class Op, int DK>
@@ -937,9 +938,9 @@ __device__ __forceinline__ bool scan_at(const BwdParams& p, int splits, ScanAt& 
 // fp32.  The serving waves watch W and dX as they store them, off the chain (no
 // difference in time).
 //
-// 16384 tokens, 16 heads, d_k = 128, d_v = 256: 770 us, 5900 cycles a chunk, of
-// which the chain waits 350; eight serving waves leave it 168 registers: 816.
-// 4 x 4096 tokens, d = 128 (a workgroup on every CU): 235 us for 0.92 GB, 75 % of
+// 16384 tokens, 16 heads, d_k = 128, d_v = 256: 784 us, some 5900 cycles a chunk,
+// of which the chain waits 350; eight serving waves leave it 168 registers: 816.
+// 4 x 4096 tokens, d = 128 (a workgroup on every CU): 243 us for 0.85 GB, 67 % of
 // a copy's rate.
 template <int DK>
 struct Scan16Lds {
@@ -1321,7 +1322,7 @@ __global__ __launch_bounds__(256 * TILES) void bwd_scan32_kernel(BwdParams p, in
 // from it on with W's rows as columns).  Then K and Q take the tiles' place and
 // the 64 x 64 products follow, right operands from the accumulators.  The
 // tiles' exponents differ; right operands are scaled to the largest.
-// 192 us for 0.84 GB at 4 x 4096 tokens, 16 heads, d = 128, bf16: 85 % of a
+// 202 us for 0.84 GB at 4 x 4096 tokens, 16 heads, d = 128, bf16: 80 % of a
 // copy's rate, two workgroups a CU (as first built, with one, 633 us).
 
 template <class Op, int DK>
@@ -1828,9 +1829,10 @@ __global__ __launch_bounds__(256, Op::kScaled ? 2 : 1) void bwd_grad_kernel(BwdP
 
 // ---------------------------------------------------------------- exact
 // bf16 heads whose inputs leave the fp16 path's domain (a key with |k|^2 >
-// 1.03125, beta or alpha outside [0, 1], a value that is not finite): the same
-// steps in fp32, one workgroup per (sequence, head), after the others (4 us where
-// no head is flagged).  The
+// 1.03125, beta or alpha outside [0, 1], a value that is not finite) or whose
+// values left fp16's range: the same steps in fp32, one workgroup per (sequence,
+// head), after the others.  5 us where no head is flagged, else 2.4 us a token at
+// d = 128 (4096 tokens 10 ms) and 3.9 at d_v = 256 (16384 tokens 64 ms).  The
 // states before the chunks are kept in fp32 where the records' S0 and dS1 were
 // (the same bytes), and everything else of the present chunk in the
 // workgroup's own scratch: a record of fp32 units and the state's gradient.

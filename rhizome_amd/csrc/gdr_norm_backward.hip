@@ -14,9 +14,9 @@
 // its columns' share of dw and db in registers; the blocks' shares go to the
 // workspace and a second kernel adds them in a fixed order.
 //
-// bf16, of a copy's 5.2 TB/s: layer norm of 16384 rows of 2048, 0.13 GB in 27 us
-// (5.0 TB/s); its backward pass, 0.21 GB in 43 us (4.9) and 4 us for the sums;
-// RMSNorm's backward pass of 262144 rows of 128, 0.20 GB in 38 us (5.3) and 4 us.
+// bf16, of a copy's 5.2 TB/s: layer norm of 16384 rows of 2048, 0.13 GB in 29 us
+// (4.6 TB/s); its backward pass, 0.21 GB in 43 us (4.9) and 4 us for the sums;
+// RMSNorm's backward pass of 262144 rows of 128, 0.20 GB in 39 us (5.1) and 4 us.
 
 #include <algorithm>
 
