@@ -52,7 +52,11 @@ def _on_stream(run, args):
     allocates is that stream's memory from the start, not memory that the
     current stream's earlier work may still use, and its results stay whole
     until the current stream's work is done with them too."""
-    stream, here = args["stream"], torch.cuda.current_stream()
+    stream = args["stream"]
+    for t in args.values():
+        if isinstance(t, torch.Tensor) and t.device != stream.device:
+            raise ValueError(f"all tensors must be on the stream's device, {stream.device}")
+    here = torch.cuda.current_stream()
     with torch.cuda.stream(stream):
         out = run(**{**args, "stream": None})
     for t in out if isinstance(out, tuple) else (out,):

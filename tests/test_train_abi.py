@@ -250,3 +250,18 @@ def test_layernorm_overlaps(over, msg):
         a.x = A + 5 * STEP
     assert _abi.lib().rhz_layernorm(byref(a), None) == _abi.ERR_INVALID_ARG
     assert "y overlaps " + msg in _abi.last_error()
+
+
+def test_a_stream_of_another_device_is_refused():
+    """Before anything is allocated or launched there."""
+    import types
+
+    import torch
+
+    import rhizome_amd
+
+    x, w = torch.empty((4, 8), device="meta"), torch.empty(8, device="meta")
+    other = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0)
+    for run in (rhizome_amd.layernorm, rhizome_amd.rmsnorm_heads):
+        with pytest.raises(ValueError, match="stream's device"):
+            run(x, w, stream=other)
