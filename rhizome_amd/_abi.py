@@ -1,4 +1,4 @@
-"""ctypes mirror of include/rhizome_gdr.h and rhizome_train.h and the loader of librhizome_gdr.so.
+"""ctypes mirror of include/rhizome_gdr.h, rhizome_train.h and rhizome_attention.h and the loader of librhizome_gdr.so.
 
 The library is loaded from this package directory only (built in-tree by
 rhizome_amd.build); if it is missing, loading raises -- there is no
@@ -19,6 +19,7 @@ ROOT = os.path.dirname(HERE)
 LIB_PATH = os.environ.get("RHIZOME_GDR_LIB") or os.path.join(HERE, "librhizome_gdr.so")
 HEADER = os.path.join(ROOT, "include", "rhizome_gdr.h")
 TRAIN_HEADER = os.path.join(ROOT, "include", "rhizome_train.h")
+ATTENTION_HEADER = os.path.join(ROOT, "include", "rhizome_attention.h")
 
 # rhz_status
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_HIP = 0, 1, 2, 3, 4
@@ -34,6 +35,9 @@ MULTISTEP_MAX = 64
 NOALLOC_MAX_SEQS = 65536
 # rhz_fill_kind
 FILL_NORMAL, FILL_UNIT_ROWS, FILL_SIGMOID, FILL_NEG_SOFTPLUS, FILL_UNIFORM = 0, 1, 2, 3, 4
+
+# rhz_rope_scaling
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_PARTS = 0, 1, 2
 
 
 class PrefillArgs(Structure):
@@ -150,6 +154,60 @@ class RmsnormArgs(Structure):
     ]
 
 
+class RopeFrequencyArgs(Structure):
+    _fields_ = [
+        ("dim", c_int32), ("scaling", c_int32), ("theta", c_double), ("factor", c_double),
+        ("trained_length", c_double), ("fast", c_double), ("slow", c_double),
+    ]
+
+
+class RopeArgs(Structure):
+    _fields_ = [
+        ("tokens", c_int32), ("heads", c_int32), ("dim", c_int32), ("offset", c_int32), ("rot", c_int32),
+        ("dtype", c_int32), ("interleaved", c_int32), ("inverse", c_int32), ("magnitude", c_float),
+        ("x_token_stride", c_int64), ("x_head_stride", c_int64), ("y_token_stride", c_int64), ("y_head_stride", c_int64),
+        ("x", c_void_p), ("positions", c_void_p), ("turns", c_void_p), ("y", c_void_p),
+    ]
+
+
+class LatentAppendArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32), ("seq_len", c_int32), ("d_c", c_int32), ("d_r", c_int32), ("page_size", c_int32),
+        ("num_pages", c_int32), ("max_pages", c_int32), ("dtype", c_int32), ("interleaved", c_int32),
+        ("magnitude", c_float), ("eps", c_float), ("latent_stride", c_int64), ("k_rope_stride", c_int64),
+        ("latent", c_void_p), ("k_rope", c_void_p), ("cu_seqlens", c_void_p), ("lengths", c_void_p),
+        ("page_table", c_void_p), ("turns", c_void_p), ("norm_scale", c_void_p), ("cache", c_void_p),
+    ]
+
+
+class LatentDecodeArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32), ("steps", c_int32), ("heads", c_int32), ("d_c", c_int32), ("d_r", c_int32),
+        ("page_size", c_int32), ("num_pages", c_int32), ("max_pages", c_int32), ("dtype", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("cache", c_void_p), ("page_table", c_void_p), ("lengths", c_void_p), ("o", c_void_p),
+        ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class LatentPrefillArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32), ("seq_len", c_int32), ("seq_len_k", c_int32), ("heads", c_int32), ("d_n", c_int32),
+        ("d_r", c_int32), ("d_v", c_int32), ("dtype", c_int32), ("causal", c_int32), ("scale", c_float),
+        ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("k_token_stride", c_int64), ("k_head_stride", c_int64),
+        ("v_token_stride", c_int64), ("v_head_stride", c_int64), ("k_rope_stride", c_int64),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("k_rope", c_void_p), ("cu_seqlens", c_void_p),
+        ("cu_seqlens_k", c_void_p), ("o", c_void_p), ("lse", c_void_p),
+    ]
+
+
+class LatentPrefillBackwardArgs(Structure):
+    _fields_ = [
+        ("forward", LatentPrefillArgs), ("grad_o", c_void_p), ("grad_lse", c_void_p), ("grad_q", c_void_p),
+        ("grad_k", c_void_p), ("grad_v", c_void_p), ("grad_k_rope", c_void_p), ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 class GdrError(RuntimeError):
     """A non-OK rhz_status, with the library's detail message."""
 
@@ -207,14 +265,20 @@ def lib():
         L.rhz_gdr_prefill_backward.argtypes = [POINTER(PrefillBackwardArgs), c_void_p]
         L.rhz_gdr_prefill_backward.restype = c_int32
         for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
-                           ("rhz_norm_backward", NormBackwardArgs)):
+                           ("rhz_norm_backward", NormBackwardArgs), ("rhz_latent_decode", LatentDecodeArgs),
+                           ("rhz_latent_prefill_backward", LatentPrefillBackwardArgs)):
             size = getattr(L, name + "_workspace_size")
             size.argtypes, size.restype = [POINTER(args), POINTER(c_size_t)], c_int32
         for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
                            ("rhz_layernorm", LayernormArgs), ("rhz_layernorm_backward", NormBackwardArgs),
-                           ("rhz_rmsnorm_heads_backward", NormBackwardArgs)):
+                           ("rhz_rmsnorm_heads_backward", NormBackwardArgs), ("rhz_rope", RopeArgs),
+                           ("rhz_latent_append", LatentAppendArgs), ("rhz_latent_decode", LatentDecodeArgs),
+                           ("rhz_latent_prefill", LatentPrefillArgs),
+                           ("rhz_latent_prefill_backward", LatentPrefillBackwardArgs)):
             run = getattr(L, name)
             run.argtypes, run.restype = [POINTER(args), c_void_p], c_int32
+        L.rhz_rope_frequencies.argtypes = [POINTER(RopeFrequencyArgs), POINTER(c_double), POINTER(c_float)]
+        L.rhz_rope_frequencies.restype = c_int32
         L.rhz_causal_conv1d.argtypes = [POINTER(Conv1dArgs), c_void_p]
         L.rhz_causal_conv1d.restype = c_int32
         L.rhz_gdr_prepare.argtypes = [POINTER(PrepareArgs), c_void_p]

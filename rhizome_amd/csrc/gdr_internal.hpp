@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "rhizome_attention.h"
 #include "rhizome_gdr.h"
 #include "rhizome_train.h"
 
@@ -92,6 +93,18 @@ hipError_t launch_layernorm(const rhz_layernorm_args& a, hipStream_t stream);
 size_t norm_backward_workspace_bytes(const rhz_norm_backward_args& a);
 // layer: layer norm's, else RMSNorm's
 hipError_t launch_norm_backward(const rhz_norm_backward_args& a, bool layer, hipStream_t stream);
+
+// The Global block's latent attention (latent_cache.hip, latent_decode.hip,
+// attn_prefill.hip, attn_backward.hip).
+hipError_t launch_rope(const rhz_rope_args& a, hipStream_t stream);
+hipError_t launch_latent_append(const rhz_latent_append_args& a, hipStream_t stream);
+size_t latent_decode_workspace_bytes(const rhz_latent_decode_args& a);
+hipError_t launch_latent_decode(const rhz_latent_decode_args& a, hipStream_t stream);
+hipError_t launch_latent_prefill(const rhz_latent_prefill_args& a, hipStream_t stream);
+size_t latent_prefill_backward_workspace_bytes(const rhz_latent_prefill_backward_args& a);
+hipError_t launch_latent_prefill_backward(const rhz_latent_prefill_backward_args& a, hipStream_t stream);
+// Whether the call's inputs can be read 16 bytes at a time.
+bool attn_vectors(const rhz_latent_prefill_args& a);
 
 // Device Philox-4x32-10 fill.
 hipError_t launch_philox_fill(int kind, uint64_t seed, uint64_t stream_id, int64_t count,
