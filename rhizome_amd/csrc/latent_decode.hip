@@ -3,17 +3,13 @@
 // of all heads.
 //
 // The rows of q of a sequence, `steps` positions by H heads, meet every cached
-// row: 2 (2 d_c + d_r) flops a value pair against (d_c + d_r) e bytes, bound by
-// memory up to some 128 rows.  A workgroup takes 32 RT rows of q and one split
-// of the sequence, whose cached rows come through LDS in tiles of 32, once for
-// the scores (rows of the tile) and once for the sum (its columns).  Of a tile
-//   scores: wave w sums q . k over its part of the columns for row tile w % RT;
-//           the parts meet in LDS and every wave adds them up and takes the
-//           softmax of all rows (cheaper than another exchange);
-//   sum:    wave w has the columns from w d_c / 4 on of all rows.
-// Splits go to the workspace unnormalised, with their maxima and sums, and are
-// joined in order by a second kernel.  Their number depends on the sequence's
-// length alone, so that a sequence's result does not depend on its batch.
+// row: 2 (2 d_c + d_r) flops a pair of rows against (d_c + d_r) e bytes a cached
+// row, bound by memory up to some 128 rows of q.  A workgroup takes one split of
+// the sequence, whose cached rows go through LDS once, there to be read along
+// the row for the scores and transposed for the sum.  Splits go to the workspace
+// unnormalised, with their maxima and sums, and are joined in order by another
+// kernel.  Their number depends on the sequence's length alone, so that a
+// sequence's result does not depend on its batch.
 #include <algorithm>
 
 #include "attn_device.hpp"
@@ -34,13 +30,13 @@ struct DecodeParams {
     float scale;
 };
 
-constexpr int kThreads = 256, kKeys = 32, kTable = 1024;
-constexpr int kMaxSplits = 128, kMinSplit = 256;
+constexpr int kTable = 1024;  // cached rows whose places are looked up at once
+constexpr int kMaxSplits = 128, kMinSplit = 256, kUnit = 32;
 
 // Cached rows of a split of a sequence of n rows.
 __host__ __device__ inline int split_rows(int n) {
     const int even = (n + kMaxSplits - 1) / kMaxSplits;
-    return max(kMinSplit, (even + kKeys - 1) / kKeys * kKeys);
+    return max(kMinSplit, (even + kUnit - 1) / kUnit * kUnit);
 }
 __host__ __device__ inline int splits_of(int n) { return n <= 0 ? 1 : (n + split_rows(n) - 1) / split_rows(n); }
 
@@ -49,182 +45,258 @@ __device__ __forceinline__ int rows_of(const DecodeParams& a, int seq) {
     return (int)min((long)max(a.lengths[seq], 0), room);
 }
 
-// Waits for all but the last n loads of a wave.
-template <int N>
-__device__ __forceinline__ void landed_but() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+// What a workgroup is to do: of sequence `seq` the positions [begin, end) for
+// the rows of q from `first_row` on.
+struct Unit {
+    int seq, split, splits, first_row, begin, end, n, length;
+};
+// The row tiles of a split follow one another on one XCD, whose L2 has the rows.
+__device__ __forceinline__ bool unit_of(const DecodeParams& a, int tile_rows, Unit& u) {
+    const int k = blockIdx.x >> 3, unit = k / a.row_tiles * 8 + (blockIdx.x & 7);
+    if (unit >= a.batch * a.splits) return false;
+    u.seq = unit / a.splits, u.split = unit % a.splits, u.first_row = k % a.row_tiles * tile_rows;
+    u.length = a.lengths[u.seq];
+    u.n = rows_of(a, u.seq);
+    u.splits = splits_of(u.n);
+    u.begin = u.split * split_rows(u.n);
+    u.end = min(u.n, u.begin + split_rows(u.n));
+    return u.split < u.splits;
 }
+// Cache row of position j, -1 where its page is outside the cache.
+__device__ __forceinline__ int cache_row(const DecodeParams& a, int seq, int j) {
+    const int page = a.table[(long)seq * a.max_pages + j / a.page];
+    return page >= 0 && page < a.num_pages ? page * a.page + j % a.page : -1;
+}
+// Positions that row r of q sees, by the length that the caller gave.
+__device__ __forceinline__ int sees(const DecodeParams& a, const Unit& u, int r) {
+    return (int)min((long)u.n, (long)u.length - a.steps + r / a.heads + 1);
+}
+
+// The unit's columns [d0, d0 + cols) of one row of q summed again over what the
+// row sees, for rows that came out not finite (attn_device.hpp).
+template <int N, typename T>
+__device__ __forceinline__ void sum_unit_row_again(const DecodeParams& a, const Unit& u, int row, int d0, int cols, float m,
+                                                   float f, int lane) {
+    const float c = a.scale * kLog2e, mc = m == -INFINITY ? 0.f : m * c;
+    const T* cache = (const T*)a.cache;
+    const long at = (long)u.seq * a.steps * a.heads + row;
+    const Rows<T> q = {(const T*)a.q + at * a.D, (const T*)a.q, 0, 0, a.D, 0}, k = {cache, cache, a.D, 0, a.D, 0};
+    sum_row_again<N>(
+        u.begin, min(u.end, sees(a, u, row)), cols, lane,
+        [&](long j) {
+            const int r = cache_row(a, u.seq, (int)j);
+            return r < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(dot_rows(q, 0, k, r), c, -mc)) * f;
+        },
+        [&](long j, int d) {
+            const int r = cache_row(a, u.seq, (int)j);
+            return r < 0 ? 0.f : Elem<T>::load(cache, (long)r * a.D + d0 + d);
+        },
+        [&](int d, float x) {
+            if (u.splits > 1)
+                a.part[(((long)u.seq * a.splits + u.split) * a.steps * a.heads + row) * a.d_c + d0 + d] = x;
+            else
+                Elem<T>::store((T*)a.o, at * a.d_c + d0 + d, x);
+        });
+}
+// Maximum and sum of row r of q: to the workspace, or the logarithm where this is all.
+__device__ __forceinline__ void store_sums(const DecodeParams& a, const Unit& u, int r, float m, float l) {
+    const int rows = a.steps * a.heads;
+    if (u.splits > 1) {
+        const long at = ((long)u.seq * a.splits + u.split) * rows + r;
+        a.part_m[at] = m, a.part_l[at] = l;
+    } else if (a.lse) {
+        a.lse[(long)u.seq * rows + r] = l == 0.f ? -INFINITY : fmaf(m, a.scale, logf(l));
+    }
+}
+
+// Waits for all but the last N loads of a wave.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// LDS reads and writes done, by all waves; loads on their way stay so.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ void load_to_lds16_from(const void* p, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
 
+// ------------------------------------------------------- many rows, or fp32
+// Eight waves, 32 RT rows of q, tiles of 32 cached rows.  Of a tile
+//   scores  wave w sums q . k of row tile w % RT over its part of the columns;
+//   weights the parts meet in LDS, and the waves of a row tile add them up and
+//           take its softmax, all of them the same; one hands the weights on;
+//   sum     wave w has the columns from w d_c / 8 on of all rows.
 template <typename T, int VD, int RT, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void latent_decode_kernel(DecodeParams a) {
-    constexpr int E = kChunkElems<T>, KD = VD + 64, BUFS = sizeof(T) == 2 ? 3 : 1;
-    constexpr int PARTS = 4 / RT, QP = KD / (2 * E) / PARTS, VTW = VD / 128;  // chunk pairs and column tiles of a wave
-    using TILE = Tile<T, KD, kKeys>;
+__global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
+    constexpr int E = kChunkElems<T>, KD = VD + 64, BUFS = sizeof(T) == 2 ? 3 : 1, NT = 512, WAVES = 8, KEYS = 32;
+    constexpr int PARTS = WAVES / RT, QP = KD / (2 * E) / PARTS, VTW = VD < 256 ? 1 : VD / 256;  // column tiles of a wave
+    static_assert(KD / (2 * E) % PARTS == 0, "whole chunk pairs for every part");
+    constexpr int WV = sizeof(T) == 2 ? 2 : 4;  // 16-byte vectors of a lane's weights
+    using TILE = Tile<T, KD, KEYS>;
     __shared__ TILE tiles[BUFS];
-    __shared__ f32x4 scores[4][4][kWave];  // [part, row tile][registers by four][lane]
+    __shared__ f32x4 scores[WAVES][4][kWave];  // [part, row tile][registers by four][lane]
+    __shared__ u32x4 handed[RT][WV][kWave];
+    __shared__ float scaled[RT][kWave], final_m[RT][kWave], final_l[RT][kWave];
     __shared__ int row_at[kTable];
     __shared__ uint32_t there[BUFS];  // a bit for every row of a tile: that its page is in the cache
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
-
-    // the row tiles of a split follow one another on one XCD, whose L2 has the rows
-    const int n_unit = blockIdx.x >> 3, unit = n_unit / a.row_tiles * 8 + (blockIdx.x & 7);
-    if (unit >= a.batch * a.splits) return;
-    const int seq = unit / a.splits, split = unit % a.splits, first_row = n_unit % a.row_tiles * 32 * RT;
-    const int n = rows_of(a, seq), splits = splits_of(n);
-    if (split >= splits) return;
-    const int begin = split * split_rows(n), end = min(n, begin + split_rows(n));
-    const int rows = a.steps * a.heads;
-    const int length = a.lengths[seq];
-
-    // cache row of position j, -1 where its page is outside the cache
-    const auto cache_row = [&](int j) {
-        const int page = a.table[(long)seq * a.max_pages + j / a.page];
-        return page >= 0 && page < a.num_pages ? page * a.page + j % a.page : -1;
-    };
-    // positions that row r of q sees, by the length that the caller gave
-    const auto sees = [&](int r) { return (int)min((long)n, (long)length - a.steps + r / a.heads + 1); };
+    Unit u;
+    if (!unit_of(a, 32 * RT, u)) return;
+    const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
 
     const int part = wave / RT, mine = wave % RT;
     u32x4 q[QP];
     {
         const Rows<T> qrows = {(const T*)a.q, (const T*)a.q, a.D, 0, a.D, 0};
-        const int r = min(first_row + 32 * mine + (lane & 31), rows - 1);
+        const int r = min(u.first_row + 32 * mine + (lane & 31), rows - 1);
 #pragma unroll
         for (int i = 0; i < QP; ++i)
-            q[i] = load_chunk<T, VEC>(qrows, (long)seq * rows + r, 0, 2 * (part * QP + i) + g);
+            q[i] = load_chunk<T, VEC>(qrows, (long)u.seq * rows + r, 0, 2 * (part * QP + i) + g);
     }
 #pragma unroll
     for (int i = 0; i < QP; ++i) settle(q[i]);
     if (a.D < TILE::kPanels * 8 * E)  // columns that no load writes
         for (int b = 0; b < BUFS; ++b)
-            for (int i = tid; i < TILE::kPanels * kKeys * 8; i += kThreads) tiles[b].chunk[i] = u32x4{0, 0, 0, 0};
+            for (int i = tid; i < TILE::kPanels * KEYS * 8; i += NT) tiles[b].chunk[i] = u32x4{0, 0, 0, 0};
 
     const auto fill_table = [&](int j0) {
-        for (int i = tid; i < kTable && j0 + i < end + kKeys; i += kThreads) row_at[i] = cache_row(min(j0 + i, end - 1));
+        for (int i = tid; i < kTable && j0 + i < end + KEYS; i += NT) row_at[i] = cache_row(a, u.seq, min(j0 + i, end - 1));
     };
     // Tile of positions j0 ..: those beyond the end repeat the last, those whose
     // page is outside the cache take row 0, which costs time if that is not
-    // finite (below).
+    // finite (sum_unit_row_again).  Half of the waves have the odd panels.
+    const int my_panel = wave >> 2;
     const auto start = [&](int j0, int b) {
-        const int r = tid >> 3, c = (tid & 7) ^ twist(r);
+        const int i = tid & 255, r = i >> 3, c = (i & 7) ^ twist(r);
         const int row = row_at[(j0 - begin + r) % kTable];
         const unsigned long long in = __ballot(row >= 0);  // eight lanes a row
         uint32_t bits = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) bits |= uint32_t(in >> (8 * k) & 1) << k;
-        if (lane == 0) reinterpret_cast<uint8_t*>(&there[b])[wave] = uint8_t(bits);
+        if (lane == 0 && wave < 4) reinterpret_cast<uint8_t*>(&there[b])[wave] = uint8_t(bits);
         const T* p = (const T*)a.cache + (long)max(row, 0) * a.D;
-        const uint32_t lds = lds_offset(&tiles[b].chunk[0]) + wave * 64 * 16;
+        const uint32_t lds = lds_offset(&tiles[b].chunk[0]) + (wave & 3) * 64 * 16;
 #pragma unroll
-        for (int k = 0; k < TILE::kPanels; ++k) {
-            const int d = (k * 8 + c) * E;
-            if (k * 8 * E >= a.D) break;
+        for (int k2 = 0; k2 < TILE::kPanels; k2 += 2) {
+            const int k = k2 + my_panel, d = (k * 8 + c) * E;
+            if (k >= TILE::kPanels || k * 8 * E >= a.D) break;
             if constexpr (VEC) {
                 if (d < a.D) load_to_lds16_from(p + d, lds + k * TILE::kPanelBytes);
             } else {
                 const Rows<T> one = {p, p, 0, 0, a.D, 0};
-                tiles[b].chunk[k * kKeys * 8 + tid] = load_chunk<T, false>(one, 0, 0, k * 8 + c);
+                tiles[b].chunk[k * KEYS * 8 + i] = load_chunk<T, false>(one, 0, 0, k * 8 + c);
             }
         }
     };
     f32x16 o[RT][VTW];
-    float m[RT], l[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        m[t] = -INFINITY, l[t] = 0.f;
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int d = 0; d < VTW; ++d) o[t][d] = f32x16{};
-    }
+    float m = -INFINITY, l = 0.f;
     const float c = a.scale * kLog2e;
-    const int least_seen = sees(first_row);
+    const int least_seen = sees(a, u, u.first_row);
+    const bool sums = wave * VTW * 32 < VD;  // the wave has columns
     fill_table(begin);
     __syncthreads();
-    const int tiles_n = (end - begin + kKeys - 1) / kKeys;
-    const bool counted = VEC && (a.D + 8 * E - 1) / (8 * E) == TILE::kPanels;  // loads of a tile as the waits count them
+    const int tiles_n = (end - begin + KEYS - 1) / KEYS;
+    // whether a tile's loads are as many as the waits below count
+    const bool counted = VEC && (a.D + 8 * E - 1) / (8 * E) == TILE::kPanels;
     if constexpr (BUFS == 3) {
         if (tiles_n > 0) start(begin, 0);
-        if (tiles_n > 1) start(begin + kKeys, 1);
+        if (tiles_n > 1) start(begin + KEYS, 1);
     }
-    for (int i = 0; i < tiles_n; ++i) {
-        const int j0 = begin + i * kKeys, b = i % BUFS, ahead = i + BUFS - 1;
-        if constexpr (BUFS == 3) {
-            if (counted && i + 1 < tiles_n)
-                landed_but<TILE::kPanels>();
+    for (int i = 0, b = 0; i < tiles_n; ++i, b = b + 1 == BUFS ? 0 : b + 1) {
+        const int j0 = begin + i * KEYS, ahead = i + BUFS - 1;
+        if (BUFS == 3 && counted && i + 1 < tiles_n) {
+            if (my_panel == 0)
+                wait_loads<(TILE::kPanels + 1) / 2>();
             else
-                landed();
+                wait_loads<TILE::kPanels / 2>();
+            lds_barrier();
         } else {
             landed();
         }
         if (ahead < tiles_n) {
-            if (ahead * kKeys % kTable == 0 && ahead > 0) {
-                fill_table(begin + ahead * kKeys);
+            if (ahead * KEYS % kTable == 0 && ahead > 0) {
+                fill_table(begin + ahead * KEYS);
                 __syncthreads();
             }
-            start(begin + ahead * kKeys, ahead % BUFS);
+            start(begin + ahead * KEYS, BUFS == 1 ? 0 : b == 0 ? BUFS - 1 : b - 1);
         }
         if constexpr (BUFS == 1) landed();
         const uint32_t tile = lds_offset(&tiles[b]);
-        {
-            f32x16 s = {};
+        f32x16 s = {};
 #pragma unroll
-            for (int k = 0; k < QP; ++k) {
-                // chunk pair part * QP + k
-                const int pair = part * QP + k;
-                const uint32_t p = ((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes;
-                dot_chunks(s, lds_read<u32x4>(p), q[k], T());
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) scores[wave][k][lane] = f32x4{s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]};
+        for (int k = 0; k < QP; ++k) {
+            // chunk pair part * QP + k
+            const int pair = part * QP + k;
+            const uint32_t p = ((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes;
+            dot_chunks(s, lds_read<u32x4>(p), q[k], T());
         }
-        // LDS alone: the next tiles' loads stay on their way
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 4; ++k) scores[wave][k][lane] = f32x4{s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]};
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f32x4 x = scores[mine][k][lane];
+#pragma unroll
+            for (int v = 1; v < PARTS; ++v) x += scores[mine + RT * v][k][lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * k + e] = x[e];
+        }
         const uint32_t in = __builtin_amdgcn_readfirstlane(there[b]);
-        const bool masked = j0 + kKeys > min(end, least_seen) || in != ~0u;
+        if (j0 + KEYS > min(end, least_seen) || in != ~0u) {
+            const int seen = min(end, sees(a, u, min(u.first_row + 32 * mine + (lane & 31), rows - 1)));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int r = (k & 3) + 8 * (k >> 2) + 4 * g;
+                if (j0 + r >= seen || !(in >> r & 1)) s[k] = -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) top = fmaxf(top, s[k]);
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        float f = 1.f;
+        if (__any((top - m) * c > 8.f)) {
+            const float up = fmaxf(m, top);
+            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
+            m = up;
+            l *= f;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            s[k] = __builtin_amdgcn_exp2f(fmaf(s[k], c, -mc));
+            l += s[k];
+        }
+        if (part == 0) {
+            Weights<T> p;
+            p.set(s);
+            u32x4 v[WV];
+            __builtin_memcpy(v, &p, sizeof v);
+#pragma unroll
+            for (int k = 0; k < WV; ++k) handed[mine][k][lane] = v[k];
+            scaled[mine][lane] = f;
+        }
+        lds_barrier();
+        if (!sums) continue;
         Weights<T> p[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            f32x16 s;
+            u32x4 v[WV];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                f32x4 x = scores[t][k][lane];
-#pragma unroll
-                for (int u = 1; u < PARTS; ++u) x += scores[t + RT * u][k][lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * k + e] = x[e];
-            }
-            if (masked) {
-                const int seen = min(end, sees(min(first_row + 32 * t + (lane & 31), rows - 1)));
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int r = (k & 3) + 8 * (k >> 2) + 4 * g;
-                    if (j0 + r >= seen || !(in >> r & 1)) s[k] = -INFINITY;
-                }
-            }
-            float top = s[0];
-#pragma unroll
-            for (int k = 1; k < 16; ++k) top = fmaxf(top, s[k]);
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            if (__any((top - m[t]) * c > 8.f)) {
-                const float up = fmaxf(m[t], top);
-                const float f = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - up) * c);
-                m[t] = up;
-                l[t] *= f;
+            for (int k = 0; k < WV; ++k) v[k] = handed[t][k][lane];
+            __builtin_memcpy(&p[t], v, sizeof v);
+            const float ft = scaled[t][lane];
+            if (__any(ft != 1.f)) {
 #pragma unroll
                 for (int d = 0; d < VTW; ++d)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[t][d][k] *= f;
+                    for (int k = 0; k < 16; ++k) o[t][d][k] *= ft;
             }
-            const float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                s[k] = __builtin_amdgcn_exp2f(fmaf(s[k], c, -mc));
-                l[t] += s[k];
-            }
-            p[t].set(s);
         }
 #pragma unroll
         for (int d = 0; d < VTW; ++d) {
@@ -235,56 +307,266 @@ __global__ __launch_bounds__(kThreads, 1) void latent_decode_kernel(DecodeParams
             for (int t = 0; t < RT; ++t) sum_rows(o[t][d], x, p[t]);
         }
     }
-
-    const long slot = (long)seq * a.splits + split;
+    l += __shfl_xor(l, 32, kWave);
+    if (part == 0) {
+        final_m[mine][lane] = m, final_l[mine][lane] = l;
+        const int r = u.first_row + 32 * mine + (lane & 31);
+        if (g == 0 && r < rows) store_sums(a, u, r, m, l);
+    }
+    lds_barrier();
+    if (!sums) return;
+    const long slot = (long)u.seq * a.splits + u.split;
     const int d0 = wave * VTW * 32, cols = min(a.d_c - d0, VTW * 32);  // the wave's columns
+    const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        l[t] += __shfl_xor(l[t], 32, kWave);
-        const int r = first_row + 32 * t + (lane & 31);
+        const int r = u.first_row + 32 * t + (lane & 31);
         bool live = r < rows;
-        const float f = splits > 1 ? 1.f : l[t] == 0.f ? 0.f : 1.f / l[t];
-        const auto out = [&](int row, int d, float x) {
-            if (splits > 1)
-                a.part[(slot * rows + row) * a.d_c + d] = x;
-            else
-                Elem<T>::store((T*)a.o, ((long)seq * rows + row) * a.d_c + d, x);
-        };
+        const float mt = final_m[t][lane], lt = final_l[t][lane];
+        const float f = u.splits > 1 ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
         uint32_t again = not_finite_rows(o[t]) & uint32_t(__ballot(live));
-        while (again) {  // the row's sum once more over what it sees
-            const int i = __ffs(again) - 1, row = first_row + 32 * t + i;
+        while (again) {
+            const int i = __ffs(again) - 1;
             again &= again - 1;
-            const float mr = __shfl(m[t], i, kWave), fr = __shfl(f, i, kWave);
-            const float mc = mr == -INFINITY ? 0.f : mr * c;
-            const Rows<T> qr = {(const T*)a.q + ((long)seq * rows + row) * a.D, (const T*)a.q, 0, 0, a.D, 0};
-            const Rows<T> kr = {(const T*)a.cache, (const T*)a.cache, a.D, 0, a.D, 0};
-            sum_row_again<VTW>(
-                begin, min(end, sees(row)), cols, lane,
-                [&](long j) {
-                    const int at = cache_row((int)j);
-                    return at < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(dot_rows(qr, 0, kr, at), c, -mc)) * fr;
-                },
-                [&](long j, int d) {
-                    const int at = cache_row((int)j);
-                    return at < 0 ? 0.f : Elem<T>::load(kr.p, (long)at * a.D + d0 + d);
-                },
-                [&](int d, float x) { out(row, d0 + d, x); });
+            sum_unit_row_again<VTW, T>(a, u, u.first_row + 32 * t + i, d0, cols, __shfl(mt, i, kWave), __shfl(f, i, kWave), lane);
             if ((lane & 31) == i) live = false;
         }
-        if (wave == 0 && g == 0 && r < rows) {
-            if (splits > 1)
-                a.part_m[slot * rows + r] = m[t], a.part_l[slot * rows + r] = l[t];
-            else if (a.lse)
-                a.lse[(long)seq * rows + r] = l[t] == 0.f ? -INFINITY : fmaf(m[t], a.scale, logf(l[t]));
-        }
         if (!live) continue;
-        const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
 #pragma unroll
         for (int d = 0; d < VTW; ++d) {
-            if (splits > 1)
+            if (u.splits > 1)
                 store_columns<float>(a.part + (slot * rows + r) * a.d_c, o[t][d], d0 + 32 * d, a.d_c, 1.f, vec, lane);
             else
-                store_columns<T>((T*)a.o + ((long)seq * rows + r) * a.d_c, o[t][d], d0 + 32 * d, a.d_c, f, vec, lane);
+                store_columns<T>((T*)a.o + ((long)u.seq * rows + r) * a.d_c, o[t][d], d0 + 32 * d, a.d_c, f, vec, lane);
+        }
+    }
+}
+
+// --------------------------------------------------- up to 16 rows, in bf16
+// Four waves, each with cached rows of its own -- every fourth tile of 16 -- and
+// a part of LDS for one tile, so that they need no barrier before their sums meet
+// at the end.  On 16x16 matrix instructions: the scores come out with the lane's
+// row of q as column and cached rows 4 g .. 4 g + 3 (g = lane / 16) in registers,
+// which is how the sum over a tile's rows takes its weights.  78 KB of LDS at d_c
+// = 512: two workgroups share a CU, and while some of its eight waves compute the
+// others' tiles are on their way.
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+
+template <int VD>
+__global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodeParams a) {
+    constexpr int KD = VD + 64, KC = KD / 32, VT = VD / 16, KEYS = 16, WAVES = 4;  // steps of the scores, column tiles
+    using T = uint16_t;
+    using TILE = Tile<T, KD, KEYS>;
+    constexpr int P = TILE::kPanels, PB = TILE::kPanelBytes;
+    __shared__ TILE tiles[WAVES];
+    __shared__ float wave_m[WAVES][16], wave_l[WAVES][16];
+    __shared__ int row_at[kTable];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    Unit u;
+    if (!unit_of(a, 16, u)) return;
+    const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
+
+    const auto fill_table = [&](int j0) {
+        for (int i = tid; i < kTable && j0 + i < end + KEYS; i += 64 * WAVES)
+            row_at[i] = cache_row(a, u.seq, min(j0 + i, end - 1));
+    };
+    if (end > begin) fill_table(begin);
+    u32x4 q[KC];
+    const Rows<T> qrows = {(const T*)a.q, (const T*)a.q, a.D, 0, a.D, 0};
+    const int kr = lane & 15, row = u.first_row + kr;  // the lane's row of q
+    const long q_row = (long)u.seq * rows + min(row, rows - 1);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) q[i] = load_chunk<T, true>(qrows, q_row, 0, 4 * i + g);
+    if (a.D < P * 64)  // columns that no load writes
+        for (int i = lane; i < P * KEYS * 8; i += 64) tiles[wave].chunk[i] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+
+    // Tile of positions j0 .., the two rows of each lane; returns a bit for every
+    // row whose page is in the cache, the others take row 0.
+    const auto start = [&](int j0) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = 8 * h + (lane >> 3), c = (lane & 7) ^ twist(r);
+            const int row = row_at[(j0 - begin + r) % kTable];
+            const unsigned long long in = __ballot(row >= 0);  // eight lanes a row
+#pragma unroll
+            for (int k = 0; k < 8; ++k) bits |= uint32_t(in >> (8 * k) & 1) << (8 * h + k);
+            const T* p = (const T*)a.cache + (long)max(row, 0) * a.D + c * 8;
+            const uint32_t lds = lds_offset(&tiles[wave].chunk[0]) + h * 1024;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if (k * 64 + 64 <= a.D)
+                    load_to_lds16_from(p + k * 64, lds + k * PB);
+                else if (k * 64 + c * 8 < a.D)
+                    load_to_lds16_from(p + k * 64, lds + k * PB);
+            }
+        }
+        return __builtin_amdgcn_readfirstlane(bits);
+    };
+
+    f32x4 o[VT];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < VT; ++d) o[d] = f32x4{};
+    const float c = a.scale * kLog2e;
+    const int least_seen = sees(a, u, u.first_row), seen = min(end, sees(a, u, min(row, rows - 1)));
+    // row lane % 16, chunk 4 i + g; and transposed: rows 4 g + (lane % 16) / 4
+    const int vr = 4 * g + (kr >> 2);
+    const uint32_t tile = lds_offset(&tiles[wave]);
+    const uint32_t k_at = tile + kr * 128 + ((twist(kr) ^ g) << 4), k_odd = k_at ^ (4 << 4);
+    const uint32_t v_at = tile + vr * 128 + ((twist(vr) ^ ((kr >> 1) & 1)) << 4) + (kr & 1) * 8;
+
+    const int tiles_n = (end - begin + KEYS - 1) / KEYS;
+    uint32_t there = 0;
+    if (wave < tiles_n) there = start(begin + wave * KEYS);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) settle(q[i]);
+    for (int i0 = 0; i0 < tiles_n; i0 += WAVES) {
+        const int i = i0 + wave, j0 = begin + i * KEYS;
+        if (i < tiles_n) {
+            wait_loads<0>();
+            // six reads ahead of the products, whatever the scheduler would have
+            constexpr int AHEAD = 6;
+            f32x4 s[2] = {};
+            u32x4 x[AHEAD];
+            const auto read = [&](int k) { return lds_read<u32x4>((k & 1 ? k_odd : k_at) + (k >> 1) * PB); };
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) x[k] = read(k);
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                s[k & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x[k % AHEAD]),
+                                                                   __builtin_bit_cast(bf16x8, q[k]), s[k & 1], 0, 0, 0);
+                if (k + AHEAD < KC) x[k % AHEAD] = read(k + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            s[0] += s[1];
+            if (j0 + KEYS > min(end, least_seen) || there != 0xffffu) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (j0 + 4 * g + k >= seen || !(there >> (4 * g + k) & 1)) s[0][k] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+            top = fmaxf(top, __shfl_xor(top, 16, kWave));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            if (__any((top - m) * c > 8.f)) {
+                const float up = fmaxf(m, top);
+                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
+                m = up;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < VT; ++d) o[d] *= f;
+            }
+            const float mc = m == -INFINITY ? 0.f : m * c;
+            bf16x4_t w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[0][k], c, -mc));
+                l += p;
+                w[k] = (__bf16)p;
+            }
+            const s16x4_t p = __builtin_bit_cast(s16x4_t, w);
+            s16x4_t y[2 * AHEAD];
+            const auto column = [&](int d) {
+                const uint32_t v = (v_at ^ ((2 * (d & 3)) << 4)) + (d >> 2) * PB;
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4_t*>(v));
+            };
+            constexpr int COLS = VT < 2 * AHEAD ? VT : 2 * AHEAD;
+#pragma unroll
+            for (int d = 0; d < COLS; ++d) y[d] = column(d);
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(y[d % COLS], p, o[d], 0, 0, 0);
+                if (d + COLS < VT) y[d % COLS] = column(d + COLS);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const int next = i0 + WAVES;
+        if (next < tiles_n && next * KEYS % kTable == 0) {  // the table ends; every wave has started all tiles before
+            __syncthreads();
+            fill_table(begin + next * KEYS);
+            __syncthreads();
+        }
+        if (next + wave < tiles_n) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile has been read
+            there = start(begin + (next + wave) * KEYS);
+        }
+    }
+
+    // The waves' sums at their common maximum: waves 2 and 3 hand theirs to 0 and
+    // 1, which exchange halves, so that each has the whole of half of the columns.
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    if (g == 0) wave_m[wave][kr] = m, wave_l[wave][kr] = l;
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, wave_m[w][kr]);
+    const float tc = top == -INFINITY ? 0.f : top * c;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum = fmaf(wave_l[w][kr], __builtin_amdgcn_exp2f(fmaf(wave_m[w][kr], c, -tc)), sum);
+    const float f = u.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    const float own = __builtin_amdgcn_exp2f(fmaf(m, c, -tc)) * f;
+    f32x4* given = reinterpret_cast<f32x4*>(&tiles[0]) + lane;
+    if (wave >= 2) {
+#pragma unroll
+        for (int d = 0; d < VT; ++d) given[((wave - 2) * VT + d) * kWave] = o[d] * own;
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int d = 0; d < VT; ++d) o[d] = o[d] * own + given[(wave * VT + d) * kWave];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int d = 0; d < VT / 2; ++d) given[(wave * (VT / 2) + d) * kWave] = wave ? o[d] : o[VT / 2 + d];
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+    bool live = row < rows;
+    if (wave == 0 && g == 0 && live) store_sums(a, u, row, top, sum);
+    const int d0 = wave * (VD / 2), cols = min(a.d_c - d0, VD / 2);
+    f32x4 x[VT / 2];
+    float bad = 0.f;  // as not_finite_rows
+#pragma unroll
+    for (int d = 0; d < VT / 2; ++d) {
+        x[d] = (wave ? o[VT / 2 + d] : o[d]) + given[((1 - wave) * (VT / 2) + d) * kWave];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bad = fmaf(x[d][k], 0.f, bad);
+    }
+    unsigned long long flags = __ballot(bad != 0.f && live);
+    flags |= flags >> 32;
+    uint32_t again = cols > 0 ? uint32_t(flags | flags >> 16) & 0xffffu : 0;
+    while (again) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        sum_unit_row_again<VD / 128, T>(a, u, u.first_row + i, d0, cols, __shfl(top, i, kWave), __shfl(f, i, kWave), lane);
+        if (kr == i) live = false;
+    }
+    if (!live) return;
+    const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
+    const long at_row = ((long)u.seq * a.splits + u.split) * rows + row;
+    float* part = a.part + at_row * a.d_c;
+    T* out = (T*)a.o + ((long)u.seq * rows + row) * a.d_c;
+#pragma unroll
+    for (int d = 0; d < VT / 2; ++d) {
+        const int at = d0 + 16 * d + 4 * g;
+        if (vec) {
+            if (at >= a.d_c) continue;
+            if (u.splits > 1)
+                *reinterpret_cast<f32x4*>(part + at) = x[d];
+            else
+                *reinterpret_cast<uint2*>(out + at) = make_uint2(pack_bf16x2(x[d][0], x[d][1]), pack_bf16x2(x[d][2], x[d][3]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (at + k >= a.d_c) continue;
+                if (u.splits > 1)
+                    part[at + k] = x[d][k];
+                else
+                    Elem<T>::store(out, at + k, x[d][k]);
+            }
         }
     }
 }
@@ -334,27 +616,52 @@ int most_splits(const rhz_latent_decode_args& a) {
     return splits_of((int)std::min<int64_t>((int64_t)a.max_pages * a.page_size, INT32_MAX));
 }
 
+hipError_t join(const DecodeParams& p, int dtype, hipStream_t stream) {
+    const int64_t joins = (int64_t)p.batch * p.steps * p.heads;
+    if (p.splits > 1) {
+        if (check_grid(joins, kJoinThreads) != hipSuccess) return hipErrorInvalidConfiguration;
+        if (dtype == RHZ_F32)
+            latent_join_kernel<float><<<(unsigned)joins, kJoinThreads, 0, stream>>>(p);
+        else
+            latent_join_kernel<uint16_t><<<(unsigned)joins, kJoinThreads, 0, stream>>>(p);
+    }
+    return hipGetLastError();
+}
+
+// Workgroups of `threads` with `tile` rows of q each; 0 if there are too many.
+unsigned blocks_of(DecodeParams& p, int tile, int threads) {
+    p.row_tiles = (p.steps * p.heads + tile - 1) / tile;
+    const int64_t blocks = ((int64_t)p.batch * p.splits + 7) / 8 * 8 * p.row_tiles;
+    return blocks > INT32_MAX || check_grid(blocks, threads) != hipSuccess ? 0 : (unsigned)blocks;
+}
+
 template <typename T, int VD, int RT, bool VEC>
 hipError_t launch(DecodeParams p, hipStream_t stream) {
-    const int rows = p.steps * p.heads;
-    p.row_tiles = (rows + 32 * RT - 1) / (32 * RT);
-    const int64_t blocks = ((int64_t)p.batch * p.splits + 7) / 8 * 8 * p.row_tiles, joins = (int64_t)p.batch * rows;
-    if (blocks > INT32_MAX || joins > INT32_MAX || check_grid(blocks, kThreads) != hipSuccess ||
-        check_grid(joins, kJoinThreads) != hipSuccess)
-        return hipErrorInvalidConfiguration;
-    latent_decode_kernel<T, VD, RT, VEC><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    if (p.splits > 1) latent_join_kernel<T><<<(unsigned)joins, kJoinThreads, 0, stream>>>(p);
-    return hipGetLastError();
+    const unsigned blocks = blocks_of(p, 32 * RT, 512);
+    if (!blocks) return hipErrorInvalidConfiguration;
+    latent_decode_kernel<T, VD, RT, VEC><<<blocks, 512, 0, stream>>>(p);
+    return join(p, sizeof(T) == 4 ? RHZ_F32 : RHZ_BF16, stream);
+}
+
+template <int VD>
+hipError_t launch_narrow(DecodeParams p, hipStream_t stream) {
+    const unsigned blocks = blocks_of(p, 16, 256);
+    if (!blocks) return hipErrorInvalidConfiguration;
+    latent_decode_narrow_kernel<VD><<<blocks, 256, 0, stream>>>(p);
+    return join(p, RHZ_BF16, stream);
 }
 
 template <typename T, int VD>
 hipError_t pick_rows(const DecodeParams& p, bool vec, hipStream_t stream) {
     const int rows = p.steps * p.heads;
-    if (!vec) return launch<T, VD, 1, false>(p, stream);
-    if (rows <= 32) return launch<T, VD, 1, true>(p, stream);
-    if constexpr (sizeof(T) == 2)  // four row tiles' accumulators and queries fill the registers in bf16
-        if (rows > 64) return launch<T, VD, 4, true>(p, stream);
-    return launch<T, VD, 2, true>(p, stream);
+    if constexpr (sizeof(T) == 4) {
+        if (!vec) return launch<T, VD, 1, false>(p, stream);
+        return rows <= 32 ? launch<T, VD, 1, true>(p, stream) : launch<T, VD, 2, true>(p, stream);
+    } else {
+        if (!vec) return launch<T, VD, 2, false>(p, stream);
+        if (rows <= 16) return launch_narrow<VD>(p, stream);
+        return rows <= 64 ? launch<T, VD, 2, true>(p, stream) : launch<T, VD, 4, true>(p, stream);
+    }
 }
 
 template <typename T>
