@@ -163,10 +163,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
                 }
             }
             if (masked) {
+                const int least = from - 4 * g, left = w.nq - qu - 4 * g;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = (i & 3) + 8 * (i >> 2) + 4 * g;
-                    if (r < from || qu + r >= w.nq) s[i] = dp[i] = 0.f;
+                    const int r = (i & 3) + 8 * (i >> 2);
+                    if (r < least || r >= left) s[i] = dp[i] = 0.f;
                 }
             }
             Weights<T> p, ds;
@@ -301,9 +302,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attn_dq_kern
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * (dp[i] - delta);
         if (masked) {
+            const int left = seen - k0 - 4 * g;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (k0 + (i & 3) + 8 * (i >> 2) + 4 * g >= seen) dp[i] = 0.f;
+                if ((i & 3) + 8 * (i >> 2) >= left) dp[i] = 0.f;
         }
         Weights<T> ds;
         ds.set(dp);

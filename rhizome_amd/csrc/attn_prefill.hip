@@ -109,11 +109,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void latent_prefi
         const int seen = a.causal ? min(w.nk, qi + shift + 1) : w.nk;  // keys that the lane's query sees
         const bool masked = k0 + BN > w.nk || (a.causal && k0 + BN > wq + shift + 1);
         if (masked) {
+            const int left = seen - k0 - 4 * g;
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (k0 + 32 * u + (i & 3) + 8 * (i >> 2) + 4 * g >= seen) s[u][i] = -INFINITY;
+                    if (32 * u + (i & 3) + 8 * (i >> 2) >= left) s[u][i] = -INFINITY;
         }
         float top = s[0][0];
 #pragma unroll

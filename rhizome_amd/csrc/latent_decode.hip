@@ -31,14 +31,22 @@ struct DecodeParams {
 };
 
 constexpr int kTable = 1024;  // cached rows whose places are looked up at once
-constexpr int kMaxSplits = 128, kMinSplit = 256, kUnit = 32;
+constexpr int kMaxSplits = 128, kMinSplit = 128, kBestSplit = 512, kUnit = 32;
 
-// Cached rows of a split of a sequence of n rows.
+// Cached rows of a split of a sequence of n rows: eighths of a short one, for
+// one request's latency, but of a long one as many as keep the parts' traffic
+// low against the cache's own (at 16 heads a part is written and read again for
+// 32 KB each against 1152 bytes a row).
 __host__ __device__ inline int split_rows(int n) {
-    const int even = (n + kMaxSplits - 1) / kMaxSplits;
-    return max(kMinSplit, (even + kUnit - 1) / kUnit * kUnit);
+    const int eighth = min(max(n / 8, kMinSplit), kBestSplit), even = max(eighth, n / kMaxSplits + (n % kMaxSplits != 0));
+    return (even + kUnit - 1) / kUnit * kUnit;
 }
 __host__ __device__ inline int splits_of(int n) { return n <= 0 ? 1 : (n + split_rows(n) - 1) / split_rows(n); }
+// No sequence of up to n rows has more: of eighths there are nine at most.
+inline int most_splits_of(int64_t n) {
+    const int64_t shortest = (n + kMinSplit - 1) / kMinSplit, best = (n + kBestSplit - 1) / kBestSplit;
+    return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(9, std::min<int64_t>(best, kMaxSplits))));
+}
 
 __device__ __forceinline__ int rows_of(const DecodeParams& a, int seq) {
     const long room = (long)a.max_pages * a.page;
@@ -116,27 +124,42 @@ __device__ __forceinline__ void wait_loads() {
 }
 // LDS reads and writes done, by all waves; loads on their way stay so.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// 16 bytes a lane from p + OFF to LDS at lds; the instruction's offset counts in LDS too.
+template <int OFF>
 __device__ __forceinline__ void load_to_lds16_from(const void* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(lds - OFF), "v"(p), "n"(OFF)
+                 : "memory");
+}
+// Panels K, K + STEP .. of a cached row from the lane's chunk of panel 0 at p on,
+// `left` bytes of the row being left from there.
+template <int K, int PANELS, int STEP>
+__device__ __forceinline__ void load_panels(const void* p, int left, int row_bytes, uint32_t lds, int panel_bytes) {
+    if constexpr (K < PANELS) {
+        if ((K + 1) * 128 <= row_bytes)
+            load_to_lds16_from<K * 128>(p, lds + K * panel_bytes);
+        else if (K * 128 < left)
+            load_to_lds16_from<K * 128>(p, lds + K * panel_bytes);
+        load_panels<K + STEP, PANELS, STEP>(p, left, row_bytes, lds, panel_bytes);
+    }
 }
 
 // ------------------------------------------------------- many rows, or fp32
-// Eight waves, 32 RT rows of q, tiles of 32 cached rows.  Of a tile
-//   scores  wave w sums q . k of row tile w % RT over its part of the columns;
-//   weights the parts meet in LDS, and the waves of a row tile add them up and
-//           take its softmax, all of them the same; one hands the weights on;
-//   sum     wave w has the columns from w d_c / 8 on of all rows.
+// Eight waves, 32 RT rows of q, tiles of 32 cached rows.  Wave w has row tile w
+// % RT, and of it a part of the columns.  Of a tile it sums q . k over its part;
+// the parts meet in LDS, and every wave of a row tile adds them up, takes the
+// softmax -- all of them the same -- and sums its part of the columns with it.
 template <typename T, int VD, int RT, bool VEC>
 __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     constexpr int E = kChunkElems<T>, KD = VD + 64, BUFS = sizeof(T) == 2 ? 3 : 1, NT = 512, WAVES = 8, KEYS = 32;
-    constexpr int PARTS = WAVES / RT, QP = KD / (2 * E) / PARTS, VTW = VD < 256 ? 1 : VD / 256;  // column tiles of a wave
+    constexpr int PARTS = WAVES / RT, QP = KD / (2 * E) / PARTS, VTW = VD / 32 < PARTS ? 1 : VD / 32 / PARTS;  // column tiles of a wave
     static_assert(KD / (2 * E) % PARTS == 0, "whole chunk pairs for every part");
-    constexpr int WV = sizeof(T) == 2 ? 2 : 4;  // 16-byte vectors of a lane's weights
     using TILE = Tile<T, KD, KEYS>;
     __shared__ TILE tiles[BUFS];
+    // 18 chunk pairs of q beside 8 column tiles of sums are four registers more
+    // than there are: one pair goes through LDS (a spilled one waits for the loads)
+    constexpr int KEPT = QP > 17 ? 17 : QP;
     __shared__ f32x4 scores[WAVES][4][kWave];  // [part, row tile][registers by four][lane]
-    __shared__ u32x4 handed[RT][WV][kWave];
-    __shared__ float scaled[RT][kWave], final_m[RT][kWave], final_l[RT][kWave];
+    __shared__ u32x4 q_rest[QP > KEPT ? WAVES : 1][kWave];
     __shared__ int row_at[kTable];
     __shared__ uint32_t there[BUFS];  // a bit for every row of a tile: that its page is in the cache
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
@@ -146,16 +169,18 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
 
     const int part = wave / RT, mine = wave % RT;
-    u32x4 q[QP];
+    u32x4 q[KEPT];
     {
         const Rows<T> qrows = {(const T*)a.q, (const T*)a.q, a.D, 0, a.D, 0};
         const int r = min(u.first_row + 32 * mine + (lane & 31), rows - 1);
+        const auto pair = [&](int i) { return load_chunk<T, VEC>(qrows, (long)u.seq * rows + r, 0, 2 * (part * QP + i) + g); };
 #pragma unroll
-        for (int i = 0; i < QP; ++i)
-            q[i] = load_chunk<T, VEC>(qrows, (long)u.seq * rows + r, 0, 2 * (part * QP + i) + g);
+        for (int i = 0; i < KEPT; ++i) q[i] = pair(i);
+        if constexpr (QP > KEPT) q_rest[wave][lane] = pair(KEPT);
     }
+    static_assert(QP <= KEPT + 1, "one pair of chunks in LDS");
 #pragma unroll
-    for (int i = 0; i < QP; ++i) settle(q[i]);
+    for (int i = 0; i < KEPT; ++i) settle(q[i]);
     if (a.D < TILE::kPanels * 8 * E)  // columns that no load writes
         for (int b = 0; b < BUFS; ++b)
             for (int i = tid; i < TILE::kPanels * KEYS * 8; i += NT) tiles[b].chunk[i] = u32x4{0, 0, 0, 0};
@@ -177,27 +202,26 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
         if (lane == 0 && wave < 4) reinterpret_cast<uint8_t*>(&there[b])[wave] = uint8_t(bits);
         const T* p = (const T*)a.cache + (long)max(row, 0) * a.D;
         const uint32_t lds = lds_offset(&tiles[b].chunk[0]) + (wave & 3) * 64 * 16;
-#pragma unroll
-        for (int k2 = 0; k2 < TILE::kPanels; k2 += 2) {
-            const int k = k2 + my_panel, d = (k * 8 + c) * E;
-            if (k >= TILE::kPanels || k * 8 * E >= a.D) break;
-            if constexpr (VEC) {
-                if (d < a.D) load_to_lds16_from(p + d, lds + k * TILE::kPanelBytes);
-            } else {
-                const Rows<T> one = {p, p, 0, 0, a.D, 0};
+        if constexpr (VEC) {
+            const int bytes = a.D * int(sizeof(T));
+            if (my_panel == 0)
+                load_panels<0, TILE::kPanels, 2>(p + c * E, bytes - c * 16, bytes, lds, TILE::kPanelBytes);
+            else
+                load_panels<1, TILE::kPanels, 2>(p + c * E, bytes - c * 16, bytes, lds, TILE::kPanelBytes);
+        } else {
+            const Rows<T> one = {p, p, 0, 0, a.D, 0};
+#pragma unroll 1
+            for (int k = my_panel; k < TILE::kPanels; k += 2)
                 tiles[b].chunk[k * KEYS * 8 + i] = load_chunk<T, false>(one, 0, 0, k * 8 + c);
-            }
         }
     };
-    f32x16 o[RT][VTW];
+    f32x16 o[VTW];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int d = 0; d < VTW; ++d) o[t][d] = f32x16{};
+    for (int d = 0; d < VTW; ++d) o[d] = f32x16{};
     float m = -INFINITY, l = 0.f;
     const float c = a.scale * kLog2e;
     const int least_seen = sees(a, u, u.first_row);
-    const bool sums = wave * VTW * 32 < VD;  // the wave has columns
+    const bool sums = part * VTW * 32 < VD;  // the wave has columns
     fill_table(begin);
     __syncthreads();
     const int tiles_n = (end - begin + KEYS - 1) / KEYS;
@@ -228,12 +252,22 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
         if constexpr (BUFS == 1) landed();
         const uint32_t tile = lds_offset(&tiles[b]);
         f32x16 s = {};
+        {
+            // reads ahead of the products, whatever the scheduler would have
+            constexpr int AHEAD = QP < 4 ? QP : 4;
+            u32x4 x[AHEAD];
+            const auto read = [&](int k) {
+                const int pair = part * QP + k;
+                return lds_read<u32x4>(((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes);
+            };
 #pragma unroll
-        for (int k = 0; k < QP; ++k) {
-            // chunk pair part * QP + k
-            const int pair = part * QP + k;
-            const uint32_t p = ((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes;
-            dot_chunks(s, lds_read<u32x4>(p), q[k], T());
+            for (int k = 0; k < AHEAD; ++k) x[k] = read(k);
+#pragma unroll
+            for (int k = 0; k < QP; ++k) {
+                dot_chunks(s, x[k % AHEAD], k < KEPT ? q[k < KEPT ? k : 0] : q_rest[wave][lane], T());
+                if (k + AHEAD < QP) x[k % AHEAD] = read(k + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) scores[wave][k][lane] = f32x4{s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]};
@@ -248,23 +282,27 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
         }
         const uint32_t in = __builtin_amdgcn_readfirstlane(there[b]);
         if (j0 + KEYS > min(end, least_seen) || in != ~0u) {
-            const int seen = min(end, sees(a, u, min(u.first_row + 32 * mine + (lane & 31), rows - 1)));
+            const int seen = min(end, sees(a, u, min(u.first_row + 32 * mine + (lane & 31), rows - 1))) - j0 - 4 * g;
+            const uint32_t mine_in = in >> (4 * g);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                const int r = (k & 3) + 8 * (k >> 2) + 4 * g;
-                if (j0 + r >= seen || !(in >> r & 1)) s[k] = -INFINITY;
+                const int r = (k & 3) + 8 * (k >> 2);
+                if (r >= seen || !(mine_in & 1u << r)) s[k] = -INFINITY;
             }
         }
         float top = s[0];
 #pragma unroll
         for (int k = 1; k < 16; ++k) top = fmaxf(top, s[k]);
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        float f = 1.f;
         if (__any((top - m) * c > 8.f)) {
             const float up = fmaxf(m, top);
-            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
             m = up;
             l *= f;
+#pragma unroll
+            for (int d = 0; d < VTW; ++d)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[d][k] *= f;
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
@@ -272,73 +310,42 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
             s[k] = __builtin_amdgcn_exp2f(fmaf(s[k], c, -mc));
             l += s[k];
         }
-        if (part == 0) {
-            Weights<T> p;
-            p.set(s);
-            u32x4 v[WV];
-            __builtin_memcpy(v, &p, sizeof v);
-#pragma unroll
-            for (int k = 0; k < WV; ++k) handed[mine][k][lane] = v[k];
-            scaled[mine][lane] = f;
-        }
-        lds_barrier();
         if (!sums) continue;
-        Weights<T> p[RT];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            u32x4 v[WV];
-#pragma unroll
-            for (int k = 0; k < WV; ++k) v[k] = handed[t][k][lane];
-            __builtin_memcpy(&p[t], v, sizeof v);
-            const float ft = scaled[t][lane];
-            if (__any(ft != 1.f)) {
-#pragma unroll
-                for (int d = 0; d < VTW; ++d)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) o[t][d][k] *= ft;
-            }
-        }
+        Weights<T> p;
+        p.set(s);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = 0; d < VTW; ++d) {
             Columns<T> x;
-            const int dt = wave * VTW + d;
-            x.template load<TILE>(tile, at, 0, dt);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) sum_rows(o[t][d], x, p[t]);
+            x.template load<TILE>(tile, at, 0, part * VTW + d);
+            sum_rows(o[d], x, p);
         }
     }
     l += __shfl_xor(l, 32, kWave);
-    if (part == 0) {
-        final_m[mine][lane] = m, final_l[mine][lane] = l;
-        const int r = u.first_row + 32 * mine + (lane & 31);
-        if (g == 0 && r < rows) store_sums(a, u, r, m, l);
-    }
-    lds_barrier();
+    const int r = u.first_row + 32 * mine + (lane & 31);
+    bool live = r < rows;
+    if (part == 0 && g == 0 && live) store_sums(a, u, r, m, l);
     if (!sums) return;
-    const long slot = (long)u.seq * a.splits + u.split;
-    const int d0 = wave * VTW * 32, cols = min(a.d_c - d0, VTW * 32);  // the wave's columns
+    const int d0 = part * VTW * 32, cols = min(a.d_c - d0, VTW * 32);  // the wave's columns
     const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
+    const float f = u.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    uint32_t again = not_finite_rows(o) & uint32_t(__ballot(live));
+    while (again) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        sum_unit_row_again<(VTW + 1) / 2, T>(a, u, u.first_row + 32 * mine + i, d0, cols, __shfl(m, i, kWave),
+                                             __shfl(f, i, kWave), lane);
+        if ((lane & 31) == i) live = false;
+    }
+    if (!live) return;
+    float* to_part = a.part + (((long)u.seq * a.splits + u.split) * rows + r) * a.d_c;
+    T* to_o = (T*)a.o + ((long)u.seq * rows + r) * a.d_c;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = u.first_row + 32 * t + (lane & 31);
-        bool live = r < rows;
-        const float mt = final_m[t][lane], lt = final_l[t][lane];
-        const float f = u.splits > 1 ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
-        uint32_t again = not_finite_rows(o[t]) & uint32_t(__ballot(live));
-        while (again) {
-            const int i = __ffs(again) - 1;
-            again &= again - 1;
-            sum_unit_row_again<VTW, T>(a, u, u.first_row + 32 * t + i, d0, cols, __shfl(mt, i, kWave), __shfl(f, i, kWave), lane);
-            if ((lane & 31) == i) live = false;
-        }
-        if (!live) continue;
-#pragma unroll
-        for (int d = 0; d < VTW; ++d) {
-            if (u.splits > 1)
-                store_columns<float>(a.part + (slot * rows + r) * a.d_c, o[t][d], d0 + 32 * d, a.d_c, 1.f, vec, lane);
-            else
-                store_columns<T>((T*)a.o + ((long)u.seq * rows + r) * a.d_c, o[t][d], d0 + 32 * d, a.d_c, f, vec, lane);
-        }
+    for (int d = 0; d < VTW; ++d) {
+        if (u.splits > 1)
+            store_columns<float>(to_part, o[d], d0 + 32 * d, a.d_c, 1.f, vec, lane);
+        else
+            store_columns<T>(to_o, o[d], d0 + 32 * d, a.d_c, f, vec, lane);
     }
 }
 
@@ -381,6 +388,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
         for (int i = lane; i < P * KEYS * 8; i += 64) tiles[wave].chunk[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
 
+    const uint32_t tile = lds_offset(&tiles[wave]);
     // Tile of positions j0 .., the two rows of each lane; returns a bit for every
     // row whose page is in the cache, the others take row 0.
     const auto start = [&](int j0) {
@@ -393,14 +401,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
 #pragma unroll
             for (int k = 0; k < 8; ++k) bits |= uint32_t(in >> (8 * k) & 1) << (8 * h + k);
             const T* p = (const T*)a.cache + (long)max(row, 0) * a.D + c * 8;
-            const uint32_t lds = lds_offset(&tiles[wave].chunk[0]) + h * 1024;
-#pragma unroll
-            for (int k = 0; k < P; ++k) {
-                if (k * 64 + 64 <= a.D)
-                    load_to_lds16_from(p + k * 64, lds + k * PB);
-                else if (k * 64 + c * 8 < a.D)
-                    load_to_lds16_from(p + k * 64, lds + k * PB);
-            }
+            load_panels<0, P, 1>(p, a.D * 2 - c * 16, a.D * 2, tile + h * 1024, PB);
         }
         return __builtin_amdgcn_readfirstlane(bits);
     };
@@ -413,7 +414,6 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     const int least_seen = sees(a, u, u.first_row), seen = min(end, sees(a, u, min(row, rows - 1)));
     // row lane % 16, chunk 4 i + g; and transposed: rows 4 g + (lane % 16) / 4
     const int vr = 4 * g + (kr >> 2);
-    const uint32_t tile = lds_offset(&tiles[wave]);
     const uint32_t k_at = tile + kr * 128 + ((twist(kr) ^ g) << 4), k_odd = k_at ^ (4 << 4);
     const uint32_t v_at = tile + vr * 128 + ((twist(vr) ^ ((kr >> 1) & 1)) << 4) + (kr & 1) * 8;
 
@@ -426,8 +426,8 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
         const int i = i0 + wave, j0 = begin + i * KEYS;
         if (i < tiles_n) {
             wait_loads<0>();
-            // six reads ahead of the products, whatever the scheduler would have
-            constexpr int AHEAD = 6;
+            // five reads ahead of the products, whatever the scheduler would have
+            constexpr int AHEAD = 5;
             f32x4 s[2] = {};
             u32x4 x[AHEAD];
             const auto read = [&](int k) { return lds_read<u32x4>((k & 1 ? k_odd : k_at) + (k >> 1) * PB); };
@@ -442,9 +442,11 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
             }
             s[0] += s[1];
             if (j0 + KEYS > min(end, least_seen) || there != 0xffffu) {
+                const int left = seen - j0 - 4 * g;
+                const uint32_t in = there >> (4 * g);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (j0 + 4 * g + k >= seen || !(there >> (4 * g + k) & 1)) s[0][k] = -INFINITY;
+                    if (k >= left || !(in & 1u << k)) s[0][k] = -INFINITY;
             }
             float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
             top = fmaxf(top, __shfl_xor(top, 16, kWave));
@@ -571,53 +573,71 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     }
 }
 
-// One row of q a workgroup: its splits' sums at their common maximum.
-constexpr int kJoinThreads = 128;
+// 256 columns of one row of q a workgroup: its splits' sums at their common
+// maximum, every fourth split on one wave, the waves' sums added in order.
+constexpr int kJoinThreads = 256, kJoinColumns = 256;
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams a) {
     __shared__ float weight[kMaxSplits];
-    const int rows = a.steps * a.heads, seq = blockIdx.x / rows, r = blockIdx.x % rows, tid = threadIdx.x;
+    __shared__ f32x4 sums[3][kWave];
+    const int rows = a.steps * a.heads, parts = (a.d_c + kJoinColumns - 1) / kJoinColumns;
+    const int d = blockIdx.x % parts * kJoinColumns + (threadIdx.x & 63) * 4;
+    const int unit = blockIdx.x / parts, seq = unit / rows, r = unit % rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int splits = splits_of(rows_of(a, seq));
     if (splits == 1) return;
     const float c = a.scale * kLog2e;
     const long first = (long)seq * a.splits * rows + r;  // slot 0's; the next split's is `rows` further
-    float top = -INFINITY, sum = 0.f;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, a.part_m[first + (long)i * rows]);
-    const float tc = top == -INFINITY ? 0.f : top * c;
-    if (tid < splits) weight[tid] = __builtin_amdgcn_exp2f(fmaf(a.part_m[first + (long)tid * rows], c, -tc));
+    float m[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool in = lane + 64 * i < splits;
+        m[i] = in ? a.part_m[first + (long)(lane + 64 * i) * rows] : -INFINITY;
+        l[i] = in ? a.part_l[first + (long)(lane + 64 * i) * rows] : 0.f;
+    }
+    const float top = wave_max(fmaxf(m[0], m[1])), tc = top == -INFINITY ? 0.f : top * c;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(m[i], c, -tc));
+        if (wave == 0) weight[lane + 64 * i] = w;
+        sum = fmaf(l[i], w, sum);
+    }
+    sum = row_sum<64>(sum);
     __syncthreads();
-    for (int i = 0; i < splits; ++i) sum = fmaf(weight[i], a.part_l[first + (long)i * rows], sum);
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
     const long row = (long)seq * rows + r;
-    if (tid == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : fmaf(top, a.scale, logf(sum));
-    const float* p = a.part + first * a.d_c;
+    if (threadIdx.x == 0 && d == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : fmaf(top, a.scale, logf(sum));
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    const float* p = a.part + first * a.d_c + d;
     const long step = (long)rows * a.d_c;
-    T* out = (T*)a.o + row * a.d_c;
-    if (a.d_c % 4 == 0 && aligned16(a.o)) {
-        for (int d = tid * 4; d < a.d_c; d += kJoinThreads * 4) {
-            f32x4 x = {};
+    const bool vec = a.d_c % 4 == 0 && aligned16(a.o), in = d < a.d_c;
+    f32x4 x = {};
+    if (vec && in) {
 #pragma unroll 8
-            for (int i = 0; i < splits; ++i) x += weight[i] * *reinterpret_cast<const f32x4*>(p + i * step + d);
-            if constexpr (sizeof(T) == 4)
-                *reinterpret_cast<f32x4*>(out + d) = x * f;
-            else
-                *reinterpret_cast<uint2*>(out + d) = make_uint2(pack_bf16x2(x[0] * f, x[1] * f), pack_bf16x2(x[2] * f, x[3] * f));
-        }
+        for (int i = wave; i < splits; i += 4) x += weight[i] * *reinterpret_cast<const f32x4*>(p + i * step);
+    } else if (in) {
+        for (int i = wave; i < splits; i += 4)
+            for (int k = 0; k < 4 && d + k < a.d_c; ++k) x[k] = fmaf(weight[i], p[i * step + k], x[k]);
+    }
+    if (wave) sums[wave - 1][lane] = x;
+    __syncthreads();
+    if (wave || !in) return;
+    x = (((x + sums[0][lane]) + sums[1][lane]) + sums[2][lane]) * f;
+    T* out = (T*)a.o + row * a.d_c + d;
+    if (!vec) {
+        for (int k = 0; k < 4 && d + k < a.d_c; ++k) Elem<T>::store(out, k, x[k]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(out) = x;
     } else {
-        for (int d = tid; d < a.d_c; d += kJoinThreads) {
-            float x = 0.f;
-            for (int i = 0; i < splits; ++i) x = fmaf(weight[i], p[i * step + d], x);
-            Elem<T>::store(out, d, x * f);
-        }
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
     }
 }
 
 int most_splits(const rhz_latent_decode_args& a) {
-    return splits_of((int)std::min<int64_t>((int64_t)a.max_pages * a.page_size, INT32_MAX));
+    return most_splits_of(std::min<int64_t>((int64_t)a.max_pages * a.page_size, INT32_MAX));
 }
 
 hipError_t join(const DecodeParams& p, int dtype, hipStream_t stream) {
-    const int64_t joins = (int64_t)p.batch * p.steps * p.heads;
+    const int64_t joins = (int64_t)p.batch * p.steps * p.heads * ((p.d_c + kJoinColumns - 1) / kJoinColumns);
     if (p.splits > 1) {
         if (check_grid(joins, kJoinThreads) != hipSuccess) return hipErrorInvalidConfiguration;
         if (dtype == RHZ_F32)

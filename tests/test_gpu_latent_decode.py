@@ -2,11 +2,13 @@
 attn_cases.py derives them), and a run of rope, append and decode against the
 expanded prefill."""
 import math
+from ctypes import byref, c_size_t
 
 import pytest
 import torch
 
 import rhizome_amd
+from rhizome_amd import _abi
 from attn_cases import DTYPES, W, half_step, near, normal, scores, weights
 
 pytestmark = pytest.mark.gpu
@@ -196,7 +198,11 @@ def test_caller_owned_buffers_and_replays(device, dtype):
     lens = [500, 20, 1000]
     q, cache, table, n = (t.to(device) for t in make(lens, 1, 16, 256, 64, 64, dtype, seed=8))
     out = torch.empty(3, 1, 16, 256, dtype=dtype, device=device)
-    ws = torch.empty(3 * 5 * 16 * 258 * 4 + 4096, dtype=torch.uint8, device=device)
+    size, args = c_size_t(), _abi.LatentDecodeArgs()
+    args.batch, args.steps, args.heads, args.d_c, args.d_r, args.scale = 3, 1, 16, 256, 64, 0.06
+    args.page_size, args.num_pages, args.max_pages, args.dtype = 64, cache.shape[0], table.shape[1], _abi.F32
+    _abi.check(_abi.lib().rhz_latent_decode_workspace_size(byref(args), byref(size)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
     rhizome_amd.latent_decode(q, cache, table, n, d_c=256, scale=0.06, out=out, workspace=ws)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
