@@ -22,35 +22,59 @@ from ctypes import byref, c_double, c_float
 import torch
 
 from . import _abi
-from .gdr import _DTYPES, _count, _empty, _on_stream, _ptr, _stream
-from .train import _same_device, _workspace
+from .gdr import _DTYPES, _count, _empty, _on_stream
+from .train import _workspace
 
 _SCALINGS = {"none": _abi.ROPE_PLAIN, "linear": _abi.ROPE_LINEAR, "by_parts": _abi.ROPE_BY_PARTS}
 
 
-def _view_ptr(t: torch.Tensor | None) -> int | None:
-    """_ptr of a tensor that need not be contiguous; its strides have been read."""
+# A decoding step's calls are bounded by the host: the device is asked for once
+# a call, and the argument structs are filled in by position, which is what
+# most of a call's time went to (rope of one position of 8 sequences: 8.0 us).
+def _here() -> int:
+    return torch.cuda.current_device()
+
+
+def _stream(here: int) -> int | None:
+    return torch._C._cuda_getCurrentRawStream(here) or None
+
+
+def _view(t: torch.Tensor | None, here: int) -> int | None:
+    """The address of a tensor whose strides have been read, on the current device."""
     if t is None:
         return None
-    if not t.is_cuda:
-        raise ValueError("all tensors must be on the GPU")
+    if t.get_device() != here:
+        if not t.is_cuda:
+            raise ValueError("all tensors must be on the GPU")
+        raise ValueError(f"all tensors must be on the current device, cuda:{here}")
     return t.data_ptr() or None
+
+
+def _dense(t: torch.Tensor | None, here: int) -> int | None:
+    """The same of a tensor that has to be contiguous."""
+    if t is not None and not t.is_contiguous():
+        raise ValueError("all tensors but those of heads must be contiguous")
+    return _view(t, here)
 
 
 def _strides(name, t, heads=True):
     """Strides in elements from token to token, and from head to head."""
-    *lead, h, d = t.shape if heads else (*t.shape[:-1], 1, t.shape[-1])
-    st = t.stride() if heads else (*t.stride()[:-1], 0, t.stride(-1))
-    if d > 1 and st[-1] != 1:
+    shape, st = t.shape, t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}'s last dimension must be dense")
-    token = st[-3] if lead[-1] > 1 or len(lead) == 1 else st[-4]
-    if len(lead) == 2 and lead[0] > 1 and lead[1] > 0 and st[-4] != token * lead[1]:
-        raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
-    return token, st[-2] if h > 1 else 0
+    at = -3 if heads else -2  # the tokens' dimension
+    token = st[at]
+    if len(shape) + at == 1:  # a batch before it
+        batch, n = shape[0], shape[at]
+        if n == 1:
+            token = st[0]
+        elif batch > 1 and st[0] != token * n and n > 0:
+            raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
+    return token, st[-2] if heads and shape[-2] > 1 else 0
 
 
 def _check_positions(name, t, shape):
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape):
+    if t.dtype != torch.int32 or t.shape != shape:
         raise ValueError(f"{name} must be int32 {tuple(shape)}")
 
 
@@ -98,14 +122,13 @@ def rope(x, positions, frequencies, *, offset: int = 0, interleaved: bool = Fals
     y = out if out is not None else _empty(x, x.shape)
     if y.shape != x.shape or y.dtype != x.dtype:
         raise ValueError("out must have x's shape and dtype")
-    a = _abi.RopeArgs()
-    a.tokens, a.heads, a.dim, a.dtype = _count(positions.numel()), x.shape[-2], x.shape[-1], _DTYPES[x.dtype]
-    a.offset, a.rot, a.interleaved, a.inverse, a.magnitude = offset, 2 * frequencies.numel(), interleaved, inverse, magnitude
-    a.x_token_stride, a.x_head_stride = _strides("x", x)
-    a.y_token_stride, a.y_head_stride = _strides("out", y)
-    _same_device(x, positions, frequencies, y)
-    a.x, a.positions, a.turns, a.y = _view_ptr(x), _ptr(positions), _ptr(frequencies), _view_ptr(y)
-    _abi.check(_abi.lib().rhz_rope(byref(a), _stream()))
+    xt, xh = _strides("x", x)
+    yt, yh = (xt, xh) if y is x else _strides("out", y)
+    here = _here()
+    a = _abi.RopeArgs(_count(positions.numel()), x.shape[-2], x.shape[-1], offset, 2 * frequencies.numel(), _DTYPES[x.dtype],
+                      interleaved, inverse, magnitude, xt, xh, yt, yh, _view(x, here), _dense(positions, here),
+                      _dense(frequencies, here), _view(y, here))
+    _abi.check(_abi.lib().rhz_rope(byref(a), _stream(here)))
     return y
 
 
@@ -146,19 +169,17 @@ def latent_append(latent, k_rope, cache, page_table, lengths, *, cu_seqlens=None
         _check_frequencies(frequencies)
         if 2 * frequencies.numel() != d_r:
             raise ValueError(f"{frequencies.numel()} frequencies for a rotary key of {d_r}")
-    if norm_scale is not None and (tuple(norm_scale.shape) != (d_c,) or norm_scale.dtype != torch.float32):
+    if norm_scale is not None and (norm_scale.shape != (d_c,) or norm_scale.dtype != torch.float32):
         raise ValueError(f"norm_scale must be fp32 ({d_c},)")
-    _same_device(latent, k_rope, cache, page_table, lengths, cu_seqlens, frequencies, norm_scale)
-    a = _abi.LatentAppendArgs()
-    a.batch, a.seq_len, a.d_c, a.d_r = batch, _count(latent.shape[-2]), d_c, d_r
-    a.page_size, a.num_pages, a.max_pages = cache.shape[1], cache.shape[0], page_table.shape[1]
-    a.dtype, a.interleaved, a.magnitude, a.eps = _DTYPES[cache.dtype], interleaved, magnitude, eps
-    a.latent_stride = _strides("latent", latent, heads=False)[0]
-    a.k_rope_stride = _strides("k_rope", k_rope, heads=False)[0] if k_rope is not None else 0
-    a.latent, a.k_rope, a.cu_seqlens = _view_ptr(latent), _view_ptr(k_rope), _ptr(cu_seqlens)
-    a.lengths, a.page_table, a.turns = _ptr(lengths), _ptr(page_table), _ptr(frequencies)
-    a.norm_scale, a.cache = _ptr(norm_scale), _ptr(cache)
-    _abi.check(_abi.lib().rhz_latent_append(byref(a), _stream()))
+    latent_stride = _strides("latent", latent, heads=False)[0]
+    k_rope_stride = _strides("k_rope", k_rope, heads=False)[0] if d_r else 0
+    here = _here()
+    a = _abi.LatentAppendArgs(
+        batch, _count(latent.shape[-2]), d_c, d_r, cache.shape[1], cache.shape[0], page_table.shape[1], _DTYPES[cache.dtype],
+        interleaved, magnitude, eps, latent_stride, k_rope_stride, _view(latent, here), _view(k_rope, here),
+        _dense(cu_seqlens, here), _dense(lengths, here), _dense(page_table, here), _dense(frequencies, here),
+        _dense(norm_scale, here), _dense(cache, here))
+    _abi.check(_abi.lib().rhz_latent_append(byref(a), _stream(here)))
     return cache
 
 
@@ -180,18 +201,17 @@ def latent_decode(q, cache, page_table, lengths, *, d_c: int, scale: float, out=
         raise ValueError(f"q is of {q.shape[0]} sequences and {q.shape[-1]} channels, the page table of {batch}, d_c is {d_c}")
     want = (*q.shape[:-1], d_c)
     o = out if out is not None else _empty(q, want)
-    if tuple(o.shape) != want or o.dtype != q.dtype:
+    if o.shape != want or o.dtype != q.dtype:
         raise ValueError(f"out must be {q.dtype} {want}")
-    _same_device(q, cache, page_table, lengths, o, workspace)
-    lse = _empty(q, q.shape[:-1], torch.float32)
-    a = _abi.LatentDecodeArgs()
-    a.batch, a.steps, a.heads, a.d_c, a.d_r = batch, q.shape[1], q.shape[2], d_c, q.shape[-1] - d_c
-    a.page_size, a.num_pages, a.max_pages = cache.shape[1], cache.shape[0], page_table.shape[1]
-    a.dtype, a.scale = _DTYPES[q.dtype], scale
-    a.q, a.cache, a.page_table, a.lengths = _ptr(q), _ptr(cache), _ptr(page_table), _ptr(lengths)
-    a.o, a.lse = _ptr(o), _ptr(lse)
+    here = _here()
+    lse = _empty(q, want[:-1], torch.float32)
+    a = _abi.LatentDecodeArgs(
+        batch, want[1], want[2], d_c, q.shape[-1] - d_c, cache.shape[1], cache.shape[0], page_table.shape[1], _DTYPES[q.dtype],
+        scale, _dense(q, here), _dense(cache, here), _dense(page_table, here), _dense(lengths, here), _dense(o, here),
+        _dense(lse, here))
     workspace = _workspace(q, a, _abi.lib().rhz_latent_decode_workspace_size, workspace)
-    _abi.check(_abi.lib().rhz_latent_decode(byref(a), _stream()))
+    _view(workspace, here)
+    _abi.check(_abi.lib().rhz_latent_decode(byref(a), _stream(here)))
     return o, lse
 
 
@@ -208,33 +228,28 @@ def _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k) -> _
         raise ValueError(f"q/k/v shapes {tuple(q.shape)} {tuple(k.shape)} {tuple(v.shape)} do not match")
     if (k_rope is None) != (d_r == 0):
         raise ValueError(f"q has {d_r} channels more than k: k_rope must have them, or be None for none")
-    if k_rope is not None and (tuple(k_rope.shape) != (*k.shape[:-2], d_r) or k_rope.dtype != q.dtype):
+    if k_rope is not None and (k_rope.shape != (*k.shape[:-2], d_r) or k_rope.dtype != q.dtype):
         raise ValueError(f"k_rope must be {q.dtype} {(*k.shape[:-2], d_r)}")
-    a = _abi.LatentPrefillArgs()
     if cu_seqlens is None:
         if cu_seqlens_k is not None:
             raise ValueError("cu_seqlens_k without cu_seqlens")
         if k.shape[0] != q.shape[0]:
             raise ValueError("q and k must have the same batch")
-        a.batch, a.seq_len, a.seq_len_k = q.shape[0], q.shape[1], k.shape[1]
+        batch, seq_len, seq_len_k = q.shape[0], q.shape[1], k.shape[1]
     else:
-        for name, cu in (("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k)):
-            if cu is not None:
-                _check_positions(name, cu, cu_seqlens.shape)
-        a.batch, a.seq_len, a.seq_len_k = cu_seqlens.numel() - 1, _count(q.shape[0]), _count(k.shape[0])
-    a.heads, a.d_n, a.d_r, a.d_v, a.dtype, a.causal = H, d_n, d_r, d_v, _DTYPES[q.dtype], causal
-    a.scale = q.shape[-1] ** -0.5 if scale is None else scale
-    a.q_token_stride, a.q_head_stride = _strides("q", q)
-    a.k_token_stride, a.k_head_stride = _strides("k", k)
-    a.v_token_stride, a.v_head_stride = _strides("v", v)
-    if k_rope is not None:
-        a.k_rope_stride = _strides("k_rope", k_rope, heads=False)[0]
-    return a
+        _check_positions("cu_seqlens", cu_seqlens, cu_seqlens.shape)
+        if cu_seqlens_k is not None:
+            _check_positions("cu_seqlens_k", cu_seqlens_k, cu_seqlens.shape)
+        batch, seq_len, seq_len_k = cu_seqlens.numel() - 1, _count(q.shape[0]), _count(k.shape[0])
+    return _abi.LatentPrefillArgs(
+        batch, seq_len, seq_len_k, H, d_n, d_r, d_v, _DTYPES[q.dtype], causal, q.shape[-1] ** -0.5 if scale is None else scale,
+        *_strides("q", q), *_strides("k", k), *_strides("v", v), _strides("k_rope", k_rope, heads=False)[0] if d_r else 0)
 
 
-def _prefill_pointers(a, q, k, v, k_rope, cu_seqlens, cu_seqlens_k):
-    a.q, a.k, a.v, a.k_rope = _view_ptr(q), _view_ptr(k), _view_ptr(v), _view_ptr(k_rope)
-    a.cu_seqlens, a.cu_seqlens_k = _ptr(cu_seqlens), _ptr(cu_seqlens_k)
+def _prefill_pointers(a, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse):
+    a.q, a.k, a.v, a.k_rope = _view(q, here), _view(k, here), _view(v, here), _view(k_rope, here)
+    a.cu_seqlens, a.cu_seqlens_k = _dense(cu_seqlens, here), _dense(cu_seqlens_k, here)
+    a.o, a.lse = _dense(o, here), _dense(lse, here)
 
 
 def latent_prefill(q, k, v, k_rope=None, *, scale=None, causal: bool = True, cu_seqlens=None, cu_seqlens_k=None,
@@ -252,13 +267,12 @@ def latent_prefill(q, k, v, k_rope=None, *, scale=None, causal: bool = True, cu_
     a = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
     want = (*q.shape[:-1], v.shape[-1])
     o = out if out is not None else _empty(q, want)
-    if tuple(o.shape) != want or o.dtype != q.dtype:
+    if o.shape != want or o.dtype != q.dtype:
         raise ValueError(f"out must be {q.dtype} {want}")
-    lse = _empty(q, q.shape[:-1], torch.float32)
-    _same_device(q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o)
-    _prefill_pointers(a, q, k, v, k_rope, cu_seqlens, cu_seqlens_k)
-    a.o, a.lse = _ptr(o), _ptr(lse)
-    _abi.check(_abi.lib().rhz_latent_prefill(byref(a), _stream()))
+    lse = _empty(q, want[:-1], torch.float32)
+    here = _here()
+    _prefill_pointers(a, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse)
+    _abi.check(_abi.lib().rhz_latent_prefill(byref(a), _stream(here)))
     return o, lse
 
 
@@ -277,17 +291,18 @@ def latent_prefill_backward(q, k, v, k_rope, o, lse, do, *, dlse=None, scale=Non
     a.forward = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
     want = (*q.shape[:-1], v.shape[-1])
     for name, t in (("o", o), ("do", do)):
-        if tuple(t.shape) != want or t.dtype != q.dtype:
+        if t.shape != want or t.dtype != q.dtype:
             raise ValueError(f"{name} must be {q.dtype} {want}")
     for name, t in (("lse", lse), ("dlse", dlse)):
         if t is not None and (t.shape != q.shape[:-1] or t.dtype != torch.float32):
             raise ValueError(f"{name} must be fp32 {tuple(q.shape[:-1])}")
-    _same_device(q, k, v, k_rope, o, lse, do, dlse, cu_seqlens, cu_seqlens_k, workspace)
-    _prefill_pointers(a.forward, q, k, v, k_rope, cu_seqlens, cu_seqlens_k)
+    here = _here()
+    _prefill_pointers(a.forward, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse)
     dq, dk, dv = _empty(q, q.shape), _empty(k, k.shape), _empty(v, v.shape)
     dr = _empty(k_rope, k_rope.shape) if k_rope is not None else None
-    a.forward.o, a.forward.lse, a.grad_o, a.grad_lse = _ptr(o), _ptr(lse), _ptr(do), _ptr(dlse)
-    a.grad_q, a.grad_k, a.grad_v, a.grad_k_rope = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dr)
+    a.grad_o, a.grad_lse = _dense(do, here), _dense(dlse, here)
+    a.grad_q, a.grad_k, a.grad_v, a.grad_k_rope = _view(dq, here), _view(dk, here), _view(dv, here), _view(dr, here)
     workspace = _workspace(q, a, _abi.lib().rhz_latent_prefill_backward_workspace_size, workspace)
-    _abi.check(_abi.lib().rhz_latent_prefill_backward(byref(a), _stream()))
+    _view(workspace, here)
+    _abi.check(_abi.lib().rhz_latent_prefill_backward(byref(a), _stream(here)))
     return dq, dk, dv, dr
