@@ -8,29 +8,12 @@
 // holds 128 keys' dk and dv, another runs over keys and holds 128 queries' dq:
 // seven products instead of the five that one kernel needs, which would have to
 // add its dq from all key tiles in memory, in no fixed order or with waits.
-#include "attn_device.hpp"
-#include "gdr_internal.hpp"
-#include "gdr_rows.hpp"
+#include "attn_params.hpp"
 
 namespace rhz {
 namespace {
 
-struct BackwardParams {
-    const void *q, *k, *v, *r, *go;
-    const int *cu_q, *cu_k;
-    const float *lse, *glse;
-    const void* o;
-    void *dq, *dk, *dv, *dr;
-    float* lse2;     // [H, queries]: lse log2 e
-    float* delta;    // [H, queries]: D
-    float* dr_part;  // [H, keys, d_r]
-    long qs, qh, ks, kh, vs, vh, rs, queries, keys;
-    int batch, len_q, len_k, heads, d_n, d_r, d_v, causal, tiles;
-    float scale;
-    bool vec_out, vec_delta;
-};
-
-constexpr int kThreads = 256, kRows = 128;
+constexpr int kThreads = kAttnThreads, kRows = 128;
 
 // ---------------------------------------------------------------- D and lse
 // 64 tokens of one head a workgroup, 16 lanes a row.
@@ -61,24 +44,11 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(BackwardParams a) 
     }
 }
 
-// Workgroup number -> (head, sequence, tile of kRows rows); false if there is none.
-__device__ __forceinline__ bool place(const BackwardParams& a, const int* cu, int total, int lane, int& head, int& seq,
-                                      int& tile) {
-    const int units = a.heads * (cu ? 1 : a.batch);
-    const int xcd = blockIdx.x & 7, n = blockIdx.x >> 3;
-    const int unit = (n / a.tiles) * 8 + xcd;
-    if (unit >= units) return false;
-    head = unit % a.heads;
-    tile = n % a.tiles;
-    seq = unit / a.heads;
-    if (cu) packed_tile(cu, a.batch, total, kRows, tile, lane, seq, tile);
-    return true;
-}
-
 // ------------------------------------------------------------------ dk, dv
-template <typename T, int DQ, int DV, bool VEC>
+template <int DQ, int DV, bool VEC>
 __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a) {
-    constexpr int E = kChunkElems<T>, BQ = sizeof(T) == 2 ? 64 : 32, SUB = BQ / 32;
+    using T = uint16_t;
+    constexpr int E = kChunkElems<T>, BQ = 64, SUB = BQ / 32;
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32, VT = DV / 32;
     using MoveQ = Mover<T, DQ, BQ, kThreads, VEC>;
     using MoveO = Mover<T, DV, BQ, kThreads, VEC>;
@@ -88,7 +58,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, a.cu_k, a.len_k, lane, head, seq, tile)) return;
+    if (!place(a, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int first = tile * kRows;
     if (first >= w.nk) return;
@@ -233,8 +203,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
 }
 
 // ---------------------------------------------------------------------- dq
-template <typename T, int DQ, int DV, bool VEC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(BackwardParams a) {
+template <int DQ, int DV, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) {
+    using T = uint16_t;
     constexpr int E = kChunkElems<T>, BN = 32;
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32;
     using MoveK = Mover<T, DQ, BN, kThreads, VEC>;
@@ -244,7 +215,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attn_dq_kern
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, a.cu_q, a.len_q, lane, head, seq, tile)) return;
+    if (!place(a, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int last_tile = (w.nq - 1) / kRows;
     if (w.nq == 0 || tile > last_tile) return;
@@ -357,41 +328,46 @@ __global__ __launch_bounds__(kThreads) void attn_rope_sum_kernel(BackwardParams 
     Elem<T>::store((T*)a.dr, at, sum);
 }
 
-int64_t tiles_of(const int* cu, int64_t total, int len, int batch) {
-    return cu ? packed_tiles(total, batch, kRows) : ((int64_t)len + kRows - 1) / kRows;
-}
-
 bool too_many(int64_t blocks) { return blocks > INT32_MAX || check_grid(blocks, kThreads) != hipSuccess; }
 
-template <typename T, int DQ, int DV, bool VEC>
+template <int DQ, int DV, bool VEC>
 hipError_t launch(BackwardParams p, hipStream_t stream) {
-    const int64_t units_q = ((int64_t)p.heads * (p.cu_q ? 1 : p.batch) + 7) / 8 * 8;
-    const int64_t tq = tiles_of(p.cu_q, p.queries, p.len_q, p.batch), tk = tiles_of(p.cu_k, p.keys, p.len_k, p.batch);
-    const int64_t delta = (p.queries + 63) / 64 * p.heads, rope = (p.keys * p.d_r + kThreads - 1) / kThreads;
-    if (too_many(units_q * tq) || too_many(units_q * tk) || too_many(delta) || too_many(rope))
-        return hipErrorInvalidConfiguration;
-    if (p.queries && p.vec_delta) attn_delta_kernel<T, true><<<(unsigned)delta, kThreads, 0, stream>>>(p);
-    if (p.queries && !p.vec_delta) attn_delta_kernel<T, false><<<(unsigned)delta, kThreads, 0, stream>>>(p);
+    const int64_t tq = attn_tiles(p.cu_q, p.queries, p.len_q, p.batch, kRows);
+    const int64_t tk = attn_tiles(p.cu_k, p.keys, p.len_k, p.batch, kRows);
     if (p.keys) {
+        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_k, tk);
+        if (!blocks) return hipErrorInvalidConfiguration;
         p.tiles = (int)tk;
-        attn_dkv_kernel<T, DQ, DV, VEC><<<(unsigned)(units_q * tk), kThreads, 0, stream>>>(p);
+        attn_dkv_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
     }
     if (p.queries) {
+        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, tq);
+        if (!blocks) return hipErrorInvalidConfiguration;
         p.tiles = (int)tq;
-        attn_dq_kernel<T, DQ, DV, VEC><<<(unsigned)(units_q * tq), kThreads, 0, stream>>>(p);
+        attn_dq_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
     }
-    if (rope) attn_rope_sum_kernel<T><<<(unsigned)rope, kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 
-template <typename T>
 hipError_t pick(const BackwardParams& p, bool vec, hipStream_t stream) {
     const int dq = p.d_n + p.d_r;
-    if (!vec) return dq <= 64 && p.d_v <= 64 ? launch<T, 64, 64, false>(p, stream) : launch<T, 192, 128, false>(p, stream);
-    if (p.d_v <= 64 && dq <= 64) return launch<T, 64, 64, true>(p, stream);
-    if (p.d_v <= 64 && dq <= 96) return launch<T, 96, 64, true>(p, stream);
-    if (dq <= 128) return launch<T, 128, 128, true>(p, stream);
-    return launch<T, 192, 128, true>(p, stream);
+    if (!vec) return dq <= 64 && p.d_v <= 64 ? launch<64, 64, false>(p, stream) : launch<192, 128, false>(p, stream);
+    if (p.d_v <= 64 && dq <= 64) return launch<64, 64, true>(p, stream);
+    if (p.d_v <= 64 && dq <= 96) return launch<96, 64, true>(p, stream);
+    if (dq <= 128) return launch<128, 128, true>(p, stream);
+    return launch<192, 128, true>(p, stream);
+}
+
+template <typename T>
+hipError_t launch_all(const BackwardParams& p, bool vec, hipStream_t stream) {
+    const int64_t delta = (p.queries + 63) / 64 * p.heads, rope = (p.keys * p.d_r + kThreads - 1) / kThreads;
+    if (too_many(delta) || too_many(rope)) return hipErrorInvalidConfiguration;
+    if (p.queries && p.vec_delta) attn_delta_kernel<T, true><<<(unsigned)delta, kThreads, 0, stream>>>(p);
+    if (p.queries && !p.vec_delta) attn_delta_kernel<T, false><<<(unsigned)delta, kThreads, 0, stream>>>(p);
+    const hipError_t e = sizeof(T) == 4 ? launch_backward_split(p, vec, stream) : pick(p, vec, stream);
+    if (e != hipSuccess) return e;
+    if (rope) attn_rope_sum_kernel<T><<<(unsigned)rope, kThreads, 0, stream>>>(p);
+    return hipGetLastError();
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -429,7 +405,7 @@ hipError_t launch_latent_prefill_backward(const rhz_latent_prefill_backward_args
     const bool vec = attn_vectors(f) && aligned16(a.grad_o);
     p.vec_delta = f.d_v % (f.dtype == RHZ_F32 ? 4 : 8) == 0 && aligned16(f.o) && aligned16(a.grad_o);
     p.vec_out = vec && aligned16(a.grad_q) && aligned16(a.grad_k) && aligned16(a.grad_v);
-    return f.dtype == RHZ_F32 ? pick<float>(p, vec, stream) : pick<uint16_t>(p, vec, stream);
+    return f.dtype == RHZ_F32 ? launch_all<float>(p, vec, stream) : launch_all<uint16_t>(p, vec, stream);
 }
 
 }  // namespace rhz

@@ -206,6 +206,11 @@ __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same of a wave's own loads and reads.
+__device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// A wave's own LDS reads are done: what it read may be written over.
+__device__ __forceinline__ void wave_read() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Makes the compiler wait for a value here: a wait that it put off into a loop
 // would count the loop's own loads into LDS along, every time.
 template <typename V>

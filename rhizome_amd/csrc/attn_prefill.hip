@@ -8,28 +8,17 @@
 // with c = scale log2 e.  The maximum is only raised, and O and l rescaled,
 // where a tile's exceeds it by 2^8 or more: p then is at most 2^8, which costs
 // neither fp32 sums nor bf16 weights any digits.
-#include "attn_device.hpp"
-#include "gdr_internal.hpp"
-#include "gdr_rows.hpp"
+#include "attn_params.hpp"
 
 namespace rhz {
 namespace {
 
-struct PrefillParams {
-    const void *q, *k, *v, *r;
-    const int *cu_q, *cu_k;
-    void* o;
-    float* lse;
-    long qs, qh, ks, kh, vs, vh, rs;
-    int batch, len_q, len_k, heads, d_n, d_r, d_v, causal, tiles;
-    float scale;
-};
+using T = uint16_t;
+constexpr int kThreads = kAttnThreads, kQueries = 128;
 
-constexpr int kThreads = 256, kQueries = 128;
-
-template <typename T, int DQ, int DV, bool VEC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void latent_prefill_kernel(PrefillParams a) {
-    constexpr int E = kChunkElems<T>, BN = sizeof(T) == 2 ? 64 : 32, SUB = BN / 32;
+template <int DQ, int DV, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillParams a) {
+    constexpr int E = kChunkElems<T>, BN = 64, SUB = BN / 32;
     constexpr int QC = DQ / (2 * E), VT = DV / 32;
     using MoveK = Mover<T, DQ, BN, kThreads, VEC>;
     using MoveV = Mover<T, DV, BN, kThreads, VEC>;
@@ -38,28 +27,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void latent_prefi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
 
-    // workgroups of one head follow one another on one XCD, whose L2 keeps
-    // its keys and values; the queries with the most keys go first
-    const int per_head = a.tiles, units = a.heads * (a.cu_q ? 1 : a.batch);
-    int unit, t;
-    {
-        const int id = blockIdx.x, xcd = id & 7, n = id >> 3;
-        unit = (n / per_head) * 8 + xcd;
-        t = n % per_head;
-        if (unit >= units) return;
-    }
-    const int head = unit % a.heads;
-    int seq, tile;
-    if (a.cu_q) {
-        packed_tile(a.cu_q, a.batch, a.len_q, kQueries, t, lane, seq, tile);
-    } else {
-        seq = unit / a.heads;
-        tile = per_head - 1 - t;
-    }
+    int head, seq, tile;
+    if (!place(a, a.cu_q, a.len_q, kQueries, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kQueries >= w.nq) return;
-    if (a.cu_q) tile = (w.nq - 1) / kQueries - tile;
-    const int first = tile * kQueries;
+    const int first = ((w.nq - 1) / kQueries - tile) * kQueries;  // the queries with the most keys go first
 
     const int wq = first + wave * 32;       // the wave's first query
     const int qi = wq + (lane & 31);        // the lane's
@@ -175,23 +147,24 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void latent_prefi
     for (int d = 0; d < VT; ++d) store_columns<T>(out, o[d], 32 * d, a.d_v, f, VEC, lane);
 }
 
-template <typename T, int DQ, int DV, bool VEC>
-hipError_t launch(const PrefillParams& p, hipStream_t stream) {
-    const int64_t units = (int64_t)p.heads * (p.cu_q ? 1 : p.batch);
-    const int64_t blocks = (units + 7) / 8 * 8 * p.tiles;
-    if (blocks > INT32_MAX || check_grid(blocks, kThreads) != hipSuccess) return hipErrorInvalidConfiguration;
-    latent_prefill_kernel<T, DQ, DV, VEC><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+template <int DQ, int DV, bool VEC>
+hipError_t launch(PrefillParams p, hipStream_t stream) {
+    const int64_t queries = p.cu_q ? (int64_t)p.len_q : (int64_t)p.batch * p.len_q;
+    const int64_t tiles = attn_tiles(p.cu_q, queries, p.len_q, p.batch, kQueries);
+    const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, tiles);
+    if (!blocks) return hipErrorInvalidConfiguration;
+    p.tiles = (int)tiles;
+    latent_prefill_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 
-template <typename T>
 hipError_t pick(const PrefillParams& p, bool vec, hipStream_t stream) {
     const int dq = p.d_n + p.d_r;
-    if (!vec) return dq <= 64 && p.d_v <= 64 ? launch<T, 64, 64, false>(p, stream) : launch<T, 192, 128, false>(p, stream);
-    if (p.d_v <= 64 && dq <= 64) return launch<T, 64, 64, true>(p, stream);
-    if (p.d_v <= 64 && dq <= 96) return launch<T, 96, 64, true>(p, stream);
-    if (dq <= 128) return launch<T, 128, 128, true>(p, stream);
-    return launch<T, 192, 128, true>(p, stream);
+    if (!vec) return dq <= 64 && p.d_v <= 64 ? launch<64, 64, false>(p, stream) : launch<192, 128, false>(p, stream);
+    if (p.d_v <= 64 && dq <= 64) return launch<64, 64, true>(p, stream);
+    if (p.d_v <= 64 && dq <= 96) return launch<96, 64, true>(p, stream);
+    if (dq <= 128) return launch<128, 128, true>(p, stream);
+    return launch<192, 128, true>(p, stream);
 }
 
 }  // namespace
@@ -207,15 +180,12 @@ bool attn_vectors(const rhz_latent_prefill_args& a) {
 hipError_t launch_latent_prefill(const rhz_latent_prefill_args& a, hipStream_t stream) {
     const int64_t queries = a.cu_seqlens ? (int64_t)a.seq_len : (int64_t)a.batch * a.seq_len;
     if (queries == 0) return hipSuccess;
-    PrefillParams p = {a.q, a.k, a.v, a.k_rope, a.cu_seqlens, a.cu_seqlens_k ? a.cu_seqlens_k : a.cu_seqlens, a.o, a.lse,
+    const PrefillParams p = {a.q, a.k, a.v, a.k_rope, a.cu_seqlens, a.cu_seqlens_k ? a.cu_seqlens_k : a.cu_seqlens, a.o, a.lse,
                        a.q_token_stride, a.q_head_stride, a.k_token_stride, a.k_head_stride, a.v_token_stride,
                        a.v_head_stride, a.k_rope_stride, a.batch, a.seq_len, a.seq_len_k, a.heads, a.d_n, a.d_r, a.d_v,
                        a.causal, 0, a.scale};
-    const int64_t tiles = a.cu_seqlens ? packed_tiles(queries, a.batch, kQueries) : ((int64_t)a.seq_len + kQueries - 1) / kQueries;
-    if (tiles > INT32_MAX) return hipErrorInvalidConfiguration;
-    p.tiles = (int)tiles;
     const bool vec = attn_vectors(a);
-    return a.dtype == RHZ_F32 ? pick<float>(p, vec, stream) : pick<uint16_t>(p, vec, stream);
+    return a.dtype == RHZ_F32 ? launch_prefill_split(p, vec, stream) : pick(p, vec, stream);
 }
 
 }  // namespace rhz
