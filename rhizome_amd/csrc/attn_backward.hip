@@ -50,8 +50,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
     using T = uint16_t;
     constexpr int E = kChunkElems<T>, BQ = 64, SUB = BQ / 32;
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32, VT = DV / 32;
-    using MoveQ = Mover<T, DQ, BQ, kThreads, VEC>;
-    using MoveO = Mover<T, DV, BQ, kThreads, VEC>;
     __shared__ Tile<T, DQ, BQ> qtiles[2];
     __shared__ Tile<T, DV, BQ> otiles[2];
     __shared__ float4 lse_s[2][16], delta_s[2][16];  // a wave's 64 floats
@@ -79,9 +77,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
     const Rows<T> orows = {(const T*)a.go + (long)head * a.d_v, (const T*)a.go, (long)a.heads * a.d_v, 0, a.d_v, 0};
     const float* lse2 = a.lse2 + head * a.queries + w.q0;
     const float* delta = a.delta + head * a.queries + w.q0;
+    const Mover<T, DQ, BQ, kThreads, VEC> move_q(qrows, tid);
+    const Mover<T, DV, BQ, kThreads, VEC> move_o(orows, tid);
     const auto start = [&](int q0, int b) {
-        MoveQ::start(qrows, (long)w.q0 + q0, w.nq - q0, qtiles[b], tid);
-        MoveO::start(orows, (long)w.q0 + q0, w.nq - q0, otiles[b], tid);
+        move_q.start((long)w.q0 + q0, w.nq - q0, qtiles[b]);
+        move_o.start((long)w.q0 + q0, w.nq - q0, otiles[b]);
         const uint32_t off = min(lane, min(BQ, w.nq - q0) - 1) * 4;
         if (wave == 0) load_to_lds4(lse2 + q0, off, lds_offset(&lse_s[b][0]));
         if (wave == 1) load_to_lds4(delta + q0, off, lds_offset(&delta_s[b][0]));
@@ -98,10 +98,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a)
     const float c = a.scale * kLog2e;
     // the first query that sees the workgroup's first key
     const int begin = a.causal ? max(0, first - shift) / BQ * BQ : 0;
-    for (int b = 0; b < 2; ++b) {
-        MoveQ::clear(qrows, qtiles[b], tid);
-        MoveO::clear(orows, otiles[b], tid);
-    }
+    for (int b = 0; b < 2; ++b) move_q.clear(qtiles[b]), move_o.clear(otiles[b]);
     __syncthreads();
     if (begin < w.nq) start(begin, 0);
     for (int q0 = begin, b = 0; q0 < w.nq; q0 += BQ, b ^= 1) {
@@ -208,8 +205,6 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
     using T = uint16_t;
     constexpr int E = kChunkElems<T>, BN = 32;
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32;
-    using MoveK = Mover<T, DQ, BN, kThreads, VEC>;
-    using MoveV = Mover<T, DV, BN, kThreads, VEC>;
     __shared__ Tile<T, DQ, BN> ktiles[2];
     __shared__ Tile<T, DV, BN> vtiles[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
@@ -245,20 +240,19 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
 #pragma unroll
     for (int d = 0; d < QT; ++d) dq[d] = f32x16{};
     const float c = a.scale * kLog2e;
-    for (int b = 0; b < 2; ++b) {
-        MoveK::clear(krows, ktiles[b], tid);
-        MoveV::clear(vrows, vtiles[b], tid);
-    }
+    const Mover<T, DQ, BN, kThreads, VEC> move_k(krows, tid);
+    const Mover<T, DV, BN, kThreads, VEC> move_v(vrows, tid);
+    for (int b = 0; b < 2; ++b) move_k.clear(ktiles[b]), move_v.clear(vtiles[b]);
     __syncthreads();
     if (end > 0) {
-        MoveK::start(krows, w.k0, w.nk, ktiles[0], tid);
-        MoveV::start(vrows, w.k0, w.nk, vtiles[0], tid);
+        move_k.start(w.k0, w.nk, ktiles[0]);
+        move_v.start(w.k0, w.nk, vtiles[0]);
     }
     for (int k0 = 0, b = 0; k0 < end; k0 += BN, b ^= 1) {
         landed();
         if (k0 + BN < end) {
-            MoveK::start(krows, (long)w.k0 + k0 + BN, w.nk - k0 - BN, ktiles[b ^ 1], tid);
-            MoveV::start(vrows, (long)w.k0 + k0 + BN, w.nk - k0 - BN, vtiles[b ^ 1], tid);
+            move_k.start((long)w.k0 + k0 + BN, w.nk - k0 - BN, ktiles[b ^ 1]);
+            move_v.start((long)w.k0 + k0 + BN, w.nk - k0 - BN, vtiles[b ^ 1]);
         }
         const uint32_t kt = lds_offset(&ktiles[b]);
         const uint32_t vt = lds_offset(&vtiles[b]);

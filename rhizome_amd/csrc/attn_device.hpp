@@ -190,13 +190,17 @@ __device__ __forceinline__ u32x4 load_chunk(const Rows<T>& s, long row0, int r, 
     }
 }
 
-// 16 (or 4) bytes a lane from memory, base + its offset, to LDS, lane i's at
-// lds + 16 i (4 i); base and lds are the same for all lanes.  Nothing waits for
-// it but landed(): the compiler, which would make every later LDS read wait for
-// a load that it knows of, does not see these.  Its own waits count them along,
-// which makes them longer, never shorter.
+// 16 (or 4) bytes a lane from memory, base + its offset + OFF, to LDS, lane i's
+// at lds + 16 i (4 i); base and lds are the same for all lanes (OFF counts in LDS
+// too, which is taken back).  Nothing waits for it but landed(): the compiler,
+// which would make every later LDS read wait for a load that it knows of, does
+// not see these.  Its own waits count them along, which makes them longer, never
+// shorter.
+template <int OFF>
 __device__ __forceinline__ void load_to_lds16(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds - OFF), "v"(off),
+                 "s"(base), "n"(OFF)
+                 : "memory");
 }
 __device__ __forceinline__ void load_to_lds4(const void* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
@@ -222,44 +226,63 @@ __device__ __forceinline__ void settle(V& v) { asm volatile("" : "+v"(v)); }
 template <typename T, int D, int ROWS, int NT, bool VEC>
 struct Mover {
     using TILE = Tile<T, D, ROWS>;
-    static constexpr int E = kChunkElems<T>, COUNT = ROWS * 8 / NT;
+    static constexpr int E = kChunkElems<T>, COUNT = ROWS * 8 / NT, PANELS = TILE::kPanels;
     static_assert(COUNT * NT == ROWS * 8, "whole chunks for every thread");
+    Rows<T> s;
+    int tid;
+    bool whole;                          // every panel is full and of one tensor
+    uint32_t off[COUNT], off_behind[COUNT];  // of the thread's chunks of a full tile, from either tensor
 
-    static __device__ __forceinline__ void clear(const Rows<T>& s, TILE& t, int tid) {
-        if (s.cols + s.extra >= TILE::kPanels * 8 * E) return;
-        for (int at = tid; at < TILE::kPanels * ROWS * 8; at += NT) t.chunk[at] = u32x4{0, 0, 0, 0};
+    __device__ __forceinline__ Mover(const Rows<T>& rows, int t) : s(rows), tid(t) {
+        whole = s.cols % (8 * E) == 0 && s.cols + s.extra == PANELS * 8 * E;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) place(i, ROWS, off[i], off_behind[i]);
+        }
+    }
+    __device__ __forceinline__ void place(int i, int valid, uint32_t& first, uint32_t& behind) const {
+        const int r = (i * NT + tid) >> 3, c = (tid & 7) ^ twist(r), rr = min(r, valid - 1);
+        first = (rr * int(s.stride) + c * E) * int(sizeof(T));
+        behind = (rr * int(s.extra_stride) + c * E) * int(sizeof(T));
+    }
+    __device__ __forceinline__ void clear(TILE& t) const {
+        if (s.cols + s.extra >= PANELS * 8 * E) return;
+        for (int at = tid; at < PANELS * ROWS * 8; at += NT) t.chunk[at] = u32x4{0, 0, 0, 0};
+    }
+    // Panels P .. of the thread's chunk i.
+    template <int P>
+    __device__ __forceinline__ void panels(int i, const T* first, const T* second, uint32_t at, uint32_t at_behind,
+                                           uint32_t lds) const {
+        if constexpr (P < PANELS) {
+            constexpr int d0 = P * 8 * E;
+            const uint32_t to = lds + P * TILE::kPanelBytes;
+            if (whole) {
+                const bool behind = d0 >= s.cols;
+                load_to_lds16<P * 128>(behind ? second : first, behind ? at_behind : at, to);
+            } else {
+                const int d = d0 + ((tid & 7) ^ twist((i * NT + tid) >> 3)) * E;
+                if (d < s.cols) load_to_lds16<P * 128>(first, at, to);
+                if (d >= s.cols && d < s.cols + s.extra) load_to_lds16<P * 128>(second, at_behind, to);
+            }
+            panels<P + 1>(i, first, second, at, at_behind, lds);
+        }
     }
     // rows row0 .. of which `valid` (>= 1) are there
-    static __device__ __forceinline__ void start(const Rows<T>& s, long row0, int valid, TILE& t, int tid) {
+    __device__ __forceinline__ void start(long row0, int valid, TILE& t) const {
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const T* first = s.p + row0 * s.stride;
         const T* second = s.extra_p + row0 * s.extra_stride - s.cols;
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
-            const int r = (i * NT + tid) >> 3, c = (tid & 7) ^ twist(r);
-            const int rr = valid >= ROWS ? r : min(r, valid - 1);
             if constexpr (VEC) {
-                const uint32_t lds = lds_offset(&t.chunk[0]) + (i * NT + wave * 64) * 16;
-                const uint32_t off = (rr * int(s.stride) + c * E) * int(sizeof(T));
-                const uint32_t off2 = (rr * int(s.extra_stride) + c * E) * int(sizeof(T));
-#pragma unroll
-                for (int p = 0; p < TILE::kPanels; ++p) {
-                    const int d0 = p * 8 * E;
-                    const T *b1 = first + d0, *b2 = second + d0;
-                    if (d0 + 8 * E <= s.cols) {
-                        load_to_lds16(b1, off, lds + p * TILE::kPanelBytes);
-                    } else if (d0 >= s.cols && d0 + 8 * E <= s.cols + s.extra) {
-                        load_to_lds16(b2, off2, lds + p * TILE::kPanelBytes);
-                    } else {
-                        const int d = d0 + c * E;
-                        if (d < s.cols) load_to_lds16(b1, off, lds + p * TILE::kPanelBytes);
-                        if (d >= s.cols && d < s.cols + s.extra) load_to_lds16(b2, off2, lds + p * TILE::kPanelBytes);
-                    }
-                }
+                uint32_t at = off[i], at_behind = off_behind[i];
+                if (valid < ROWS) place(i, valid, at, at_behind);
+                panels<0>(i, first, second, at, at_behind, lds_offset(&t.chunk[0]) + (i * NT + wave * 64) * 16);
             } else {
+                const int r = (i * NT + tid) >> 3, c = (tid & 7) ^ twist(r);
 #pragma unroll 1
-                for (int p = 0; p < TILE::kPanels; ++p)
-                    t.chunk[p * ROWS * 8 + i * NT + tid] = load_chunk<T, false>(s, row0, rr, p * 8 + c);
+                for (int p = 0; p < PANELS; ++p)
+                    t.chunk[p * ROWS * 8 + i * NT + tid] = load_chunk<T, false>(s, row0, min(r, valid - 1), p * 8 + c);
             }
         }
     }
@@ -288,6 +311,20 @@ __device__ __forceinline__ void store_columns(T* out, const f32x16& acc, int d0,
                 if (d + j < D) Elem<T>::store(out, d + j, x[j]);
         }
     }
+}
+
+// The other half's value beside one's own.
+__device__ __forceinline__ float2 both_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_of_halves(float x) {
+    const float2 v = both_halves(x);
+    return fmaxf(v.x, v.y);
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+    const float2 v = both_halves(x);
+    return v.x + v.y;
 }
 
 // ---- rows with an infinity or NaN

@@ -20,8 +20,6 @@ template <int DQ, int DV, bool VEC>
 __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillParams a) {
     constexpr int E = kChunkElems<T>, BN = 64, SUB = BN / 32;
     constexpr int QC = DQ / (2 * E), VT = DV / 32;
-    using MoveK = Mover<T, DQ, BN, kThreads, VEC>;
-    using MoveV = Mover<T, DV, BN, kThreads, VEC>;
     __shared__ Tile<T, DQ, BN> ktiles[2];
     __shared__ Tile<T, DV, BN> vtiles[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
@@ -53,20 +51,19 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
     for (int d = 0; d < VT; ++d) o[d] = f32x16{};
     const float c = a.scale * kLog2e;
     float m = -INFINITY, l = 0.f;
-    for (int b = 0; b < 2; ++b) {
-        MoveK::clear(krows, ktiles[b], tid);
-        MoveV::clear(vrows, vtiles[b], tid);
-    }
+    const Mover<T, DQ, BN, kThreads, VEC> move_k(krows, tid);
+    const Mover<T, DV, BN, kThreads, VEC> move_v(vrows, tid);
+    for (int b = 0; b < 2; ++b) move_k.clear(ktiles[b]), move_v.clear(vtiles[b]);
     __syncthreads();
     if (end > 0) {
-        MoveK::start(krows, w.k0, w.nk, ktiles[0], tid);
-        MoveV::start(vrows, w.k0, w.nk, vtiles[0], tid);
+        move_k.start(w.k0, w.nk, ktiles[0]);
+        move_v.start(w.k0, w.nk, vtiles[0]);
     }
     for (int k0 = 0, b = 0; k0 < end; k0 += BN, b ^= 1) {
         landed();
         if (k0 + BN < end) {
-            MoveK::start(krows, (long)w.k0 + k0 + BN, w.nk - k0 - BN, ktiles[b ^ 1], tid);
-            MoveV::start(vrows, (long)w.k0 + k0 + BN, w.nk - k0 - BN, vtiles[b ^ 1], tid);
+            move_k.start((long)w.k0 + k0 + BN, w.nk - k0 - BN, ktiles[b ^ 1]);
+            move_v.start((long)w.k0 + k0 + BN, w.nk - k0 - BN, vtiles[b ^ 1]);
         }
         const uint32_t kt = lds_offset(&ktiles[b]);
         const uint32_t vt = lds_offset(&vtiles[b]);
@@ -93,7 +90,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = max_of_halves(top);
         if (__any((top - m) * c > 8.f)) {
             const float up = fmaxf(m, top);
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
@@ -122,7 +119,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
             }
         }
     }
-    l += __shfl_xor(l, 32, kWave);
+    l = sum_of_halves(l);
     const float f = l == 0.f ? 0.f : 1.f / l;
     uint32_t again = not_finite_rows(o) & uint32_t(__ballot(live));
     while (again) {

@@ -52,8 +52,6 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
     constexpr int QC = DQ / (2 * E), VT = DV / 32;
     using TileK = Tile<T, DQ, kTile>;
     using TileV = Tile<T, DV, kTile>;
-    using MoveK = Mover<T, DQ, kTile, kWave, VEC>;
-    using MoveV = Mover<T, DV, kTile, kWave, VEC>;
     __shared__ WaveTiles<DQ, DV> tiles[kWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
@@ -75,12 +73,13 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
 #pragma unroll
     for (int c = 0; c < QC; ++c) settle(q[c]);
     WaveTiles<DQ, DV>& mine = tiles[wave];
-    MoveK::clear(krows, mine.a, lane);
-    MoveV::clear(vrows, mine.b, lane);
+    const Mover<T, DQ, kTile, kWave, VEC> move_a(krows, lane);
+    const Mover<T, DV, kTile, kWave, VEC> move_b(vrows, lane);
+    move_a.clear(mine.a), move_b.clear(mine.b);
     wave_read();
     const auto start = [&](int k0) {
-        MoveK::start(krows, (long)w.k0 + k0, w.nk - k0, mine.a, lane);
-        MoveV::start(vrows, (long)w.k0 + k0, w.nk - k0, mine.b, lane);
+        move_a.start((long)w.k0 + k0, w.nk - k0, mine.a);
+        move_b.start((long)w.k0 + k0, w.nk - k0, mine.b);
     };
     f32x16 o[VT];
 #pragma unroll
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = max_of_halves(top);
         if (__any((top - m) * c > 8.f)) {
             const float up = fmaxf(m, top);
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
@@ -134,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
         if (k0 + kWaves * kTile < end) start(k0 + kWaves * kTile);
     }
     // the waves' sums at their common maximum, over the tiles' memory
-    l += __shfl_xor(l, 32, kWave);
+    l = sum_of_halves(l);
     const Sums<VT> sums = {reinterpret_cast<f32x4*>(&tiles[0]), lane};
     float2* stats = reinterpret_cast<float2*>(&sums.at[kWaves * VT * 4 * kWave]);
     static_assert(sizeof(tiles) >= kWaves * (VT * 4096 + kWave * 8), "room for the sums");
@@ -184,8 +183,6 @@ __global__ __launch_bounds__(kThreads) void attn_dkv_split_kernel(BackwardParams
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32, VT = DV / 32;
     using TileQ = Tile<T, DQ, kTile>;
     using TileO = Tile<T, DV, kTile>;
-    using MoveQ = Mover<T, DQ, kTile, kWave, VEC>;
-    using MoveO = Mover<T, DV, kTile, kWave, VEC>;
     __shared__ WaveTiles<DQ, DV> tiles[kWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
@@ -212,16 +209,17 @@ __global__ __launch_bounds__(kThreads) void attn_dkv_split_kernel(BackwardParams
 #pragma unroll
     for (int c = 0; c < VC; ++c) settle(vf[c]);
     WaveTiles<DQ, DV>& mine = tiles[wave];
-    MoveQ::clear(qrows, mine.a, lane);
-    MoveO::clear(orows, mine.b, lane);
+    const Mover<T, DQ, kTile, kWave, VEC> move_a(qrows, lane);
+    const Mover<T, DV, kTile, kWave, VEC> move_b(orows, lane);
+    move_a.clear(mine.a), move_b.clear(mine.b);
     wave_read();
     const float *lse2 = a.lse2 + head * a.queries + w.q0, *delta = a.delta + head * a.queries + w.q0;
     float lse_r = 0.f, delta_r = 0.f;  // of query lane % 32 of the tile
     const auto start = [&](int q0) {
         const int i = q0 + min(lane & 31, w.nq - q0 - 1);
         lse_r = lse2[i], delta_r = delta[i];
-        MoveQ::start(qrows, (long)w.q0 + q0, w.nq - q0, mine.a, lane);
-        MoveO::start(orows, (long)w.q0 + q0, w.nq - q0, mine.b, lane);
+        move_a.start((long)w.q0 + q0, w.nq - q0, mine.a);
+        move_b.start((long)w.q0 + q0, w.nq - q0, mine.b);
     };
     f32x16 dk[QT], dv[VT];
 #pragma unroll
@@ -328,8 +326,6 @@ __global__ __launch_bounds__(kThreads) void attn_dq_split_kernel(BackwardParams 
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32;
     using TileK = Tile<T, DQ, kTile>;
     using TileV = Tile<T, DV, kTile>;
-    using MoveK = Mover<T, DQ, kTile, kWave, VEC>;
-    using MoveV = Mover<T, DV, kTile, kWave, VEC>;
     __shared__ WaveTiles<DQ, DV> tiles[kWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
@@ -358,12 +354,13 @@ __global__ __launch_bounds__(kThreads) void attn_dq_split_kernel(BackwardParams 
     for (int c = 0; c < VC; ++c) settle(of[c]);
     settle(lse2), settle(delta);
     WaveTiles<DQ, DV>& mine = tiles[wave];
-    MoveK::clear(krows, mine.a, lane);
-    MoveV::clear(vrows, mine.b, lane);
+    const Mover<T, DQ, kTile, kWave, VEC> move_a(krows, lane);
+    const Mover<T, DV, kTile, kWave, VEC> move_b(vrows, lane);
+    move_a.clear(mine.a), move_b.clear(mine.b);
     wave_read();
     const auto start = [&](int k0) {
-        MoveK::start(krows, (long)w.k0 + k0, w.nk - k0, mine.a, lane);
-        MoveV::start(vrows, (long)w.k0 + k0, w.nk - k0, mine.b, lane);
+        move_a.start((long)w.k0 + k0, w.nk - k0, mine.a);
+        move_b.start((long)w.k0 + k0, w.nk - k0, mine.b);
     };
     f32x16 dq[QT];
 #pragma unroll

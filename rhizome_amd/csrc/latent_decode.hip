@@ -293,7 +293,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
         float top = s[0];
 #pragma unroll
         for (int k = 1; k < 16; ++k) top = fmaxf(top, s[k]);
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = max_of_halves(top);
         if (__any((top - m) * c > 8.f)) {
             const float up = fmaxf(m, top);
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
             sum_rows(o[d], x, p);
         }
     }
-    l += __shfl_xor(l, 32, kWave);
+    l = sum_of_halves(l);
     const int r = u.first_row + 32 * mine + (lane & 31);
     bool live = r < rows;
     if (part == 0 && g == 0 && live) store_sums(a, u, r, m, l);
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
             }
             float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
             top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            top = max_of_halves(top);
             if (__any((top - m) * c > 8.f)) {
                 const float up = fmaxf(m, top);
                 const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - up) * c);
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     // The waves' sums at their common maximum: waves 2 and 3 hand theirs to 0 and
     // 1, which exchange halves, so that each has the whole of half of the columns.
     l += __shfl_xor(l, 16, kWave);
-    l += __shfl_xor(l, 32, kWave);
+    l = sum_of_halves(l);
     if (g == 0) wave_m[wave][kr] = m, wave_l[wave][kr] = l;
     __syncthreads();
     float top = -INFINITY, sum = 0.f;
