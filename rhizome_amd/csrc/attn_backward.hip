@@ -45,155 +45,220 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(BackwardParams a) 
 }
 
 // ------------------------------------------------------------------ dk, dv
+// Eight waves for 128 keys, two for every 32 of them: the first forms the
+// weights p and sums dv = p^T do, the second forms dp, takes p from the first
+// through LDS a tile later, and sums dk = ds^T q.  That halves what a wave holds
+// (keys or values as operands, and one of the sums), so that each SIMD has one of
+// either kind, whose matrix and vector instructions overlap.
 template <int DQ, int DV, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BackwardParams a) {
+__global__ __launch_bounds__(512, 2) void attn_dkv_kernel(BackwardParams a) {
     using T = uint16_t;
-    constexpr int E = kChunkElems<T>, BQ = 64, SUB = BQ / 32;
+    constexpr int E = kChunkElems<T>, BQ = 32, RING = 4;
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32, VT = DV / 32;
-    __shared__ Tile<T, DQ, BQ> qtiles[2];
-    __shared__ Tile<T, DV, BQ> otiles[2];
-    __shared__ float4 lse_s[2][16], delta_s[2][16];  // a wave's 64 floats
+    using TileQ = Tile<T, DQ, BQ>;
+    using TileO = Tile<T, DV, BQ>;
+    __shared__ TileQ qtiles[RING];
+    __shared__ TileO otiles[RING];
+    __shared__ f32x4 handed[2][4][4][kWave];                 // p: [tile][32 keys][registers by four][lane]
+    __shared__ float4 lse_s[RING][16], delta_s[RING][16];  // a wave's 64 floats
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
+    const int second = wave >> 2, group = wave & 3;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
     if (!place(a, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int first = tile * kRows;
     if (first >= w.nk) return;
-    const int wk = first + wave * 32, kj = wk + (lane & 31);
+    const int wk = first + group * 32, kj = wk + (lane & 31);
     const int shift = w.nk - w.nq;
+    bool live = kj < w.nk;
+    const long token = (long)w.k0 + min(kj, w.nk - 1), row = token * a.heads + head;
 
-    u32x4 kf[QC], vf[VC];
     const Rows<T> krows = {(const T*)a.k + head * a.kh, (const T*)(a.r ? a.r : a.k), a.ks, a.rs, a.d_n, a.d_r};
     const Rows<T> vrows = {(const T*)a.v + head * a.vh, (const T*)a.v, a.vs, 0, a.d_v, 0};
-    {
-        const int r = min(kj, w.nk - 1) - first;
-#pragma unroll
-        for (int c = 0; c < QC; ++c) kf[c] = load_chunk<T, VEC>(krows, (long)w.k0 + first, r, 2 * c + g);
-#pragma unroll
-        for (int c = 0; c < VC; ++c) vf[c] = load_chunk<T, VEC>(vrows, (long)w.k0 + first, r, 2 * c + g);
-    }
     const Rows<T> qrows = {(const T*)a.q + head * a.qh, (const T*)a.q, a.qs, 0, a.d_n + a.d_r, 0};
     const Rows<T> orows = {(const T*)a.go + (long)head * a.d_v, (const T*)a.go, (long)a.heads * a.d_v, 0, a.d_v, 0};
     const float* lse2 = a.lse2 + head * a.queries + w.q0;
     const float* delta = a.delta + head * a.queries + w.q0;
-    const Mover<T, DQ, BQ, kThreads, VEC> move_q(qrows, tid);
-    const Mover<T, DV, BQ, kThreads, VEC> move_o(orows, tid);
-    const auto start = [&](int q0, int b) {
-        move_q.start((long)w.q0 + q0, w.nq - q0, qtiles[b]);
-        move_o.start((long)w.q0 + q0, w.nq - q0, otiles[b]);
-        const uint32_t off = min(lane, min(BQ, w.nq - q0) - 1) * 4;
-        if (wave == 0) load_to_lds4(lse2 + q0, off, lds_offset(&lse_s[b][0]));
-        if (wave == 1) load_to_lds4(delta + q0, off, lds_offset(&delta_s[b][0]));
-    };
-#pragma unroll
-    for (int c = 0; c < QC; ++c) settle(kf[c]);
-#pragma unroll
-    for (int c = 0; c < VC; ++c) settle(vf[c]);
-    f32x16 dk[QT], dv[VT];
-#pragma unroll
-    for (int d = 0; d < QT; ++d) dk[d] = f32x16{};
-#pragma unroll
-    for (int d = 0; d < VT; ++d) dv[d] = f32x16{};
     const float c = a.scale * kLog2e;
-    // the first query that sees the workgroup's first key
+    // from the first query that sees the workgroup's first key on
     const int begin = a.causal ? max(0, first - shift) / BQ * BQ : 0;
-    for (int b = 0; b < 2; ++b) move_q.clear(qtiles[b]), move_o.clear(otiles[b]);
-    __syncthreads();
-    if (begin < w.nq) start(begin, 0);
-    for (int q0 = begin, b = 0; q0 < w.nq; q0 += BQ, b ^= 1) {
-        landed();
-        if (q0 + BQ < w.nq) start(q0 + BQ, b ^ 1);
-        const uint32_t qt = lds_offset(&qtiles[b]);
-        const uint32_t ot = lds_offset(&otiles[b]);
-        if (a.causal && q0 + BQ - 1 + shift < wk) continue;  // sees none of the wave's keys
-#pragma unroll 1  // both halves at once take more registers than there are
-        for (int u = 0; u < SUB; ++u) {
-            f32x16 s = {}, dp = {};
+    const int tiles = w.nq > begin ? (w.nq - begin + BQ - 1) / BQ : 0;
+
+    // The first kind moves q, the second do and what belongs to the queries.
+    const Mover<T, DQ, BQ, kThreads, VEC> move_q(qrows, tid & 255);
+    const Mover<T, DV, BQ, kThreads, VEC> move_o(orows, tid & 255);
+    const auto start = [&](int j) {
+        const int q0 = begin + j * BQ, left = w.nq - q0, slot = j % RING;
+        if (!second) {
+            move_q.start((long)w.q0 + q0, left, qtiles[slot]);
+        } else {
+            move_o.start((long)w.q0 + q0, left, otiles[slot]);
+            const uint32_t off = min(lane, min(BQ, left) - 1) * 4;
+            if (group == 0) load_to_lds4(lse2 + q0, off, lds_offset(&lse_s[slot][0]));
+            if (group == 1) load_to_lds4(delta + q0, off, lds_offset(&delta_s[slot][0]));
+        }
+    };
+    for (int i = 0; i < RING; ++i) {
+        if (!second) move_q.clear(qtiles[i]);
+        if (second) move_o.clear(otiles[i]);
+    }
+    // Tile j is there, for all waves, while j + 1 may be on its way.
+    const bool counted = VEC && move_q.whole && move_o.whole;
+    const auto wait = [&](int j) {
+        if (counted && j + 1 < tiles) {
+            if (!second)
+                wait_loads<TileQ::kPanels>();
+            else if (group < 2)
+                wait_loads<TileO::kPanels + 1>();
+            else
+                wait_loads<TileO::kPanels>();
+        } else {
+            wait_loads<0>();
+        }
+        lds_barrier();
+    };
+    const auto hidden = [&](int j) { return a.causal && begin + j * BQ + BQ - 1 + shift < wk; };  // sees none of the keys
+    // p or ds of what is not seen: of the lane's key rows below `least`, and those behind the last query
+    const auto clip = [&](int j, f32x16& x) {
+        const int qu = begin + j * BQ;
+        if (qu + BQ <= w.nq && !(a.causal && wk + 31 - shift > qu)) return;
+        const int least = (a.causal ? kj - shift - qu : 0) - 4 * g, left = w.nq - qu - 4 * g;
 #pragma unroll
-            for (int i = 0; i < QC; ++i) dot_chunks(s, read_row<Tile<T, DQ, BQ>>(qt, at, u, i), kf[i], T());
+        for (int i = 0; i < 16; ++i) {
+            const int r = (i & 3) + 8 * (i >> 2);
+            if (r < least || r >= left) x[i] = 0.f;
+        }
+    };
+
+    if (!second) {
+        u32x4 kf[QC];
 #pragma unroll
-            for (int i = 0; i < VC; ++i) dot_chunks(dp, read_row<Tile<T, DV, BQ>>(ot, at, u, i), vf[i], T());
-            const int qu = q0 + 32 * u;
-            // the lane's key is seen by the tile's queries from number `from` on
-            const int from = a.causal ? kj - shift - qu : 0;
-            const bool masked = qu + 32 > w.nq || (a.causal && wk + 31 - shift > qu);
+        for (int i = 0; i < QC; ++i)
+            kf[i] = load_chunk<T, VEC>(krows, (long)w.k0 + first, min(kj, w.nk - 1) - first, 2 * i + g);
+#pragma unroll
+        for (int i = 0; i < QC; ++i) settle(kf[i]);
+        f32x16 dv[VT];
+#pragma unroll
+        for (int d = 0; d < VT; ++d) dv[d] = f32x16{};
+        lds_barrier();
+        if (tiles > 0) start(0);
+        if (tiles > 1) start(1);
+        for (int j = 0; j < tiles; ++j) {
+            wait(j);
+            if (j + 2 < tiles) start(j + 2);
+            if (hidden(j)) continue;
+            const uint32_t qt = lds_offset(&qtiles[j % RING]), ot = lds_offset(&otiles[j % RING]);
+            f32x16 s = {};
+            dot_ahead<QC, 6>(s, kf, [&](int i) { return read_row<TileQ>(qt, at, 0, i); }, T());
+            SumAhead<T, TileO, VT, 2> sum;
+            sum.begin(ot, at, 0);
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
-                const float4 lq = lse_s[b][8 * u + 2 * i4 + g], dq = delta_s[b][8 * u + 2 * i4 + g];
-                const float ls[4] = {lq.x, lq.y, lq.z, lq.w}, ds[4] = {dq.x, dq.y, dq.z, dq.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = 4 * i4 + j;
-                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ls[j]));
-                    dp[i] = s[i] * (dp[i] - ds[j]);
-                }
+                const float4 l = lse_s[j % RING][2 * i4 + g];
+                s[4 * i4] = __builtin_amdgcn_exp2f(fmaf(s[4 * i4], c, -l.x));
+                s[4 * i4 + 1] = __builtin_amdgcn_exp2f(fmaf(s[4 * i4 + 1], c, -l.y));
+                s[4 * i4 + 2] = __builtin_amdgcn_exp2f(fmaf(s[4 * i4 + 2], c, -l.z));
+                s[4 * i4 + 3] = __builtin_amdgcn_exp2f(fmaf(s[4 * i4 + 3], c, -l.w));
             }
-            if (masked) {
-                const int least = from - 4 * g, left = w.nq - qu - 4 * g;
+            clip(j, s);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                handed[j & 1][group][k][lane] = f32x4{s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]};
+            Weights<T> p;
+            p.set(s);
+            sum.run(dv, ot, at, 0, p);
+        }
+        lds_barrier();  // the last tile's weights are handed on
+        uint32_t again = not_finite_rows(dv) & uint32_t(__ballot(live));
+        while (again) {
+            const int r = __ffs(again) - 1;
+            again &= again - 1;
+            const long mine = (long)w.k0 + wk + r;
+            const int from = a.causal ? max(0, wk + r - shift) : 0;  // the first query that sees the key
+            sum_row_again<2>(
+                (long)w.q0 + from, (long)w.q0 + w.nq, a.d_v, lane,
+                [&](long i) { return __builtin_amdgcn_exp2f(fmaf(dot_rows(qrows, i, krows, mine), c, -lse2[i - w.q0])); },
+                [&](long i, int d) { return value(orows, i, d); },
+                [&](int d, float x) { Elem<T>::store((T*)a.dv + (mine * a.heads + head) * a.d_v, d, x); });
+            if ((lane & 31) == r) live = false;
+        }
+        if (!live) return;
+#pragma unroll
+        for (int d = 0; d < VT; ++d) store_columns<T>((T*)a.dv + row * a.d_v, dv[d], 32 * d, a.d_v, 1.f, a.vec_out, lane);
+    } else {
+        u32x4 vf[VC];
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+            vf[i] = load_chunk<T, VEC>(vrows, (long)w.k0 + first, min(kj, w.nk - 1) - first, 2 * i + g);
+#pragma unroll
+        for (int i = 0; i < VC; ++i) settle(vf[i]);
+        f32x16 dk[QT];
+#pragma unroll
+        for (int d = 0; d < QT; ++d) dk[d] = f32x16{};
+        lds_barrier();
+        if (tiles > 0) start(0);
+        if (tiles > 1) start(1);
+        for (int j1 = 0; j1 <= tiles; ++j1) {  // a tile behind the first kind
+            if (j1 < tiles)
+                wait(j1);
+            else
+                lds_barrier();
+            if (j1 + 2 < tiles) start(j1 + 2);
+            const int j = j1 - 1;
+            if (j < 0 || hidden(j)) continue;
+            const uint32_t qt = lds_offset(&qtiles[j % RING]), ot = lds_offset(&otiles[j % RING]);
+            f32x16 dp = {};
+            dot_ahead<VC, 6>(dp, vf, [&](int i) { return read_row<TileO>(ot, at, 0, i); }, T());
+            SumAhead<T, TileQ, QT, 2> sum;
+            sum.begin(qt, at, 0);
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const f32x4 p = handed[j & 1][group][i4][lane];
+                const float4 l = delta_s[j % RING][2 * i4 + g];
+                dp[4 * i4] = p[0] * (dp[4 * i4] - l.x);
+                dp[4 * i4 + 1] = p[1] * (dp[4 * i4 + 1] - l.y);
+                dp[4 * i4 + 2] = p[2] * (dp[4 * i4 + 2] - l.z);
+                dp[4 * i4 + 3] = p[3] * (dp[4 * i4 + 3] - l.w);
+            }
+            clip(j, dp);
+            Weights<T> ds;
+            ds.set(dp);
+            sum.run(dk, qt, at, 0, ds);
+        }
+        uint32_t again = not_finite_rows(dk) & uint32_t(__ballot(live));
+        while (again) {
+            const int r = __ffs(again) - 1;
+            again &= again - 1;
+            const long mine = (long)w.k0 + wk + r;
+            const int from = a.causal ? max(0, wk + r - shift) : 0;
+            sum_row_again<3>(
+                (long)w.q0 + from, (long)w.q0 + w.nq, a.d_n + a.d_r, lane,
+                [&](long i) {
+                    return __builtin_amdgcn_exp2f(fmaf(dot_rows(qrows, i, krows, mine), c, -lse2[i - w.q0])) *
+                           (dot_rows(orows, i, vrows, mine) - delta[i - w.q0]) * a.scale;
+                },
+                [&](long i, int d) { return value(qrows, i, d); },
+                [&](int d, float x) {
+                    if (d < a.d_n)
+                        Elem<T>::store((T*)a.dk + (mine * a.heads + head) * a.d_n, d, x);
+                    else
+                        a.dr_part[(head * a.keys + mine) * a.d_r + d - a.d_n] = x;
+                });
+            if ((lane & 31) == r) live = false;
+        }
+        if (!live) return;
+        T* gk = (T*)a.dk + row * a.d_n;
+        float* gr = a.dr_part + (head * a.keys + token) * a.d_r;
+#pragma unroll
+        for (int d = 0; d < QT; ++d) {
+            if (32 * d < a.d_n) store_columns<T>(gk, dk[d], 32 * d, a.d_n, a.scale, a.vec_out, lane);
+            if (32 * d + 32 > a.d_n) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = (i & 3) + 8 * (i >> 2);
-                    if (r < least || r >= left) s[i] = dp[i] = 0.f;
+                    const int e = 32 * d + (i & 3) + 8 * (i >> 2) + 4 * g - a.d_n;
+                    if (e >= 0 && e < a.d_r) gr[e] = dk[d][i] * a.scale;
                 }
-            }
-            Weights<T> p, ds;
-            p.set(s);
-            ds.set(dp);
-#pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                Columns<T> x;
-                x.template load<Tile<T, DV, BQ>>(ot, at, u, d);
-                sum_rows(dv[d], x, p);
-            }
-#pragma unroll
-            for (int d = 0; d < QT; ++d) {
-                Columns<T> x;
-                x.template load<Tile<T, DQ, BQ>>(qt, at, u, d);
-                sum_rows(dk[d], x, ds);
-            }
-        }
-    }
-    bool live = kj < w.nk;
-    uint32_t again = (not_finite_rows(dv) | not_finite_rows(dk)) & uint32_t(__ballot(live));
-    while (again) {
-        const int r = __ffs(again) - 1;
-        again &= again - 1;
-        const long mine = (long)w.k0 + wk + r, row = mine * a.heads + head;
-        const int from = a.causal ? max(0, wk + r - shift) : 0;  // the first query that sees the key
-        const auto weight = [&](long i) {
-            return __builtin_amdgcn_exp2f(fmaf(dot_rows(qrows, i, krows, mine), c, -lse2[i - w.q0]));
-        };
-        sum_row_again<2>((long)w.q0 + from, (long)w.q0 + w.nq, a.d_v, lane, weight,
-                         [&](long i, int d) { return value(orows, i, d); },
-                         [&](int d, float x) { Elem<T>::store((T*)a.dv + row * a.d_v, d, x); });
-        sum_row_again<3>(
-            (long)w.q0 + from, (long)w.q0 + w.nq, a.d_n + a.d_r, lane,
-            [&](long i) { return weight(i) * (dot_rows(orows, i, vrows, mine) - delta[i - w.q0]) * a.scale; },
-            [&](long i, int d) { return value(qrows, i, d); },
-            [&](int d, float x) {
-                if (d < a.d_n)
-                    Elem<T>::store((T*)a.dk + row * a.d_n, d, x);
-                else
-                    a.dr_part[(head * a.keys + mine) * a.d_r + d - a.d_n] = x;
-            });
-        if ((lane & 31) == r) live = false;
-    }
-    if (!live) return;
-    const long token = (long)w.k0 + kj, row = token * a.heads + head;
-    T* gv = (T*)a.dv + row * a.d_v;
-#pragma unroll
-    for (int d = 0; d < VT; ++d) store_columns<T>(gv, dv[d], 32 * d, a.d_v, 1.f, a.vec_out, lane);
-    T* gk = (T*)a.dk + row * a.d_n;
-    float* gr = a.dr_part + (head * a.keys + token) * a.d_r;
-#pragma unroll
-    for (int d = 0; d < QT; ++d) {
-        if (32 * d < a.d_n) store_columns<T>(gk, dk[d], 32 * d, a.d_n, a.scale, a.vec_out, lane);
-        if (32 * d + 32 > a.d_n) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int e = 32 * d + (i & 3) + 8 * (i >> 2) + 4 * g - a.d_n;
-                if (e >= 0 && e < a.d_r) gr[e] = dk[d][i] * a.scale;
             }
         }
     }
@@ -258,10 +323,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
         const uint32_t vt = lds_offset(&vtiles[b]);
         if (a.causal && k0 > wq + 31 + shift) continue;
         f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int i = 0; i < QC; ++i) dot_chunks(s, read_row<Tile<T, DQ, BN>>(kt, at, 0, i), qf[i], T());
-#pragma unroll
-        for (int i = 0; i < VC; ++i) dot_chunks(dp, read_row<Tile<T, DV, BN>>(vt, at, 0, i), of[i], T());
+        dot_ahead<QC, 4>(s, qf, [&](int i) { return read_row<Tile<T, DQ, BN>>(kt, at, 0, i); }, T());
+        dot_ahead<VC, 4>(dp, of, [&](int i) { return read_row<Tile<T, DV, BN>>(vt, at, 0, i); }, T());
+        SumAhead<T, Tile<T, DQ, BN>, QT, 2> sum;
+        sum.begin(kt, at, 0);
         const int seen = a.causal ? min(w.nk, qi + shift + 1) : w.nk;
         const bool masked = k0 + BN > w.nk || (a.causal && k0 + BN > wq + shift + 1);
 #pragma unroll
@@ -274,12 +339,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
         }
         Weights<T> ds;
         ds.set(dp);
-#pragma unroll
-        for (int d = 0; d < QT; ++d) {
-            Columns<T> x;
-            x.template load<Tile<T, DQ, BN>>(kt, at, 0, d);
-            sum_rows(dq[d], x, ds);
-        }
+        sum.run(dq, kt, at, 0, ds);
     }
     bool live = qi < w.nq;
     uint32_t again = not_finite_rows(dq) & uint32_t(__ballot(live));
@@ -329,10 +389,10 @@ hipError_t launch(BackwardParams p, hipStream_t stream) {
     const int64_t tq = attn_tiles(p.cu_q, p.queries, p.len_q, p.batch, kRows);
     const int64_t tk = attn_tiles(p.cu_k, p.keys, p.len_k, p.batch, kRows);
     if (p.keys) {
-        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_k, tk);
+        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_k, tk, 512);
         if (!blocks) return hipErrorInvalidConfiguration;
         p.tiles = (int)tk;
-        attn_dkv_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
+        attn_dkv_kernel<DQ, DV, VEC><<<blocks, 512, 0, stream>>>(p);
     }
     if (p.queries) {
         const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, tq);

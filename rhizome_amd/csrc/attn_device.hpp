@@ -210,7 +210,14 @@ __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The same of a wave's own loads and reads.
+// Waits for all but the last N loads of a wave.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// LDS reads and writes done, by all waves; loads on their way stay so.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// A wave's own loads and reads.
 __device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 // A wave's own LDS reads are done: what it read may be written over.
 __device__ __forceinline__ void wave_read() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -312,6 +319,45 @@ __device__ __forceinline__ void store_columns(T* out, const f32x16& acc, int d0,
         }
     }
 }
+
+// LDS reads some steps ahead of the products that take them, pinned there: left
+// to itself the scheduler reads, waits and multiplies by turns, 130 clocks of
+// LDS's latency for every 32 of the product.
+// acc += sum over i < N of read(i) . own[i]
+template <int N, int AHEAD, typename T, typename READ>
+__device__ __forceinline__ void dot_ahead(f32x16& acc, const u32x4 (&own)[N], READ read, T) {
+    constexpr int A = AHEAD < N ? AHEAD : N;
+    u32x4 x[A];
+#pragma unroll
+    for (int i = 0; i < A; ++i) x[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        dot_chunks(acc, x[i % A], own[i], T());
+        if (i + A < N) x[i % A] = read(i + A);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// acc[d] += tile's columns d, transposed, times p, of N column tiles; begin() may
+// come long before run().
+template <typename T, typename TILE, int N, int AHEAD>
+struct SumAhead {
+    static constexpr int A = AHEAD < N ? AHEAD : N;
+    Columns<T> x[A];
+    __device__ __forceinline__ void begin(uint32_t tile, const LaneReads& at, int u) {
+#pragma unroll
+        for (int d = 0; d < A; ++d) x[d].template load<TILE>(tile, at, u, d);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void run(f32x16 (&acc)[N], uint32_t tile, const LaneReads& at, int u, const Weights<T>& p) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) {
+            sum_rows(acc[d], x[d % A], p);
+            if (d + A < N) x[d % A].template load<TILE>(tile, at, u, d + A);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
 
 // The other half's value beside one's own.
 __device__ __forceinline__ float2 both_halves(float x) {

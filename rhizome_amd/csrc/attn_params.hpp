@@ -54,10 +54,10 @@ __device__ __forceinline__ bool place(const PARAMS& a, const int* cu, int total,
     return true;
 }
 // Workgroups for `tiles` tiles of every head; 0 if there are too many.
-inline unsigned attn_blocks(int heads, int batch, const int* cu, int64_t tiles) {
+inline unsigned attn_blocks(int heads, int batch, const int* cu, int64_t tiles, int threads = kAttnThreads) {
     const int64_t units = ((int64_t)heads * (cu ? 1 : batch) + 7) / 8 * 8;
     const int64_t blocks = tiles > INT32_MAX ? INT64_MAX / 2 : units * tiles;
-    return blocks > INT32_MAX || check_grid(blocks, kAttnThreads) != hipSuccess ? 0 : (unsigned)blocks;
+    return blocks > INT32_MAX || check_grid(blocks, threads) != hipSuccess ? 0 : (unsigned)blocks;
 }
 inline int64_t attn_tiles(const int* cu, int64_t total, int len, int batch, int size) {
     return cu ? packed_tiles(total, batch, size) : ((int64_t)len + size - 1) / size;

@@ -72,8 +72,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             s[u] = f32x16{};
-#pragma unroll
-            for (int i = 0; i < QC; ++i) dot_chunks(s[u], read_row<Tile<T, DQ, BN>>(kt, at, u, i), q[i], T());
+            dot_ahead<QC, 6>(s[u], q, [&](int i) { return read_row<Tile<T, DQ, BN>>(kt, at, u, i); }, T());
         }
         const int seen = a.causal ? min(w.nk, qi + shift + 1) : w.nk;  // keys that the lane's query sees
         const bool masked = k0 + BN > w.nk || (a.causal && k0 + BN > wq + shift + 1);
@@ -104,6 +103,8 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
         const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
+            SumAhead<T, Tile<T, DV, BN>, VT, 2> sum;
+            sum.begin(vt, at, u);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], c, -mc));
@@ -111,12 +112,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
             }
             Weights<T> p;
             p.set(s[u]);
-#pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                Columns<T> x;
-                x.template load<Tile<T, DV, BN>>(vt, at, u, d);
-                sum_rows(o[d], x, p);
-            }
+            sum.run(o, vt, at, u, p);
         }
     }
     l = sum_of_halves(l);

@@ -117,13 +117,6 @@ __device__ __forceinline__ void store_sums(const DecodeParams& a, const Unit& u,
     }
 }
 
-// Waits for all but the last N loads of a wave.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// LDS reads and writes done, by all waves; loads on their way stay so.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // 16 bytes a lane from p + OFF to LDS at lds; the instruction's offset counts in LDS too.
 template <int OFF>
 __device__ __forceinline__ void load_to_lds16_from(const void* p, uint32_t lds) {
