@@ -37,18 +37,27 @@ struct BackwardParams {
 
 constexpr int kAttnThreads = 256;
 
+// Heads (of sequences) whose workgroups are mixed on an XCD.
+constexpr int kMixed = 4;
+
 // Workgroup number -> head, sequence and tile of `size` rows of the side whose
-// offsets are `cu`; false if there is none.  Workgroups of one head follow one
-// another on one XCD, whose L2 keeps what they all read.
+// offsets are `cu`; false if there is none.  A head's workgroups are on one XCD,
+// whose L2 keeps what they all read.  There they start in order, by turns on its
+// quarters, so that a place stays empty until its turn comes: kMixed heads' tiles
+// of one number, which take about as long, follow one another.
 template <typename PARAMS>
 __device__ __forceinline__ bool place(const PARAMS& a, const int* cu, int total, int size, int lane, int& head, int& seq,
                                       int& tile) {
     const int units = a.heads * (cu ? 1 : a.batch);
     const int xcd = blockIdx.x & 7, n = blockIdx.x >> 3;
-    const int unit = (n / a.tiles) * 8 + xcd;
-    if (unit >= units) return false;
+    const int here = (units - xcd + 7) >> 3;  // units of this XCD
+    const int group = n / (kMixed * a.tiles), mixed = min(kMixed, here - group * kMixed);
+    if (mixed <= 0) return false;
+    const int m = n - group * kMixed * a.tiles;
+    if (m >= mixed * a.tiles) return false;
+    const int unit = (group * kMixed + m % mixed) * 8 + xcd;
     head = unit % a.heads;
-    tile = n % a.tiles;
+    tile = m / mixed;
     seq = unit / a.heads;
     if (cu) packed_tile(cu, a.batch, total, size, tile, lane, seq, tile);
     return true;
