@@ -125,8 +125,8 @@ rhz_status rhz_latent_append(const rhz_latent_append_args* args, void* stream);
 
 /* Attention of the last `steps` positions of every sequence over its cached
  * latents, absorbed (mla_decode, attention.rs:226-300): query i of sequence b
- * sees positions 0 .. lengths[b] - steps + i.  Rows beyond the table and pages
- * outside the cache hold no keys.  A sequence is split over workgroups by its
+ * sees positions 0 .. lengths[b] - steps + i.  Positions beyond the table, or
+ * from 2^31 - 4097 on, and pages outside the cache hold no keys.  A sequence is split over workgroups by its
  * own length alone and joined in order. */
 typedef struct rhz_latent_decode_args {
     int32_t batch;     /* >= 1 */

@@ -48,8 +48,9 @@ inline int most_splits_of(int64_t n) {
     return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(9, std::min<int64_t>(best, kMaxSplits))));
 }
 
+constexpr int64_t kMostRows = INT32_MAX - 4096;  // numbers of tiles' rows behind the last stay in 32 bits
 __device__ __forceinline__ int rows_of(const DecodeParams& a, int seq) {
-    const long room = (long)a.max_pages * a.page;
+    const long room = min((long)a.max_pages * a.page, (long)kMostRows);
     return (int)min((long)max(a.lengths[seq], 0), room);
 }
 
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     const float c = a.scale * kLog2e;
     const int least_seen = sees(a, u, u.first_row);
     const bool sums = part * VTW * 32 < VD;  // the wave has columns
-    fill_table(begin);
+    if (end > begin) fill_table(begin);
     __syncthreads();
     const int tiles_n = (end - begin + KEYS - 1) / KEYS;
     // whether a tile's loads are as many as the waits below count
@@ -626,7 +627,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams 
 }
 
 int most_splits(const rhz_latent_decode_args& a) {
-    return most_splits_of(std::min<int64_t>((int64_t)a.max_pages * a.page_size, INT32_MAX));
+    return most_splits_of(std::min<int64_t>((int64_t)a.max_pages * a.page_size, kMostRows));
 }
 
 hipError_t join(const DecodeParams& p, int dtype, hipStream_t stream) {

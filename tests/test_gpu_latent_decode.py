@@ -109,6 +109,13 @@ def test_pages(device, dtype, page):
 
 
 @both
+@pytest.mark.parametrize("H", [2, 20])
+def test_empty_sequences_and_pages_of_one_row(device, dtype, H):
+    """The first table entry of all has nothing before it to be looked up."""
+    check([0, 3, 0], 1, H, 128, 16, 1, dtype, device)
+
+
+@both
 def test_long_contexts(device, dtype):
     """More than 128 splits' worth of rows, and a table of rows refilled on the way."""
     check([40000, 2500], 1, 2, 64, 0, 64, dtype, device, seed=1)
