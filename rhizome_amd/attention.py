@@ -67,7 +67,7 @@ def _strides(name, t, heads=True):
     if len(shape) + at == 1:  # a batch before it
         batch, n = shape[0], shape[at]
         if n == 1:
-            token = st[0]
+            token = st[0] if batch > 1 else 0
         elif batch > 1 and st[0] != token * n and n > 0:
             raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
     return token, st[-2] if heads and shape[-2] > 1 else 0

@@ -215,6 +215,19 @@ def test_strides_and_alignment(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+def test_one_token_of_a_long_tensor(device, dtype):
+    """Its batch of one is 2^23 elements long, which no token's distance from the next is."""
+    H, d, m = 2, 64, 50
+    q, kv, _, _ = make([1], [m], H, d, 0, d, dtype, seed=18)
+    long = torch.zeros(1, (1 << 23) // (H * d), H, d, dtype=dtype, device=device)
+    long[:, 5:6] = q.to(device)
+    k, v = (t[None].to(device) for t in (kv[..., :d], kv[..., d:]))
+    got = rhizome_amd.latent_prefill(long[:, 5:6], k, v)
+    want = rhizome_amd.latent_prefill(q[None].to(device), k, v)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_a_sequence_alone_and_in_a_pack(device, dtype):
     """Batch-invariance, bit for bit; rows outside every sequence are left as they were."""
     lens, H, d = [37, 150, 64], 2, 64
