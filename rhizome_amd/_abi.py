@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t,
                     c_uint32, c_uint64, c_void_p)
 
@@ -208,6 +209,23 @@ class LatentPrefillBackwardArgs(Structure):
     ]
 
 
+def _codes(args) -> str:
+    codes = {c_int32: "i", c_int64: "q", c_float: "f", c_void_p: "P", c_size_t: "N"}
+    return "".join(codes.get(t) or _codes(t) for _, t in args._fields_)
+
+
+def _packer(args):
+    """A call that lays the values of args' fields out, in order, as C does (addresses
+    as numbers, 0 for NULL): a quarter of the time that filling in a Structure takes."""
+    s = struct.Struct("@" + _codes(args))
+    assert s.size == ctypes.sizeof(args)
+    return s.pack
+
+
+pack_rope, pack_latent_append, pack_latent_decode = _packer(RopeArgs), _packer(LatentAppendArgs), _packer(LatentDecodeArgs)
+pack_latent_prefill, pack_latent_prefill_backward = _packer(LatentPrefillArgs), _packer(LatentPrefillBackwardArgs)
+
+
 class GdrError(RuntimeError):
     """A non-OK rhz_status, with the library's detail message."""
 
@@ -265,18 +283,20 @@ def lib():
         L.rhz_gdr_prefill_backward.argtypes = [POINTER(PrefillBackwardArgs), c_void_p]
         L.rhz_gdr_prefill_backward.restype = c_int32
         for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
-                           ("rhz_norm_backward", NormBackwardArgs), ("rhz_latent_decode", LatentDecodeArgs),
-                           ("rhz_latent_prefill_backward", LatentPrefillBackwardArgs)):
+                           ("rhz_norm_backward", NormBackwardArgs)):
             size = getattr(L, name + "_workspace_size")
             size.argtypes, size.restype = [POINTER(args), POINTER(c_size_t)], c_int32
         for name, args in (("rhz_gdr_conv_prepare_backward", ConvPrepareBackwardArgs),
                            ("rhz_layernorm", LayernormArgs), ("rhz_layernorm_backward", NormBackwardArgs),
-                           ("rhz_rmsnorm_heads_backward", NormBackwardArgs), ("rhz_rope", RopeArgs),
-                           ("rhz_latent_append", LatentAppendArgs), ("rhz_latent_decode", LatentDecodeArgs),
-                           ("rhz_latent_prefill", LatentPrefillArgs),
-                           ("rhz_latent_prefill_backward", LatentPrefillBackwardArgs)):
+                           ("rhz_rmsnorm_heads_backward", NormBackwardArgs)):
             run = getattr(L, name)
             run.argtypes, run.restype = [POINTER(args), c_void_p], c_int32
+        for name in ("rhz_rope", "rhz_latent_append", "rhz_latent_decode", "rhz_latent_prefill", "rhz_latent_prefill_backward"):
+            run = getattr(L, name)
+            run.argtypes, run.restype = [c_void_p, c_void_p], c_int32  # what a packer lays out, or byref() of a Structure
+        for name in ("rhz_latent_decode_workspace_size", "rhz_latent_prefill_backward_workspace_size"):
+            size = getattr(L, name)
+            size.argtypes, size.restype = [c_void_p, POINTER(c_size_t)], c_int32
         L.rhz_rope_frequencies.argtypes = [POINTER(RopeFrequencyArgs), POINTER(c_double), POINTER(c_float)]
         L.rhz_rope_frequencies.restype = c_int32
         L.rhz_causal_conv1d.argtypes = [POINTER(Conv1dArgs), c_void_p]

@@ -17,20 +17,19 @@ A decoding step of the block, with the projections around it:
 """
 from __future__ import annotations
 
-from ctypes import byref, c_double, c_float
+from ctypes import byref, c_double, c_float, c_size_t
 
 import torch
 
 from . import _abi
 from .gdr import _DTYPES, _count, _empty, _on_stream
-from .train import _workspace
 
 _SCALINGS = {"none": _abi.ROPE_PLAIN, "linear": _abi.ROPE_LINEAR, "by_parts": _abi.ROPE_BY_PARTS}
 
 
 # A decoding step's calls are bounded by the host: the device is asked for once
-# a call, and the argument structs are filled in by position, which is what
-# most of a call's time went to (rope of one position of 8 sequences: 8.0 us).
+# a call, shapes are taken apart once, and the arguments are laid out in one go
+# (_abi.pack_*): a rope of 8 tokens takes 6.8 us a call instead of 8.6.
 def _here() -> int:
     return torch.cuda.current_device()
 
@@ -39,38 +38,53 @@ def _stream(here: int) -> int | None:
     return torch._C._cuda_getCurrentRawStream(here) or None
 
 
-def _view(t: torch.Tensor | None, here: int) -> int | None:
-    """The address of a tensor whose strides have been read, on the current device."""
+def _view(t: torch.Tensor | None, here: int) -> int:
+    """The address of a tensor whose strides have been read, on the current device; 0 for None."""
     if t is None:
-        return None
+        return 0
     if t.get_device() != here:
         if not t.is_cuda:
             raise ValueError("all tensors must be on the GPU")
         raise ValueError(f"all tensors must be on the current device, cuda:{here}")
-    return t.data_ptr() or None
+    return t.data_ptr()
 
 
-def _dense(t: torch.Tensor | None, here: int) -> int | None:
+def _dense(t: torch.Tensor | None, here: int) -> int:
     """The same of a tensor that has to be contiguous."""
     if t is not None and not t.is_contiguous():
         raise ValueError("all tensors but those of heads must be contiguous")
     return _view(t, here)
 
 
-def _strides(name, t, heads=True):
-    """Strides in elements from token to token, and from head to head."""
-    shape, st = t.shape, t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
+def _token_stride(name, t, batch, n):
+    """In elements, of a tensor of n tokens of every sequence of a batch, whose
+    last dimension has to be dense; batch None: of tokens alone."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}'s last dimension must be dense")
-    at = -3 if heads else -2  # the tokens' dimension
-    token = st[at]
-    if len(shape) + at == 1:  # a batch before it
-        batch, n = shape[0], shape[at]
-        if n == 1:
-            token = st[0] if batch > 1 else 0
-        elif batch > 1 and st[0] != token * n and n > 0:
-            raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
-    return token, st[-2] if heads and shape[-2] > 1 else 0
+    if batch is None:
+        return st[0]
+    if st[0] == st[1] * n:
+        return st[1]
+    if batch <= 1:
+        return st[1] if n > 1 else 0
+    if n == 1:
+        return st[0]
+    if n > 0:
+        raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
+    return st[1]
+
+
+def _workspace(size, a, like, workspace, here):
+    """Address and bytes of the caller's workspace, or of a new one of the size
+    that `size` gives for the arguments; and the new one, to be kept until the call."""
+    if workspace is None:
+        need = c_size_t()
+        _abi.check(size(a, byref(need)))
+        if not need.value:
+            return 0, 0, None
+        workspace = like.new_empty((need.value,), dtype=torch.uint8)
+    return _dense(workspace, here), workspace.numel() * workspace.element_size(), workspace
 
 
 def _check_positions(name, t, shape):
@@ -115,31 +129,37 @@ def rope(x, positions, frequencies, *, offset: int = 0, interleaved: bool = Fals
     """
     if stream is not None:
         return _on_stream(rope, locals())
-    if x.dim() not in (3, 4) or x.dtype not in _DTYPES:
+    dtype, shape = _DTYPES.get(x.dtype), x.shape
+    if dtype is None or len(shape) not in (3, 4):
         raise ValueError("x must be fp32 or bf16 [tokens, H, d] or [B, T, H, d]")
-    _check_positions("positions", positions, x.shape[:-2])
+    batch, n = (shape[0], shape[1]) if len(shape) == 4 else (None, shape[0])
+    H, d = shape[-2], shape[-1]
+    _check_positions("positions", positions, (n,) if batch is None else (batch, n))
     _check_frequencies(frequencies)
-    y = out if out is not None else _empty(x, x.shape)
-    if y.shape != x.shape or y.dtype != x.dtype:
+    y = out if out is not None else _empty(x, shape)
+    if y is not x and (y.shape != shape or y.dtype != x.dtype):
         raise ValueError("out must have x's shape and dtype")
-    xt, xh = _strides("x", x)
-    yt, yh = (xt, xh) if y is x else _strides("out", y)
+    xt, xh = _token_stride("x", x, batch, n), x.stride(-2) if H > 1 else 0
+    yt, yh = (xt, xh) if y is x else (_token_stride("out", y, batch, n), y.stride(-2) if H > 1 else 0)
     here = _here()
-    a = _abi.RopeArgs(_count(positions.numel()), x.shape[-2], x.shape[-1], offset, 2 * frequencies.numel(), _DTYPES[x.dtype],
-                      interleaved, inverse, magnitude, xt, xh, yt, yh, _view(x, here), _dense(positions, here),
-                      _dense(frequencies, here), _view(y, here))
-    _abi.check(_abi.lib().rhz_rope(byref(a), _stream(here)))
+    a = _abi.pack_rope(_count(n if batch is None else batch * n), H, d, offset, 2 * frequencies.numel(), dtype, interleaved,
+                       inverse, magnitude, xt, xh, yt, yh, _view(x, here), _dense(positions, here), _dense(frequencies, here),
+                       _view(y, here))
+    _abi.check(_abi.lib().rhz_rope(a, _stream(here)))
     return y
 
 
 def _check_paged(cache, page_table, lengths, D):
-    if cache.dim() != 3 or cache.dtype not in _DTYPES or cache.shape[-1] != D:
+    """Sequences, and what the argument structs have of the cache: page_size, num_pages, max_pages, dtype."""
+    dtype, at, table = _DTYPES.get(cache.dtype), cache.shape, page_table.shape
+    if len(at) != 3 or dtype is None or at[2] != D:
         raise ValueError(f"cache must be fp32 or bf16 [pages, page_size, {D}]")
-    if page_table.dim() != 2:
+    if len(table) != 2 or page_table.dtype != torch.int32:
         raise ValueError("page_table must be int32 [sequences, pages]")
-    _check_positions("page_table", page_table, page_table.shape)
-    _check_positions("lengths", lengths, page_table.shape[:1])
-    return page_table.shape[0]
+    batch, width = table
+    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.numel() != batch:
+        raise ValueError(f"lengths must be int32 ({batch},)")
+    return batch, (at[1], at[0], width, dtype)
 
 
 def latent_append(latent, k_rope, cache, page_table, lengths, *, cu_seqlens=None, frequencies=None,
@@ -154,15 +174,16 @@ def latent_append(latent, k_rope, cache, page_table, lengths, *, cu_seqlens=None
     """
     if stream is not None:
         return _on_stream(latent_append, locals())
-    dense = cu_seqlens is None
-    if latent.dim() != (3 if dense else 2) or latent.dtype != cache.dtype:
+    shape, dense = latent.shape, cu_seqlens is None
+    if len(shape) != (3 if dense else 2) or latent.dtype != cache.dtype:
         raise ValueError(f"latent must be {'[B, n, d_c]' if dense else '[tokens, d_c]'} of the cache's dtype")
-    if k_rope is not None and (k_rope.shape[:-1] != latent.shape[:-1] or k_rope.dtype != cache.dtype):
+    n, d_c = shape[-2], shape[-1]
+    d_r = k_rope.shape[-1] if k_rope is not None else 0
+    if k_rope is not None and (k_rope.shape != ((shape[0], n, d_r) if dense else (n, d_r)) or k_rope.dtype != cache.dtype):
         raise ValueError("k_rope must have latent's tokens and dtype")
-    d_c, d_r = latent.shape[-1], k_rope.shape[-1] if k_rope is not None else 0
-    batch = _check_paged(cache, page_table, lengths, d_c + d_r)
-    if dense and latent.shape[0] != batch:
-        raise ValueError(f"latent has {latent.shape[0]} sequences, the page table {batch}")
+    batch, paged = _check_paged(cache, page_table, lengths, d_c + d_r)
+    if dense and shape[0] != batch:
+        raise ValueError(f"latent has {shape[0]} sequences, the page table {batch}")
     if not dense:
         _check_positions("cu_seqlens", cu_seqlens, (batch + 1,))
     if frequencies is not None:
@@ -171,15 +192,14 @@ def latent_append(latent, k_rope, cache, page_table, lengths, *, cu_seqlens=None
             raise ValueError(f"{frequencies.numel()} frequencies for a rotary key of {d_r}")
     if norm_scale is not None and (norm_scale.shape != (d_c,) or norm_scale.dtype != torch.float32):
         raise ValueError(f"norm_scale must be fp32 ({d_c},)")
-    latent_stride = _strides("latent", latent, heads=False)[0]
-    k_rope_stride = _strides("k_rope", k_rope, heads=False)[0] if d_r else 0
+    rows = batch if dense else None
+    latent_stride, k_rope_stride = _token_stride("latent", latent, rows, n), _token_stride("k_rope", k_rope, rows, n) if d_r else 0
     here = _here()
-    a = _abi.LatentAppendArgs(
-        batch, _count(latent.shape[-2]), d_c, d_r, cache.shape[1], cache.shape[0], page_table.shape[1], _DTYPES[cache.dtype],
-        interleaved, magnitude, eps, latent_stride, k_rope_stride, _view(latent, here), _view(k_rope, here),
-        _dense(cu_seqlens, here), _dense(lengths, here), _dense(page_table, here), _dense(frequencies, here),
-        _dense(norm_scale, here), _dense(cache, here))
-    _abi.check(_abi.lib().rhz_latent_append(byref(a), _stream(here)))
+    a = _abi.pack_latent_append(
+        batch, _count(n), d_c, d_r, *paged, interleaved, magnitude, eps, latent_stride, k_rope_stride, _view(latent, here),
+        _view(k_rope, here), _dense(cu_seqlens, here), _dense(lengths, here), _dense(page_table, here),
+        _dense(frequencies, here), _dense(norm_scale, here), _dense(cache, here))
+    _abi.check(_abi.lib().rhz_latent_append(a, _stream(here)))
     return cache
 
 
@@ -194,62 +214,61 @@ def latent_decode(q, cache, page_table, lengths, *, d_c: int, scale: float, out=
     """
     if stream is not None:
         return _on_stream(latent_decode, locals())
-    if q.dim() != 4 or q.dtype != cache.dtype:
+    shape = q.shape
+    if len(shape) != 4 or q.dtype != cache.dtype:
         raise ValueError("q must be [B, n, H, d_c + d_r] of the cache's dtype")
-    batch = _check_paged(cache, page_table, lengths, q.shape[-1])
-    if q.shape[0] != batch or not 0 < d_c <= q.shape[-1]:
-        raise ValueError(f"q is of {q.shape[0]} sequences and {q.shape[-1]} channels, the page table of {batch}, d_c is {d_c}")
-    want = (*q.shape[:-1], d_c)
-    o = out if out is not None else _empty(q, want)
+    rows, steps, H, D = shape
+    batch, paged = _check_paged(cache, page_table, lengths, D)
+    if rows != batch or not 0 < d_c <= D:
+        raise ValueError(f"q is of {rows} sequences and {D} channels, the page table of {batch}, d_c is {d_c}")
+    want = (batch, steps, H, d_c)
+    o = out if out is not None else q.new_empty(want)
     if o.shape != want or o.dtype != q.dtype:
         raise ValueError(f"out must be {q.dtype} {want}")
-    here = _here()
-    lse = _empty(q, want[:-1], torch.float32)
-    a = _abi.LatentDecodeArgs(
-        batch, want[1], want[2], d_c, q.shape[-1] - d_c, cache.shape[1], cache.shape[0], page_table.shape[1], _DTYPES[q.dtype],
-        scale, _dense(q, here), _dense(cache, here), _dense(page_table, here), _dense(lengths, here), _dense(o, here),
-        _dense(lse, here))
-    workspace = _workspace(q, a, _abi.lib().rhz_latent_decode_workspace_size, workspace)
-    _view(workspace, here)
-    _abi.check(_abi.lib().rhz_latent_decode(byref(a), _stream(here)))
+    here, L = _here(), _abi.lib()
+    lse = q.new_empty((batch, steps, H), dtype=torch.float32)
+    args = (batch, steps, H, d_c, D - d_c, *paged, scale, _dense(q, here), _dense(cache, here), _dense(page_table, here),
+            _dense(lengths, here), _dense(o, here), _view(lse, here))
+    at, size, workspace = _workspace(L.rhz_latent_decode_workspace_size, _abi.pack_latent_decode(*args, 0, 0), q, workspace, here)
+    _abi.check(L.rhz_latent_decode(_abi.pack_latent_decode(*args, at, size), _stream(here)))
     return o, lse
 
 
-def _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k) -> _abi.LatentPrefillArgs:
-    """Check the shapes and fill in sizes and strides; _prefill_pointers does the rest."""
-    nd = 4 if cu_seqlens is None else 3
-    if q.dim() != nd or k.dim() != nd or v.dim() != nd:
+def _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k):
+    """Check the shapes; (the argument struct's sizes and strides, the shapes of the queries' rows and of their outputs)."""
+    qs, ks, vs, nd = q.shape, k.shape, v.shape, 4 if cu_seqlens is None else 3
+    if len(qs) != nd or len(ks) != nd or len(vs) != nd:
         raise ValueError("q, k and v must be [B, T, H, d], or [tokens, H, d] with cu_seqlens")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k, v must share one dtype, fp32 or bf16")
-    H, d_n, d_v = q.shape[-2], k.shape[-1], v.shape[-1]
-    d_r = q.shape[-1] - d_n
-    if v.shape[:-1] != k.shape[:-1] or k.shape[-2] != H or d_r < 0:
-        raise ValueError(f"q/k/v shapes {tuple(q.shape)} {tuple(k.shape)} {tuple(v.shape)} do not match")
-    if (k_rope is None) != (d_r == 0):
-        raise ValueError(f"q has {d_r} channels more than k: k_rope must have them, or be None for none")
-    if k_rope is not None and (k_rope.shape != (*k.shape[:-2], d_r) or k_rope.dtype != q.dtype):
-        raise ValueError(f"k_rope must be {q.dtype} {(*k.shape[:-2], d_r)}")
     if cu_seqlens is None:
         if cu_seqlens_k is not None:
             raise ValueError("cu_seqlens_k without cu_seqlens")
-        if k.shape[0] != q.shape[0]:
+        (batch, n_q, H, d_q), (batch_k, n_k, H_k, d_n), d_v = qs, ks, vs[3]
+        if batch_k != batch:
             raise ValueError("q and k must have the same batch")
-        batch, seq_len, seq_len_k = q.shape[0], q.shape[1], k.shape[1]
+        spread, rows = batch, (batch, n_q, H)
     else:
+        (n_q, H, d_q), (n_k, H_k, d_n), d_v = qs, ks, vs[2]
         _check_positions("cu_seqlens", cu_seqlens, cu_seqlens.shape)
         if cu_seqlens_k is not None:
             _check_positions("cu_seqlens_k", cu_seqlens_k, cu_seqlens.shape)
-        batch, seq_len, seq_len_k = cu_seqlens.numel() - 1, _count(q.shape[0]), _count(k.shape[0])
-    return _abi.LatentPrefillArgs(
-        batch, seq_len, seq_len_k, H, d_n, d_r, d_v, _DTYPES[q.dtype], causal, q.shape[-1] ** -0.5 if scale is None else scale,
-        *_strides("q", q), *_strides("k", k), *_strides("v", v), _strides("k_rope", k_rope, heads=False)[0] if d_r else 0)
-
-
-def _prefill_pointers(a, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse):
-    a.q, a.k, a.v, a.k_rope = _view(q, here), _view(k, here), _view(v, here), _view(k_rope, here)
-    a.cu_seqlens, a.cu_seqlens_k = _dense(cu_seqlens, here), _dense(cu_seqlens_k, here)
-    a.o, a.lse = _dense(o, here), _dense(lse, here)
+        batch, spread, rows = cu_seqlens.numel() - 1, None, (n_q, H)
+    d_r = d_q - d_n
+    if vs[:-1] != ks[:-1] or H_k != H or d_r < 0:
+        raise ValueError(f"q/k/v shapes {tuple(qs)} {tuple(ks)} {tuple(vs)} do not match")
+    if (k_rope is None) != (d_r == 0):
+        raise ValueError(f"q has {d_r} channels more than k: k_rope must have them, or be None for none")
+    if k_rope is not None and (k_rope.shape != (*ks[:-2], d_r) or k_rope.dtype != q.dtype):
+        raise ValueError(f"k_rope must be {q.dtype} {(*ks[:-2], d_r)}")
+    one = H == 1  # whose distance to a next one is nothing's
+    sizes = (batch, _count(n_q), _count(n_k), H, d_n, d_r, d_v, dtype, causal, d_q ** -0.5 if scale is None else scale,
+             _token_stride("q", q, spread, n_q), 0 if one else q.stride(-2),
+             _token_stride("k", k, spread, n_k), 0 if one else k.stride(-2),
+             _token_stride("v", v, spread, n_k), 0 if one else v.stride(-2),
+             _token_stride("k_rope", k_rope, spread, n_k) if d_r else 0)
+    return sizes, rows, (*rows, d_v)
 
 
 def latent_prefill(q, k, v, k_rope=None, *, scale=None, causal: bool = True, cu_seqlens=None, cu_seqlens_k=None,
@@ -264,15 +283,15 @@ def latent_prefill(q, k, v, k_rope=None, *, scale=None, causal: bool = True, cu_
     """
     if stream is not None:
         return _on_stream(latent_prefill, locals())
-    a = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
-    want = (*q.shape[:-1], v.shape[-1])
-    o = out if out is not None else _empty(q, want)
+    sizes, rows, want = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
+    o = out if out is not None else q.new_empty(want)
     if o.shape != want or o.dtype != q.dtype:
         raise ValueError(f"out must be {q.dtype} {want}")
-    lse = _empty(q, want[:-1], torch.float32)
+    lse = q.new_empty(rows, dtype=torch.float32)
     here = _here()
-    _prefill_pointers(a, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse)
-    _abi.check(_abi.lib().rhz_latent_prefill(byref(a), _stream(here)))
+    a = _abi.pack_latent_prefill(*sizes, _view(q, here), _view(k, here), _view(v, here), _view(k_rope, here),
+                                 _dense(cu_seqlens, here), _dense(cu_seqlens_k, here), _dense(o, here), _view(lse, here))
+    _abi.check(_abi.lib().rhz_latent_prefill(a, _stream(here)))
     return o, lse
 
 
@@ -287,22 +306,20 @@ def latent_prefill_backward(q, k, v, k_rope, o, lse, do, *, dlse=None, scale=Non
     """
     if stream is not None:
         return _on_stream(latent_prefill_backward, locals())
-    a = _abi.LatentPrefillBackwardArgs()
-    a.forward = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
-    want = (*q.shape[:-1], v.shape[-1])
+    sizes, rows, want = _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k)
     for name, t in (("o", o), ("do", do)):
         if t.shape != want or t.dtype != q.dtype:
             raise ValueError(f"{name} must be {q.dtype} {want}")
     for name, t in (("lse", lse), ("dlse", dlse)):
-        if t is not None and (t.shape != q.shape[:-1] or t.dtype != torch.float32):
-            raise ValueError(f"{name} must be fp32 {tuple(q.shape[:-1])}")
-    here = _here()
-    _prefill_pointers(a.forward, here, q, k, v, k_rope, cu_seqlens, cu_seqlens_k, o, lse)
-    dq, dk, dv = _empty(q, q.shape), _empty(k, k.shape), _empty(v, v.shape)
-    dr = _empty(k_rope, k_rope.shape) if k_rope is not None else None
-    a.grad_o, a.grad_lse = _dense(do, here), _dense(dlse, here)
-    a.grad_q, a.grad_k, a.grad_v, a.grad_k_rope = _view(dq, here), _view(dk, here), _view(dv, here), _view(dr, here)
-    workspace = _workspace(q, a, _abi.lib().rhz_latent_prefill_backward_workspace_size, workspace)
-    _view(workspace, here)
-    _abi.check(_abi.lib().rhz_latent_prefill_backward(byref(a), _stream(here)))
+        if t is not None and (t.shape != rows or t.dtype != torch.float32):
+            raise ValueError(f"{name} must be fp32 {rows}")
+    here, L = _here(), _abi.lib()
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dr = k_rope.new_empty(k_rope.shape) if k_rope is not None else None
+    args = (*sizes, _view(q, here), _view(k, here), _view(v, here), _view(k_rope, here), _dense(cu_seqlens, here),
+            _dense(cu_seqlens_k, here), _dense(o, here), _dense(lse, here), _dense(do, here), _dense(dlse, here),
+            _view(dq, here), _view(dk, here), _view(dv, here), _view(dr, here))
+    at, size, workspace = _workspace(L.rhz_latent_prefill_backward_workspace_size,
+                                     _abi.pack_latent_prefill_backward(*args, 0, 0), q, workspace, here)
+    _abi.check(L.rhz_latent_prefill_backward(_abi.pack_latent_prefill_backward(*args, at, size), _stream(here)))
     return dq, dk, dv, dr
