@@ -46,10 +46,10 @@ constexpr int kMixed = 4;
 // quarters, so that a place stays empty until its turn comes: kMixed heads' tiles
 // of one number, which take about as long, follow one another.
 template <typename PARAMS>
-__device__ __forceinline__ bool place(const PARAMS& a, const int* cu, int total, int size, int lane, int& head, int& seq,
-                                      int& tile) {
+__device__ __forceinline__ bool place(const PARAMS& a, unsigned block, const int* cu, int total, int size, int lane, int& head,
+                                      int& seq, int& tile) {
     const int units = a.heads * (cu ? 1 : a.batch);
-    const int xcd = blockIdx.x & 7, n = blockIdx.x >> 3;
+    const int xcd = block & 7, n = block >> 3;
     const int here = (units - xcd + 7) >> 3;  // units of this XCD
     const int group = n / (kMixed * a.tiles), mixed = min(kMixed, here - group * kMixed);
     if (mixed <= 0) return false;

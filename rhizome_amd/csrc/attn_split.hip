@@ -4,8 +4,13 @@
 // through a sequence is long and the tiles' traffic small against it.  A
 // workgroup therefore has 32 rows only, and its four waves share the other
 // side: each has all 32 rows on every fourth tile, with a tile of LDS of its own
-// and no barrier, and their sums are added in order at the end (2 x 1003 tokens,
-// 8 heads of 64 + 32: see the table of the design notes for both).
+// and no barrier, and their sums are added in order at the end.  Against 32 rows
+// on each of four waves that share the tiles, as the bf16 kernels have it (2 x 2048
+// tokens, 16 heads of 64 + 32 channels): 355 -> 213 us for the prefill, 100 of the
+// 154 TFLOP/s of a large matrix product, 1205 -> 718 for the backward pass; and of
+// few rows, 513, 1, 190 and 1003 tokens, 8 heads, 103 -> 42 us.
+#include <algorithm>
+
 #include "attn_params.hpp"
 
 namespace rhz {
@@ -56,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
+    if (!place(a, blockIdx.x, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kRows >= w.nq) return;
     const int first = ((w.nq - 1) / kRows - tile) * kRows;  // the queries with the most keys go first
@@ -179,15 +184,14 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
 
 // -------------------------------------------------------------------- dk, dv
 template <int DQ, int DV, bool VEC>
-__global__ __launch_bounds__(kThreads) void attn_dkv_split_kernel(BackwardParams a) {
+__device__ __forceinline__ void dkv(const BackwardParams& a, unsigned block, WaveTiles<DQ, DV> (&tiles)[kWaves]) {
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32, VT = DV / 32;
     using TileQ = Tile<T, DQ, kTile>;
     using TileO = Tile<T, DV, kTile>;
-    __shared__ WaveTiles<DQ, DV> tiles[kWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
+    if (!place(a, block, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int first = tile * kRows;
     if (first >= w.nk) return;
@@ -322,15 +326,14 @@ __global__ __launch_bounds__(kThreads) void attn_dkv_split_kernel(BackwardParams
 
 // ------------------------------------------------------------------------ dq
 template <int DQ, int DV, bool VEC>
-__global__ __launch_bounds__(kThreads) void attn_dq_split_kernel(BackwardParams a) {
+__device__ __forceinline__ void dq(const BackwardParams& a, unsigned block, WaveTiles<DQ, DV> (&tiles)[kWaves]) {
     constexpr int QC = DQ / (2 * E), VC = DV / (2 * E), QT = DQ / 32;
     using TileK = Tile<T, DQ, kTile>;
     using TileV = Tile<T, DV, kTile>;
-    __shared__ WaveTiles<DQ, DV> tiles[kWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
+    if (!place(a, block, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kRows >= w.nq) return;
     const int first = ((w.nq - 1) / kRows - tile) * kRows;
@@ -424,6 +427,30 @@ __global__ __launch_bounds__(kThreads) void attn_dq_split_kernel(BackwardParams 
     }
 }
 
+// One launch of both, dk and dv first, so that neither ends on a card half empty:
+// 64 + 32 channels, 1080 tokens of 8 heads 68 -> 52 us, 2 x 2048 of 16 heads 792
+// -> 724, at two workgroups a CU.  Wider ones have the LDS for one only, and each
+// kernel then is faster by itself: 128 + 64 channels, 1631 us against 1694 in one.
+template <int DQ, int DV, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void attn_backward_split_kernel(BackwardParams a) {
+    __shared__ WaveTiles<DQ, DV> tiles[kWaves];
+    const unsigned half = gridDim.x / 2;
+    if (blockIdx.x < half)
+        dkv<DQ, DV, VEC>(a, blockIdx.x, tiles);
+    else
+        dq<DQ, DV, VEC>(a, blockIdx.x - half, tiles);
+}
+template <int DQ, int DV, bool VEC>
+__global__ __launch_bounds__(kThreads) void attn_dkv_split_kernel(BackwardParams a) {
+    __shared__ WaveTiles<DQ, DV> tiles[kWaves];
+    dkv<DQ, DV, VEC>(a, blockIdx.x, tiles);
+}
+template <int DQ, int DV, bool VEC>
+__global__ __launch_bounds__(kThreads) void attn_dq_split_kernel(BackwardParams a) {
+    __shared__ WaveTiles<DQ, DV> tiles[kWaves];
+    dq<DQ, DV, VEC>(a, blockIdx.x, tiles);
+}
+
 template <int DQ, int DV, bool VEC>
 hipError_t prefill(PrefillParams p, hipStream_t stream) {
     const int64_t queries = p.cu_q ? (int64_t)p.len_q : (int64_t)p.batch * p.len_q;
@@ -439,19 +466,21 @@ template <int DQ, int DV, bool VEC>
 hipError_t backward(BackwardParams p, hipStream_t stream) {
     const int64_t tq = attn_tiles(p.cu_q, p.queries, p.len_q, p.batch, kRows);
     const int64_t tk = attn_tiles(p.cu_k, p.keys, p.len_k, p.batch, kRows);
-    if (p.keys) {
-        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_k, tk);
+    if constexpr (DQ <= 96 && DV <= 64) {
+        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, 2 * std::max(tq, tk));
         if (!blocks) return hipErrorInvalidConfiguration;
+        p.tiles = (int)std::max(tq, tk);
+        attn_backward_split_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
+        return hipGetLastError();
+    } else {
+        const unsigned dkv = attn_blocks(p.heads, p.batch, p.cu_k, tk), dq = attn_blocks(p.heads, p.batch, p.cu_q, tq);
+        if ((p.keys && !dkv) || (p.queries && !dq)) return hipErrorInvalidConfiguration;
         p.tiles = (int)tk;
-        attn_dkv_split_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
-    }
-    if (p.queries) {
-        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, tq);
-        if (!blocks) return hipErrorInvalidConfiguration;
+        if (p.keys) attn_dkv_split_kernel<DQ, DV, VEC><<<dkv, kThreads, 0, stream>>>(p);
         p.tiles = (int)tq;
-        attn_dq_split_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
+        if (p.queries) attn_dq_split_kernel<DQ, DV, VEC><<<dq, kThreads, 0, stream>>>(p);
+        return hipGetLastError();
     }
-    return hipGetLastError();
 }
 
 }  // namespace
