@@ -36,16 +36,19 @@ constexpr int kMaxSplits = 128, kMinSplit = 128, kBestSplit = 512, kUnit = 32;
 // Cached rows of a split of a sequence of n rows: eighths of a short one, for
 // one request's latency, but of a long one as many as keep the parts' traffic
 // low against the cache's own (at 16 heads a part is written and read again for
-// 32 KB each against 1152 bytes a row).
+// 32 KB each against 1152 bytes a row).  Eighths of 64, 128, 256 rows at least: one
+// sequence of 517 positions 15.1, 15.3, 18.0 us.  Of 256, 512, 1024 at most: one of
+// 16384 - / 25 / 37 us, eight of them - / 38 / 46, 64 of 2048 to 6084 97 / 87 / 76
+// (where the splits of 512 are a few more than the card has places).
 __host__ __device__ inline int split_rows(int n) {
-    const int eighth = min(max(n / 8, kMinSplit), kBestSplit), even = max(eighth, n / kMaxSplits + (n % kMaxSplits != 0));
+    const int eighth = min(max((n + 7) / 8, kMinSplit), kBestSplit), even = max(eighth, n / kMaxSplits + (n % kMaxSplits != 0));
     return (even + kUnit - 1) / kUnit * kUnit;
 }
 __host__ __device__ inline int splits_of(int n) { return n <= 0 ? 1 : (n + split_rows(n) - 1) / split_rows(n); }
-// No sequence of up to n rows has more: of eighths there are nine at most.
+// No sequence of up to n rows has more.
 inline int most_splits_of(int64_t n) {
     const int64_t shortest = (n + kMinSplit - 1) / kMinSplit, best = (n + kBestSplit - 1) / kBestSplit;
-    return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(9, std::min<int64_t>(best, kMaxSplits))));
+    return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(8, std::min<int64_t>(best, kMaxSplits))));
 }
 
 constexpr int64_t kMostRows = INT32_MAX - 4096;  // numbers of tiles' rows behind the last stay in 32 bits
@@ -60,10 +63,14 @@ struct Unit {
     int seq, split, splits, first_row, begin, end, n, length;
 };
 // The row tiles of a split follow one another on one XCD, whose L2 has the rows.
+// First splits of all sequences come first: those that a sequence is too short to
+// have are behind the others, where their workgroups, which end at once, do not
+// disturb their distribution over the CUs (32 x 4096 positions, 128 rows: 73 us, and
+// 113 with every ninth workgroup such a one).
 __device__ __forceinline__ bool unit_of(const DecodeParams& a, int tile_rows, Unit& u) {
     const int k = blockIdx.x >> 3, unit = k / a.row_tiles * 8 + (blockIdx.x & 7);
     if (unit >= a.batch * a.splits) return false;
-    u.seq = unit / a.splits, u.split = unit % a.splits, u.first_row = k % a.row_tiles * tile_rows;
+    u.seq = unit % a.batch, u.split = unit / a.batch, u.first_row = k % a.row_tiles * tile_rows;
     u.length = a.lengths[u.seq];
     u.n = rows_of(a, u.seq);
     u.splits = splits_of(u.n);
@@ -138,10 +145,17 @@ __device__ __forceinline__ void load_panels(const void* p, int left, int row_byt
 }
 
 // ------------------------------------------------------- many rows, or fp32
-// Eight waves, 32 RT rows of q, tiles of 32 cached rows.  Wave w has row tile w
-// % RT, and of it a part of the columns.  Of a tile it sums q . k over its part;
-// the parts meet in LDS, and every wave of a row tile adds them up, takes the
-// softmax -- all of them the same -- and sums its part of the columns with it.
+// Eight waves, 32 RT rows of q, tiles of 32 cached rows.  8 / RT waves share a row
+// tile, each with a part of the columns.  Of a tile a wave sums q . k over its
+// part; the parts meet in LDS, and every wave of a row tile adds them up, takes the
+// softmax -- all of them the same -- and sums its part of the columns with it.  In
+// bf16 the second half of the row tiles is half a tile behind the first: between
+// two barriers one wave of a SIMD multiplies queries and keys while the other is at
+// the softmax and the sums (16 x 4096 positions at 128 rows 64 -> 59 us against all
+// in step, at 256 rows 130 -> 114).  What bounds it is the loads, 2.2 to 2.6 us for
+// the 36 KB of a tile on each CU with two tiles on their way, 3.7 to 4.3 TB/s: LDS
+// has no room for a fourth, and reading the sums' columns ahead of the products
+// changes nothing.
 template <typename T, int VD, int RT, bool VEC>
 __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     constexpr int E = kChunkElems<T>, KD = VD + 64, BUFS = sizeof(T) == 2 ? 3 : 1, NT = 512, WAVES = 8, KEYS = 32;
@@ -162,7 +176,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     if (!unit_of(a, 32 * RT, u)) return;
     const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
 
-    const int part = wave / RT, mine = wave % RT;
+    const int part = wave % PARTS, mine = wave / PARTS;
     u32x4 q[KEPT];
     {
         const Rows<T> qrows = {(const T*)a.q, (const T*)a.q, a.D, 0, a.D, 0};
@@ -221,60 +235,42 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     const int tiles_n = (end - begin + KEYS - 1) / KEYS;
     // whether a tile's loads are as many as the waits below count
     const bool counted = VEC && (a.D + 8 * E - 1) / (8 * E) == TILE::kPanels;
-    if constexpr (BUFS == 3) {
-        if (tiles_n > 0) start(begin, 0);
-        if (tiles_n > 1) start(begin + KEYS, 1);
-    }
-    for (int i = 0, b = 0; i < tiles_n; ++i, b = b + 1 == BUFS ? 0 : b + 1) {
-        const int j0 = begin + i * KEYS, ahead = i + BUFS - 1;
-        if (BUFS == 3 && counted && i + 1 < tiles_n) {
-            if (my_panel == 0)
-                wait_loads<(TILE::kPanels + 1) / 2>();
-            else
-                wait_loads<TILE::kPanels / 2>();
-            lds_barrier();
-        } else {
-            landed();
-        }
-        if (ahead < tiles_n) {
-            if (ahead * KEYS % kTable == 0 && ahead > 0) {
-                fill_table(begin + ahead * KEYS);
-                __syncthreads();
-            }
-            start(begin + ahead * KEYS, BUFS == 1 ? 0 : b == 0 ? BUFS - 1 : b - 1);
-        }
-        if constexpr (BUFS == 1) landed();
-        const uint32_t tile = lds_offset(&tiles[b]);
+    // The wave's part of tile i's scores, to LDS.
+    const auto score = [&](int i) {
+        const uint32_t tile = lds_offset(&tiles[i % BUFS]);
         f32x16 s = {};
-        {
-            // reads ahead of the products, whatever the scheduler would have
-            constexpr int AHEAD = QP < 4 ? QP : 4;
-            u32x4 x[AHEAD];
-            const auto read = [&](int k) {
-                const int pair = part * QP + k;
-                return lds_read<u32x4>(((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes);
-            };
+        // reads ahead of the products, whatever the scheduler would have
+        constexpr int AHEAD = QP < 4 ? QP : 4;
+        u32x4 x[AHEAD];
+        const auto read = [&](int k) {
+            const int pair = part * QP + k;
+            return lds_read<u32x4>(((tile + at.row) ^ (((2 * pair) & 7) << 4)) + (pair >> 2) * TILE::kPanelBytes);
+        };
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) x[k] = read(k);
+        for (int k = 0; k < AHEAD; ++k) x[k] = read(k);
 #pragma unroll
-            for (int k = 0; k < QP; ++k) {
-                dot_chunks(s, x[k % AHEAD], k < KEPT ? q[k < KEPT ? k : 0] : q_rest[wave][lane], T());
-                if (k + AHEAD < QP) x[k % AHEAD] = read(k + AHEAD);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int k = 0; k < QP; ++k) {
+            dot_chunks(s, x[k % AHEAD], k < KEPT ? q[k < KEPT ? k : 0] : q_rest[wave][lane], T());
+            if (k + AHEAD < QP) x[k % AHEAD] = read(k + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) scores[wave][k][lane] = f32x4{s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]};
-        lds_barrier();
+    };
+    // All parts of tile i's scores, their softmax, and the wave's columns of the sum.
+    const auto sum = [&](int i) {
+        const uint32_t tile = lds_offset(&tiles[i % BUFS]);
+        const int j0 = begin + i * KEYS;
+        f32x16 s;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            f32x4 x = scores[mine][k][lane];
+            f32x4 x = scores[mine * PARTS][k][lane];
 #pragma unroll
-            for (int v = 1; v < PARTS; ++v) x += scores[mine + RT * v][k][lane];
+            for (int v = 1; v < PARTS; ++v) x += scores[mine * PARTS + v][k][lane];
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * k + e] = x[e];
         }
-        const uint32_t in = __builtin_amdgcn_readfirstlane(there[b]);
+        const uint32_t in = __builtin_amdgcn_readfirstlane(there[i % BUFS]);
         if (j0 + KEYS > min(end, least_seen) || in != ~0u) {
             const int seen = min(end, sees(a, u, min(u.first_row + 32 * mine + (lane & 31), rows - 1))) - j0 - 4 * g;
             const uint32_t mine_in = in >> (4 * g);
@@ -304,7 +300,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
             s[k] = __builtin_amdgcn_exp2f(fmaf(s[k], c, -mc));
             l += s[k];
         }
-        if (!sums) continue;
+        if (!sums) return;
         Weights<T> p;
         p.set(s);
         __builtin_amdgcn_sched_barrier(0);
@@ -313,6 +309,64 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
             Columns<T> x;
             x.template load<TILE>(tile, at, 0, part * VTW + d);
             sum_rows(o[d], x, p);
+        }
+    };
+    if constexpr (BUFS == 3) {
+        if (tiles_n > 0) start(begin, 0);
+        if (tiles_n > 1) start(begin + KEYS, 1);
+        // Tile i has landed for all, while the next may be on its way.
+        const auto arrive = [&](int i) {
+            if (counted && i + 1 < tiles_n) {
+                if (my_panel == 0)
+                    wait_loads<(TILE::kPanels + 1) / 2>();
+                else
+                    wait_loads<TILE::kPanels / 2>();
+            } else {
+                wait_loads<0>();
+            }
+            lds_barrier();
+        };
+        // Tile i - 1 has been read by all: its place takes the next but one.
+        const auto leave = [&](int i) {
+            lds_barrier();
+            if (i + 2 >= tiles_n) return;
+            if ((i + 2) * KEYS % kTable == 0) {
+                fill_table(begin + (i + 2) * KEYS);
+                __syncthreads();
+            }
+            start(begin + (i + 2) * KEYS, (i + 2) % BUFS);
+        };
+        // both kinds of waves meet 2 tiles_n + 1 barriers
+        if (tiles_n > 0 && mine < RT / 2) {
+            for (int i = 0; i < tiles_n; ++i) {
+                arrive(i);
+                score(i);
+                leave(i);
+                sum(i);
+            }
+            lds_barrier();
+        } else if (tiles_n > 0) {
+            arrive(0);
+            leave(0);
+            for (int i = 0; i < tiles_n; ++i) {
+                score(i);
+                arrive(i + 1);
+                sum(i);
+                if (i + 1 < tiles_n) leave(i + 1);
+            }
+        }
+    } else {
+        for (int i = 0; i < tiles_n; ++i) {
+            if (i * KEYS % kTable == 0 && i > 0) {
+                __syncthreads();
+                fill_table(begin + i * KEYS);
+            }
+            __syncthreads();
+            start(begin + i * KEYS, 0);
+            landed();
+            score(i);
+            lds_barrier();
+            sum(i);
         }
     }
     l = sum_of_halves(l);
@@ -343,7 +397,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     }
 }
 
-// --------------------------------------------------- up to 16 rows, in bf16
+// ----------------------------------------- 16 rows a workgroup, up to 32, in bf16
 // Four waves, each with cached rows of its own -- every fourth tile of 16 -- and
 // a part of LDS for one tile, so that they need no barrier before their sums meet
 // at the end.  On 16x16 matrix instructions: the scores come out with the lane's
@@ -665,15 +719,18 @@ hipError_t launch_narrow(DecodeParams p, hipStream_t stream) {
     return join(p, RHZ_BF16, stream);
 }
 
+// By the rows of q of a sequence.  bf16, 32 sequences of 4096 positions, by the
+// kernel of 16 rows, of 64, of 128: at 32 rows 42 / 49 / - us, at 64 68 / 54 / 69,
+// at 96 94 / 93 / 66, at 128 119 / 95 / 72.  fp32, 16 sequences, by tiles of 32 or
+// 64 rows: at 32 rows 116 / 173, at 64 121 / 178, so that all have 32.
 template <typename T, int VD>
 hipError_t pick_rows(const DecodeParams& p, bool vec, hipStream_t stream) {
-    const int rows = p.steps * p.heads;
     if constexpr (sizeof(T) == 4) {
-        if (!vec) return launch<T, VD, 1, false>(p, stream);
-        return rows <= 32 ? launch<T, VD, 1, true>(p, stream) : launch<T, VD, 2, true>(p, stream);
+        return vec ? launch<T, VD, 1, true>(p, stream) : launch<T, VD, 1, false>(p, stream);
     } else {
+        const int rows = p.steps * p.heads;
         if (!vec) return launch<T, VD, 2, false>(p, stream);
-        if (rows <= 16) return launch_narrow<VD>(p, stream);
+        if (rows <= 32) return launch_narrow<VD>(p, stream);
         return rows <= 64 ? launch<T, VD, 2, true>(p, stream) : launch<T, VD, 4, true>(p, stream);
     }
 }
