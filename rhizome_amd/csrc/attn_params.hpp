@@ -44,7 +44,9 @@ constexpr int kMixed = 4;
 // offsets are `cu`; false if there is none.  A head's workgroups are on one XCD,
 // whose L2 keeps what they all read.  There they start in order, by turns on its
 // quarters, so that a place stays empty until its turn comes: kMixed heads' tiles
-// of one number, which take about as long, follow one another.
+// of one number, which take about as long, follow one another.  2 x 4096 tokens, 32
+// heads, by 1, 2, 4 and 8 of them: prefill 411, 386, 374, 375 us, backward 1487,
+// 1432, 1402, 1411.
 template <typename PARAMS>
 __device__ __forceinline__ bool place(const PARAMS& a, unsigned block, const int* cu, int total, int size, int lane, int& head,
                                       int& seq, int& tile) {

@@ -8,6 +8,16 @@
 // with c = scale log2 e.  The maximum is only raised, and O and l rescaled,
 // where a tile's exceeds it by 2^8 or more: p then is at most 2^8, which costs
 // neither fp32 sums nor bf16 weights any digits.
+//
+// Tiles of 64 keys, twice, take 80 KB at 192 + 128 channels, so that two
+// workgroups share a CU and one's products run beside the other's softmax.
+// 2 x 4096 tokens, 32 heads of 128 + 64 channels, causal: 364 us, 944 TFLOP/s of
+// the two products' 344 GF, against 298 us at the 1152 TFLOP/s of a large matrix
+// product.  What bounds it: matrix instructions take 42 % of the time and the
+// vector unit 36 % (the exponentials above all); without the loads and their
+// barriers it would still be 322 us.  Measured at 371 us for this shape and not
+// better: S of the next tile ahead of the softmax within a wave 385, eight waves a
+// workgroup 382, loads spread over the products 391, tile loads behind S 392.
 #include "attn_params.hpp"
 
 namespace rhz {
@@ -151,6 +161,11 @@ hipError_t launch(PrefillParams p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// The narrowest kernel that holds the channels.  2 x 4096 tokens, 16 heads, by the
+// kernels for (64, 64), (96, 64), (128, 128) and (192, 128) channels of keys and
+// values: of 64 and 64 104 / - / 164 / 187 us, of 96 and 64 - / 115 / 150 / 169, of
+// 128 and 128 - / - / 162 / 184.  Not vec, values are loaded one by one and tiles
+// written by the threads: 526 us instead of 115 at 96 and 64.
 hipError_t pick(const PrefillParams& p, bool vec, hipStream_t stream) {
     const int dq = p.d_n + p.d_r;
     if (!vec) return dq <= 64 && p.d_v <= 64 ? launch<64, 64, false>(p, stream) : launch<192, 128, false>(p, stream);

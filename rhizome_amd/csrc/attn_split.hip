@@ -485,6 +485,10 @@ hipError_t backward(BackwardParams p, hipStream_t stream) {
 
 }  // namespace
 
+// The narrowest kernel that holds the channels: 2 x 4096 tokens, 16 heads, prefill,
+// by the kernels for (64, 64), (96, 64), (128, 128) and (192, 128) channels: of 64
+// and 64 643 / - / 1703 / 2168 us, of 96 and 64 - / 779 / 1709 / 2172, of 128 and
+// 128 - / - / 1495 / 2058.
 hipError_t launch_prefill_split(PrefillParams p, bool vec, hipStream_t stream) {
     const int dq = p.d_n + p.d_r;
     if (!vec) return dq <= 64 && p.d_v <= 64 ? prefill<64, 64, false>(p, stream) : prefill<192, 128, false>(p, stream);
