@@ -328,3 +328,56 @@ def test_python_refusals(call, message):
     i = lambda *shape: torch.zeros(shape, dtype=torch.int32)
     with pytest.raises((ValueError, RuntimeError), match=message):
         call(t, i)
+
+
+def test_rust_bindings_agree():
+    """The Rust declarations written out for maintainers have the header's constants, fields and parameters."""
+    import re
+
+    import test_integration_bindings as T
+
+    to_rust = lambda t: T.c_to_rust(t).replace("double", "f64")
+    text = T.strip_c_comments(open(_abi.ATTENTION_HEADER).read())
+    text = re.sub(r"int64_t (\w+), (\w+);", r"int64_t \1; int64_t \2;", text)
+    doc = open(os.path.join(_abi.ROOT, "INTEGRATION.md")).read()
+    start = doc.index("```rust", doc.index("### src/sys_attention.rs"))
+    rust = doc[start:doc.index("```", start + 7)]
+    structs, found = {}, {}
+    for name, body in re.findall(r"typedef struct (\w+) \{(.*?)\} \1;", text, flags=re.S):
+        decls = [re.fullmatch(r"(.+?)\s*(\w+)", " ".join(d.split())) for d in body.split(";") if d.strip()]
+        structs[name] = [(m.group(2), to_rust(m.group(1))) for m in decls]
+    for name, body in re.findall(r"#\[repr\(C\)\]\s*pub struct (\w+) \{(.*?)\}", rust, flags=re.S):
+        found[name] = [re.fullmatch(r"pub (\w+): (.+)", " ".join(f.split())).groups() for f in body.split(",") if f.strip()]
+    assert found == structs and len(structs) == 6
+    consts = dict(re.findall(r"(RHZ_ROPE_\w+)\s*=\s*(\d+)", text))
+    assert dict(re.findall(r"pub const (RHZ_\w+): i32 = (\d+);", rust)) == consts and len(consts) == 3
+    declared = re.findall(r"rhz_status\s+(rhz_\w+)\(([^)]*)\);", text)
+    assert len(declared) == 8
+    for name, params in declared:
+        m = re.search(r"pub fn %s\(([^)]*)\)\s*->\s*i32;" % name, rust)
+        assert m, name
+        want = [to_rust(re.fullmatch(r"(.+?)\s*(\w+)", " ".join(x.split())).group(1)) for x in params.split(",")]
+        assert [" ".join(x.split()).split(": ")[1] for x in m.group(1).split(",")] == want, name
+
+
+def test_packed_arguments_are_the_structures():
+    """What the front end lays out is what filling in the Structure gives."""
+    for name in ("Rope", "LatentAppend", "LatentDecode", "LatentPrefill", "LatentPrefillBackward"):
+        struct = getattr(_abi, name + "Args")
+        flat = []
+        for field, t in struct._fields_:
+            flat += [(field, f, u) for f, u in t._fields_] if hasattr(t, "_fields_") else [(None, field, t)]
+        a, values = struct(), []
+        for i, (outer, field, t) in enumerate(flat):
+            v = 0.5 * i if t is c_float else 3 * i + 1
+            setattr(getattr(a, outer) if outer else a, field, v)
+            values.append(v)
+        pack = getattr(_abi, "pack_" + {"Rope": "rope", "LatentAppend": "latent_append", "LatentDecode": "latent_decode",
+                                        "LatentPrefill": "latent_prefill",
+                                        "LatentPrefillBackward": "latent_prefill_backward"}[name])
+        got, want = pack(*values), bytes(a)
+        assert len(got) == len(want)
+        for outer, field, t in flat:  # padding may differ
+            at = getattr(struct, outer).offset + getattr(dict(struct._fields_)[outer], field).offset if outer else \
+                getattr(struct, field).offset
+            assert got[at:at + ctypes.sizeof(t)] == want[at:at + ctypes.sizeof(t)], (name, field)
