@@ -128,11 +128,14 @@ struct AppendParams {
     float magnitude, eps;
 };
 
-constexpr int kMaxChunks = 8;  // of a lane: 4096 bf16 latents; fp32 reads those behind 2048 twice
+// Chunks of a lane that stay in registers: 1024 bf16 or 512 fp32 latents, those
+// behind are read twice.  With eight, for 4096, the registers leave room for fewer
+// waves: 10333 tokens of 512 + 64, 11.0 us instead of 10.1.
+constexpr int kMaxChunks = 2;
 
 // A wave a token: the latent is read once and kept in registers while its norm is
-// formed.  10333 tokens of 512 + 64, 24 MB: 10.8 us, values one by one 13.4; one
-// token each of 8 sequences 3.8.
+// formed.  10333 tokens of 512 + 64, 24 MB: 10.1 us, values one by one 13.4; one
+// token each of 8 sequences 4.4.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void latent_append_kernel(AppendParams a) {
     using V = Vec<T, VEC>;
@@ -140,6 +143,22 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(AppendParams a)
     const int lane = threadIdx.x & 63;
     const long t = (long)blockIdx.x * (kThreads / kWave) + (threadIdx.x >> 6);
     if (t >= a.tokens) return;
+    // The token's values are on their way while its place is looked up.
+    const T* x = (const T*)a.latent + t * a.ls;
+    const int chunks = a.d_c / E;
+    typename V::Raw keep[kMaxChunks];
+#pragma unroll
+    for (int k = 0; k < kMaxChunks; ++k) {
+        const int i = k * kWave + lane;
+        if (i < chunks) keep[k] = V::load_raw(x + i * E);
+    }
+    const T* r = (const T*)a.key + t * a.ks;
+    const int half = a.d_r / 2;
+    const auto pair = [&](int i) { return a.inter ? 2 * i : i; };
+    const auto partner = [&](int i) { return a.inter ? 2 * i + 1 : i + half; };
+    float p0 = 0.f, q0 = 0.f;
+    double f0 = 0.0;
+    if (a.turns && lane < half) p0 = Elem<T>::load(r, pair(lane)), q0 = Elem<T>::load(r, partner(lane)), f0 = a.turns[lane];
     int seq, left;  // tokens of the sequence from this one on
     if (a.cu) {
         seq = 0;  // sequences that end at or before t
@@ -163,16 +182,7 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(AppendParams a)
     const int page = a.table[(long)seq * a.max_pages + pos / a.page];
     if (page < 0 || page >= a.num_pages) return;
     T* out = (T*)a.cache + ((long)page * a.page + pos % a.page) * (a.d_c + a.d_r);
-    const T* x = (const T*)a.latent + t * a.ls;
-    const int chunks = a.d_c / E;
-    typename V::Raw keep[kMaxChunks];
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMaxChunks; ++k) {
-        const int i = k * kWave + lane;
-        if (i < chunks) keep[k] = V::load_raw(x + i * E);
-    }
-    float f = 1.f;
+    float sum = 0.f, f = 1.f;
     if (a.norm) {
 #pragma unroll
         for (int k = 0; k < kMaxChunks; ++k) {
@@ -209,19 +219,16 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(AppendParams a)
         V::load(x + i * E, v);
         put(i, v);
     }
-    const T* r = (const T*)a.key + t * a.ks;
     out += a.d_c;
     if (!a.turns) {
         for (int d = lane; d < a.d_r; d += kWave) out[d] = r[d];
         return;
     }
-    const int half = a.d_r / 2;
     for (int i = lane; i < half; i += kWave) {
-        const int d = a.inter ? 2 * i : i, e = a.inter ? d + 1 : d + half;
-        const float2 cs = rotation(a.turns[i], (int)pos, a.magnitude);
-        const float p = Elem<T>::load(r, d), q = Elem<T>::load(r, e);
-        Elem<T>::store(out, d, p * cs.x - q * cs.y);
-        Elem<T>::store(out, e, p * cs.y + q * cs.x);
+        if (i != lane) p0 = Elem<T>::load(r, pair(i)), q0 = Elem<T>::load(r, partner(i)), f0 = a.turns[i];
+        const float2 cs = rotation(f0, (int)pos, a.magnitude);
+        Elem<T>::store(out, pair(i), p0 * cs.x - q0 * cs.y);
+        Elem<T>::store(out, partner(i), p0 * cs.y + q0 * cs.x);
     }
 }
 
