@@ -280,6 +280,7 @@ def latent_prefill(q, k, v, k_rope=None, *, scale=None, causal: bool = True, cu_
     where the keys are others, ``cu_seqlens_k``.  Causal: the last query of a
     sequence sees all of its keys.  scale defaults to (d_n + d_r) ** -0.5.
     Returns (o [B, T, H, d_v], lse fp32 [B, T, H]), which the backward pass takes.
+    Rows of a pack outside every sequence are not written.
     """
     if stream is not None:
         return _on_stream(latent_prefill, locals())
@@ -301,8 +302,9 @@ def latent_prefill_backward(q, k, v, k_rope, o, lse, do, *, dlse=None, scale=Non
 
     The forward call's inputs again, its o and lse, ``do`` the gradient of o and
     ``dlse`` that of lse (None: zeros).  Returns (dq, dk, dv, dk_rope or None),
-    contiguous and of q's dtype, dk_rope summed over the heads.  Two calls that
-    may run at the same time must not share a workspace.
+    contiguous and of q's dtype, dk_rope summed over the heads.  Rows of a pack
+    outside every sequence are not written.  Two calls that may run at the same
+    time must not share a workspace.
     """
     if stream is not None:
         return _on_stream(latent_prefill_backward, locals())

@@ -188,3 +188,34 @@ def test_tensors_elsewhere(device):
     for i in range(3):
         with pytest.raises(ValueError, match="on the GPU"):
             rhizome_amd.latent_prefill_backward(q, q, q, None, *(t.cpu() if k == i else t for k, t in enumerate((o, lse, q))))
+
+
+@both
+def test_tokens_beyond_32_bits(device, dtype):
+    """The last tokens of tensors of more than 2^32 bytes, of a pack whose other tokens are in no sequence."""
+    n, H, d_n, d_r, d_v = 140, 64, 128, 64, 128
+    total = (5 << 30) // (H * (d_n + d_r) * (2 if dtype == torch.bfloat16 else 4))
+    q, kv, r, do = (t.to(device) for t in make([n], [n], H, d_n, d_r, d_v, dtype, seed=19))
+
+    def far(t):
+        out = torch.empty(total, *t.shape[1:], dtype=t.dtype, device=device)
+        out[-n:] = t
+        return out
+
+    long = [far(t) for t in (q, kv, r, do)]
+    pos = torch.arange(total, dtype=torch.int32, device=device)
+    freq = rhizome_amd.rope_frequencies(d_r, device=device)[0]
+    rhizome_amd.rope(long[0], pos, freq, offset=d_n, out=long[0])
+    rhizome_amd.rope(q, pos[-n:], freq, offset=d_n, out=q)
+    assert torch.equal(long[0][-n:], q)
+    cu = torch.tensor([total - n, total], dtype=torch.int32, device=device)
+    run = lambda q, kv, r, do, cu: [t[-n:].clone() for t in _both_passes(q, kv, r, do, cu, d_n)]
+    got = run(*long, cu)
+    want = run(q, kv, r, do, torch.tensor([0, n], dtype=torch.int32, device=device))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _both_passes(q, kv, r, do, cu, d_n):
+    k, v = kv[..., :d_n], kv[..., d_n:]
+    o, lse = rhizome_amd.latent_prefill(q, k, v, r, cu_seqlens=cu)
+    return o, lse, *rhizome_amd.latent_prefill_backward(q, k, v, r, o, lse, do, cu_seqlens=cu)

@@ -102,6 +102,13 @@ def test_widths(device, dtype, d_c, d_r):
 
 
 @both
+@pytest.mark.parametrize("d_c,d_r", [(130, 6), (100, 28), (1, 7), (497, 15), (251, 5), (12, 4)])
+def test_rows_of_whole_chunks_with_latents_that_are_not(device, dtype, d_c, d_r):
+    for steps, H in ((1, 8), (2, 16), (3, 16), (2, 40)):
+        check([130, 300], steps, H, d_c, d_r, 64, dtype, device, seed=d_c)
+
+
+@both
 @pytest.mark.parametrize("page", [1, 3, 16, 31, 100, 1000])
 def test_pages(device, dtype, page):
     """Pages that end inside a tile, of one row, and longer than a split."""
