@@ -74,7 +74,7 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_kernel(BackwardParams a) {
     const int second = wave >> 2, group = wave & 3;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, blockIdx.x, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
+    if (!place<kRows, true>(a, blockIdx.x, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int first = tile * kRows;
     if (first >= w.nk) return;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, blockIdx.x, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
+    if (!place<kRows, false>(a, blockIdx.x, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int last_tile = (w.nq - 1) / kRows;
     if (w.nq == 0 || tile > last_tile) return;

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
     const LaneReads at = lane_reads<T>(lane);
 
     int head, seq, tile;
-    if (!place(a, blockIdx.x, a.cu_q, a.len_q, kQueries, lane, head, seq, tile)) return;
+    if (!place<kQueries, false>(a, blockIdx.x, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kQueries >= w.nq) return;
     const int first = ((w.nq - 1) / kQueries - tile) * kQueries;  // the queries with the most keys go first

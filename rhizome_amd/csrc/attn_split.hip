@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, blockIdx.x, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
+    if (!place<kRows, false>(a, blockIdx.x, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kRows >= w.nq) return;
     const int first = ((w.nq - 1) / kRows - tile) * kRows;  // the queries with the most keys go first
@@ -191,7 +191,7 @@ __device__ __forceinline__ void dkv(const BackwardParams& a, unsigned block, Wav
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, block, a.cu_k, a.len_k, kRows, lane, head, seq, tile)) return;
+    if (!place<kRows, true>(a, block, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     const int first = tile * kRows;
     if (first >= w.nk) return;
@@ -333,7 +333,7 @@ __device__ __forceinline__ void dq(const BackwardParams& a, unsigned block, Wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     int head, seq, tile;
-    if (!place(a, block, a.cu_q, a.len_q, kRows, lane, head, seq, tile)) return;
+    if (!place<kRows, false>(a, block, lane, head, seq, tile)) return;
     const Range w = seq_range(a.cu_q, a.cu_k, seq, a.len_q, a.len_k);
     if (tile * kRows >= w.nq) return;
     const int first = ((w.nq - 1) / kRows - tile) * kRows;

@@ -83,6 +83,25 @@ def test_packs(device, dtype, causal, lens, keys):
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+@pytest.mark.parametrize("lens,keys", [
+    ([300, 0, 700, 1, 129, 128, 513], [300, 5, 900, 400, 129, 100, 513]),
+    ([128, 256, 384], [128, 256, 384]),
+    ([700, 20], [100, 650]),  # most of its queries see nothing, few see much
+    ([1, 600], [600, 1]),
+])
+def test_packs_of_many_tiles(device, dtype, lens, keys):
+    """Whose tiles are worked on by the length of their way, over all sequences."""
+    check(lens, keys, 2, 64, 16, 64, dtype, device, seed=len(lens))
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+@pytest.mark.parametrize("count", [2, 63, 64, 65])
+def test_numbers_of_sequences(device, dtype, count):
+    lens = [int(x) for x in torch.randint(0, 200, (count,), generator=torch.Generator().manual_seed(count))]
+    check(lens, lens, 2, 32, 0, 32, dtype, device, seed=4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_many_sequences(device, dtype):
     """More sequences than a wave has lanes, empty ones among them."""
     lens = [int(x) for x in torch.randint(0, 9, (150,), generator=torch.Generator().manual_seed(2))]
