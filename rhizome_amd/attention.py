@@ -263,7 +263,7 @@ def _prefill_args(q, k, v, k_rope, scale, causal, cu_seqlens, cu_seqlens_k):
     if k_rope is not None and (k_rope.shape != (*ks[:-2], d_r) or k_rope.dtype != q.dtype):
         raise ValueError(f"k_rope must be {q.dtype} {(*ks[:-2], d_r)}")
     one = H == 1  # whose distance to a next one is nothing's
-    sizes = (batch, _count(n_q), _count(n_k), H, d_n, d_r, d_v, dtype, causal, d_q ** -0.5 if scale is None else scale,
+    sizes = (batch, _count(n_q), _count(n_k), H, d_n, d_r, d_v, dtype, causal, (d_q or 1) ** -0.5 if scale is None else scale,
              _token_stride("q", q, spread, n_q), 0 if one else q.stride(-2),
              _token_stride("k", k, spread, n_k), 0 if one else k.stride(-2),
              _token_stride("v", v, spread, n_k), 0 if one else v.stride(-2),
