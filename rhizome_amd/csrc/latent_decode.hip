@@ -19,6 +19,37 @@
 namespace rhz {
 namespace {
 
+constexpr int kTable = 1024;  // cached rows whose places are looked up at once
+constexpr int kMaxSplits = 128, kUnit = 32;
+
+// Cached rows of a split of a sequence of n rows: eighths of a short one, for one
+// request's latency, of `least` rows at least, but of a long one `best` at most, as
+// many as keep the parts' traffic low against the cache's own (at 16 heads a part is
+// written and read again for 32 KB each against 1152 bytes a row).
+//   bf16, 16 heads, least 64, 128, 256: one sequence of 517 positions 15.1, 15.3, 18.0
+// us.  best 256, 512, 1024: one of 16384 - / 25 / 37 us, eight of them - / 38 / 46, 64
+// of 2048 to 6084 97 / 87 / 76 (where splits of 512 are a few more than the card has
+// places).
+//   fp32 takes sixteen times as long for a row: best 128, 256, 512: one of 16384 39 /
+// 60 / 107 us, sixteen of 4096 77 / 72 / 115, 32 of them 153 / 139 / 132; least 64,
+// 128: one of 517 26 / 32.
+struct SplitRule {
+    int least, best;
+};
+template <typename T> constexpr SplitRule kRule = sizeof(T) == 4 ? SplitRule{64, 128} : SplitRule{128, 512};
+__device__ __forceinline__ int split_rows(SplitRule r, int n) {
+    const int eighth = min(max((n + 7) / 8, r.least), r.best), even = max(eighth, n / kMaxSplits + (n % kMaxSplits != 0));
+    return (even + kUnit - 1) / kUnit * kUnit;
+}
+__device__ __forceinline__ int splits_of(SplitRule r, int n) {
+    return n <= 0 ? 1 : (n + split_rows(r, n) - 1) / split_rows(r, n);
+}
+// No sequence of up to n rows has more.
+inline int most_splits_of(SplitRule r, int64_t n) {
+    const int64_t shortest = (n + r.least - 1) / r.least, best = (n + r.best - 1) / r.best;
+    return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(8, std::min<int64_t>(best, kMaxSplits))));
+}
+
 struct DecodeParams {
     const void *q, *cache;
     const int *table, *lengths;
@@ -29,27 +60,6 @@ struct DecodeParams {
     int batch, steps, heads, d_c, D, page, num_pages, max_pages, splits, row_tiles;
     float scale;
 };
-
-constexpr int kTable = 1024;  // cached rows whose places are looked up at once
-constexpr int kMaxSplits = 128, kMinSplit = 128, kBestSplit = 512, kUnit = 32;
-
-// Cached rows of a split of a sequence of n rows: eighths of a short one, for
-// one request's latency, but of a long one as many as keep the parts' traffic
-// low against the cache's own (at 16 heads a part is written and read again for
-// 32 KB each against 1152 bytes a row).  Eighths of 64, 128, 256 rows at least: one
-// sequence of 517 positions 15.1, 15.3, 18.0 us.  Of 256, 512, 1024 at most: one of
-// 16384 - / 25 / 37 us, eight of them - / 38 / 46, 64 of 2048 to 6084 97 / 87 / 76
-// (where the splits of 512 are a few more than the card has places).
-__host__ __device__ inline int split_rows(int n) {
-    const int eighth = min(max((n + 7) / 8, kMinSplit), kBestSplit), even = max(eighth, n / kMaxSplits + (n % kMaxSplits != 0));
-    return (even + kUnit - 1) / kUnit * kUnit;
-}
-__host__ __device__ inline int splits_of(int n) { return n <= 0 ? 1 : (n + split_rows(n) - 1) / split_rows(n); }
-// No sequence of up to n rows has more.
-inline int most_splits_of(int64_t n) {
-    const int64_t shortest = (n + kMinSplit - 1) / kMinSplit, best = (n + kBestSplit - 1) / kBestSplit;
-    return (int)std::max<int64_t>(1, std::min(shortest, std::max<int64_t>(8, std::min<int64_t>(best, kMaxSplits))));
-}
 
 constexpr int64_t kMostRows = INT32_MAX - 4096;  // numbers of tiles' rows behind the last stay in 32 bits
 __device__ __forceinline__ int rows_of(const DecodeParams& a, int seq) {
@@ -67,15 +77,16 @@ struct Unit {
 // have are behind the others, where their workgroups, which end at once, do not
 // disturb their distribution over the CUs (32 x 4096 positions, 128 rows: 73 us, and
 // 113 with every ninth workgroup such a one).
+template <typename T>
 __device__ __forceinline__ bool unit_of(const DecodeParams& a, int tile_rows, Unit& u) {
     const int k = blockIdx.x >> 3, unit = k / a.row_tiles * 8 + (blockIdx.x & 7);
     if (unit >= a.batch * a.splits) return false;
     u.seq = unit % a.batch, u.split = unit / a.batch, u.first_row = k % a.row_tiles * tile_rows;
     u.length = a.lengths[u.seq];
     u.n = rows_of(a, u.seq);
-    u.splits = splits_of(u.n);
-    u.begin = u.split * split_rows(u.n);
-    u.end = min(u.n, u.begin + split_rows(u.n));
+    u.splits = splits_of(kRule<T>, u.n);
+    u.begin = u.split * split_rows(kRule<T>, u.n);
+    u.end = min(u.n, u.begin + split_rows(kRule<T>, u.n));
     return u.split < u.splits;
 }
 // Cache row of position j, -1 where its page is outside the cache.
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     const LaneReads at = lane_reads<T>(lane);
     Unit u;
-    if (!unit_of(a, 32 * RT, u)) return;
+    if (!unit_of<T>(a, 32 * RT, u)) return;
     const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
 
     const int part = wave % PARTS, mine = wave / PARTS;
@@ -419,7 +430,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     __shared__ int row_at[kTable];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     Unit u;
-    if (!unit_of(a, 16, u)) return;
+    if (!unit_of<T>(a, 16, u)) return;
     const int rows = a.steps * a.heads, begin = u.begin, end = u.end;
 
     const auto fill_table = [&](int j0) {
@@ -632,7 +643,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams 
     const int rows = a.steps * a.heads, parts = (a.d_c + kJoinColumns - 1) / kJoinColumns;
     const int d = blockIdx.x % parts * kJoinColumns + (threadIdx.x & 63) * 4;
     const int unit = blockIdx.x / parts, seq = unit / rows, r = unit % rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int splits = splits_of(rows_of(a, seq));
+    const int splits = splits_of(kRule<T>, rows_of(a, seq));
     if (splits == 1) return;
     const float c = a.scale * kLog2e;
     const long first = (long)seq * a.splits * rows + r;  // slot 0's; the next split's is `rows` further
@@ -682,7 +693,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams 
 }
 
 int most_splits(const rhz_latent_decode_args& a) {
-    return most_splits_of(std::min<int64_t>((int64_t)a.max_pages * a.page_size, kMostRows));
+    return most_splits_of(a.dtype == RHZ_F32 ? kRule<float> : kRule<uint16_t>, std::min<int64_t>((int64_t)a.max_pages * a.page_size, kMostRows));
 }
 
 hipError_t join(const DecodeParams& p, int dtype, hipStream_t stream) {
