@@ -234,6 +234,21 @@ def test_strides_and_alignment(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+def test_expanded_inputs(device, dtype):
+    """One head's keys and values for all heads, one token's for all tokens: strides of zero."""
+    n, H, d = 150, 4, 64
+    q, kv, _, do = (t[None].to(device) if t is not None else None for t in make([n], [n], H, d, 0, d, dtype, seed=21))
+    for whole in (kv[:, :, :1], kv[:, :1]):
+        k, v = (t.expand(1, n, H, d) for t in (whole[..., :d], whole[..., d:]))
+        o, lse = rhizome_amd.latent_prefill(q, k, v)
+        got = o, lse, *rhizome_amd.latent_prefill_backward(q, k, v, None, o, lse, do)[:3]
+        k, v = k.contiguous(), v.contiguous()
+        o, lse = rhizome_amd.latent_prefill(q, k, v)
+        want = o, lse, *rhizome_amd.latent_prefill_backward(q, k, v, None, o, lse, do)[:3]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_one_token_of_a_long_tensor(device, dtype):
     """Its batch of one is 2^23 elements long, which no token's distance from the next is."""
     H, d, m = 2, 64, 50

@@ -199,3 +199,16 @@ def test_append_to_many_sequences(device):
     pos = lens - 1
     assert torch.equal(cache[table[torch.arange(n), pos // page].long().to(device), (pos % page).to(device)], new)
     assert int((cache.abs().sum(-1) > 0).sum()) == n
+
+
+@both
+def test_expanded_tokens(device, dtype):
+    """One token's heads turned to every position; an output of rows that share memory is refused."""
+    n, H, d = 33, 4, 64
+    freq = rhizome_amd.rope_frequencies(d, device=device)[0]
+    pos = torch.arange(n, dtype=torch.int32, device=device)
+    x = normal((1, H, d), torch.Generator().manual_seed(3), dtype).to(device)
+    got = rhizome_amd.rope(x.expand(n, H, d), pos, freq, out=torch.empty(n, H, d, dtype=dtype, device=device))
+    assert torch.equal(got, rhizome_amd.rope(x.expand(n, H, d).contiguous(), pos, freq))
+    with pytest.raises(RuntimeError, match="overlap"):
+        rhizome_amd.rope(got, pos, freq, out=x.clone().expand(n, H, d))
