@@ -110,10 +110,11 @@ def rope_frequencies(dim: int, *, theta: float = 10000.0, scaling: str = "none",
     """
     if scaling not in _SCALINGS:
         raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}")
+    _count(abs(dim))  # the struct's field would take it modulo 2^32, the table's size not
     a = _abi.RopeFrequencyArgs(dim, _SCALINGS[scaling], theta, factor, trained_length, fast, slow)
-    turns, magnitude = (c_double * max(dim // 2, 1))(), c_float(0.0)
+    turns, magnitude = (c_double * 512)(), c_float(0.0)  # of the widest that is supported
     _abi.check(_abi.lib().rhz_rope_frequencies(byref(a), turns, byref(magnitude)))
-    return torch.tensor(list(turns), dtype=torch.float64, device=device), magnitude.value
+    return torch.tensor(turns[:dim // 2], dtype=torch.float64, device=device), magnitude.value
 
 
 def rope(x, positions, frequencies, *, offset: int = 0, interleaved: bool = False, magnitude: float = 1.0,

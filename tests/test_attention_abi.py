@@ -84,6 +84,13 @@ def test_frequencies():
     assert between.any() and bool(((parts < f) & (parts > f / 40))[between].all())
 
 
+@pytest.mark.parametrize("dim", [-2 ** 32 + 1024, 2 ** 32 + 64, 2 ** 31, -2 ** 31 - 2, 2 ** 31 - 2, 1026, -2, 0, 3])
+def test_frequencies_of_a_dimension_out_of_range(dim):
+    """Refused, and not taken modulo 2^32: the library would write a table wider than the one it is given."""
+    with pytest.raises((ValueError, _abi.GdrError), match="dim|2\\^31"):
+        rhizome_amd.rope_frequencies(dim, device="cpu")
+
+
 FREQ = dict(dim=64, scaling=_abi.ROPE_BY_PARTS, theta=1e4, factor=4.0, trained_length=4096.0, fast=32.0, slow=1.0)
 
 
