@@ -179,7 +179,11 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_kernel(BackwardParams a) {
             sum.run(dv, ot, at, 0, p);
         }
         lds_barrier();  // the last tile's weights are handed on
-        uint32_t again = not_finite_rows(dv) & uint32_t(__ballot(live));
+        uint32_t again = not_finite_rows(dv) & rows_with(live);
+        if (again) {  // but for keys that a query with a NaN sees
+            const int last = last_with(w.nq, lane, [&](int i) { return lse2[i] != lse2[i]; });
+            again &= rows_with((a.causal ? max(0, kj - shift) : 0) > last);
+        }
         while (again) {
             const int r = __ffs(again) - 1;
             again &= again - 1;
@@ -235,7 +239,11 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_kernel(BackwardParams a) {
             ds.set(dp);
             sum.run(dk, qt, at, 0, ds);
         }
-        uint32_t again = not_finite_rows(dk) & uint32_t(__ballot(live));
+        uint32_t again = not_finite_rows(dk) & rows_with(live);
+        if (again) {
+            const int last = last_with(w.nq, lane, [&](int i) { return lse2[i] != lse2[i] || delta[i] != delta[i]; });
+            again &= rows_with((a.causal ? max(0, kj - shift) : 0) > last);
+        }
         while (again) {
             const int r = __ffs(again) - 1;
             again &= again - 1;
@@ -353,7 +361,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(BackwardParams a) 
         sum.run(dq, kt, at, 0, ds);
     }
     bool live = qi < w.nq;
-    uint32_t again = not_finite_rows(dq) & uint32_t(__ballot(live));
+    const bool nan = (lse2 != lse2 || delta != delta) && (a.causal ? min(w.nk, qi + shift + 1) : w.nk) > 0;
+    uint32_t again = not_finite_rows(dq) & rows_with(live && !nan);
     while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;

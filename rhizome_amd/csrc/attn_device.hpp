@@ -377,7 +377,13 @@ __device__ __forceinline__ float sum_of_halves(float x) {
 // Weight 0 does not take a hidden row out of a product if that row holds an
 // infinity or NaN: whoever's result is not finite sums again over the rows that
 // it sees, in plain fp32, a wave a row.  (Scores are masked one by one, so that
-// the maxima, sums and weights are right in any case.)
+// the maxima, sums and weights are right in any case.)  That takes a time of its
+// own for every pair of rows, so it is for rows of which it can say more than NaN:
+// those whose own statistic is NaN, which only what they see can make it, are NaN
+// in every column as they are, and a sum that is NaN in every column stays so.  4096
+// tokens, 16 heads of 128 + 64 channels, bf16, NaN in all queries: prefill 112 ->
+// 0.13 ms; in all values 2.0.  An infinity in one value that all later rows see
+// takes 113 ms (finite 0.14), in one gradient of o 227 (0.45).
 template <int N>
 __device__ __forceinline__ uint32_t not_finite_rows(const f32x16 (&acc)[N]) {
     float sum = 0.f;  // 0 * x is NaN where x is not finite, and a sum keeps it
@@ -387,6 +393,17 @@ __device__ __forceinline__ uint32_t not_finite_rows(const f32x16 (&acc)[N]) {
         for (int i = 0; i < 16; ++i) sum = fmaf(acc[d][i], 0.f, sum);
     const unsigned long long b = __ballot(sum != 0.f);
     return uint32_t(b) | uint32_t(b >> 32);
+}
+// The rows of lanes that have `is`, the same in either half.
+__device__ __forceinline__ uint32_t rows_with(bool is) { return uint32_t(__ballot(is)); }
+// The last of n for which is(i), -1 for none, by all lanes of a wave together.
+template <typename IS>
+__device__ __forceinline__ int last_with(int n, int lane, IS is) {
+    for (int i0 = (n - 1) / kWave * kWave; i0 >= 0; i0 -= kWave) {
+        const unsigned long long b = __ballot(i0 + lane < n && is(i0 + lane));
+        if (b) return i0 + 63 - __clzll((long long)b);
+    }
+    return -1;
 }
 template <typename T>
 __device__ __forceinline__ float value(const Rows<T>& s, long r, int d) {
@@ -418,6 +435,10 @@ __device__ __forceinline__ void sum_row_again(long lo, long hi, int cols, int la
             for (int k = 0; k < N; ++k)
                 if (lane + 64 * k < cols) sum[k] = fmaf(pi, x(j0 + i, lane + 64 * k), sum[k]);
         }
+        bool nan = true;  // in all of the lane's columns
+#pragma unroll
+        for (int k = 0; k < N; ++k) nan = nan && (lane + 64 * k >= cols || sum[k] != sum[k]);
+        if (__all(nan)) break;
     }
 #pragma unroll
     for (int k = 0; k < N; ++k)

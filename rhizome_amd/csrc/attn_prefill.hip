@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill_kernel(PrefillPara
     }
     l = sum_of_halves(l);
     const float f = l == 0.f ? 0.f : 1.f / l;
-    uint32_t again = not_finite_rows(o) & uint32_t(__ballot(live));
+    uint32_t again = not_finite_rows(o) & rows_with(live && l == l);
     while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;

@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void latent_prefill_split_kernel(PrefillP
     if (wave == 0 && g == 0 && live) a.lse[row] = total == 0.f ? -INFINITY : fmaf(top, a.scale, logf(total));
     for (int d = wave; d < VT; d += kWaves) {
         f32x16 x[1] = {sums.sum(d)};
-        const uint32_t again = not_finite_rows(x) & uint32_t(__ballot(live));
+        const uint32_t again = not_finite_rows(x) & rows_with(live && total == total);
         for (uint32_t left = again; left; left &= left - 1) {
             const int r = __ffs(left) - 1;
             const long to = (long)w.q0 + first + r;
@@ -287,7 +287,11 @@ __device__ __forceinline__ void dkv(const BackwardParams& a, unsigned block, Wav
         const bool is_v = d >= QT;
         const int d0 = 32 * (is_v ? d - QT : d);
         f32x16 x[1] = {sums.sum(d)};
-        const uint32_t again = not_finite_rows(x) & uint32_t(__ballot(live));
+        uint32_t again = not_finite_rows(x) & rows_with(live);
+        if (again) {  // but for keys that a query with a NaN sees
+            const int last = last_with(w.nq, lane, [&](int i) { return lse2[i] != lse2[i] || (!is_v && delta[i] != delta[i]); });
+            again &= rows_with((a.causal ? max(0, kj - shift) : 0) > last);
+        }
         const auto put = [&](long to, int e, float y) {  // to column e of a key's row
             if (is_v)
                 ((T*)a.dv)[(to * a.heads + head) * a.d_v + e] = y;
@@ -405,9 +409,10 @@ __device__ __forceinline__ void dq(const BackwardParams& a, unsigned block, Wave
     for (int d = 0; d < QT; ++d) sums.put(wave, d, dq[d]);
     __syncthreads();
     const int cols = a.d_n + a.d_r;
+    const bool nan = (lse2 != lse2 || delta != delta) && seen > 0;
     for (int d = wave; d < QT; d += kWaves) {
         f32x16 x[1] = {sums.sum(d)};
-        const uint32_t again = not_finite_rows(x) & uint32_t(__ballot(live));
+        const uint32_t again = not_finite_rows(x) & rows_with(live && !nan);
         for (uint32_t left = again; left; left &= left - 1) {
             const int r = __ffs(left) - 1;
             const long to = (long)w.q0 + first + r;

@@ -388,7 +388,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     const int d0 = part * VTW * 32, cols = min(a.d_c - d0, VTW * 32);  // the wave's columns
     const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
     const float f = u.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-    uint32_t again = not_finite_rows(o) & uint32_t(__ballot(live));
+    uint32_t again = not_finite_rows(o) & rows_with(live && l == l);
     while (again) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
 #pragma unroll
         for (int k = 0; k < 4; ++k) bad = fmaf(x[d][k], 0.f, bad);
     }
-    unsigned long long flags = __ballot(bad != 0.f && live);
+    unsigned long long flags = __ballot(bad != 0.f && live && sum == sum);
     flags |= flags >> 32;
     uint32_t again = cols > 0 ? uint32_t(flags | flags >> 16) & 0xffffu : 0;
     while (again) {
