@@ -580,9 +580,14 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
         for (int d = 0; d < VT; ++d) o[d] = o[d] * own + given[(wave * VT + d) * kWave];
     }
     __syncthreads();
+    // by value: a choice between two places of o is an index, which would put o into memory
+    const auto of_half = [&](int half, int d) {
+        const f32x4 first = o[d], second = o[VT / 2 + d];
+        return half ? second : first;
+    };
     if (wave < 2) {
 #pragma unroll
-        for (int d = 0; d < VT / 2; ++d) given[(wave * (VT / 2) + d) * kWave] = wave ? o[d] : o[VT / 2 + d];
+        for (int d = 0; d < VT / 2; ++d) given[(wave * (VT / 2) + d) * kWave] = of_half(1 - wave, d);
     }
     __syncthreads();
     if (wave >= 2) return;
@@ -593,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     float bad = 0.f;  // as not_finite_rows
 #pragma unroll
     for (int d = 0; d < VT / 2; ++d) {
-        x[d] = (wave ? o[VT / 2 + d] : o[d]) + given[((1 - wave) * (VT / 2) + d) * kWave];
+        x[d] = of_half(wave, d) + given[((1 - wave) * (VT / 2) + d) * kWave];
 #pragma unroll
         for (int k = 0; k < 4; ++k) bad = fmaf(x[d][k], 0.f, bad);
     }
@@ -748,8 +753,8 @@ hipError_t pick_rows(const DecodeParams& p, bool vec, hipStream_t stream) {
 }
 
 // By the width of a latent: 32 sequences of 4096 positions, d_c 128 on the kernels
-// of 128 and of 512 at 16 rows 25.8 / 26.7 us, at 64 rows 36.6 / 44.4, d_c 256 on
-// those of 256 and of 512 24.7 / 29.3 and 41 / 45.  Not vec, the wide kernel reads
+// of 128 and of 512 at 16 rows 18.4 / 27.0 us, at 64 rows 36.3 / 43.9, d_c 256 on
+// those of 256 and of 512 24.6 / 29.1 and 41 / 45.  Not vec, the wide kernel reads
 // values one by one: d_c 512, 64 rows 54 -> 128 us.
 template <typename T>
 hipError_t pick(const DecodeParams& p, hipStream_t stream) {
