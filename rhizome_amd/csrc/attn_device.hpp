@@ -198,12 +198,11 @@ __device__ __forceinline__ u32x4 load_chunk(const Rows<T>& s, long row0, int r, 
 // shorter.
 template <int OFF>
 __device__ __forceinline__ void load_to_lds16(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds - OFF), "v"(off),
-                 "s"(base), "n"(OFF)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"{m0}"(lds - OFF), "v"(off), "s"(base), "n"(OFF)
                  : "memory");
 }
 __device__ __forceinline__ void load_to_lds4(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
 }
 // Until every wave's loads into LDS have landed and its LDS reads are done.
 __device__ __forceinline__ void landed() {

@@ -139,8 +139,7 @@ __device__ __forceinline__ void store_sums(const DecodeParams& a, const Unit& u,
 // 16 bytes a lane from p + OFF to LDS at lds; the instruction's offset counts in LDS too.
 template <int OFF>
 __device__ __forceinline__ void load_to_lds16_from(const void* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(lds - OFF), "v"(p), "n"(OFF)
-                 : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"{m0}"(lds - OFF), "v"(p), "n"(OFF) : "memory");
 }
 // Panels K, K + STEP .. of a cached row from the lane's chunk of panel 0 at p on,
 // `left` bytes of the row being left from there.
