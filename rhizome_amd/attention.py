@@ -58,19 +58,16 @@ def _dense(t: torch.Tensor | None, here: int) -> int:
 
 def _token_stride(name, t, batch, n):
     """In elements, of a tensor of n tokens of every sequence of a batch, whose
-    last dimension has to be dense; batch None: of tokens alone."""
+    last dimension has to be dense; batch None: of tokens alone.  A single token
+    has no distance to a next one."""
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}'s last dimension must be dense")
-    if batch is None:
+    if (n if batch is None else batch * n) <= 1:
+        return 0
+    if batch is None or n == 1:
         return st[0]
-    if st[0] == st[1] * n:
-        return st[1]
-    if batch <= 1:
-        return st[1] if n > 1 else 0
-    if n == 1:
-        return st[0]
-    if n > 0:
+    if batch > 1 and st[0] != st[1] * n:
         raise ValueError(f"{name}'s tokens must be evenly spaced over the batch")
     return st[1]
 

@@ -13,6 +13,7 @@ from hypothesis import given, settings, strategies as st
 
 import rhizome_amd
 from rhizome_amd import _abi
+from rhizome_amd.attention import _token_stride
 
 A = 1 << 40  # fake device addresses, 2^32 apart; never dereferenced
 STEP = 1 << 32
@@ -388,3 +389,22 @@ def test_packed_arguments_are_the_structures():
             at = getattr(struct, outer).offset + getattr(dict(struct._fields_)[outer], field).offset if outer else \
                 getattr(struct, field).offset
             assert got[at:at + ctypes.sizeof(t)] == want[at:at + ctypes.sizeof(t)], (name, field)
+
+
+def test_token_strides():
+    """The distance of a token from the next one, which a single token does not have, whatever its view says."""
+    far = torch.empty(0).as_strided  # nothing is read
+    stride = lambda shape, strides, batch, n: _token_stride("x", far(shape, strides), batch, n)
+    big = 1 << 30
+    for shape, strides, batch, n in (((1, 2, 0), (big, 8, 1), None, 1), ((1, 1, 2, 0), (big, big, 8, 1), 1, 1),
+                                     ((1, 1, 2, 0), (big, 16, 8, 1), 1, 1), ((0, 2, 0), (big, 8, 1), None, 0),
+                                     ((3, 0, 2, 0), (big, 16, 8, 1), 3, 0)):
+        assert stride(shape, strides, batch, n) == 0
+    assert stride((5, 2, 0), (40, 8, 1), None, 5) == 40
+    assert stride((3, 5, 2, 0), (200, 40, 8, 1), 3, 5) == 40
+    assert stride((1, 5, 2, 0), (big, 40, 8, 1), 1, 5) == 40
+    assert stride((3, 1, 2, 0), (200, 40, 8, 1), 3, 1) == 200
+    with pytest.raises(ValueError, match="evenly"):
+        stride((3, 5, 2, 0), (300, 40, 8, 1), 3, 5)
+    with pytest.raises(ValueError, match="dense"):
+        _token_stride("x", torch.empty(5, 2, 8)[..., ::2], None, 5)

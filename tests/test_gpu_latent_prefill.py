@@ -262,6 +262,24 @@ def test_one_token_of_a_long_tensor(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+def test_one_packed_token_far_from_a_next_one(device, dtype):
+    """A sequence of one query, 2^23 elements from where the next would be, and of one key."""
+    H, d = 2, 64
+    q, kv, _, do = make([1], [1], H, d, 0, d, dtype, seed=19)
+    long = torch.zeros(2, (1 << 23) // (H * d), H, d, dtype=dtype, device=device)
+    long[1, 5] = q[0].to(device)
+    far = long[1:, 5]
+    assert far.shape == q.shape and far.stride(0) == 1 << 23
+    k, v, cu = kv[..., :d].to(device), kv[..., d:].to(device), starts([1]).to(device)
+    got = rhizome_amd.latent_prefill(far, k, v, cu_seqlens=cu)
+    want = rhizome_amd.latent_prefill(q.to(device), k, v, cu_seqlens=cu)
+    grads = [rhizome_amd.latent_prefill_backward(x, k, v, None, *want, do.to(device), cu_seqlens=cu) for x in (far, q.to(device))]
+    turned = [rhizome_amd.rope(x, cu[:1], torch.ones(8, dtype=torch.float64, device=device)) for x in (far, q.to(device))]
+    assert all(torch.equal(a, b) for a, b in zip((*got, *grads[0][:3], turned[0]), (*want, *grads[1][:3], turned[1])))
+
+
+
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_a_sequence_alone_and_in_a_pack(device, dtype):
     """Batch-invariance, bit for bit; rows outside every sequence are left as they were."""
     lens, H, d = [37, 150, 64], 2, 64
