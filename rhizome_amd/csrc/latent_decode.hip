@@ -7,8 +7,9 @@
 // row, bound by memory up to some 128 rows of q.  A workgroup takes one split of
 // the sequence, whose cached rows go through LDS once, there to be read along
 // the row for the scores and transposed for the sum.  Splits go to the workspace
-// unnormalised, with their maxima and sums, and are joined in order by another
-// kernel.  Their number depends on the sequence's length alone, so that a
+// with their maxima and sums, each normalised by its own, since a sum of weights
+// times values can leave fp32's range where their mean does not, and are joined in
+// order by another kernel.  Their number depends on the sequence's length alone, so that a
 // sequence's result does not depend on its batch.
 #include <algorithm>
 
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     if (!sums) return;
     const int d0 = part * VTW * 32, cols = min(a.d_c - d0, VTW * 32);  // the wave's columns
     const bool vec = a.d_c % 4 == 0 && aligned16(a.o);
-    const float f = u.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const float f = l == 0.f ? 0.f : 1.f / l;
     uint32_t again = not_finite_rows(o) & rows_with(live && l == l);
     while (again) {
         const int i = __ffs(again) - 1;
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
 #pragma unroll
     for (int d = 0; d < VTW; ++d) {
         if (u.splits > 1)
-            store_columns<float>(to_part, o[d], d0 + 32 * d, a.d_c, 1.f, vec, lane);
+            store_columns<float>(to_part, o[d], d0 + 32 * d, a.d_c, f, vec, lane);
         else
             store_columns<T>(to_o, o[d], d0 + 32 * d, a.d_c, f, vec, lane);
     }
@@ -566,7 +567,7 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     const float tc = top == -INFINITY ? 0.f : top * c;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum = fmaf(wave_l[w][kr], __builtin_amdgcn_exp2f(fmaf(wave_m[w][kr], c, -tc)), sum);
-    const float f = u.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
     const float own = __builtin_amdgcn_exp2f(fmaf(m, c, -tc)) * f;
     f32x4* given = reinterpret_cast<f32x4*>(&tiles[0]) + lane;
     if (wave >= 2) {
@@ -637,8 +638,8 @@ __global__ __launch_bounds__(256, 2) void latent_decode_narrow_kernel(DecodePara
     }
 }
 
-// 256 columns of one row of q a workgroup: its splits' sums at their common
-// maximum, every fourth split on one wave, the waves' sums added in order.
+// 256 columns of one row of q a workgroup: its splits by their shares of the sum
+// of weights, every fourth split on one wave, the waves' sums added in order.
 constexpr int kJoinThreads = 256, kJoinColumns = 256;
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams a) {
@@ -662,15 +663,17 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams 
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(m[i], c, -tc));
-        if (wave == 0) weight[lane + 64 * i] = w;
-        sum = fmaf(l[i], w, sum);
+        l[i] *= __builtin_amdgcn_exp2f(fmaf(m[i], c, -tc));
+        sum += l[i];
     }
     sum = row_sum<64>(sum);
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    if (wave == 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) weight[lane + 64 * i] = l[i] * f;
     __syncthreads();
     const long row = (long)seq * rows + r;
     if (threadIdx.x == 0 && d == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : fmaf(top, a.scale, logf(sum));
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
     const float* p = a.part + first * a.d_c + d;
     const long step = (long)rows * a.d_c;
     const bool vec = a.d_c % 4 == 0 && aligned16(a.o), in = d < a.d_c;
@@ -685,7 +688,7 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(DecodeParams 
     if (wave) sums[wave - 1][lane] = x;
     __syncthreads();
     if (wave || !in) return;
-    x = (((x + sums[0][lane]) + sums[1][lane]) + sums[2][lane]) * f;
+    x = ((x + sums[0][lane]) + sums[1][lane]) + sums[2][lane];
     T* out = (T*)a.o + row * a.d_c + d;
     if (!vec) {
         for (int k = 0; k < 4 && d + k < a.d_c; ++k) Elem<T>::store(out, k, x[k]);

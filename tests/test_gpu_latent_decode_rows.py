@@ -64,3 +64,17 @@ def test_splits_longer_than_the_table_of_places(device, dtype, steps, H, d_c):
     want, tol = exact(q, cache, table, lens, d_c, 0.2, dtype, 128)
     near(got[0], want[0], tol[0], "o")
     near(got[1], want[1], tol[1], "lse")
+
+
+@both
+@pytest.mark.parametrize("H", [8, 40, 100])
+@pytest.mark.parametrize("length", [40, 2000])
+def test_values_near_the_largest(device, dtype, H, length):
+    """Latents whose sum over some hundred rows leaves fp32's range, and whose mean does not."""
+    q, cache, table, n = make([length], 1, H, 128, 16, 64, dtype, seed=23)
+    cache[..., 5], q[..., 5] = 1.5e37, 0.0
+    cache[..., 6], q[..., 6] = 1e36 * cache[..., 6], 0.0
+    got = run(q, cache, table, n, 128, 0.05, device)
+    want, tol = exact(q, cache, table, n, 128, 0.05, dtype, 64)
+    near(got[0], want[0], tol[0], "o")
+    near(got[1], want[1], tol[1], "lse")
