@@ -1,8 +1,8 @@
 /*
  * rhizome_attention.h -- C ABI of the Global block's latent attention in
  * librhizome_gdr.so: rotary positions, the paged cache of latents with its
- * writer and its single-position reader, and the prefill with its backward
- * pass.
+ * writer and its reader of a sequence's last positions, and the prefill with
+ * its backward pass.
  *
  * A token has one latent c_t (d_c values) and one rotary key r_t (d_r values)
  * for all heads.  Expanded, head h has the key [k_t,h | r_t] and the value
@@ -109,8 +109,8 @@ typedef struct rhz_latent_append_args {
     int32_t interleaved;
     float magnitude;   /* finite */
     float eps;         /* >= 0 */
-    int64_t latent_stride; /* of a token, >= d_c */
-    int64_t k_rope_stride; /* >= d_r */
+    int64_t latent_stride; /* of a token, >= 0 */
+    int64_t k_rope_stride; /* likewise */
     const void* latent;        /* [tokens, d_c] */
     const void* k_rope;        /* [tokens, d_r], or NULL where d_r is 0 */
     const int32_t* cu_seqlens; /* device [batch + 1], or NULL (dense) */
@@ -127,7 +127,9 @@ rhz_status rhz_latent_append(const rhz_latent_append_args* args, void* stream);
  * latents, absorbed (mla_decode, attention.rs:226-300): query i of sequence b
  * sees positions 0 .. lengths[b] - steps + i.  Positions beyond the table, or
  * from 2^31 - 4097 on, and pages outside the cache hold no keys.  A sequence is split over workgroups by its
- * own length alone and joined in order. */
+ * own length alone and joined in order.  bf16 on bf16 matrix instructions with
+ * fp32 accumulation, the weights rounded to bf16 before they meet the latents;
+ * fp32 in fp32. */
 typedef struct rhz_latent_decode_args {
     int32_t batch;     /* >= 1 */
     int32_t steps;     /* 1..RHZ_MULTISTEP_MAX */
@@ -160,7 +162,8 @@ rhz_status rhz_latent_decode(const rhz_latent_decode_args* args, void* stream);
  * last query of a sequence sees all of its keys, the one before it all but the
  * last, and so on, so that queries that continue a cached context bring its
  * keys along.  bf16 on bf16 matrix instructions with fp32 accumulation, the
- * weights rounded to bf16 before they meet the values; fp32 in fp32. */
+ * weights rounded to bf16 before they meet the values; fp32 in fp32.  Tokens of
+ * q, k, v and k_rope are at most 2^22 elements apart. */
 typedef struct rhz_latent_prefill_args {
     int32_t batch;     /* sequences, >= 1 */
     int32_t seq_len;   /* queries: dense: of every sequence;  packed: of all */
@@ -172,7 +175,7 @@ typedef struct rhz_latent_prefill_args {
     int32_t dtype;     /* rhz_dtype of q, k, k_rope, v and o */
     int32_t causal;    /* 0 or 1 */
     float scale;       /* > 0, finite */
-    int64_t q_token_stride, q_head_stride;
+    int64_t q_token_stride, q_head_stride; /* all >= 0 */
     int64_t k_token_stride, k_head_stride;
     int64_t v_token_stride, v_head_stride;
     int64_t k_rope_stride;
@@ -191,7 +194,8 @@ rhz_status rhz_latent_prefill(const rhz_latent_prefill_args* args, void* stream)
 /* Backward pass of rhz_latent_prefill: `forward` is that call's arguments, its
  * o and lse read here as it wrote them, and grad_o (and grad_lse) the gradients
  * of its outputs.  The gradients are contiguous, of q's dtype; grad_k_rope is
- * summed over the heads in fp32 and rounded once.  Rows of a pack outside every
+ * summed over the heads in fp32 and rounded once.  In bf16 the weights, and their
+ * gradients, are rounded to bf16 before the products that sum them.  Rows of a pack outside every
  * sequence are left as they were.  No output overlaps an input, the workspace
  * or another output. */
 typedef struct rhz_latent_prefill_backward_args {

@@ -21,7 +21,6 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // 16 bytes: 8 bf16 or 4 fp32 values
 template <typename T> constexpr int kChunkElems = 16 / int(sizeof(T));
@@ -91,7 +90,10 @@ __device__ __forceinline__ void dot_chunks(f32x16& acc, const u32x4& a, const u3
 }
 
 // ---- products over the tile's rows: acc[column d, lane's row] += sum_r tile[r][d] p[r, lane's row]
-// p of 32 tile rows as the operand: registers 8 s .. 8 s + 7 are step s.
+// p of 32 tile rows as the operand: registers 8 s .. 8 s + 7 are step s.  Where the
+// tensors are bf16 the weights (and in the backward pass their gradients) are
+// rounded to it: an fp32 product takes sixteen times as long.  The error against 64
+// bits grows from 1.6e-3, the result's own rounding, to 2.0 to 2.3e-3 of its size.
 template <typename T> struct Weights;
 template <> struct Weights<uint16_t> {
     bf16x8 x[2];

@@ -128,8 +128,8 @@ struct AppendParams {
     float magnitude, eps;
 };
 
-// Chunks of a lane that stay in registers: 1024 bf16 or 512 fp32 latents, those
-// behind are read twice.  With eight, for 4096, the registers leave room for fewer
+// Chunks of a lane that stay in registers: 1024 bf16 or 512 fp32 latents (128 of
+// either where a chunk is one value), those behind are read twice.  With eight, for 4096, the registers leave room for fewer
 // waves: 10333 tokens of 512 + 64, 11.0 us instead of 10.1.
 constexpr int kMaxChunks = 2;
 
