@@ -9,10 +9,11 @@
 // seven products instead of the five that one kernel needs, which would have to
 // add its dq from all key tiles in memory, in no fixed order or with waits.
 //
-// 2 x 4096 tokens, 32 heads of 128 + 64 channels, causal: 1357 us, of which D and
-// lse 33 (134 MB, 4.1 TB/s), dk and dv 870 (790 TFLOP/s of its four
-// products), dq 505 (1090 of its three), the sum over heads 14.  The seven products
-// at the 1152 TFLOP/s of a large one: 1074 us, the formula's five 775.
+// 2 x 4096 tokens, 32 heads of 128 + 64 channels, causal: 1350 to 1420 us by the
+// card's clocks.  Of 1394 by one trace of the kernels, D and lse take 31 (134 MB, 4.4
+// TB/s), dk and dv 838 (820 TFLOP/s of its four products), dq 511 (1075 of its
+// three), the sum over heads 15.  The seven products at the 1152 TFLOP/s of a large
+// one: 1074 us, the formula's five 775.
 #include "attn_params.hpp"
 
 namespace rhz {
@@ -112,7 +113,9 @@ __global__ __launch_bounds__(512, 2) void attn_dkv_kernel(BackwardParams a) {
         if (!second) move_q.clear(qtiles[i]);
         if (second) move_o.clear(otiles[i]);
     }
-    // Tile j is there, for all waves, while j + 1 may be on its way.
+    // Tile j is there, for all waves, while j + 1 may be on its way -- if every panel is
+    // full and of one tensor: the waits count panels.  Else (64 + 32 channels) j + 1 has
+    // to be there too.
     const bool counted = VEC && move_q.whole && move_o.whole;
     const auto wait = [&](int j) {
         if (counted && j + 1 < tiles) {

@@ -93,7 +93,7 @@ __device__ __forceinline__ void dot_chunks(f32x16& acc, const u32x4& a, const u3
 // p of 32 tile rows as the operand: registers 8 s .. 8 s + 7 are step s.  Where the
 // tensors are bf16 the weights (and in the backward pass their gradients) are
 // rounded to it: an fp32 product takes sixteen times as long.  The error against 64
-// bits grows from 1.6e-3, the result's own rounding, to 2.0 to 2.3e-3 of its size.
+// bits grows from 1.6 to 1.8e-3 of a result, its own rounding, to 1.7 to 2.4e-3.
 template <typename T> struct Weights;
 template <> struct Weights<uint16_t> {
     bf16x8 x[2];

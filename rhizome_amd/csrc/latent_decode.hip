@@ -163,10 +163,12 @@ __device__ __forceinline__ void load_panels(const void* p, int left, int row_byt
 // bf16 the second half of the row tiles is half a tile behind the first: between
 // two barriers one wave of a SIMD multiplies queries and keys while the other is at
 // the softmax and the sums (16 x 4096 positions at 128 rows 64 -> 59 us against all
-// in step, at 256 rows 130 -> 114).  What bounds it is the loads, 2.2 to 2.6 us for
-// the 36 KB of a tile on each CU with two tiles on their way, 3.7 to 4.3 TB/s: LDS
-// has no room for a fourth, and reading the sums' columns ahead of the products
-// changes nothing.
+// in step, at 256 rows 130 -> 114).  What bounds it is a workgroup's own way from
+// tile to tile -- scores, their exchange, softmax and sums between two barriers --
+// and the card's memory little: the 16 tiles of a split take 37, 39 and 45 us at 64
+// rows with 64, 128 and 256 workgroups (8, 16 and 32 x 4096 positions), 48, 50 and 58
+// at 128.  LDS has no room for a fourth tile, and reading the sums' columns ahead of
+// the products changes nothing.
 template <typename T, int VD, int RT, bool VEC>
 __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     constexpr int E = kChunkElems<T>, KD = VD + 64, BUFS = sizeof(T) == 2 ? 3 : 1, NT = 512, WAVES = 8, KEYS = 32;
@@ -244,7 +246,9 @@ __global__ __launch_bounds__(512, 2) void latent_decode_kernel(DecodeParams a) {
     if (end > begin) fill_table(begin);
     __syncthreads();
     const int tiles_n = (end - begin + KEYS - 1) / KEYS;
-    // whether a tile's loads are as many as the waits below count
+    // Whether a tile's loads are as many as the waits below count: not where the last
+    // panel has no columns (d_r = 0), where a tile waits for the next one's loads too
+    // (32 x 4096 positions at 64 rows, 512 + 0 channels 44 us, 512 + 64 45).
     const bool counted = VEC && (a.D + 8 * E - 1) / (8 * E) == TILE::kPanels;
     // The wave's part of tile i's scores, to LDS.
     const auto score = [&](int i) {
