@@ -411,18 +411,12 @@ template <int DQ, int DV, bool VEC>
 hipError_t launch(BackwardParams p, hipStream_t stream) {
     const int64_t tq = attn_tiles(p.cu_q, p.queries, p.len_q, p.batch, kRows);
     const int64_t tk = attn_tiles(p.cu_k, p.keys, p.len_k, p.batch, kRows);
-    if (p.keys) {
-        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_k, tk, 512);
-        if (!blocks) return hipErrorInvalidConfiguration;
-        p.tiles = (int)tk;
-        attn_dkv_kernel<DQ, DV, VEC><<<blocks, 512, 0, stream>>>(p);
-    }
-    if (p.queries) {
-        const unsigned blocks = attn_blocks(p.heads, p.batch, p.cu_q, tq);
-        if (!blocks) return hipErrorInvalidConfiguration;
-        p.tiles = (int)tq;
-        attn_dq_kernel<DQ, DV, VEC><<<blocks, kThreads, 0, stream>>>(p);
-    }
+    const unsigned dkv = attn_blocks(p.heads, p.batch, p.cu_k, tk, 512), dq = attn_blocks(p.heads, p.batch, p.cu_q, tq);
+    if ((p.keys && !dkv) || (p.queries && !dq)) return hipErrorInvalidConfiguration;
+    p.tiles = (int)tk;
+    if (p.keys) attn_dkv_kernel<DQ, DV, VEC><<<dkv, 512, 0, stream>>>(p);
+    p.tiles = (int)tq;
+    if (p.queries) attn_dq_kernel<DQ, DV, VEC><<<dq, kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 

@@ -707,15 +707,15 @@ int most_splits(const rhz_latent_decode_args& a) {
     return most_splits_of(a.dtype == RHZ_F32 ? kRule<float> : kRule<uint16_t>, std::min<int64_t>((int64_t)a.max_pages * a.page_size, kMostRows));
 }
 
-hipError_t join(const DecodeParams& p, int dtype, hipStream_t stream) {
-    const int64_t joins = (int64_t)p.batch * p.steps * p.heads * ((p.d_c + kJoinColumns - 1) / kJoinColumns);
-    if (p.splits > 1) {
-        if (check_grid(joins, kJoinThreads) != hipSuccess) return hipErrorInvalidConfiguration;
-        if (dtype == RHZ_F32)
-            latent_join_kernel<float><<<(unsigned)joins, kJoinThreads, 0, stream>>>(p);
-        else
-            latent_join_kernel<uint16_t><<<(unsigned)joins, kJoinThreads, 0, stream>>>(p);
-    }
+// The join's workgroups, none where no sequence can have two splits; -1 if there are too many.
+int64_t join_blocks(const DecodeParams& p) {
+    const int64_t blocks = (int64_t)p.batch * p.steps * p.heads * ((p.d_c + kJoinColumns - 1) / kJoinColumns);
+    if (p.splits == 1) return 0;
+    return check_grid(blocks, kJoinThreads) == hipSuccess ? blocks : -1;
+}
+template <typename T>
+hipError_t join(const DecodeParams& p, int64_t blocks, hipStream_t stream) {
+    if (blocks) latent_join_kernel<T><<<(unsigned)blocks, kJoinThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -729,17 +729,19 @@ unsigned blocks_of(DecodeParams& p, int tile, int threads) {
 template <typename T, int VD, int RT, bool VEC>
 hipError_t launch(DecodeParams p, hipStream_t stream) {
     const unsigned blocks = blocks_of(p, 32 * RT, 512);
-    if (!blocks) return hipErrorInvalidConfiguration;
+    const int64_t joins = join_blocks(p);
+    if (!blocks || joins < 0) return hipErrorInvalidConfiguration;
     latent_decode_kernel<T, VD, RT, VEC><<<blocks, 512, 0, stream>>>(p);
-    return join(p, sizeof(T) == 4 ? RHZ_F32 : RHZ_BF16, stream);
+    return join<T>(p, joins, stream);
 }
 
 template <int VD>
 hipError_t launch_narrow(DecodeParams p, hipStream_t stream) {
     const unsigned blocks = blocks_of(p, 16, 256);
-    if (!blocks) return hipErrorInvalidConfiguration;
+    const int64_t joins = join_blocks(p);
+    if (!blocks || joins < 0) return hipErrorInvalidConfiguration;
     latent_decode_narrow_kernel<VD><<<blocks, 256, 0, stream>>>(p);
-    return join(p, RHZ_BF16, stream);
+    return join<uint16_t>(p, joins, stream);
 }
 
 // By the rows of q of a sequence.  bf16, 32 sequences of 4096 positions, by the

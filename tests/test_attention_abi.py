@@ -178,6 +178,14 @@ def test_decode_validation(over, status, msg):
     refused("rhz_latent_decode", _fill(_abi.LatentDecodeArgs, DECODE, DECODE_PTRS, over), status, msg)
 
 
+def test_decode_with_more_rows_than_a_grid_can_join():
+    """Refused before the first of its two kernels: 65537 sequences of 128 heads, 512 channels and up to two splits."""
+    far = {name: A + (i << 37) for i, name in enumerate((*DECODE_PTRS, "workspace"))}
+    a = _fill(_abi.LatentDecodeArgs, DECODE, (), dict(batch=65537, steps=1, heads=128, page_size=256, max_pages=1,
+                                                      workspace_bytes=1 << 36, **far))
+    assert _abi.lib().rhz_latent_decode(byref(a), None) == _abi.ERR_HIP and "invalid configuration" in _abi.last_error()
+
+
 def test_decode_workspace_size():
     query = "rhz_latent_decode_workspace_size"
     make = lambda **over: _fill(_abi.LatentDecodeArgs, DECODE, DECODE_PTRS, over)
