@@ -126,10 +126,10 @@ rhz_status rhz_latent_append(const rhz_latent_append_args* args, void* stream);
 /* Attention of the last `steps` positions of every sequence over its cached
  * latents, absorbed (mla_decode, attention.rs:226-300): query i of sequence b
  * sees positions 0 .. lengths[b] - steps + i.  Positions beyond the table, or
- * from 2^31 - 4097 on, and pages outside the cache hold no keys.  A sequence is split over workgroups by its
- * own length alone and joined in order.  bf16 on bf16 matrix instructions with
- * fp32 accumulation, the weights rounded to bf16 before they meet the latents;
- * fp32 in fp32. */
+ * from 2^31 - 4097 on, and pages outside the cache hold no keys.  A sequence is
+ * split over workgroups by its own length alone and joined in order.  bf16 on
+ * bf16 matrix instructions with fp32 accumulation, the weights rounded to bf16
+ * before they meet the latents; fp32 in fp32. */
 typedef struct rhz_latent_decode_args {
     int32_t batch;     /* >= 1 */
     int32_t steps;     /* 1..RHZ_MULTISTEP_MAX */
@@ -195,9 +195,9 @@ rhz_status rhz_latent_prefill(const rhz_latent_prefill_args* args, void* stream)
  * o and lse read here as it wrote them, and grad_o (and grad_lse) the gradients
  * of its outputs.  The gradients are contiguous, of q's dtype; grad_k_rope is
  * summed over the heads in fp32 and rounded once.  In bf16 the weights, and their
- * gradients, are rounded to bf16 before the products that sum them.  Rows of a pack outside every
- * sequence are left as they were.  No output overlaps an input, the workspace
- * or another output. */
+ * gradients, are rounded to bf16 before the products that sum them.  Rows of a
+ * pack outside every sequence are left as they were.  No output overlaps an
+ * input, the workspace or another output. */
 typedef struct rhz_latent_prefill_backward_args {
     rhz_latent_prefill_args forward;
     const void* grad_o;    /* [queries, H, d_v] */

@@ -129,8 +129,9 @@ struct AppendParams {
 };
 
 // Chunks of a lane that stay in registers: 1024 bf16 or 512 fp32 latents (128 of
-// either where a chunk is one value), those behind are read twice.  With eight, for 4096, the registers leave room for fewer
-// waves: 10333 tokens of 512 + 64, 11.0 us instead of 10.1.
+// either where a chunk is one value), those behind are read twice.  With eight, for
+// 4096, the registers leave room for fewer waves: 10333 tokens of 512 + 64, 11.0 us
+// instead of 10.1.
 constexpr int kMaxChunks = 2;
 
 // A wave a token: the latent is read once and kept in registers while its norm is
