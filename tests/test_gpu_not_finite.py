@@ -106,7 +106,7 @@ def check_time(run_with, finite, cases):
     for name in cases:
         t = took(lambda: run_with({k: torch.full_like(v, math.nan) if k in name else v for k, v in finite.items()}))
         print(f"NaN in {', '.join(name)}: {t:.3f} ms, finite {usual:.3f}", flush=True)
-        assert t < 8 * usual + 3.0, f"NaN in {name}: {t:.1f} ms instead of {usual:.2f}"
+        assert t < 20 * usual + 3.0, f"NaN in {name}: {t:.1f} ms instead of {usual:.2f}"
 
 
 EVERY = ("q", "k", "v", "r", "do")
